@@ -366,6 +366,156 @@ size_t pal_epilogue_bwd_workspace_bytes(const PalGlueDims *dims);
 int pal_epilogue_bwd(const PalGlueDims *dims, const PalEpilogueTensors *t, const PalEpilogueGrads *gr,
                      void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---------------------------------------------- residual norm, 8-bit rows */
+
+/* Pre-norm between two blocks with the residual's addition (the block's fla.modules.RMSNorm with prenorm: the
+ * reference's PalimpsaBlock calls it between its mixer and its MLP; restated from its published behaviour):
+ *   s = x + residual, rounded to res_dtype and handed on;  y = s * rsqrt(mean(s^2) + eps) * weight
+ * Rows of any length up to 16384 at any element's address. */
+typedef struct PalNormDims {
+  int64_t rows;
+  int64_t x_stride;     /* elements between rows of x (>= dim); every other row tensor is packed, but: */
+  int64_t res_stride;   /* elements between rows of residual (>= dim)           */
+  int32_t dim;          /* entries per row                                      */
+  int32_t dtype;        /* PAL_DTYPE_* of x, y, dy, dx                          */
+  int32_t res_dtype;    /* of residual, residual_out and their gradients: F32, or BF16 if dtype is BF16 */
+  int32_t weight_dtype; /* of weight                                            */
+  int32_t group;        /* entries per 8-bit scale: 32, 64, 128 or 256 and a divisor of dim, or 0 for the whole row */
+  float eps;
+} PalNormDims;
+
+typedef struct PalNormTensors {
+  const void *x;        /* dtype [rows,dim]                                     */
+  const void *residual; /* res_dtype [rows,dim] or NULL (the first block)       */
+  const void *weight;   /* weight_dtype [dim]                                   */
+  void *residual_out;   /* res_dtype [rows,dim]                                 */
+  void *y;              /* dtype [rows,dim]; with scales: OCP e4m3 [rows,dim], one byte each */
+  float *scales;        /* fp32 [rows, dim / group] ([rows, 1] for group 0), or NULL: scale = max(max|y|, 1e-12) / 448,
+                           rows hold round(y / scale); NaN for a row whose sum of squares is not finite */
+} PalNormTensors;
+
+typedef struct PalNormGrads {
+  const void *dy;            /* dtype [rows,dim] or NULL (zero)                 */
+  const void *dresidual_out; /* res_dtype [rows,dim] or NULL (zero)             */
+  void *dx;                  /* dtype [rows,dim]                                */
+  void *dresidual;           /* res_dtype [rows,dim]; may be NULL where res_dtype == dtype (it is dx) */
+  float *dweight;            /* fp32 [dim]                                      */
+} PalNormGrads;
+
+int pal_residual_norm_fwd(const PalNormDims *dims, const PalNormTensors *t, void *stream);
+/* Backward: reads t->weight and t->residual_out (as the forward call wrote it); the other tensors of t are not touched. */
+size_t pal_residual_norm_bwd_workspace_bytes(const PalNormDims *dims);
+int pal_residual_norm_bwd(const PalNormDims *dims, const PalNormTensors *t, const PalNormGrads *gr,
+                          void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------ short causal convolution */
+
+/* The depthwise causal convolution in front of the operator (fla.modules.ShortConvolution in palimpsa/layers/palimpsa.py:240-257,
+ * conv1d in layers/meta_mamba2.py), restated from its published behaviour:
+ *   p[t,c] = bias[c] + sum_{i < width} weight[c, width-1-i] x[t-i,c],   y = p or p * sigmoid(p)
+ * with x[t-i] of tokens before the sequence taken from init (column width - i + t), or zero.  States hold the last `width`
+ * inputs, oldest first. */
+#define PAL_CONV_MAX_WIDTH 8
+
+typedef struct PalConvDims {
+  int32_t batch, seq_len, n_seqs; /* as in PalDims; a packed batch may hold empty sequences, n_seqs is not bound by seq_len */
+  int32_t channels;
+  int32_t width;          /* taps, 2 .. PAL_CONV_MAX_WIDTH                      */
+  int32_t total_chunks;   /* packed: rows of chunk_table                        */
+  int32_t dtype;          /* PAL_DTYPE_* of x, y, init, final and their gradients */
+  int32_t weight_dtype;   /* of weight and bias                                 */
+  int32_t silu;           /* 1: y = p sigmoid(p); 0: y = p                      */
+  uint32_t flags;         /* PAL_FLAG_VARLEN, PAL_FLAG_HAS_INIT, PAL_FLAG_STORE_FINAL */
+  int64_t x_batch_stride; /* elements between batch rows and between tokens of x; y and all gradients are packed */
+  int64_t x_token_stride;
+} PalConvDims;
+
+typedef struct PalConvTensors {
+  const void *x;              /* dtype [B,T,D]                                  */
+  const void *weight;         /* weight_dtype [D,width]                         */
+  const void *bias;           /* weight_dtype [D] or NULL                       */
+  void *y;                    /* dtype [B,T,D]                                  */
+  const void *init;           /* dtype [N,D,width] or NULL                      */
+  void *final_;               /* dtype [N,D,width] or NULL; not init            */
+  const int32_t *cu_seqlens;  /* device int32 [N+1] or NULL                     */
+  const int32_t *chunk_table; /* device int32 [total_chunks,4] (pal_build_chunk_table) or NULL */
+} PalConvTensors;
+
+typedef struct PalConvGrads {
+  const void *dy;             /* dtype [B,T,D]                                  */
+  const void *d_final;        /* dtype [N,D,width] or NULL (zero)               */
+  void *dx;                   /* dtype [B,T,D]                                  */
+  float *dweight, *dbias;     /* fp32 [D,width], [D] (NULL iff bias is NULL)    */
+  void *d_init;               /* dtype [N,D,width] or NULL                      */
+} PalConvGrads;
+
+int pal_short_conv_fwd(const PalConvDims *dims, const PalConvTensors *t, void *stream);
+size_t pal_short_conv_bwd_workspace_bytes(const PalConvDims *dims);
+int pal_short_conv_bwd(const PalConvDims *dims, const PalConvTensors *t, const PalConvGrads *gr,
+                       void *workspace, size_t workspace_bytes, void *stream);
+/* Tokens of a generation: batch sequences of seq_len tokens (a few), the state in t->final_ [B,D,width] is read and written in
+ * place (t->init is not looked at; flags other than PAL_FLAG_VARLEN, which is refused, are ignored). */
+int pal_short_conv_step(const PalConvDims *dims, const PalConvTensors *t, void *stream);
+
+/* ---------------------------------------------------------- selective scan */
+
+/* The third recurrence of this family, with a decay of its own for every channel d and state entry n (selective state
+ * spaces; Gu and Dao, "Mamba: Linear-Time Sequence Modeling with Selective State Spaces", 2023, equations 2 and 4):
+ *   dt = softplus(delta + delta_bias)  (or delta + delta_bias),   h[d,n] = exp(dt A[d,n]) h[d,n] + dt u[d] B[n],
+ *   y[d] = (sum_n C[n] h[d,n] + D[d] u[d]) * z sigmoid(z)
+ * B and C are shared by the channels of a group (channel d reads group d / (channels / groups)). */
+#define PAL_SCAN_MAX_STATE 64
+/* tokens between two kept states (PalScanTensors.checkpoints) */
+#define PAL_SCAN_BLOCK 16
+
+typedef struct PalScanDims {
+  int32_t batch, seq_len, n_seqs; /* as in PalDims; a packed batch may hold empty sequences, n_seqs is not bound by seq_len */
+  int32_t channels;       /* D                                                  */
+  int32_t state;          /* N: entries of the state per channel, 1 .. PAL_SCAN_MAX_STATE */
+  int32_t groups;         /* G: groups of B and C, a divisor of channels        */
+  int32_t dtype;          /* PAL_DTYPE_* of the rows: u, delta, B, C, z, y and their gradients */
+  int32_t softplus;       /* 1: dt = softplus(delta + delta_bias); 0: their sum as it is */
+  uint32_t flags;         /* PAL_FLAG_VARLEN, PAL_FLAG_HAS_INIT, PAL_FLAG_STORE_FINAL */
+  /* elements between batch rows and between tokens; y and all gradients are packed */
+  int64_t u_batch, u_token, delta_batch, delta_token, z_batch, z_token, B_batch, B_token, C_batch, C_token;
+} PalScanDims;
+
+typedef struct PalScanTensors {
+  const void *u, *delta;      /* dtype [B,T,D]                                  */
+  const float *A;             /* fp32 [D,N]                                     */
+  const void *B, *C;          /* dtype [B,T,G,N]                                */
+  const float *D;             /* fp32 [D] or NULL                               */
+  const void *z;              /* dtype [B,T,D] or NULL (no gate)                */
+  const float *delta_bias;    /* fp32 [D] or NULL                               */
+  void *y;                    /* dtype [B,T,D]                                  */
+  const float *init;          /* fp32 [N_seqs,D,N] or NULL                      */
+  float *final_;              /* fp32 [N_seqs,D,N] or NULL; may be init where no gradient is wanted */
+  const int32_t *cu_seqlens;  /* device int32 [n_seqs+1] or NULL                */
+  float *checkpoints;         /* pal_scan_checkpoint_bytes(dims), for the backward, or NULL */
+} PalScanTensors;
+
+typedef struct PalScanGrads {
+  const void *dy;             /* dtype [B,T,D]                                  */
+  const float *d_final;       /* fp32 [N_seqs,D,N] or NULL (zero)               */
+  void *du, *ddelta;          /* dtype [B,T,D]                                  */
+  float *dA;                  /* fp32 [D,N]                                     */
+  void *dB, *dC;              /* dtype [B,T,G,N]                                */
+  float *dD;                  /* fp32 [D], NULL iff D is NULL                   */
+  void *dz;                   /* dtype [B,T,D], NULL iff z is NULL              */
+  float *ddelta_bias;         /* fp32 [D], NULL iff delta_bias is NULL          */
+  float *d_init;              /* fp32 [N_seqs,D,N] or NULL                      */
+} PalScanGrads;
+
+/* Forward; seq_len = 1 with final_ == init is a step of a generation.  workspace: pal_scan_fwd_workspace_bytes(dims) bytes
+ * (0 for many calls: NULL is fine then). */
+size_t pal_scan_checkpoint_bytes(const PalScanDims *dims);
+size_t pal_scan_fwd_workspace_bytes(const PalScanDims *dims);
+int pal_scan_fwd(const PalScanDims *dims, const PalScanTensors *t, void *workspace, size_t workspace_bytes, void *stream);
+/* Backward: t as in the forward call, with the checkpoints as that call left them; t->y and t->final_ are not touched. */
+size_t pal_scan_bwd_workspace_bytes(const PalScanDims *dims);
+int pal_scan_bwd(const PalScanDims *dims, const PalScanTensors *t, const PalScanGrads *gr, void *workspace,
+                 size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------------------ shape queries */
 
 /* 1 if the chunked entry points would build the tile-start states of this call (dims as handed to them,

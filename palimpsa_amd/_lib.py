@@ -75,6 +75,51 @@ class PalEpilogueGrads(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("dy", "d_o", "dx", "dgate", "dD", "dweight")]
 
 
+class PalNormDims(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("x_stride", C.c_int64), ("res_stride", C.c_int64), ("dim", C.c_int32),
+                ("dtype", C.c_int32), ("res_dtype", C.c_int32), ("weight_dtype", C.c_int32), ("group", C.c_int32),
+                ("eps", C.c_float)]
+
+
+class PalNormTensors(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "residual", "weight", "residual_out", "y", "scales")]
+
+
+class PalNormGrads(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("dy", "dresidual_out", "dx", "dresidual", "dweight")]
+
+
+class PalConvDims(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("batch", "seq_len", "n_seqs", "channels", "width", "total_chunks", "dtype",
+                                          "weight_dtype", "silu")] + [("flags", C.c_uint32)] +
+                [(n, C.c_int64) for n in ("x_batch_stride", "x_token_stride")])
+
+
+class PalConvTensors(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "weight", "bias", "y", "init", "final_", "cu_seqlens", "chunk_table")]
+
+
+class PalConvGrads(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("dy", "d_final", "dx", "dweight", "dbias", "d_init")]
+
+
+class PalScanDims(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("batch", "seq_len", "n_seqs", "channels", "state", "groups", "dtype", "softplus")] +
+                [("flags", C.c_uint32)] +
+                [(n, C.c_int64) for n in ("u_batch", "u_token", "delta_batch", "delta_token", "z_batch", "z_token",
+                                          "B_batch", "B_token", "C_batch", "C_token")])
+
+
+class PalScanTensors(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "y", "init", "final_",
+                                          "cu_seqlens", "checkpoints")]
+
+
+class PalScanGrads(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("dy", "d_final", "du", "ddelta", "dA", "dB", "dC", "dD", "dz", "ddelta_bias",
+                                          "d_init")]
+
+
 class PalimpsaHipError(RuntimeError):
     def __init__(self, code: int, where: str, text: str):
         super().__init__(f"{where} failed with code {code}: {text}")
@@ -131,6 +176,22 @@ def load() -> C.CDLL:
         fn = getattr(lib, name)
         fn.restype = C.c_size_t
         fn.argtypes = [P(PalGlueDims)]
+    for name, dims, tensors, grads in (("pal_residual_norm", PalNormDims, PalNormTensors, PalNormGrads),
+                                       ("pal_short_conv", PalConvDims, PalConvTensors, PalConvGrads),
+                                       ("pal_scan", PalScanDims, PalScanTensors, PalScanGrads)):
+        fwd, bwd, ws = (getattr(lib, name + x) for x in ("_fwd", "_bwd", "_bwd_workspace_bytes"))
+        fwd.restype = bwd.restype = C.c_int
+        fwd.argtypes = [P(dims), P(tensors), C.c_void_p]
+        bwd.argtypes = [P(dims), P(tensors), P(grads), C.c_void_p, C.c_size_t, C.c_void_p]
+        ws.restype = C.c_size_t
+        ws.argtypes = [P(dims)]
+    lib.pal_short_conv_step.restype = C.c_int
+    lib.pal_short_conv_step.argtypes = [P(PalConvDims), P(PalConvTensors), C.c_void_p]
+    lib.pal_scan_fwd.argtypes = [P(PalScanDims), P(PalScanTensors), C.c_void_p, C.c_size_t, C.c_void_p]
+    for name in ("pal_scan_fwd_workspace_bytes", "pal_scan_checkpoint_bytes"):
+        fn = getattr(lib, name)
+        fn.restype = C.c_size_t
+        fn.argtypes = [P(PalScanDims)]
     lib.pal_state_pass_applies.restype = C.c_int
     lib.pal_state_pass_applies.argtypes = [P(PalDims), C.c_int]
     lib.pal_chunk_fwd_segments.restype = C.c_int

@@ -32,6 +32,19 @@ enum KernelId {
   kKernGlaBwdTile,
   kKernBwdPartsSum,
   kKernRecurrentSeg,
+  kKernResidualNormFwd,
+  kKernResidualNormBwd,
+  kKernResidualNormReduce,
+  kKernShortConvFwd,
+  kKernShortConvBwd,
+  kKernShortConvReduce,
+  kKernShortConvStep,
+  kKernScanFwd,
+  kKernScanSegment,
+  kKernScanJoin,
+  kKernScanBwd,
+  kKernScanBwdRows,
+  kKernScanBwdParams,
   kKernCount
 };
 

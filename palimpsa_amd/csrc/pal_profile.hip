@@ -54,7 +54,10 @@ static const char* kNames[kKernCount] = {
     "gla_dq_kernel", "gla_dv_kernel", "gla_dk_kernel", "gla_bwd_scan_kernel", "gla_bwd_gate_kernel",
     "prologue_fwd_kernel", "prologue_bwd_kernel", "epilogue_fwd_kernel", "epilogue_bwd_kernel",
     "gla_recurrent_fwd_kernel", "chunk_states_kernel", "gla_bwd_states_kernel", "gla_bwd_tile_kernel",
-    "chunk_bwd_parts_sum_kernel", "recurrent_seg_kernel"};
+    "chunk_bwd_parts_sum_kernel", "recurrent_seg_kernel", "residual_norm_fwd_kernel", "residual_norm_bwd_kernel",
+    "residual_norm_reduce_kernel", "short_conv_fwd_kernel", "short_conv_bwd_kernel", "short_conv_reduce_kernel",
+    "short_conv_step_kernel", "scan_fwd_kernel", "scan_segment_kernel", "scan_join_kernel", "scan_bwd_kernel",
+    "scan_bwd_rows_kernel", "scan_bwd_params_kernel"};
 
 }  // namespace pal
 

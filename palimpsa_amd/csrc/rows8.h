@@ -1,0 +1,74 @@
+// Rows of any length and alignment, eight consecutive elements per lane: whole pieces move as 16-byte accesses (which the
+// global memory path takes at any element's address), the last piece of a row whose length is no multiple of eight
+// element by element.
+#pragma once
+#include <type_traits>
+
+#include "pal_common.h"
+
+namespace pal {
+
+typedef bf16x8 bf16x8_any __attribute__((aligned(2)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+
+// eight elements as fetched, converted when they are used
+template <typename T>
+struct Piece8;
+template <>
+struct Piece8<bf16_t> {
+  bf16x8 v;
+  __device__ __forceinline__ void load(const bf16_t* p) { v = *(const bf16x8_any*)p; }
+  __device__ __forceinline__ float get(int e) const { return (float)v[e]; }
+  __device__ __forceinline__ void set(int e, bf16_t x) { v[e] = x; }
+};
+template <>
+struct Piece8<float> {
+  f32x4 lo, hi;
+  __device__ __forceinline__ void load(const float* p) { lo = *(const f32x4_any*)p; hi = *(const f32x4_any*)(p + 4); }
+  __device__ __forceinline__ float get(int e) const { return e < 4 ? lo[e & 3] : hi[e & 3]; }
+  __device__ __forceinline__ void set(int e, float x) { if (e < 4) lo[e & 3] = x; else hi[e & 3] = x; }
+};
+
+// `n` elements of the piece are there (8 or more: all; 0 or less: none, and nothing is read), the others are zero
+template <typename T>
+__device__ __forceinline__ void load_piece(Piece8<T>& d, const T* p, int n) {
+  if (n >= 8) {
+    d.load(p);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d.set(e, e < n ? p[e] : (T)0.f);
+  }
+}
+__device__ __forceinline__ void store_piece(bf16_t* p, const float* x, int n) {
+  if (n >= 8) {
+    const bf16x2 a = pack2(x[0], x[1]), b = pack2(x[2], x[3]), c = pack2(x[4], x[5]), d = pack2(x[6], x[7]);
+    const bf16x8 v = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+    *(bf16x8_any*)p = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = (bf16_t)x[e];
+  }
+}
+__device__ __forceinline__ void store_piece(float* p, const float* x, int n) {
+  if (n >= 8) {
+    const f32x4 a = {x[0], x[1], x[2], x[3]}, b = {x[4], x[5], x[6], x[7]};
+    *(f32x4_any*)p = a;
+    *(f32x4_any*)(p + 4) = b;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) p[e] = x[e];
+  }
+}
+
+// per-channel parameters of either type, eight at a time
+__device__ __forceinline__ void load_params(float* out, const void* p, int64_t i, int is_bf16, int n) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) out[e] = e < n ? load_rt(p, i + e, is_bf16) : 0.f;
+}
+
+// reciprocal to 1 ulp (one instruction; an IEEE division is ten), logistic function
+__device__ __forceinline__ float logistic(float x) { return fast_rcp(1.f + __expf(-x)); }
+
+}  // namespace pal

@@ -1,0 +1,530 @@
+// Short causal convolution, one filter of `width` taps per channel, with its activation and its state:
+//     p[t,c] = bias[c] + sum_{i<W} w[c, W-1-i] x[t-i,c],    y = p  or  p sigmoid(p),
+// x before the first token of a sequence taken from the state it starts with (column W + t of [N,D,W]), or zero.
+// Backward, with dp = dy act'(p):  dx[t] = sum_i w[W-1-i] dp[t+i] (the tokens of the sequence),  dw[W-1-i] = sum_t dp[t] x[t-i],
+// dbias = sum_t dp[t]; the state's gradient is dx at t < 0.
+//
+// Bound by HBM: a thread owns a few neighbouring channels of a run of tokens of one sequence and walks the run with the last
+// inputs in registers, so a row is read once (and its last W - 1 tokens once more by the run after it).  Dense batches are cut into
+// runs of equal length; packed ones take the tiles of the chunk table (64 tokens of one sequence at most), cut the same way, so
+// that no thread looks for its sequence.  Partial sums of dw and dbias are added over the runs of a workgroup, then over the
+// workgroups, in a fixed order.
+#include "pal_common.h"
+#include "pal_host.h"
+#include "pal_profile.h"
+#include "rows8.h"
+
+namespace pal {
+
+struct ConvArgs {
+  const void *x, *weight, *bias, *init, *dy, *d_final;
+  void *y, *final_, *dx, *d_init;
+  const int32_t *cu, *table;
+  float *part, *dweight, *dbias;
+  int64_t xb, xt;          // strides of x
+  int32_t T, D, N, chunks, weight_bf16, silu;
+  int32_t run, runs;       // tokens per run, runs of the pass
+  int32_t pieces;          // pieces of channels
+  int32_t blocks;          // workgroups that convolve; the ones behind them write states
+  int32_t per_tile;        // runs per tile of the table (packed), or per batch row
+};
+
+// run r: its sequence, the tokens [t0, t1) it covers and those of the sequence, [s0, s1), all counted in rows of the tensors
+struct ConvRun {
+  int32_t seq;
+  int64_t t0, t1, s0, s1, row0;   // row0: first token of the batch row
+  __device__ __forceinline__ ConvRun(const ConvArgs& a, int r) {
+    const int tile = r / a.per_tile, sub = r - tile * a.per_tile;
+    if (a.cu) {
+      const int32_t* e = a.table + 4 * (int64_t)tile;
+      seq = min(max(e[0], 0), a.N - 1);
+      int bos, len;
+      packed_seq_bounds(a.cu, seq, a.T, bos, len);
+      s0 = bos;
+      s1 = (int64_t)bos + len;
+      row0 = 0;
+      const int64_t first = min(max((int64_t)e[1], s0), s1), last = min(first + min(max(e[2], 0), PAL_CHUNK), s1);
+      t0 = min(first + (int64_t)sub * a.run, last);
+      t1 = min(t0 + a.run, last);
+    } else {
+      seq = tile;
+      s0 = row0 = (int64_t)tile * a.T;
+      s1 = s0 + a.T;
+      t0 = s0 + (int64_t)sub * a.run;
+      t1 = min(t0 + a.run, s1);
+    }
+  }
+  // element of x at token t (a row of this run's batch row)
+  __device__ __forceinline__ int64_t at(const ConvArgs& a, int64_t t) const {
+    return a.cu ? t * a.xt : (int64_t)seq * a.xb + (t - row0) * a.xt;
+  }
+};
+
+// VW neighbouring channels: pieces of eight for bf16 rows in the forward, of four elsewhere
+template <typename T, int VW>
+struct Chans;
+template <typename T>
+struct Chans<T, 8> {
+  Piece8<T> v;
+  __device__ __forceinline__ void load(const T* p, int n) { load_piece(v, p, n); }
+  __device__ __forceinline__ float get(int e) const { return v.get(e); }
+};
+template <>
+struct Chans<bf16_t, 4> {
+  typedef bf16x4 any __attribute__((aligned(2)));
+  bf16x4 v;
+  __device__ __forceinline__ void load(const bf16_t* p, int n) {
+    if (n >= 4) {
+      v = *(const any*)p;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = e < n ? p[e] : (bf16_t)0.f;
+    }
+  }
+  __device__ __forceinline__ float get(int e) const { return (float)v[e]; }
+};
+template <>
+struct Chans<float, 4> {
+  f32x4 v;
+  __device__ __forceinline__ void load(const float* p, int n) {
+    if (n >= 4) {
+      v = *(const f32x4_any*)p;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = e < n ? p[e] : 0.f;
+    }
+  }
+  __device__ __forceinline__ float get(int e) const { return v[e]; }
+};
+template <int VW>
+__device__ __forceinline__ void store_chans(bf16_t* p, const float* x, int n) {
+  if constexpr (VW == 8) {
+    store_piece(p, x, n);
+  } else if (n >= 4) {
+    typedef bf16x4 any __attribute__((aligned(2)));
+    const bf16x2 a = pack2(x[0], x[1]), b = pack2(x[2], x[3]);
+    const bf16x4 v = {a[0], a[1], b[0], b[1]};
+    *(any*)p = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) p[e] = (bf16_t)x[e];
+  }
+}
+template <int VW>
+__device__ __forceinline__ void store_chans(float* p, const float* x, int n) {
+  if (n >= 4) {
+    const f32x4 v = {x[0], x[1], x[2], x[3]};
+    *(f32x4_any*)p = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < n) p[e] = x[e];
+  }
+}
+
+template <int W, int VW>
+__device__ __forceinline__ void load_taps(float (*w)[VW], float* bias, const ConvArgs& a, int c, int n) {
+#pragma unroll
+  for (int e = 0; e < VW; ++e) {
+#pragma unroll
+    for (int k = 0; k < W; ++k) w[k][e] = e < n ? load_rt(a.weight, (int64_t)(c + e) * W + k, a.weight_bf16) : 0.f;
+    bias[e] = a.bias && e < n ? load_rt(a.bias, c + e, a.weight_bf16) : 0.f;
+  }
+}
+// the W - 1 inputs before token t: rows of the sequence, or the state it starts with, or zero; h[0] the oldest
+template <typename T, int W, int VW>
+__device__ __forceinline__ void load_before(float (*h)[VW], const ConvArgs& a, const ConvRun& r, int64_t t, int c, int n) {
+#pragma unroll
+  for (int k = 0; k < W - 1; ++k) {
+    const int64_t tk = t - (W - 1) + k;
+    if (tk >= r.s0) {
+      Chans<T, VW> x;
+      x.load((const T*)a.x + r.at(a, tk) + c, n);
+#pragma unroll
+      for (int e = 0; e < VW; ++e) h[k][e] = x.get(e);
+    } else {
+      const int slot = (int)(tk - r.s0) + W;   // 1 .. W - 1
+#pragma unroll
+      for (int e = 0; e < VW; ++e) h[k][e] = a.init && e < n ? to_f32(((const T*)a.init)[((int64_t)r.seq * a.D + c + e) * W + slot]) : 0.f;
+    }
+  }
+}
+
+// final states: the last W inputs of a sequence, its old state moved up where it is shorter
+template <typename T>
+__device__ __forceinline__ void conv_states(const ConvArgs& a, int W, int block) {
+  const int64_t total = (int64_t)a.N * a.D * W;
+  for (int64_t i = (int64_t)block * 256 + threadIdx.x; i < total; i += (int64_t)(gridDim.x - a.blocks) * 256) {
+    const int k = (int)(i % W);
+    const int64_t nc = i / W;
+    const int c = (int)(nc % a.D), seq = (int)(nc / a.D);
+    int64_t s0 = (int64_t)seq * a.T, len = a.T;
+    if (a.cu) {
+      int bos, l;
+      packed_seq_bounds(a.cu, seq, a.T, bos, l);
+      s0 = bos;
+      len = l;
+    }
+    const int64_t t = len - W + k;
+    T v = (T)0.f;
+    if (t >= 0) v = ((const T*)a.x)[(a.cu ? (s0 + t) * a.xt : (int64_t)seq * a.xb + t * a.xt) + c];
+    else if (a.init) v = ((const T*)a.init)[nc * W + k + len];
+    ((T*)a.final_)[i] = v;
+  }
+}
+
+constexpr int kConvBatch = 4;   // rows fetched before the first of them is used
+
+template <typename T, int W, int VW>
+__global__ __launch_bounds__(256) void short_conv_fwd_kernel(ConvArgs a) {
+  if ((int)blockIdx.x >= a.blocks) {
+    conv_states<T>(a, W, blockIdx.x - a.blocks);
+    return;
+  }
+  const unsigned idx = blockIdx.x * 256u + threadIdx.x;
+  const int run = idx / a.pieces, c = (int)(idx - (unsigned)run * a.pieces) * VW;
+  if (run >= a.runs) return;
+  const ConvRun r(a, run);
+  if (r.t0 >= r.t1) return;
+  const int n = a.D - c;
+  float w[W][VW], bias[VW], h[W][VW];
+  load_taps<W, VW>(w, bias, a, c, n);
+  load_before<T, W, VW>(h, a, r, r.t0, c, n);
+  const T* px = (const T*)a.x + r.at(a, r.t0) + c;
+  T* py = (T*)a.y + r.t0 * a.D + c;
+  const int len = (int)(r.t1 - r.t0);
+  for (int tb = 0; tb < len; tb += kConvBatch) {
+    Chans<T, VW> xb[kConvBatch];
+#pragma unroll
+    for (int u = 0; u < kConvBatch; ++u) xb[u].load(px + (int64_t)min(tb + u, len - 1) * a.xt, n);
+#pragma unroll
+    for (int u = 0; u < kConvBatch; ++u) {
+      if (tb + u >= len) break;
+      float p[VW];
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        h[W - 1][e] = xb[u].get(e);
+        p[e] = bias[e];
+#pragma unroll
+        for (int k = 0; k < W; ++k) p[e] = fmaf(w[k][e], h[k][e], p[e]);
+        if (a.silu) p[e] *= logistic(p[e]);
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) h[k][e] = h[k + 1][e];
+      }
+      store_chans<VW>(py + (int64_t)(tb + u) * a.D, p, n);
+    }
+  }
+}
+
+// workgroups: (group of 4 runs, 64 pieces of channels), the pieces of a group next to each other; a wave walks one run, the
+// four waves' shares of dw and dbias meet in LDS
+template <typename T, int W>
+__global__ __launch_bounds__(256) void short_conv_bwd_kernel(ConvArgs a) {
+  constexpr int VW = 4;
+  __shared__ float sW[4][W + 1][64 * VW + 4];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int spans = (a.pieces + 63) / 64, group = blockIdx.x / spans, span = blockIdx.x - group * spans;
+  const int c = (span * 64 + lane) * VW, n = a.D - c;
+  const int run = group * 4 + wave;
+  float dw[W][VW], db[VW];
+#pragma unroll
+  for (int e = 0; e < VW; ++e) {
+    db[e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) dw[k][e] = 0.f;
+  }
+  if (run < a.runs && n > 0) {
+    const ConvRun r(a, run);
+    if (r.t0 < r.t1) {
+      float w[W][VW], bias[VW], h[W][VW], dp[W][VW];   // dp[k]: token t - (W - 1) + k
+      load_taps<W, VW>(w, bias, a, c, n);
+      load_before<T, W, VW>(h, a, r, r.t0, c, n);
+#pragma unroll
+      for (int e = 0; e < VW; ++e)
+#pragma unroll
+        for (int k = 0; k < W; ++k) dp[k][e] = 0.f;
+      const T* px = (const T*)a.x + r.at(a, r.t0) + c;
+      const T* pg = (const T*)a.dy + r.t0 * a.D + c;
+      const int len = (int)(r.t1 - r.t0), left = (int)min(r.s1 - r.t0, (int64_t)len + W - 1);   // tokens to walk, past the run
+      const bool first = r.t0 == r.s0;
+      for (int tb = 0; tb < len + W - 1; tb += kConvBatch) {
+        Chans<T, VW> xb[kConvBatch], gb[kConvBatch];
+#pragma unroll
+        for (int u = 0; u < kConvBatch; ++u) {
+          const int64_t t = min(tb + u, left - 1);
+          xb[u].load(px + t * a.xt, n);
+          gb[u].load(pg + t * a.D, n);
+        }
+#pragma unroll
+        for (int u = 0; u < kConvBatch; ++u) {
+          const int t = tb + u;
+          if (t >= len + W - 1) break;
+          const bool in = t < left, own = t < len;
+          float dx[VW];
+#pragma unroll
+          for (int e = 0; e < VW; ++e) {
+            h[W - 1][e] = xb[u].get(e);
+            float p = bias[e];
+#pragma unroll
+            for (int k = 0; k < W; ++k) p = fmaf(w[k][e], h[k][e], p);
+            float g = in ? gb[u].get(e) : 0.f;
+            if (a.silu) {
+              const float s = logistic(p);
+              g = in ? g * (s + p * s * (1.f - s)) : 0.f;
+            }
+            dp[W - 1][e] = g;
+            dx[e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < W; ++k) dx[e] = fmaf(w[W - 1 - k][e], dp[k][e], dx[e]);
+            if (own) {
+              db[e] += g;
+#pragma unroll
+              for (int k = 0; k < W; ++k) dw[k][e] = fmaf(g, h[k][e], dw[k][e]);
+            }
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k) { h[k][e] = h[k + 1][e]; dp[k][e] = dp[k + 1][e]; }
+          }
+          const int64_t to = r.t0 + t - (W - 1);   // the token whose gradient is whole now
+          if (to < r.t0 && !(first && a.d_init)) continue;
+          const int64_t slot = to - r.s1 + W;      // its column of the final state, if it is there
+          if (a.d_final && slot >= 0)
+#pragma unroll
+            for (int e = 0; e < VW; ++e)
+              if (e < n) dx[e] += to_f32(((const T*)a.d_final)[((int64_t)r.seq * a.D + c + e) * W + slot]);
+          if (to >= r.t0) {
+            store_chans<VW>((T*)a.dx + to * a.D + c, dx, n);
+          } else {
+#pragma unroll
+            for (int e = 0; e < VW; ++e)
+              if (e < n) {
+                T* d = (T*)a.d_init + ((int64_t)r.seq * a.D + c + e) * W;
+                d[to - r.s0 + W] = from_f32<T>(dx[e]);
+                if (t == 0) d[0] = (T)0.f;         // the oldest input of the state meets no tap
+              }
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k <= W; ++k) {
+    const f32x4 x = k < W ? (f32x4){dw[k < W ? k : 0][0], dw[k < W ? k : 0][1], dw[k < W ? k : 0][2], dw[k < W ? k : 0][3]}
+                          : (f32x4){db[0], db[1], db[2], db[3]};
+    *(f32x4*)&sW[wave][k][VW * lane] = x;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < (W + 1) * 256; i += 256) {
+    const int k = i >> 8, cc = i & 255, ch = span * 256 + cc;
+    if (ch < a.D) a.part[((int64_t)group * (W + 1) + k) * a.D + ch] = sW[0][k][cc] + sW[1][k][cc] + sW[2][k][cc] + sW[3][k][cc];
+  }
+}
+
+// dweight [D,W], dbias [D] from the workgroups' shares [groups][W+1][D] (16 waves, each its share in order), and behind these
+// workgroups the gradient of the state of sequences without a token: it went straight through
+template <typename T>
+__global__ __launch_bounds__(1024) void short_conv_reduce_kernel(ConvArgs a, int W, int groups, int sum_blocks) {
+  __shared__ float s[16][64];
+  if ((int)blockIdx.x >= sum_blocks) {
+    const int64_t total = (int64_t)a.N * a.D * W;
+    for (int64_t i = (int64_t)(blockIdx.x - sum_blocks) * 1024 + threadIdx.x; i < total; i += (int64_t)(gridDim.x - sum_blocks) * 1024) {
+      int bos, len;
+      packed_seq_bounds(a.cu, (int)(i / ((int64_t)a.D * W)), a.T, bos, len);
+      if (len == 0) ((T*)a.d_init)[i] = a.d_final ? ((const T*)a.d_final)[i] : (T)0.f;
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t col = (int64_t)blockIdx.x * 64 + lane, cols = (int64_t)(W + 1) * a.D;
+  float t = 0.f;
+  if (col < cols)
+    for (int g = w; g < groups; g += 16) t += a.part[g * cols + col];
+  s[w][lane] = t;
+  __syncthreads();
+  if (w == 0 && col < cols) {
+    t = s[0][lane];
+#pragma unroll
+    for (int k = 1; k < 16; ++k) t += s[k][lane];
+    const int k = (int)(col / a.D), c = (int)(col - (int64_t)k * a.D);
+    if (k < W) a.dweight[(int64_t)c * W + k] = t;
+    else if (a.dbias) a.dbias[c] = t;
+  }
+}
+
+// a few tokens of a generation: thread = channel of a sequence, state in place
+template <typename T, int W>
+__global__ __launch_bounds__(256) void short_conv_step_kernel(ConvArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (int64_t)a.N * a.D) return;
+  const int seq = (int)(i / a.D), c = (int)(i - (int64_t)seq * a.D);
+  T* st = (T*)a.final_ + i * W;
+  T h[W];
+  float w[W];
+#pragma unroll
+  for (int k = 0; k < W; ++k) { h[k] = st[k]; w[k] = load_rt(a.weight, (int64_t)c * W + k, a.weight_bf16); }
+  const float bias = a.bias ? load_rt(a.bias, c, a.weight_bf16) : 0.f;
+  const T* px = (const T*)a.x + (int64_t)seq * a.xb + c;
+  T* py = (T*)a.y + (int64_t)seq * a.T * a.D + c;
+  for (int t = 0; t < a.T; ++t) {
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) h[k] = h[k + 1];
+    h[W - 1] = px[t * a.xt];
+    float p = bias;
+#pragma unroll
+    for (int k = 0; k < W; ++k) p = fmaf(w[k], to_f32(h[k]), p);
+    if (a.silu) p *= logistic(p);
+    py[(int64_t)t * a.D] = from_f32<T>(p);
+  }
+#pragma unroll
+  for (int k = 0; k < W; ++k) st[k] = h[k];
+}
+
+static int check_conv(const PalConvDims* d, const PalConvTensors* t) {
+  if (!d || !t) return PAL_E_NULL;
+  if (d->batch <= 0 || d->seq_len <= 0 || d->n_seqs <= 0 || d->channels <= 0) return PAL_E_DIM;
+  if ((int64_t)d->batch * d->seq_len > (int64_t)1 << 30 || d->channels > 1 << 20) return PAL_E_DIM;
+  if (d->width < 2 || d->width > PAL_CONV_MAX_WIDTH) return PAL_E_DIM;
+  if (d->dtype != PAL_DTYPE_F32 && d->dtype != PAL_DTYPE_BF16) return PAL_E_DTYPE;
+  if (d->weight_dtype != PAL_DTYPE_F32 && d->weight_dtype != PAL_DTYPE_BF16) return PAL_E_DTYPE;
+  if (d->x_token_stride < d->channels && d->seq_len > 1) return PAL_E_DIM;
+  if (d->x_batch_stride < 0) return PAL_E_DIM;
+  if (!t->x || !t->weight || !t->y) return PAL_E_NULL;
+  return PAL_OK;
+}
+static int check_conv_seqs(const PalConvDims* d, const PalConvTensors* t) {
+  const bool packed = d->flags & PAL_FLAG_VARLEN;
+  if (packed && d->batch != 1) return PAL_E_VARLEN_BATCH;
+  if (packed != (t->cu_seqlens != nullptr)) return PAL_E_CU_SEQLENS;
+  if (!packed && d->n_seqs != d->batch) return PAL_E_DIM;
+  if (packed && !t->chunk_table) return PAL_E_NULL;
+  if (packed) {
+    const int64_t lo = ((int64_t)d->seq_len + PAL_CHUNK - 1) / PAL_CHUNK, hi = (int64_t)d->seq_len / PAL_CHUNK + d->n_seqs;
+    if (d->total_chunks < lo || d->total_chunks > hi) return PAL_E_CHUNK;
+  }
+  if (((d->flags & PAL_FLAG_HAS_INIT) != 0) != (t->init != nullptr)) return PAL_E_STATE;
+  return PAL_OK;
+}
+
+static ConvArgs conv_args(const PalConvDims* d, const PalConvTensors* t) {
+  ConvArgs a{};
+  a.x = t->x; a.weight = t->weight; a.bias = t->bias; a.init = t->init; a.y = t->y; a.final_ = t->final_;
+  a.cu = t->cu_seqlens; a.table = t->chunk_table;
+  a.xb = d->x_batch_stride; a.xt = d->x_token_stride;
+  a.T = d->seq_len; a.D = d->channels; a.N = d->n_seqs; a.chunks = d->total_chunks;
+  a.weight_bf16 = d->weight_dtype == PAL_DTYPE_BF16; a.silu = d->silu;
+  return a;
+}
+// Tokens per run: 64, halved down to 8 while the pass has less than 16 waves a compute unit.
+static void conv_runs(ConvArgs& a, const PalConvDims* d, int vw) {
+  a.pieces = (a.D + vw - 1) / vw;
+  a.run = PAL_CHUNK;
+  const int64_t tokens = (int64_t)d->batch * d->seq_len;
+  while (a.run > 8 && tokens / a.run * a.pieces < 256 * 16 * 64) a.run >>= 1;
+  a.per_tile = a.cu ? PAL_CHUNK / a.run : (a.T + a.run - 1) / a.run;
+  a.runs = a.per_tile * (a.cu ? a.chunks : d->batch);
+}
+
+template <typename T, int VW>
+static void conv_fwd_launch(const ConvArgs& a, int W, int grid, hipStream_t s) {
+#define PAL_CONV(W_)                                                                                                     \
+  case W_:                                                                                                               \
+    PAL_TIMED_LAUNCH(kKernShortConvFwd, s, (short_conv_fwd_kernel<T, W_, VW>), dim3(grid), dim3(256), 0, s, a);           \
+    break;
+  switch (W) { PAL_CONV(2) PAL_CONV(3) PAL_CONV(4) PAL_CONV(5) PAL_CONV(6) PAL_CONV(7) PAL_CONV(8) }
+#undef PAL_CONV
+}
+template <typename T>
+static void conv_bwd_launch(const ConvArgs& a, int W, dim3 grid, hipStream_t s) {
+#define PAL_CONV(W_)                                                                                            \
+  case W_: PAL_TIMED_LAUNCH(kKernShortConvBwd, s, (short_conv_bwd_kernel<T, W_>), grid, dim3(256), 0, s, a); break;
+  switch (W) { PAL_CONV(2) PAL_CONV(3) PAL_CONV(4) PAL_CONV(5) PAL_CONV(6) PAL_CONV(7) PAL_CONV(8) }
+#undef PAL_CONV
+}
+template <typename T>
+static void conv_step_launch(const ConvArgs& a, int W, hipStream_t s) {
+  const unsigned grid = (unsigned)(((int64_t)a.N * a.D + 255) / 256);
+#define PAL_CONV(W_)                                                                                                  \
+  case W_: PAL_TIMED_LAUNCH(kKernShortConvStep, s, (short_conv_step_kernel<T, W_>), dim3(grid), dim3(256), 0, s, a); break;
+  switch (W) { PAL_CONV(2) PAL_CONV(3) PAL_CONV(4) PAL_CONV(5) PAL_CONV(6) PAL_CONV(7) PAL_CONV(8) }
+#undef PAL_CONV
+}
+static int conv_state_blocks(const PalConvDims* d) {
+  const int64_t b = ((int64_t)d->n_seqs * d->channels * d->width + 1023) / 1024;
+  return (int)(b < 1024 ? b : 1024);
+}
+// runs of the backward pass and the groups of four whose shares it leaves
+static int conv_groups(const ConvArgs& a) { return (a.runs + 3) / 4; }
+
+}  // namespace pal
+
+extern "C" int pal_short_conv_fwd(const PalConvDims* d, const PalConvTensors* t, void* stream) {
+  using namespace pal;
+  if (int rc = check_conv(d, t)) return rc;
+  if (int rc = check_conv_seqs(d, t)) return rc;
+  if (((d->flags & PAL_FLAG_STORE_FINAL) != 0) != (t->final_ != nullptr)) return PAL_E_STATE;
+  ConvArgs a = conv_args(d, t);
+  const int vw = d->dtype == PAL_DTYPE_BF16 ? 8 : 4;
+  conv_runs(a, d, vw);
+  const int64_t threads = (int64_t)a.runs * a.pieces;
+  if (threads > (int64_t)1 << 31) return PAL_E_DIM;
+  a.blocks = (int)((threads + 255) / 256);
+  const int grid = a.blocks + (t->final_ ? conv_state_blocks(d) : 0);
+  hipStream_t s = (hipStream_t)stream;
+  if (d->dtype == PAL_DTYPE_BF16) conv_fwd_launch<bf16_t, 8>(a, d->width, grid, s);
+  else conv_fwd_launch<float, 4>(a, d->width, grid, s);
+  PAL_HIP_LAUNCH_CHECK();
+  return PAL_OK;
+}
+
+extern "C" size_t pal_short_conv_bwd_workspace_bytes(const PalConvDims* d) {
+  using namespace pal;
+  PalConvTensors any{};
+  any.x = any.weight = d; any.y = (void*)d;
+  if (check_conv(d, &any) != PAL_OK) return 0;
+  if (d->flags & PAL_FLAG_VARLEN) any.cu_seqlens = (const int32_t*)d;
+  ConvArgs a = conv_args(d, &any);
+  conv_runs(a, d, 4);
+  return sizeof(float) * (size_t)conv_groups(a) * (d->width + 1) * d->channels;
+}
+
+extern "C" int pal_short_conv_bwd(const PalConvDims* d, const PalConvTensors* t, const PalConvGrads* gr, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  using namespace pal;
+  if (int rc = check_conv(d, t)) return rc;
+  if (int rc = check_conv_seqs(d, t)) return rc;
+  if (!gr || !gr->dy || !gr->dx || !gr->dweight || (t->bias != nullptr) != (gr->dbias != nullptr)) return PAL_E_NULL;
+  if (gr->d_init && !t->init) return PAL_E_STATE;
+  if (!workspace || workspace_bytes < pal_short_conv_bwd_workspace_bytes(d)) return PAL_E_WORKSPACE;
+  ConvArgs a = conv_args(d, t);
+  conv_runs(a, d, 4);
+  a.dy = gr->dy; a.dx = gr->dx; a.dweight = gr->dweight; a.dbias = gr->dbias; a.d_init = gr->d_init; a.d_final = gr->d_final;
+  a.part = (float*)workspace;
+  const int groups = conv_groups(a);
+  const int64_t blocks = (int64_t)((a.pieces + 63) / 64) * groups;
+  if (blocks > (int64_t)1 << 31) return PAL_E_DIM;
+  hipStream_t s = (hipStream_t)stream;
+  const dim3 grid((unsigned)blocks);
+  if (d->dtype == PAL_DTYPE_BF16) conv_bwd_launch<bf16_t>(a, d->width, grid, s);
+  else conv_bwd_launch<float>(a, d->width, grid, s);
+  PAL_HIP_LAUNCH_CHECK();
+  const int sums = (int)(((int64_t)(d->width + 1) * a.D + 63) / 64), more = a.cu && a.d_init ? conv_state_blocks(d) : 0;
+  if (d->dtype == PAL_DTYPE_BF16)
+    PAL_TIMED_LAUNCH(kKernShortConvReduce, s, short_conv_reduce_kernel<bf16_t>, dim3(sums + more), dim3(1024), 0, s, a, d->width, groups, sums);
+  else
+    PAL_TIMED_LAUNCH(kKernShortConvReduce, s, short_conv_reduce_kernel<float>, dim3(sums + more), dim3(1024), 0, s, a, d->width, groups, sums);
+  PAL_HIP_LAUNCH_CHECK();
+  return PAL_OK;
+}
+
+extern "C" int pal_short_conv_step(const PalConvDims* d, const PalConvTensors* t, void* stream) {
+  using namespace pal;
+  if (int rc = check_conv(d, t)) return rc;
+  if (d->flags & PAL_FLAG_VARLEN) return PAL_E_VARLEN_BATCH;
+  if (d->n_seqs != d->batch) return PAL_E_DIM;
+  if (!t->final_) return PAL_E_STATE;
+  ConvArgs a = conv_args(d, t);
+  if (d->dtype == PAL_DTYPE_BF16) conv_step_launch<bf16_t>(a, d->width, (hipStream_t)stream);
+  else conv_step_launch<float>(a, d->width, (hipStream_t)stream);
+  PAL_HIP_LAUNCH_CHECK();
+  return PAL_OK;
+}

@@ -18,6 +18,12 @@ in different element-wise work (:283-299 before, :355-363 after); the same kerne
     v, b, dt = metamamba2_inputs(x, dt_raw, dt_bias, b_raw, b_scale, dt_limit)     # dt clamped, v = x dt, b = .. dt
     o = chunk_palimpsa(C, B, v, b, dt, A, Ip, scale=1.0, ...)                       # B, C rows as they are
     y = metamamba2_output_norm(o, x, D, gate, weight, eps)                          # gate first, norm over the token
+
+Between two blocks stands a norm with the residual's addition (the pre-norm of the reference's blocks, ``fla.modules.RMSNorm`` called with
+a residual; models/palimpsa/modeling_palimpsa.py:84-114), for training and, with rows in 8 bits, for serving:
+
+    y, residual = residual_rms_norm(x, residual, weight, eps)
+    q, scales, residual = residual_rms_norm_fp8(x, residual, weight, eps, group_size=128)   # y = q * scales, e4m3
 """
 from __future__ import annotations
 
@@ -25,12 +31,14 @@ import ctypes as C
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ... import _lib as L
 from ..palimpsa import _common as cm
 
 __all__ = ["palimpsa_inputs", "palimpsa_output_norm", "PalimpsaInputs", "PalimpsaOutputNorm",
-           "metamamba2_inputs", "metamamba2_output_norm", "MetaMamba2Inputs", "MetaMamba2OutputNorm"]
+           "metamamba2_inputs", "metamamba2_output_norm", "MetaMamba2Inputs", "MetaMamba2OutputNorm",
+           "residual_rms_norm", "residual_rms_norm_fp8", "ResidualRmsNorm"]
 
 
 def _rows_dtype(*tensors) -> torch.dtype:
@@ -343,6 +351,137 @@ class MetaMamba2OutputNorm(torch.autograd.Function):
         return (d_o.to(dt[0]), None if dx is None else dx.reshape(sh[1]).to(dt[1]),
                 None if dD is None else dD.reshape(sh[2]).to(dt[2]),
                 None if dgate is None else dgate.reshape(sh[3]).to(dt[3]), dw.reshape(sh[4]).to(dt[4]), None)
+
+
+MAX_NORM_ROW = 16384
+
+
+def _norm_rows(x: torch.Tensor, dtype: torch.dtype):
+    """x ``[.., D]`` in ``dtype`` with one distance between its rows, and that distance (a slice of a wider tensor stays where it is)."""
+    x = x if x.dtype == dtype else x.to(dtype)
+    D = x.shape[-1]
+    if x.stride(-1) == 1 or D == 1:
+        stride = None
+        for d in range(x.dim() - 2, -1, -1):
+            if x.shape[d] == 1:
+                continue
+            if stride is None:
+                stride, span = x.stride(d), x.stride(d) * x.shape[d]
+                if stride < D:
+                    break
+            elif x.stride(d) == span:
+                span *= x.shape[d]
+            else:
+                break
+        else:
+            return x, D if stride is None else stride
+    x = x.contiguous()
+    return x, D
+
+
+def _norm_call(x, residual, weight, eps, residual_in_fp32, group=None):
+    """Checks a norm call and fills its structs: (dims, tensors, outputs) with everything that has to stay alive in ``outputs``."""
+    dev = cm._require_gpu(x, residual, weight)
+    if x.dim() < 1 or x.numel() == 0:
+        raise ValueError(f"x must be [.., D] with at least one row, got {tuple(x.shape)}")
+    D = x.shape[-1]
+    if D > MAX_NORM_ROW:
+        raise ValueError(f"the norm serves rows of up to {MAX_NORM_ROW} entries, got {D}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual must have the shape of x, {tuple(x.shape)}, got {tuple(residual.shape)}")
+    if tuple(weight.shape) != (D,):
+        raise ValueError(f"weight must be [{D}], got {tuple(weight.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    cd = _rows_dtype(x)
+    rd = torch.float32 if residual_in_fp32 or _rows_dtype(x, residual) == torch.float32 else torch.bfloat16
+    xc, xs = _norm_rows(x, cd)
+    rc, rs = (None, D) if residual is None else _norm_rows(residual, rd)
+    w = cm.param(weight)
+    res_out = torch.empty(x.shape, dtype=rd, device=dev)
+    dims = L.PalNormDims(rows=x.numel() // D, x_stride=xs, res_stride=rs, dim=D, dtype=cm._pal_dtype(cd), res_dtype=cm._pal_dtype(rd),
+                         weight_dtype=cm._pal_dtype(w.dtype), group=group or 0, eps=float(eps))
+    tens = L.PalNormTensors(x=cm._ptr(xc), residual=cm._ptr(rc), weight=cm._ptr(w), residual_out=cm._ptr(res_out))
+    return dims, tens, (dev, cd, rd, xc, rc, w, res_out)
+
+
+class ResidualRmsNorm(torch.autograd.Function):
+    """forward(ctx, x, residual, weight, eps, residual_in_fp32) -> (y, residual_out): s = x + residual, y = rmsnorm(s) * weight."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, residual_in_fp32):
+        dims, tens, (dev, cd, rd, xc, rc_, w, res_out) = _norm_call(x, residual, weight, eps, residual_in_fp32)
+        y = torch.empty(x.shape, dtype=cd, device=dev)
+        tens.y = y.data_ptr()
+        with torch.cuda.device(dev):
+            rc = L.load().pal_residual_norm_fwd(dims, tens, cm.current_stream_ptr(dev))
+        L.check(rc, "pal_residual_norm_fwd")
+        ctx.set_materialize_grads(False)
+        if any(ctx.needs_input_grad):
+            ctx.save_for_backward(res_out, w)
+            ctx.dims = dims
+            ctx.meta = dict(cd=cd, rd=rd, dtypes=[None if t is None else t.dtype for t in (x, residual, weight)])
+        return (y if y.dtype == x.dtype else y.to(x.dtype)), res_out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dres):
+        res_out, w = ctx.saved_tensors
+        m = ctx.meta
+        dev, cd, rd = res_out.device, m["cd"], m["rd"]
+        if dy is None and dres is None:
+            return None, None, None, None, None
+        dy = None if dy is None else cm._plain(dy, cd)
+        dres = None if dres is None else cm._plain(dres, rd)
+        dx = torch.empty(res_out.shape, dtype=cd, device=dev)
+        d_res = dx if cd == rd else torch.empty(res_out.shape, dtype=rd, device=dev)
+        dw = torch.empty(w.shape, dtype=torch.float32, device=dev)
+        pt = cm._ptr
+        tens = L.PalNormTensors(weight=pt(w), residual_out=pt(res_out))
+        grads = L.PalNormGrads(dy=pt(dy), dresidual_out=pt(dres), dx=pt(dx), dresidual=None if cd == rd else pt(d_res), dweight=pt(dw))
+        lib = L.load()
+        ws_bytes = int(lib.pal_residual_norm_bwd_workspace_bytes(ctx.dims))
+        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev):
+            rc = lib.pal_residual_norm_bwd(ctx.dims, tens, grads, C.c_void_p(ws.data_ptr()), ws_bytes, cm.current_stream_ptr(dev))
+        L.check(rc, "pal_residual_norm_bwd")
+        dt = m["dtypes"]
+        return dx.to(dt[0]), None if dt[1] is None else d_res.to(dt[1]), dw.to(dt[2]), None, None
+
+
+@cm.no_compile
+def residual_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-5,
+                      residual_in_fp32: bool = False):
+    """``s = x + residual``, ``y = s * rsqrt(mean(s ** 2) + eps) * weight``; returns ``(y, s)``: the block's input and the residual
+    stream to hand on.  x, residual ``[.., D]`` (D up to 16384, residual None for the first block), weight ``[D]``.
+
+    y has the type of x; s is bf16 where x and residual are bf16 and ``residual_in_fp32`` is not set, else fp32 (bf16 rows beside an
+    fp32 stream are the usual choice for deep models).  The norm is that of s as it is handed on.  Gradients for x, residual and weight."""
+    cm._require_gpu(x, residual, weight)
+    return ResidualRmsNorm.apply(x, residual, weight, eps, residual_in_fp32)
+
+
+@cm.no_compile
+def residual_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-5,
+                          group_size: Optional[int] = None, residual_in_fp32: bool = False):
+    """``residual_rms_norm`` with y in 8 bits for a projection that takes such rows; returns ``(q, scales, s)`` with ``y = q * scales``:
+    q ``[.., D]`` ``torch.float8_e4m3fn``, scales fp32 ``[.., D / group_size]``, one for each group of ``group_size`` entries (32, 64, 128
+    or 256, a divisor of D), or ``[.., 1]``, one for the row (``group_size`` None).  A scale is the largest absolute y of its group (at least
+    1e-12) over 448.  A row whose sum of squares is not a finite number has NaN scales.  No gradients: call it under ``torch.no_grad()``."""
+    cm._require_gpu(x, residual, weight)
+    if cm.wants_grad(x, residual, weight):
+        raise ValueError("residual_rms_norm_fp8 has no gradient: use residual_rms_norm, or torch.no_grad()")
+    D = x.shape[-1] if x.dim() else 0
+    if group_size is not None and (group_size not in (32, 64, 128, 256) or D % group_size):
+        raise ValueError(f"group_size must be 32, 64, 128 or 256 and divide the {D} entries of a row, or None; got {group_size}")
+    dims, tens, (dev, _, _, xc, rc_, w, res_out) = _norm_call(x, residual, weight, eps, residual_in_fp32, group_size)
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
+    scales = torch.empty(x.shape[:-1] + (D // group_size if group_size else 1,), dtype=torch.float32, device=dev)
+    tens.y, tens.scales = q.data_ptr(), scales.data_ptr()
+    with torch.cuda.device(dev):
+        rc = L.load().pal_residual_norm_fwd(dims, tens, cm.current_stream_ptr(dev))
+    L.check(rc, "pal_residual_norm_fwd")
+    return q, scales, res_out
 
 
 @cm.no_compile

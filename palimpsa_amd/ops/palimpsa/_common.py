@@ -238,6 +238,56 @@ def current_stream_ptr(dev: torch.device):
     return C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
+def token_rows(x: torch.Tensor, inner: int = 1) -> torch.Tensor:
+    """x ``[B, T, ...]`` as the kernels with strides take it: the last ``inner`` dims packed, any non-negative distance
+    between batch rows and at least a row between tokens (a slice of a wider projection stays where it is)."""
+    if x.numel() == 0:
+        return x.contiguous()
+    row = 1
+    for d in range(x.dim() - 1, x.dim() - 1 - inner, -1):
+        if x.shape[d] != 1 and x.stride(d) != row:
+            return x.contiguous()
+        row *= x.shape[d]
+    if (x.shape[1] > 1 and x.stride(1) < row) or x.stride(0) < 0:
+        return x.contiguous()
+    return x
+
+
+def token_strides(x: torch.Tensor, inner: int = 1):
+    """(batch, token) strides of ``token_rows(x, inner)``; a dim of one entry counts as packed."""
+    row = 1
+    for d in range(x.dim() - inner, x.dim()):
+        row *= x.shape[d]
+    token = x.stride(1) if x.shape[1] > 1 else row
+    return (x.stride(0) if x.shape[0] > 1 else token * x.shape[1]), token
+
+
+def param(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """A per-channel parameter as the kernels read it: bf16 or fp32, packed."""
+    if x is None:
+        return None
+    return _plain(x, x.dtype if x.dtype in (torch.float32, torch.bfloat16) else torch.float32)
+
+
+def packed_batch(cu_seqlens: torch.Tensor, B: int, T: int, dev: torch.device):
+    """(cu_seqlens int32 on ``dev``, chunk table, chunks, sequences) of a packed batch; ValueError for one that is none."""
+    if B != 1:
+        raise ValueError(f"Batch size must be 1 for Varlen, got {B}")
+    meta, total = chunk_meta(cu_seqlens, T, dev)
+    n = int(cu_seqlens.numel()) - 1
+    return cu_seqlens.to(device=dev, dtype=torch.int32).contiguous(), meta[n + 1:], total, n
+
+
+def wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def bump_version(x: torch.Tensor) -> None:
+    """Tell autograd that a kernel wrote x in place."""
+    if not x.is_inference():
+        torch.autograd.graph.increment_version(x)
+
+
 def unpad_state(x: Optional[torch.Tensor], p: Prepared):
     if x is None or (p.dk_p == p.dk and p.dv_p == p.dv):
         return x
