@@ -466,7 +466,7 @@ int pal_short_conv_step(const PalConvDims *dims, const PalConvTensors *t, void *
  * B and C are shared by the channels of a group (channel d reads group d / (channels / groups)). */
 #define PAL_SCAN_MAX_STATE 64
 /* tokens between two kept states (PalScanTensors.checkpoints) */
-#define PAL_SCAN_BLOCK 16
+#define PAL_SCAN_BLOCK 8
 
 typedef struct PalScanDims {
   int32_t batch, seq_len, n_seqs; /* as in PalDims; a packed batch may hold empty sequences, n_seqs is not bound by seq_len */

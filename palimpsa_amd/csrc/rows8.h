@@ -17,16 +17,37 @@ struct Piece8;
 template <>
 struct Piece8<bf16_t> {
   bf16x8 v;
-  __device__ __forceinline__ void load(const bf16_t* p) { v = *(const bf16x8_any*)p; }
   __device__ __forceinline__ float get(int e) const { return (float)v[e]; }
+  __device__ __forceinline__ bf16_t at(int e) const { return v[e]; }
   __device__ __forceinline__ void set(int e, bf16_t x) { v[e] = x; }
+  template <typename P>   // (pointers of any address space)
+  __device__ __forceinline__ void load(P p) { v = *(const __attribute__((address_space(1))) bf16x8_any*)p; }
+  template <typename P>
+  __device__ __forceinline__ void store(P p) const { *(__attribute__((address_space(1))) bf16x8_any*)p = v; }
+  // a use of the value: whoever loaded it waits here
+  __device__ __forceinline__ void settle() {
+    f32x4 x = __builtin_bit_cast(f32x4, v);
+    asm volatile("" : "+v"(x));
+    v = __builtin_bit_cast(bf16x8, x);
+  }
 };
 template <>
 struct Piece8<float> {
   f32x4 lo, hi;
-  __device__ __forceinline__ void load(const float* p) { lo = *(const f32x4_any*)p; hi = *(const f32x4_any*)(p + 4); }
   __device__ __forceinline__ float get(int e) const { return e < 4 ? lo[e & 3] : hi[e & 3]; }
+  __device__ __forceinline__ float at(int e) const { return get(e); }
   __device__ __forceinline__ void set(int e, float x) { if (e < 4) lo[e & 3] = x; else hi[e & 3] = x; }
+  template <typename P>
+  __device__ __forceinline__ void load(P p) {
+    lo = *(const __attribute__((address_space(1))) f32x4_any*)p;
+    hi = *(const __attribute__((address_space(1))) f32x4_any*)(p + 4);
+  }
+  template <typename P>
+  __device__ __forceinline__ void store(P p) const {
+    *(__attribute__((address_space(1))) f32x4_any*)p = lo;
+    *(__attribute__((address_space(1))) f32x4_any*)(p + 4) = hi;
+  }
+  __device__ __forceinline__ void settle() { asm volatile("" : "+v"(lo), "+v"(hi)); }
 };
 
 // `n` elements of the piece are there (8 or more: all; 0 or less: none, and nothing is read), the others are zero

@@ -18,11 +18,17 @@
 // batch segments know nothing of sequences: a token that starts a sequence takes that sequence's initial state in place of the
 // state before it, and a segment that holds such a token lets nothing through.
 //
-// For the backward the forward keeps the state before every 16th token in fp32; the backward computes the 16 tokens again, four
-// at a time, and keeps a and a h' of four tokens in registers.
+// Rows are fetched eight tokens at a time, one block ahead: a lane takes eight neighbouring channels of one token, the block passes
+// through LDS, and what a lane computes for its channel goes back the same way.  (A two-byte access per token and array instead
+// took eight times the memory instructions.)  Results are stored at the top of the next block, before its fetch: loads and stores
+// leave the memory queue in order, and a store issued after a fetch is waited for with it.
+//
+// For the backward the forward keeps the state before every 8th token in fp32; the backward computes the 8 tokens again, two
+// at a time, and keeps a and a h' of two tokens in registers.
 #include "pal_common.h"
 #include "pal_host.h"
 #include "pal_profile.h"
+#include "rows8.h"
 
 namespace pal {
 
@@ -34,7 +40,8 @@ struct ScanArgs {
   float *seg_h, *seg_dt, *part_bc, *part_a, *part_c;
   int32_t *seg_cut;
   const int32_t* cu;
-  int64_t ub, ut, db, dt, zb, zt, Bb, Bt, Cb, Ct;   // strides
+  int64_t ub, db, zb, Bb, Cb;                        // strides between batch rows
+  int32_t ut, dt, zt, Bt, Ct;                        // and between tokens (below 2^24)
   int32_t rows, T, seqs, D_, N, G, per_group, tiles_g, tiles, softplus, vec;
   int32_t seg, segs, ckpts;                          // tokens per segment (a multiple of PAL_SCAN_BLOCK), segments and kept states per row
 };
@@ -52,21 +59,27 @@ __device__ __forceinline__ float log1p_full(float e) {
   const float s = 1.f + e;
   return fmaf(e - (s - 1.f), fast_rcp(s), __builtin_amdgcn_logf(s) * 0.6931471806f);
 }
-// time step from the raw one (already with its bias); softplus is the identity above 20, as torch computes it
+// time step from the raw one (already with its bias); softplus is the identity above 20, as torch computes it (and for a NaN)
 __device__ __forceinline__ float time_step(float raw, int softplus) {
-  return softplus && raw <= 20.f ? log1p_full(exp_full(raw)) : raw;
+  const float s = log1p_full(exp_full(raw));
+  return softplus && raw <= 20.f ? s : raw;
 }
 __device__ __forceinline__ float sigmoid_full(float x) { return fast_rcp(1.f + exp_full(-x)); }
 
 // ------------------------------------------------------------------------------------------------ lanes
 // lane 4 q + j of a wave: channels 16 k + q (k = 0 .. 3) by entries 4 j + i (i = 0 .. 3) of the state; its own channel is 16 j + q
+// (moves inside a quad have a source for every lane: nothing is kept in the target, and the compiler may fold them into their use)
+template <int CTRL>
+__device__ __forceinline__ float in_quad(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
 template <int K>
-__device__ __forceinline__ float of_channel(float x) { return quad_move<K * 0x55>(x); }   // the value of the lane that owns channel k
+__device__ __forceinline__ float of_channel(float x) { return in_quad<K * 0x55>(x); }   // the value of the lane that owns channel k
 // four sums over a quad: lane j gets the total of p_j
 __device__ __forceinline__ float quad_total4(float p0, float p1, float p2, float p3, bool odd, bool high) {
-  const float a = (odd ? p1 : p0) + quad_move<0xB1>(odd ? p0 : p1);
-  const float b = (odd ? p3 : p2) + quad_move<0xB1>(odd ? p2 : p3);
-  return (high ? b : a) + quad_move<0x4E>(high ? a : b);
+  const float a = (odd ? p1 : p0) + in_quad<0xB1>(odd ? p0 : p1);
+  const float b = (odd ? p3 : p2) + in_quad<0xB1>(odd ? p2 : p3);
+  return (high ? b : a) + in_quad<0x4E>(high ? a : b);
 }
 
 // a sequence: its number and its tokens [s, e) in the row
@@ -84,38 +97,44 @@ __device__ __forceinline__ ScanSeq seq_at(const ScanArgs& a, int row, int t) {
   return {lo, a.cu[lo], a.cu[lo + 1]};
 }
 
-template <typename T>
+// The lane's number, hidden from the compiler: what rare paths compute from it stays in them instead of being kept in
+// registers for all of the loop.
+__device__ __forceinline__ int hidden_lane() {
+  int l = threadIdx.x & 63;
+  asm volatile("" : "+v"(l));
+  return l;
+}
+
 struct Lane {
-  int w, j, q, n0, own, row, tile, group;
+  int w, j, row, tile, group, base, end;   // wave, place in the quad, batch row, tile and its group, first channel of the tile, end of the group
+  unsigned own;                            // own channel
   bool on, odd, high;
-  int chan[4], valid[4];
+  bool full;                               // all 64 channels of the tile are there
   __device__ __forceinline__ Lane(const ScanArgs& a) {
     const int l = threadIdx.x & 63;
     w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    q = l >> 2; j = l & 3;
+    j = l & 3;
     odd = j & 1; high = j & 2;
-    n0 = 16 * w + 4 * j;
     tile = blockIdx.x;
     row = blockIdx.z;
     group = tile / a.tiles_g;
-    const int base = group * a.per_group + (tile - group * a.tiles_g) * 64, end = (group + 1) * a.per_group;
-    own = base + 16 * j + q;
-    on = own < end;
-    own = min(own, end - 1);        // (lanes beyond the group compute its last channel again and store nothing)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      chan[k] = base + 16 * k + q;
-      valid[k] = chan[k] < end;
-      chan[k] = min(chan[k], end - 1);
-    }
+    base = group * a.per_group + (tile - group * a.tiles_g) * 64;
+    end = (group + 1) * a.per_group;
+    full = base + 64 <= end;
+    const int c = base + 16 * j + (l >> 2);
+    on = c < end;
+    own = min(c, end - 1);        // (lanes beyond the group compute its last channel again and store nothing)
   }
-  // the lane's 4 x 4 entries of a [.., channels, N] fp32 array, zero beyond N
+  // The lane's 4 x 4 entries of a [.., channels, N] fp32 array, zero beyond N: where sequences start and end, not in the loops over tokens.
   __device__ __forceinline__ void load(const ScanArgs& a, const float* p, float (*x)[4]) const {
+    const int l = hidden_lane();
+    const int n0 = 16 * w + 4 * (l & 3);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const float* s = p + (int64_t)chan[k] * a.N + n0;
-      if (a.vec && n0 < a.N) {
-        const f32x4 v = *(const f32x4*)s;
+      const float* s = p + (int64_t)min(base + 16 * k + (l >> 2), end - 1) * a.N + n0;
+      if (a.vec) {
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (n0 < a.N) v = *(const f32x4*)s;
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[k][i] = v[i];
       } else {
@@ -123,15 +142,22 @@ struct Lane {
         for (int i = 0; i < 4; ++i) x[k][i] = n0 + i < a.N ? s[i] : 0.f;
       }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(x[k][i]));   // (see settle below)
   }
   __device__ __forceinline__ void store(const ScanArgs& a, float* p, const float (*x)[4]) const {
+    const int l = hidden_lane();
+    const int n0 = 16 * w + 4 * (l & 3);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (!valid[k]) continue;
-      float* d = p + (int64_t)chan[k] * a.N + n0;
-      if (a.vec && n0 < a.N) {
+      const int c = base + 16 * k + (l >> 2);
+      if (c >= end) continue;
+      float* d = p + (int64_t)c * a.N + n0;
+      if (a.vec) {
         const f32x4 v = {x[k][0], x[k][1], x[k][2], x[k][3]};
-        *(f32x4*)d = v;
+        if (n0 < a.N) *(f32x4*)d = v;
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -139,67 +165,198 @@ struct Lane {
       }
     }
   }
-  __device__ __forceinline__ void store_zero(const ScanArgs& a, float* p) const {
-    const float z[4][4] = {};
-    store(a, p, z);
-  }
-  // four entries of B or C of a token as fetched (zero beyond N)
-  __device__ __forceinline__ void fetch_bc(const ScanArgs& a, const void* base, int64_t at, int n, float* x) const {
-    const T* p = (const T*)base + at + (int64_t)group * a.N + n;
-    if constexpr (sizeof(T) == 2) {
-      typedef bf16x4 any __attribute__((aligned(2)));
-      if (n + 4 <= a.N) {
-        const bf16x4 v = *(const any*)p;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = (float)v[i];
-        return;
-      }
+};
+// An element of a row: the row's address is the same for the whole wave, the lane adds 32 bits.  The empty assembly keeps the address
+// in scalar registers: left alone, the compiler adds the lane's part first and carries one 64-bit address per array and lane
+// through the loops.
+#define PAL_GLOBAL __attribute__((address_space(1)))
+template <typename T>
+__device__ __forceinline__ PAL_GLOBAL T* row_element(const T* row, unsigned bytes) {
+  const uint64_t p = (uint64_t)row;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((int)p), hi = __builtin_amdgcn_readfirstlane((int)(p >> 32));
+  auto base = (PAL_GLOBAL char*)((uint64_t)hi << 32 | lo);
+  asm("" : "+s"(base));
+  asm("" : "+v"(bytes));
+  return (PAL_GLOBAL T*)(base + bytes);
+}
+template <typename T>
+__device__ __forceinline__ T row_load(const T* row, unsigned i) { return *row_element(row, i * (unsigned)sizeof(T)); }
+template <typename T>
+__device__ __forceinline__ void row_store(T* row, unsigned i, T x) { *row_element(row, i * (unsigned)sizeof(T)) = x; }
+// A load that only some paths make has to be waited for on those paths: where they meet the others again, the compiler would wait for
+// every load in flight on any of them, the next block's rows among them.  The empty assembly is a use of the value.
+__device__ __forceinline__ void settle(f32x4& x) { asm volatile("" : "+v"(x)); }
+__device__ __forceinline__ void settle(float& x) { asm volatile("" : "+v"(x)); }
+
+// Four entries of B or C, from entry n on (zero beyond N), as fetched.  p: the group's entries of the block's first token; the
+// lane's token is `bytes` behind it.
+template <typename T>
+struct Four {
+  typename Raw4<T>::type v;
+  __device__ __forceinline__ void fetch(const ScanArgs& a, const T* p, unsigned bytes, int n) {
+    typedef typename Raw4<T>::type any __attribute__((aligned(sizeof(T))));
+    if (a.vec) {
+      v = *(const PAL_GLOBAL any*)row_element(p, bytes + (n < a.N ? n : 0) * (unsigned)sizeof(T));
     } else {
-      typedef f32x4 any __attribute__((aligned(4)));
-      if (n + 4 <= a.N) {
-        const f32x4 v = *(const any*)p;
+      asm volatile("" : "+v"(n));
+      const T* q = (const T*)((const char*)p + bytes) + n;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = v[i];
-        return;
+      for (int i = 0; i < 4; ++i) v[i] = n + i < a.N ? q[i] : (T)0.f;
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = (float)v[i];
+        settle(x[i]);
+        v[i] = (T)x[i];
       }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = n + i < a.N ? to_f32(p[i]) : 0.f;
+  }
+  __device__ __forceinline__ f32x4 get(const ScanArgs& a, int n) const {
+    const f32x4 x = {(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+    return n < a.N ? x : (f32x4){0.f, 0.f, 0.f, 0.f};
   }
 };
-// index of a lane's four entries in an array of one float4 for each lane, channel piece and wave of every tile
+// index of a wave's entries in an array of one float4 for each channel piece and lane of every wave and tile
 __device__ __forceinline__ int64_t packed_at(int64_t slot, const ScanArgs& a, int tile, int nw, int w, int k) {
-  return (((slot * a.tiles + tile) * nw + w) * 4 + k) * 64 + (threadIdx.x & 63);
+  return (((slot * a.tiles + tile) * nw + w) * 4 + k) * 64;
+}
+__device__ __forceinline__ void load_packed(const float* p, int64_t at, float (*x)[4]) {
+  const unsigned l = threadIdx.x & 63;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const f32x4 v = row_load((const f32x4*)p + at, 64 * k + l);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[k][i] = v[i];
+  }
+}
+__device__ __forceinline__ void store_packed(float* p, int64_t at, const float (*x)[4]) {
+  const unsigned l = threadIdx.x & 63;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) row_store((f32x4*)p + at, 64 * k + l, (f32x4){x[k][0], x[k][1], x[k][2], x[k][3]});
+}
+__device__ __forceinline__ void zero44(float (*x)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[k][i] = 0.f;
+}
+// Nothing is moved across by the scheduler.  The sixteen entries of a lane go through each kind of operation together: left alone,
+// the scheduler walks entry by entry to save registers, and the product, its exponential and what uses that wait for
+// each other.
+__device__ __forceinline__ void stage() { __builtin_amdgcn_sched_barrier(0); }
+// decays of a token, and its input to the states
+__device__ __forceinline__ void decays(float (*e)[4], const float* dk, const float (*A2)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[k][i] = dk[k] * A2[k][i];
+  stage();
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[k][i] = fast_exp2(e[k][i]);
 }
 __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
-
-// a sequence's state where it starts
-template <typename T>
-__device__ __forceinline__ void start_state(const ScanArgs& a, const Lane<T>& ln, int seq, float (*h)[4]) {
-  if (a.init) {
-    ln.load(a, a.init + (int64_t)seq * a.D_ * a.N, h);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h[k][i] = 0.f;
+// a sequence's entries of a [seqs, channels, N] array, or zero where there is none
+__device__ __forceinline__ void load_state(const ScanArgs& a, const Lane& ln, const float* p, int seq, float (*h)[4]) {
+  if (p) ln.load(a, p + (int64_t)seq * a.D_ * a.N, h);
+  else zero44(h);
+}
+__device__ __forceinline__ void store_state(const ScanArgs& a, const Lane& ln, float* p, int seq, const float (*h)[4]) {
+  ln.store(a, p + (int64_t)seq * a.D_ * a.N, h);
+}
+// sequences [n, end) have no token: what they start with is what they end with
+__device__ __forceinline__ void hand_over(const ScanArgs& a, const Lane& ln, const float* from, float* to, int n, int end) {
+  if (!to) return;
+  for (; n < end; ++n) {
+    float x[4][4];
+    load_state(a, ln, from, n, x);
+    store_state(a, ln, to, n, x);
   }
 }
+// the sequence after / before `s` that has a token (the last one / first one: itself)
+__device__ __forceinline__ ScanSeq next_seq(const ScanArgs& a, const ScanSeq& s) {
+  int n = s.n + 1;
+  while (n < a.seqs && a.cu[n + 1] <= s.e) ++n;
+  return n < a.seqs ? ScanSeq{n, s.e, a.cu[n + 1]} : ScanSeq{a.seqs, s.e, a.T + 1};
+}
+__device__ __forceinline__ ScanSeq prev_seq(const ScanArgs& a, const ScanSeq& s) {
+  int n = s.n - 1;
+  while (n >= 0 && a.cu[n] >= s.s) --n;
+  return n >= 0 ? ScanSeq{n, a.cu[n], s.s} : ScanSeq{-1, -1, s.s};
+}
+// the tokens of a block that are walked: all of them, known to the compiler, or [lo, hi)
+struct Whole {
+  static constexpr bool whole = true;
+  int lo, hi;
+};
+struct Part {
+  static constexpr bool whole = false;
+  int lo, hi;
+};
+template <typename R>
+__device__ __forceinline__ bool walks(const R& r, int t) { return R::whole || (t >= r.lo && t < r.hi); }
+
+constexpr int kTok = PAL_SCAN_BLOCK;   // tokens of a block
+
+// A block of one array: lane l takes channels 8 (l % 8) .. of token l / 8 (of the last token where the block has fewer).  Whole tiles
+// without a branch; of the last tile of a group what is there, the channels beyond it are zero.
+template <typename T>
+struct BlockRows {
+  Piece8<T> v;
+  // row: the block's first token; left: tokens behind it
+  __device__ __forceinline__ void fetch(const Lane& ln, const T* row, int stride, int left) {
+    const int l = threadIdx.x & 63;
+    const unsigned at = __umul24(min(l >> 3, left), stride) + ln.base + 8 * (l & 7);
+    if (ln.full) {
+      v.load(row_element(row, at * (unsigned)sizeof(T)));
+    } else {
+      const int h = hidden_lane();
+      load_piece(v, row + __umul24(min(h >> 3, left), stride) + ln.base + 8 * (h & 7), ln.end - ln.base - 8 * (h & 7));
+      v.settle();
+    }
+  }
+  __device__ __forceinline__ void to_lds(T (*to)[64]) const {
+    const int l = threadIdx.x & 63;
+    *(Piece8<T>*)&to[l >> 3][8 * (l & 7)] = v;
+  }
+  // and back: a block of results, nt tokens of it
+  __device__ __forceinline__ void from_lds(const T (*from)[64]) {
+    const int l = threadIdx.x & 63;
+    v = *(const Piece8<T>*)&from[l >> 3][8 * (l & 7)];
+  }
+  __device__ __forceinline__ void store(const Lane& ln, T* row, int stride, int nt) const {
+    const int l = threadIdx.x & 63;
+    const unsigned at = __umul24(l >> 3, stride) + ln.base + 8 * (l & 7);
+    if (ln.full && nt == kTok) {
+      v.store(row_element(row, at * (unsigned)sizeof(T)));
+    } else {
+      const int h = hidden_lane();
+      T* to = row + __umul24(h >> 3, stride) + ln.base + 8 * (h & 7);
+      if ((h >> 3) < nt)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < ln.end - ln.base - 8 * (h & 7)) to[e] = v.at(e);
+    }
+  }
+};
+// element of a block in LDS that belongs to a lane's own channel
+__device__ __forceinline__ int own_at() { return 16 * (threadIdx.x & 3) + ((threadIdx.x & 63) >> 2); }
 
 // ------------------------------------------------------------------------------------------------ forward
-constexpr int kScanTok = 8;   // tokens fetched together
-
 // OUT: the pass itself.  Otherwise the walk of a segment from zero: its last state, the sum of its dt, and whether a sequence starts in it.
 template <typename T, int NW, bool OUT>
 __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs a) {
-  __shared__ float sBC[NW][kScanTok][2][16];
-  __shared__ float sY[NW > 1 && OUT ? 2 : 1][NW > 1 && OUT ? NW : 1][kScanTok][64];
-  const Lane<T> ln(a);
-  const int l = threadIdx.x & 63, w = ln.w, row = ln.row;
+  __shared__ float sBC[NW][kTok][2][16];
+  __shared__ __attribute__((aligned(16))) T sRow[NW][OUT ? 3 : 2][kTok][64];   // u, delta, z
+  __shared__ __attribute__((aligned(16))) T sOut[OUT && NW == 1 ? kTok : 1][64];
+  __shared__ float sY[NW > 1 && OUT ? 2 : 1][NW > 1 && OUT ? NW : 1][kTok][64];
+  const Lane ln(a);
+  const int l = threadIdx.x & 63, w = ln.w, row = ln.row, own = own_at();
   const int t0 = blockIdx.y * a.seg, t1 = min(a.T, t0 + a.seg);
   const float bias = a.bias ? a.bias[ln.own] : 0.f, Dc = a.D ? a.D[ln.own] : 0.f;
   float A2[4][4], h[4][4], dt_sum = 0.f;
@@ -207,147 +364,150 @@ __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs a) {
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { A2[k][i] *= kLog2e; h[k][i] = 0.f; }
+    for (int i = 0; i < 4; ++i) A2[k][i] *= kLog2e;
   ScanSeq cur = seq_at(a, row, t0);
   int cut = 0;
-  if (OUT && t0 > 0 && cur.s != t0) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const f32x4 v = ((const f32x4*)a.seg_h)[packed_at((int64_t)row * a.segs + blockIdx.y, a, ln.tile, NW, w, k)];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h[k][i] = v[i];
-    }
-  }
-  if (OUT && t0 == 0 && a.final_ && a.cu)
-    for (int n = 0; n < cur.n; ++n) {   // sequences without a token before the first one
-      float x[4][4];
-      start_state(a, ln, n, x);
-      ln.store(a, a.final_ + (int64_t)n * a.D_ * a.N, x);
-    }
-  const T* pu = (const T*)a.u + row * a.ub + ln.own;
-  const T* pd = (const T*)a.delta + row * a.db + ln.own;
-  const T* pz = a.z ? (const T*)a.z + row * a.zb + ln.own : nullptr;
-  T* py = (T*)a.y + (int64_t)row * a.T * a.D_ + ln.own;
+  if (OUT && t0 > 0 && cur.s != t0) load_packed(a.seg_h, packed_at((int64_t)row * a.segs + blockIdx.y, a, ln.tile, NW, w, 0), h);
+  else zero44(h);
+  if (OUT && t0 == 0 && a.cu) hand_over(a, ln, a.init, a.final_, 0, cur.n);   // sequences without a token before the first one
+  const T* pu = (const T*)a.u + row * a.ub;
+  const T* pd = (const T*)a.delta + row * a.db;
+  const T* pz = a.z ? (const T*)a.z + row * a.zb : nullptr;
+  T* py = (T*)a.y + (int64_t)row * a.T * a.D_;
 
-  T ur[kScanTok], dr[kScanTok], zr[kScanTok];
-  float bc[4];
+  const T* pB = (const T*)a.Bm + row * a.Bb + (int64_t)ln.group * a.N;
+  const T* pC = (const T*)a.Cm + row * a.Cb + (int64_t)ln.group * a.N;
+  const int n4 = 16 * w + 4 * (l & 3);     // B and C: lane l takes these entries of token l / 4 (of the last token there is)
+
+  BlockRows<T> ru, rd, rz;
+  Four<T> rb, rc;
   auto fetch = [&](int tb) {
-#pragma unroll
-    for (int t = 0; t < kScanTok; ++t) {
-      const int64_t at = min(tb + t, t1 - 1);
-      ur[t] = pu[at * a.ut];
-      dr[t] = pd[at * a.dt];
-      if (OUT && a.z) zr[t] = pz[at * a.zt];
-    }
-    const int64_t at = min(tb + (l >> 3), t1 - 1);
-    const bool c = l & 4;
-    if (OUT || !c) ln.fetch_bc(a, c ? a.Cm : a.Bm, c ? row * a.Cb + at * a.Ct : row * a.Bb + at * a.Bt, 16 * w + 4 * (l & 3), bc);
+    const int left = min(kTok, t1 - tb) - 1;
+    ru.fetch(ln, pu + (int64_t)tb * a.ut, a.ut, left);
+    rd.fetch(ln, pd + (int64_t)tb * a.dt, a.dt, left);
+    if (OUT && a.z) rz.fetch(ln, pz + (int64_t)tb * a.zt, a.zt, left);
+    const int t = min((l >> 2) & 7, left);
+    rb.fetch(a, pB + (int64_t)tb * a.Bt, __umul24(t, a.Bt) * (unsigned)sizeof(T), n4);
+    if (OUT) rc.fetch(a, pC + (int64_t)tb * a.Ct, __umul24(t, a.Ct) * (unsigned)sizeof(T), n4);
   };
   fetch(t0);
   int turn = 0;
-  for (int tb = t0; tb < t1; tb += kScanTok) {
-    if (OUT && a.ckpt && (tb & (PAL_SCAN_BLOCK - 1)) == 0) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const f32x4 v = {h[k][0], h[k][1], h[k][2], h[k][3]};
-        ((f32x4*)a.ckpt)[packed_at((int64_t)row * a.ckpts + tb / PAL_SCAN_BLOCK, a, ln.tile, NW, w, k)] = v;
+  for (int tb = t0; tb < t1; tb += kTok) {
+    ru.to_lds(sRow[w][0]);
+    rd.to_lds(sRow[w][1]);
+    if (OUT && a.z) rz.to_lds(sRow[w][OUT ? 2 : 0]);
+    *(f32x4*)&sBC[w][(l >> 2) & 7][0][4 * (l & 3)] = rb.get(a, n4);     // (the upper half of the wave holds the same as the lower)
+    if (OUT) *(f32x4*)&sBC[w][(l >> 2) & 7][1][4 * (l & 3)] = rc.get(a, n4);
+    if constexpr (OUT && NW == 1) {
+      if (tb > t0) {
+        BlockRows<T> done;
+        done.from_lds(sOut);
+        done.store(ln, py + (int64_t)(tb - kTok) * a.D_, a.D_, kTok);
       }
     }
-    const int nt = min(kScanTok, t1 - tb);
-    float dt[kScanTok], x[kScanTok], uv[kScanTok], zv[kScanTok];
-#pragma unroll
-    for (int t = 0; t < kScanTok; ++t) {
-      uv[t] = to_f32(ur[t]);
-      dt[t] = time_step(to_f32(dr[t]) + bias, a.softplus);
-      x[t] = dt[t] * uv[t];
-      zv[t] = OUT && a.z ? to_f32(zr[t]) : 0.f;
-    }
-    if (OUT || !(l & 4)) *(f32x4*)&sBC[w][l >> 3][(l >> 2) & 1][4 * (l & 3)] = (f32x4){bc[0], bc[1], bc[2], bc[3]};
+    if (OUT && a.ckpt) store_packed(a.ckpt, packed_at((int64_t)row * a.ckpts + tb / kTok, a, ln.tile, NW, w, 0), h);
     wave_lds_fence();
-    if (tb + kScanTok < t1) fetch(tb + kScanTok);
+    if (tb + kTok < t1) fetch(tb + kTok);
+    const int nt = min(kTok, t1 - tb);
+    float dt[kTok], uv[kTok], gate[kTok];
 #pragma unroll
-    for (int t = 0; t < kScanTok; ++t) {
-      if (t >= nt) break;
-      const int tok = tb + t;
-      if (tok == cur.s) {
-        start_state(a, ln, cur.n, h);
+    for (int t = 0; t < kTok; ++t) {
+      uv[t] = to_f32(sRow[w][0][t][own]);
+      dt[t] = time_step(to_f32(sRow[w][1][t][own]) + bias, a.softplus);
+      gate[t] = 1.f;
+    }
+    if (OUT && a.z)
+#pragma unroll
+      for (int t = 0; t < kTok; ++t) {
+        const float z = to_f32(sRow[w][OUT ? 2 : 0][t][own]);
+        gate[t] = z * sigmoid_full(z);
+      }
+    auto walk = [&](auto r) {
+#pragma unroll
+      for (int t = 0; t < kTok; ++t) {
+        if (!walks(r, t)) continue;
+        const f32x4 Bv = *(const f32x4*)&sBC[w][t][0][4 * ln.j];
+        f32x4 Cv;
+        if (OUT) Cv = *(const f32x4*)&sBC[w][t][1][4 * ln.j];
+        const float x = dt[t] * uv[t];
+        const float dk[4] = {of_channel<0>(dt[t]), of_channel<1>(dt[t]), of_channel<2>(dt[t]), of_channel<3>(dt[t])};
+        const float xk[4] = {of_channel<0>(x), of_channel<1>(x), of_channel<2>(x), of_channel<3>(x)};
+        float e[4][4], s[4];
+        stage();
+        decays(e, dk, A2);
+        stage();
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) h[k][i] = fmaf(e[k][i], h[k][i], xk[k] * Bv[i]);
+        stage();
+        if (OUT) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[k] = i ? fmaf(Cv[i], h[k][i], s[k]) : Cv[i] * h[k][i];
+
+          const float y = quad_total4(s[0], s[1], s[2], s[3], ln.odd, ln.high);
+          if constexpr (NW == 1) sOut[t][own] = from_f32<T>(fmaf(Dc, uv[t], y) * gate[t]);
+          else sY[turn][w][t][l] = y;
+        } else {
+          dt_sum += dt[t];
+        }
+      }
+    };
+    for (int lo = 0, hi; lo < nt; lo = hi) {   // the parts of the block that belong to one sequence each: one, nearly always
+      if (tb + lo == cur.s) {
+        load_state(a, ln, a.init, cur.n, h);
         cut = 1;
       }
-      const f32x4 Bv = *(const f32x4*)&sBC[w][t][0][4 * ln.j];
-      f32x4 Cv;
-      if (OUT) Cv = *(const f32x4*)&sBC[w][t][1][4 * ln.j];
-      const float dk[4] = {of_channel<0>(dt[t]), of_channel<1>(dt[t]), of_channel<2>(dt[t]), of_channel<3>(dt[t])};
-      const float xk[4] = {of_channel<0>(x[t]), of_channel<1>(x[t]), of_channel<2>(x[t]), of_channel<3>(x[t])};
-      float s[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        s[k] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          h[k][i] = fmaf(fast_exp2(dk[k] * A2[k][i]), h[k][i], xk[k] * Bv[i]);
-          if (OUT) s[k] = fmaf(Cv[i], h[k][i], s[k]);
-        }
-      }
-      if (OUT) {
-        float yv = quad_total4(s[0], s[1], s[2], s[3], ln.odd, ln.high);
-        if constexpr (NW == 1) {
-          yv = fmaf(Dc, uv[t], yv);
-          if (a.z) yv *= zv[t] * sigmoid_full(zv[t]);
-          if (ln.on) py[(int64_t)tok * a.D_] = from_f32<T>(yv);
-        } else {
-          sY[turn][w][t][l] = yv;
-        }
-      } else {
-        dt_sum += dt[t];
-      }
-      if (tok + 1 == cur.e) {
-        if (OUT && a.final_) ln.store(a, a.final_ + (int64_t)cur.n * a.D_ * a.N, h);
+      hi = max(lo + 1, min(nt, cur.e - tb));
+      if (hi - lo == kTok) walk(Whole{0, 0});
+      else walk(Part{lo, hi});
+      if (tb + hi == cur.e) {
+        if (OUT && a.final_) store_state(a, ln, a.final_, cur.n, h);
         if (a.cu) {
-          int n = cur.n + 1;
-          for (; n < a.seqs && a.cu[n + 1] <= tok + 1; ++n)   // sequences without a token
-            if (OUT && a.final_) {
-              float e[4][4];
-              start_state(a, ln, n, e);
-              ln.store(a, a.final_ + (int64_t)n * a.D_ * a.N, e);
-            }
-          if (n < a.seqs) cur = {n, tok + 1, a.cu[n + 1]};
+          const ScanSeq next = next_seq(a, cur);
+          if (OUT) hand_over(a, ln, a.init, a.final_, cur.n + 1, next.n);
+          cur = next;
         }
       }
     }
     if constexpr (NW > 1 && OUT) {
       __syncthreads();
 #pragma unroll
-      for (int t = 0; t < kScanTok; ++t) {
+      for (int t = 0; t < kTok; ++t) {
         if (t % NW != w || t >= nt) continue;
-        float yv = Dc * uv[t];
+        float y = Dc * uv[t];
 #pragma unroll
-        for (int k = 0; k < NW; ++k) yv += sY[turn][k][t][l];
-        if (a.z) yv *= zv[t] * sigmoid_full(zv[t]);
-        if (ln.on) py[(int64_t)(tb + t) * a.D_] = from_f32<T>(yv);
+        for (int k = 0; k < NW; ++k) y += sY[turn][k][t][l];
+        if (ln.on) row_store(py + (int64_t)(tb + t) * a.D_, ln.own, from_f32<T>(y * gate[t]));
       }
       turn ^= 1;
     }
     wave_lds_fence();
   }
+  if constexpr (OUT && NW == 1) {
+    const int tb = t0 + (t1 - 1 - t0) / kTok * kTok;
+    BlockRows<T> done;
+    done.from_lds(sOut);
+    done.store(ln, py + (int64_t)tb * a.D_, a.D_, t1 - tb);
+  }
   if (!OUT) {
     const int64_t slot = (int64_t)row * a.segs + blockIdx.y;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const f32x4 v = {h[k][0], h[k][1], h[k][2], h[k][3]};
-      ((f32x4*)a.seg_h)[packed_at(slot, a, ln.tile, NW, w, k)] = v;
-    }
+    store_packed(a.seg_h, packed_at(slot, a, ln.tile, NW, w, 0), h);
     if (w == 0) a.seg_dt[(slot * a.tiles + ln.tile) * 64 + l] = dt_sum;
     if (ln.tile == 0 && threadIdx.x == 0) a.seg_cut[slot] = cut;
   }
 }
 
-// What comes back over a segment from its end with nothing coming in: a thread-for-thread copy of the backward's carry,
-// g <- a (g + C Y) from the last token to the first.
+// What comes back over a segment from its end with nothing coming in: the backward's carry, g <- a (g + C Y) from the last
+// token to the first.
 template <typename T, int NW>
 __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) {
-  __shared__ float sC[NW][kScanTok][16];
-  const Lane<T> ln(a);
-  const int l = threadIdx.x & 63, w = ln.w, row = ln.row;
+  __shared__ float sC[NW][kTok][16];
+  __shared__ __attribute__((aligned(16))) T sRow[NW][3][kTok][64];   // dy, delta, z
+  const Lane ln(a);
+  const int l = threadIdx.x & 63, w = ln.w, row = ln.row, own = own_at();
   const int t0 = blockIdx.y * a.seg, t1 = min(a.T, t0 + a.seg);
   const float bias = a.bias ? a.bias[ln.own] : 0.f;
   float A2[4][4], g[4][4], dt_sum = 0.f;
@@ -355,77 +515,83 @@ __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) 
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { A2[k][i] *= kLog2e; g[k][i] = 0.f; }
+    for (int i = 0; i < 4; ++i) A2[k][i] *= kLog2e;
+  zero44(g);
   ScanSeq cur = seq_at(a, row, t1 - 1);
   int cut = 0;
-  const T* pd = (const T*)a.delta + row * a.db + ln.own;
-  const T* pz = a.z ? (const T*)a.z + row * a.zb + ln.own : nullptr;
-  const T* pg = (const T*)a.dy + (int64_t)row * a.T * a.D_ + ln.own;
-  T dr[kScanTok], zr[kScanTok], gr[kScanTok];
-  float bc[4];
+  const T* pd = (const T*)a.delta + row * a.db;
+  const T* pz = a.z ? (const T*)a.z + row * a.zb : nullptr;
+  const T* pg = (const T*)a.dy + (int64_t)row * a.T * a.D_;
+  const T* pC = (const T*)a.Cm + row * a.Cb + (int64_t)ln.group * a.N;
+  const int n4 = 16 * w + 4 * (l & 3);
+  BlockRows<T> rg, rd, rz;
+  Four<T> rc;
   auto fetch = [&](int tb) {
-#pragma unroll
-    for (int t = 0; t < kScanTok; ++t) {
-      const int64_t at = min(tb + t, t1 - 1);
-      dr[t] = pd[at * a.dt];
-      gr[t] = pg[at * a.D_];
-      if (a.z) zr[t] = pz[at * a.zt];
-    }
-    if (!(l & 32)) ln.fetch_bc(a, a.Cm, row * a.Cb + (int64_t)min(tb + (l >> 2), t1 - 1) * a.Ct, 16 * w + 4 * (l & 3), bc);
+    const int left = min(kTok, t1 - tb) - 1;
+    rg.fetch(ln, pg + (int64_t)tb * a.D_, a.D_, left);
+    rd.fetch(ln, pd + (int64_t)tb * a.dt, a.dt, left);
+    if (a.z) rz.fetch(ln, pz + (int64_t)tb * a.zt, a.zt, left);
+    rc.fetch(a, pC + (int64_t)tb * a.Ct, __umul24(min((l >> 2) & 7, left), a.Ct) * (unsigned)sizeof(T), n4);
   };
-  const int last = t0 + (t1 - 1 - t0) / kScanTok * kScanTok;
+  const int last = t0 + (t1 - 1 - t0) / kTok * kTok;
   fetch(last);
-  for (int tb = last; tb >= t0; tb -= kScanTok) {
-    const int nt = min(kScanTok, t1 - tb);
-    float dt[kScanTok], Y[kScanTok];
+  for (int tb = last; tb >= t0; tb -= kTok) {
+    rg.to_lds(sRow[w][0]);
+    rd.to_lds(sRow[w][1]);
+    if (a.z) rz.to_lds(sRow[w][2]);
+    *(f32x4*)&sC[w][(l >> 2) & 7][4 * (l & 3)] = rc.get(a, n4);
+    wave_lds_fence();
+    if (tb > t0) fetch(tb - kTok);
+    const int nt = min(kTok, t1 - tb);
+    float dt[kTok], Y[kTok];
 #pragma unroll
-    for (int t = 0; t < kScanTok; ++t) {
-      dt[t] = time_step(to_f32(dr[t]) + bias, a.softplus);
-      Y[t] = to_f32(gr[t]);
-      if (a.z) {
-        const float z = to_f32(zr[t]);
+    for (int t = 0; t < kTok; ++t) {
+      dt[t] = time_step(to_f32(sRow[w][1][t][own]) + bias, a.softplus);
+      Y[t] = to_f32(sRow[w][0][t][own]);
+    }
+    if (a.z)
+#pragma unroll
+      for (int t = 0; t < kTok; ++t) {
+        const float z = to_f32(sRow[w][2][t][own]);
         Y[t] *= z * sigmoid_full(z);
       }
-    }
-    if (!(l & 32)) *(f32x4*)&sC[w][l >> 2][4 * (l & 3)] = (f32x4){bc[0], bc[1], bc[2], bc[3]};
-    wave_lds_fence();
-    if (tb > t0) fetch(tb - kScanTok);
+    auto walk = [&](auto r) {
 #pragma unroll
-    for (int t = kScanTok - 1; t >= 0; --t) {
-      if (t >= nt) continue;
-      const int tok = tb + t;
-      if (tok + 1 == cur.e) {
+      for (int t = kTok - 1; t >= 0; --t) {
+        if (!walks(r, t)) continue;
+        const f32x4 Cv = *(const f32x4*)&sC[w][t][4 * ln.j];
+        const float dk[4] = {of_channel<0>(dt[t]), of_channel<1>(dt[t]), of_channel<2>(dt[t]), of_channel<3>(dt[t])};
+        const float Yk[4] = {of_channel<0>(Y[t]), of_channel<1>(Y[t]), of_channel<2>(Y[t]), of_channel<3>(Y[t])};
+        float e[4][4];
+        stage();
+        decays(e, dk, A2);
 #pragma unroll
         for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) g[k][i] = 0.f;
-        if (a.d_final) ln.load(a, a.d_final + (int64_t)cur.n * a.D_ * a.N, g);
+          for (int i = 0; i < 4; ++i) g[k][i] = fmaf(Cv[i], Yk[k], g[k][i]);
+        stage();
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) g[k][i] *= e[k][i];
+        dt_sum += dt[t];
       }
-      const f32x4 Cv = *(const f32x4*)&sC[w][t][4 * ln.j];
-      const float dk[4] = {of_channel<0>(dt[t]), of_channel<1>(dt[t]), of_channel<2>(dt[t]), of_channel<3>(dt[t])};
-      const float Yk[4] = {of_channel<0>(Y[t]), of_channel<1>(Y[t]), of_channel<2>(Y[t]), of_channel<3>(Y[t])};
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) g[k][i] = fast_exp2(dk[k] * A2[k][i]) * fmaf(Cv[i], Yk[k], g[k][i]);
-      dt_sum += dt[t];
-      if (tok == cur.s) {
+    };
+    for (int hi = nt, lo; hi > 0; hi = lo) {
+      if (tb + hi == cur.e) load_state(a, ln, a.d_final, cur.n, g);
+      lo = min(hi - 1, max(0, cur.s - tb));
+      if (hi - lo == kTok) walk(Whole{0, 0});
+      else walk(Part{lo, hi});
+      if (tb + lo == cur.s) {
         cut = 1;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) g[k][i] = 0.f;
-        if (tok > t0) cur = seq_at(a, row, tok - 1);
+        zero44(g);
+        if (a.cu) cur = prev_seq(a, cur);
       }
     }
     wave_lds_fence();
   }
   const int64_t slot = (int64_t)row * a.segs + blockIdx.y;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const f32x4 v = {g[k][0], g[k][1], g[k][2], g[k][3]};
-    ((f32x4*)a.seg_h)[packed_at(slot, a, ln.tile, NW, w, k)] = v;
-  }
+  store_packed(a.seg_h, packed_at(slot, a, ln.tile, NW, w, 0), g);
   if (w == 0) a.seg_dt[(slot * a.tiles + ln.tile) * 64 + l] = dt_sum;
   if (ln.tile == 0 && threadIdx.x == 0) a.seg_cut[slot] = cut;
 }
@@ -449,7 +615,7 @@ __global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs a) {
     for (int x = 0; x < kAhead; ++x) {
       const int s = min(b + x, a.segs - 1);
       const int64_t slot = (int64_t)row * a.segs + (BACK ? a.segs - 1 - s : s);
-      v[x] = H[packed_at(slot, a, tile, NW, w, k)];
+      v[x] = H[packed_at(slot, a, tile, NW, w, k) + l];
       d[x] = a.seg_dt[(slot * a.tiles + tile) * 64 + (l & ~3) + k];
       c[x] = a.seg_cut[slot];
     }
@@ -457,7 +623,7 @@ __global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs a) {
     for (int x = 0; x < kAhead; ++x) {
       if (b + x >= a.segs) break;
       const int64_t slot = (int64_t)row * a.segs + (BACK ? a.segs - 1 - (b + x) : b + x);
-      H[packed_at(slot, a, tile, NW, w, k)] = (f32x4){h[0], h[1], h[2], h[3]};
+      H[packed_at(slot, a, tile, NW, w, k) + l] = (f32x4){h[0], h[1], h[2], h[3]};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         // (a state of zero stays zero whatever the decay over the segment has overflowed to)
@@ -469,17 +635,19 @@ __global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-constexpr int kSub = 4;   // tokens whose decays and states are in registers
+constexpr int kSub = 2;   // tokens whose decays and states are in registers
 
 template <typename T, int NW>
-__global__ __launch_bounds__(64 * NW) void scan_bwd_kernel(ScanArgs a) {
-  constexpr int kBlk = PAL_SCAN_BLOCK;
-  __shared__ float sBC[NW][kBlk][2][16];
-  __shared__ float sDt[NW][kBlk][64];
-  __shared__ f32x4 sH[NW][kBlk / kSub - 1][4][64];
+__global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
+  constexpr int kOwn = (4 + NW - 1) / NW;   // arrays that a wave fetches for the workgroup
+  __shared__ float sBC[NW][kTok][2][16];
+  __shared__ __attribute__((aligned(16))) T sRow[4][kTok][64];   // u, delta, z, dy; then du, ddelta, dz in the places of the first three
+  __shared__ float sDt[kTok][64];
+  __shared__ f32x4 sH[NW][kTok / kSub - 1][4][64];
+  __shared__ __attribute__((aligned(16))) float sP[NW][kTok][32];   // the waves' shares of dB and dC
   __shared__ float sS[NW > 1 ? 2 : 1][NW > 1 ? NW : 1][kSub][3][64];
-  const Lane<T> ln(a);
-  const int l = threadIdx.x & 63, w = ln.w, row = ln.row;
+  const Lane ln(a);
+  const int l = threadIdx.x & 63, w = ln.w, row = ln.row, own = own_at();
   const int t0 = blockIdx.y * a.seg, t1 = min(a.T, t0 + a.seg);
   const float bias = a.bias ? a.bias[ln.own] : 0.f, Dc = a.D ? a.D[ln.own] : 0.f;
   float A2[4][4], carry[4][4], dA[4][4];
@@ -488,205 +656,247 @@ __global__ __launch_bounds__(64 * NW) void scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
   for (int k = 0; k < 4; ++k)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { A2[k][i] *= kLog2e; carry[k][i] = dA[k][i] = 0.f; }
+    for (int i = 0; i < 4; ++i) A2[k][i] *= kLog2e;
+  zero44(dA);
   const int64_t slot = (int64_t)row * a.segs + blockIdx.y;
-  if (t1 < a.T)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const f32x4 v = ((const f32x4*)a.seg_h)[packed_at(slot, a, ln.tile, NW, w, k)];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) carry[k][i] = v[i];
-    }
+  if (t1 < a.T) load_packed(a.seg_h, packed_at(slot, a, ln.tile, NW, w, 0), carry);
+  else zero44(carry);
   ScanSeq cur = seq_at(a, row, t1 - 1);
-  if (t1 == a.T && a.d_init && a.cu)
-    for (int n = cur.n + 1; n < a.seqs; ++n) {   // sequences without a token behind the last one
-      float e[4][4] = {};
-      if (a.d_final) ln.load(a, a.d_final + (int64_t)n * a.D_ * a.N, e);
-      ln.store(a, a.d_init + (int64_t)n * a.D_ * a.N, e);
-    }
-  const T* pu = (const T*)a.u + row * a.ub + ln.own;
-  const T* pd = (const T*)a.delta + row * a.db + ln.own;
-  const T* pz = a.z ? (const T*)a.z + row * a.zb + ln.own : nullptr;
-  const int64_t out0 = (int64_t)row * a.T * a.D_ + ln.own;
-  const T* pg = (const T*)a.dy + out0;
+  if (t1 == a.T && a.cu) hand_over(a, ln, a.d_final, a.d_init, cur.n + 1, a.seqs);   // sequences without a token behind the last one
+  const int64_t out0 = (int64_t)row * a.T * a.D_;
+  const int shares = ((l >> 4) & 1) * 16 + 4 * (l & 3) + ((l >> 2) & 1) * 2 + ((l >> 3) & 1);   // a lane's sum among dB and dC (below)
   int turn = 0;
+  auto sync = [&]() {
+    if constexpr (NW == 1) wave_lds_fence();
+    else __syncthreads();
+  };
 
-  for (int tb = t0 + (t1 - 1 - t0) / kBlk * kBlk; tb >= t0; tb -= kBlk) {
-    const int nt = min(kBlk, t1 - tb);
-    // ---- the block's time steps, B and C, and its states before tokens 4, 8 and 12
-    T ur[kBlk], dr[kBlk];
+  const T* pB = (const T*)a.Bm + row * a.Bb + (int64_t)ln.group * a.N;
+  const T* pC = (const T*)a.Cm + row * a.Cb + (int64_t)ln.group * a.N;
+  const int n4 = 16 * w + 4 * (l & 3);
+  BlockRows<T> rows[kOwn];
+  Four<T> rb, rc;
+  float h0[4][4];              // the state kept before the block
+  auto fetch = [&](int tb) {
+    const int left = min(kTok, t1 - tb) - 1;
 #pragma unroll
-    for (int t = 0; t < kBlk; ++t) {
-      const int64_t at = min(tb + t, t1 - 1);
-      dr[t] = pd[at * a.dt];
-      if (t < kBlk - kSub) ur[t] = pu[at * a.ut];
+    for (int m = 0; m < kOwn; ++m) {
+      const int i = w + NW * m;
+      if (i > 3 || (i == 2 && !a.z)) continue;
+      const T* p = (const T*)(i == 0 ? a.u : i == 1 ? a.delta : i == 2 ? a.z : a.dy);
+      const int64_t batch = i == 0 ? a.ub : i == 1 ? a.db : i == 2 ? a.zb : (int64_t)a.T * a.D_;
+      const int stride = i == 0 ? a.ut : i == 1 ? a.dt : i == 2 ? a.zt : a.D_;
+      rows[m].fetch(ln, p + row * batch + (int64_t)tb * stride, stride, left);
     }
-    {
-      const int64_t at = min(tb + (l >> 2), t1 - 1);
-      float b[4], c[4];
-      ln.fetch_bc(a, a.Bm, row * a.Bb + at * a.Bt, 16 * w + 4 * (l & 3), b);
-      ln.fetch_bc(a, a.Cm, row * a.Cb + at * a.Ct, 16 * w + 4 * (l & 3), c);
-      *(f32x4*)&sBC[w][l >> 2][0][4 * (l & 3)] = (f32x4){b[0], b[1], b[2], b[3]};
-      *(f32x4*)&sBC[w][l >> 2][1][4 * (l & 3)] = (f32x4){c[0], c[1], c[2], c[3]};
+    const int t = min((l >> 2) & 7, left);
+    rb.fetch(a, pB + (int64_t)tb * a.Bt, __umul24(t, a.Bt) * (unsigned)sizeof(T), n4);
+    rc.fetch(a, pC + (int64_t)tb * a.Ct, __umul24(t, a.Ct) * (unsigned)sizeof(T), n4);
+  };
+  auto fetch_kept = [&](int tb) { load_packed(a.ckpt, packed_at((int64_t)row * a.ckpts + tb / kTok, a, ln.tile, NW, w, 0), h0); };
+  // results of a block: out of LDS, and on their way
+  BlockRows<T> done[kOwn];
+  f32x4 done_bc;
+  auto take = [&]() {
+#pragma unroll
+    for (int m = 0; m < kOwn; ++m) done[m].from_lds(sRow[min(w + NW * m, 2)]);
+    done_bc = *(const f32x4*)&sP[w][l >> 3][4 * (l & 7)];
+  };
+  auto put = [&](int tb, int nt) {
+#pragma unroll
+    for (int m = 0; m < kOwn; ++m) {
+      const int i = w + NW * m;
+      if (i > 2 || (i == 2 && !a.z)) continue;
+      done[m].store(ln, (T*)(i == 0 ? a.du : i == 1 ? a.ddelta : a.dz) + out0 + (int64_t)tb * a.D_, a.D_, nt);
     }
-    const f32x4* kept = (const f32x4*)a.ckpt + packed_at((int64_t)row * a.ckpts + tb / kBlk, a, ln.tile, NW, w, 0);
-    ScanSeq fw = cur.s <= tb ? cur : seq_at(a, row, tb);   // sequence of the block's first token
-    const ScanSeq fw0 = fw;
+    const float* to = a.part_bc + ((((int64_t)row * a.T + tb) * a.tiles + ln.tile) * NW + w) * 32;
+    if ((l >> 3) < nt) *(PAL_GLOBAL f32x4*)row_element(to, ((l >> 3) * a.tiles * NW * 32 + 4 * (l & 7)) * 4u) = done_bc;
+  };
+  const int last = t0 + (t1 - 1 - t0) / kTok * kTok;
+  fetch(last);
+  fetch_kept(last);
+
+  for (int tb = last; tb >= t0; tb -= kTok) {
+    const int nt = min(kTok, t1 - tb);
+    // ---- the block's rows, time steps, and its states before tokens 2, 4 and 6
+    take();     // (before the first block: nothing, and it goes nowhere)
+    sync();
+#pragma unroll
+    for (int m = 0; m < kOwn; ++m) {
+      const int i = w + NW * m;
+      if (i <= 3) rows[m].to_lds(sRow[i]);
+    }
+    *(f32x4*)&sBC[w][(l >> 2) & 7][0][4 * (l & 3)] = rb.get(a, n4);
+    *(f32x4*)&sBC[w][(l >> 2) & 7][1][4 * (l & 3)] = rc.get(a, n4);
+    sync();
+    // (the stores after the wait for this block's rows and before the next fetch: they are never waited for by themselves)
+    if (tb < last) put(tb + kTok, min(kTok, t1 - tb - kTok));
+    if (tb > t0) fetch(tb - kTok);
+#pragma unroll
+    for (int t = 0; t < kTok; ++t)
+      if (t % NW == w) sDt[t][l] = time_step(to_f32(sRow[1][t][own]) + bias, a.softplus);
+    sync();
     {
       float h[4][4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const f32x4 v = kept[k * 64];
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[k][i] = v[i];
-      }
-      wave_lds_fence();
+        for (int i = 0; i < 4; ++i) h[k][i] = h0[k][i];
+      auto walk = [&](auto r) {
 #pragma unroll
-      for (int t = 0; t < kBlk; ++t) {
-        const float dt = time_step(to_f32(dr[t]) + bias, a.softplus);
-        sDt[w][t][l] = dt;
-        if (t >= kBlk - kSub || t >= nt) continue;
-        const int tok = tb + t;
-        if (tok == fw.s) start_state(a, ln, fw.n, h);
-        const float x = dt * to_f32(ur[t]);
-        const f32x4 Bv = *(const f32x4*)&sBC[w][t][0][4 * ln.j];
-        const float dk[4] = {of_channel<0>(dt), of_channel<1>(dt), of_channel<2>(dt), of_channel<3>(dt)};
-        const float xk[4] = {of_channel<0>(x), of_channel<1>(x), of_channel<2>(x), of_channel<3>(x)};
+        for (int t = 0; t < kTok - kSub; ++t) {
+          if (walks(r, t)) {
+            const float dt = sDt[t][l], x = dt * to_f32(sRow[0][t][own]);
+            const f32x4 Bv = *(const f32x4*)&sBC[w][t][0][4 * ln.j];
+            const float dk[4] = {of_channel<0>(dt), of_channel<1>(dt), of_channel<2>(dt), of_channel<3>(dt)};
+            const float xk[4] = {of_channel<0>(x), of_channel<1>(x), of_channel<2>(x), of_channel<3>(x)};
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) h[k][i] = fmaf(fast_exp2(dk[k] * A2[k][i]), h[k][i], xk[k] * Bv[i]);
-        if (t % kSub == kSub - 1)
+              for (int i = 0; i < 4; ++i) h[k][i] = fmaf(fast_exp2(dk[k] * A2[k][i]), h[k][i], xk[k] * Bv[i]);
+            if (t % kSub == kSub - 1)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) sH[w][t / kSub][k][l] = (f32x4){h[k][0], h[k][1], h[k][2], h[k][3]};
-        if (tok + 1 == fw.e) fw = seq_at(a, row, min(tok + 1, a.T - 1));
+              for (int k = 0; k < 4; ++k) sH[w][t / kSub][k][l] = (f32x4){h[k][0], h[k][1], h[k][2], h[k][3]};
+          }
+        }
+      };
+      const int most = min(nt, kTok - kSub);
+      ScanSeq fw = cur.s <= tb ? cur : seq_at(a, row, tb);
+      for (int lo = 0, hi; lo < most; lo = hi) {
+        if (tb + lo == fw.s) load_state(a, ln, a.init, fw.n, h);
+        hi = max(lo + 1, min(most, fw.e - tb));
+        if (hi - lo == kTok - kSub) walk(Whole{0, 0});
+        else walk(Part{lo, hi});
+        if (hi < most) fw = next_seq(a, fw);
       }
     }
     wave_lds_fence();
-    // ---- four tokens at a time from the end
+    // ---- two tokens at a time from the end
     for (int sub = (nt - 1) / kSub; sub >= 0; --sub) {
       const int ts = tb + sub * kSub, ns = min(kSub, t1 - ts);
-      float h[4][4], av[kSub][4][4], ah[kSub][4][4];
-      float uv[kSub], zv[kSub], gv[kSub], raw[kSub];
+      // what the tokens take and, in the same place, what they give once they are done: Y -> du, slope (of the softplus) -> ddelta,
+      // gz (dy silu'(z)) -> dz
+      float uv[kSub], Y[kSub], slope[kSub], gz[kSub];
 #pragma unroll
       for (int t = 0; t < kSub; ++t) {
-        const int64_t at = min(ts + t, t1 - 1);
-        uv[t] = to_f32(pu[at * a.ut]);
-        raw[t] = to_f32(pd[at * a.dt]) + bias;
-        zv[t] = a.z ? to_f32(pz[at * a.zt]) : 0.f;
-        gv[t] = ln.on ? to_f32(pg[at * a.D_]) : 0.f;     // (a lane beyond the group adds nothing to dB and dC)
-        if (!ln.on) uv[t] = 0.f;
+        const float raw = to_f32(sRow[1][sub * kSub + t][own]) + bias, sg = sigmoid_full(raw);
+        uv[t] = to_f32(sRow[0][sub * kSub + t][own]);
+        Y[t] = to_f32(sRow[3][sub * kSub + t][own]);
+        slope[t] = a.softplus && raw <= 20.f ? sg : 1.f;
+        gz[t] = 0.f;
       }
+      if (a.z)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const f32x4 v = sub ? sH[w][sub ? sub - 1 : 0][k][l] : kept[k * 64];
+        for (int t = 0; t < kSub; ++t) {
+          const float z = to_f32(sRow[2][sub * kSub + t][own]), sg = sigmoid_full(z);
+          gz[t] = Y[t] * (sg + z * sg * (1.f - sg));
+          Y[t] *= z * sg;
+        }
+      auto finish = [&](int t, float dt, float ypre, float sumB, float sumA) {
+        const float ddt = fmaf(uv[t], sumB, sumA * 0.6931471806f);
+        gz[t] *= fmaf(Dc, uv[t], ypre);
+        dD = fmaf(Y[t], uv[t], dD);
+        slope[t] *= ddt;
+        dbias += slope[t];
+        Y[t] = fmaf(dt, sumB, Dc * Y[t]);
+        sRow[0][sub * kSub + t][own] = from_f32<T>(Y[t]);
+        sRow[1][sub * kSub + t][own] = from_f32<T>(slope[t]);
+        sRow[2][sub * kSub + t][own] = from_f32<T>(gz[t]);
+      };
+      float h[4][4];
+      auto walk = [&](auto r, bool ends) {
+        float av[kSub][4][4], ah[kSub][4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) h[k][i] = v[i];
-      }
-      ScanSeq sq = cur.s <= ts ? cur : fw0.e > ts ? fw0 : seq_at(a, row, ts);
-#pragma unroll
-      for (int t = 0; t < kSub; ++t) {
-        if (t >= ns) break;
-        const int tok = ts + t;
-        if (tok == sq.s) start_state(a, ln, sq.n, h);
-        const float dt = sDt[w][sub * kSub + t][l], x = dt * uv[t];
-        const f32x4 Bv = *(const f32x4*)&sBC[w][sub * kSub + t][0][4 * ln.j];
-        const float dk[4] = {of_channel<0>(dt), of_channel<1>(dt), of_channel<2>(dt), of_channel<3>(dt)};
-        const float xk[4] = {of_channel<0>(x), of_channel<1>(x), of_channel<2>(x), of_channel<3>(x)};
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            av[t][k][i] = fast_exp2(dk[k] * A2[k][i]);
-            ah[t][k][i] = av[t][k][i] * h[k][i];
-            h[k][i] = fmaf(xk[k], Bv[i], ah[t][k][i]);
-          }
-        if (tok + 1 == sq.e && t + 1 < ns) sq = seq_at(a, row, tok + 1);
-      }
-#pragma unroll
-      for (int t = kSub - 1; t >= 0; --t) {
-        if (t >= ns) continue;
-        const int tok = ts + t;
-        if (tok + 1 == cur.e) {
+        for (int t = 0; t < kSub; ++t) {
+          if (!walks(r, t)) continue;
+          const float dt = sDt[sub * kSub + t][l], x = dt * uv[t];
+          const f32x4 Bv = *(const f32x4*)&sBC[w][sub * kSub + t][0][4 * ln.j];
+          const float dk[4] = {of_channel<0>(dt), of_channel<1>(dt), of_channel<2>(dt), of_channel<3>(dt)};
+          const float xk[4] = {of_channel<0>(x), of_channel<1>(x), of_channel<2>(x), of_channel<3>(x)};
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) carry[k][i] = 0.f;
-          if (a.d_final) ln.load(a, a.d_final + (int64_t)cur.n * a.D_ * a.N, carry);
+            for (int i = 0; i < 4; ++i) {
+              av[t][k][i] = fast_exp2(dk[k] * A2[k][i]);
+              ah[t][k][i] = av[t][k][i] * h[k][i];
+              h[k][i] = fmaf(xk[k], Bv[i], ah[t][k][i]);
+            }
         }
-        const float dt = sDt[w][sub * kSub + t][l], x = dt * uv[t];
-        const float sz = a.z ? sigmoid_full(zv[t]) : 0.f;
-        const float Y = a.z ? gv[t] * zv[t] * sz : gv[t];
-        const f32x4 Bv = *(const f32x4*)&sBC[w][sub * kSub + t][0][4 * ln.j];
-        const f32x4 Cv = *(const f32x4*)&sBC[w][sub * kSub + t][1][4 * ln.j];
-        const float dk[4] = {of_channel<0>(dt), of_channel<1>(dt), of_channel<2>(dt), of_channel<3>(dt)};
-        const float xk[4] = {of_channel<0>(x), of_channel<1>(x), of_channel<2>(x), of_channel<3>(x)};
-        const float Yk[4] = {of_channel<0>(Y), of_channel<1>(Y), of_channel<2>(Y), of_channel<3>(Y)};
-        float gB[4] = {0.f, 0.f, 0.f, 0.f}, gC[4] = {0.f, 0.f, 0.f, 0.f}, sy[4], sb[4], sa[4];
+        if (ends) load_state(a, ln, a.d_final, cur.n, carry);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          sy[k] = sb[k] = sa[k] = 0.f;
+        for (int t = kSub - 1; t >= 0; --t) {
+          if (!walks(r, t)) continue;
+          const float dt = sDt[sub * kSub + t][l], x = dt * uv[t];
+          const f32x4 Bv = *(const f32x4*)&sBC[w][sub * kSub + t][0][4 * ln.j];
+          const f32x4 Cv = *(const f32x4*)&sBC[w][sub * kSub + t][1][4 * ln.j];
+          const float dk[4] = {of_channel<0>(dt), of_channel<1>(dt), of_channel<2>(dt), of_channel<3>(dt)};
+          const float xk[4] = {of_channel<0>(x), of_channel<1>(x), of_channel<2>(x), of_channel<3>(x)};
+          const float Yk[4] = {of_channel<0>(Y[t]), of_channel<1>(Y[t]), of_channel<2>(Y[t]), of_channel<3>(Y[t])};
+          float gB[4], gC[4], sy[4], sb[4], sa[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float hv = fmaf(xk[k], Bv[i], ah[t][k][i]);
-            const float g = fmaf(Cv[i], Yk[k], carry[k][i]), p = g * ah[t][k][i];
-            gC[i] = fmaf(Yk[k], hv, gC[i]);
-            gB[i] = fmaf(g, xk[k], gB[i]);
-            sy[k] = fmaf(Cv[i], hv, sy[k]);
-            sb[k] = fmaf(g, Bv[i], sb[k]);
-            sa[k] = fmaf(p, A2[k][i], sa[k]);
-            dA[k][i] = fmaf(p, dk[k], dA[k][i]);
-            carry[k][i] = g * av[t][k][i];
+          for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float hv = fmaf(xk[k], Bv[i], ah[t][k][i]);
+              const float g = fmaf(Cv[i], Yk[k], carry[k][i]), p = g * ah[t][k][i];
+              gC[i] = k ? fmaf(Yk[k], hv, gC[i]) : Yk[k] * hv;
+              gB[i] = k ? fmaf(g, xk[k], gB[i]) : g * xk[k];
+              sy[k] = i ? fmaf(Cv[i], hv, sy[k]) : Cv[i] * hv;
+              sb[k] = i ? fmaf(g, Bv[i], sb[k]) : g * Bv[i];
+              sa[k] = i ? fmaf(p, A2[k][i], sa[k]) : p * A2[k][i];
+              dA[k][i] = fmaf(p, dk[k], dA[k][i]);
+              carry[k][i] = g * av[t][k][i];
+            }
+          }
+          // dB, dC: eight sums over the sixteen quads; lane bits 3, 2, 4 choose among them, bit 5 holds the same twice
+          {
+            const float p0 = pair_bit3(gB[0], gB[1]), p1 = pair_bit3(gB[2], gB[3]);
+            const float p2 = pair_bit3(gC[0], gC[1]), p3 = pair_bit3(gC[2], gC[3]);
+            float r0 = pair_bit2(p0, p1), r1 = pair_bit2(p2, p3);
+            swap_rows(r0, r1);
+            float s = r0 + r1, s2 = s;
+            swap_halves(s, s2);
+            sP[w][sub * kSub + t][shares] = s + s2;
+          }
+          const float ty = quad_total4(sy[0], sy[1], sy[2], sy[3], ln.odd, ln.high);
+          const float tB = quad_total4(sb[0], sb[1], sb[2], sb[3], ln.odd, ln.high);
+          const float tA = quad_total4(sa[0], sa[1], sa[2], sa[3], ln.odd, ln.high);
+          if constexpr (NW == 1) {
+            finish(t, dt, ty, tB, tA);
+          } else {
+            sS[turn][w][t][0][l] = ty;
+            sS[turn][w][t][1][l] = tB;
+            sS[turn][w][t][2][l] = tA;
           }
         }
-        // dB, dC: eight sums over the sixteen quads; lane bits 3, 2, 4 choose among them, bit 5 holds the same twice
-        {
-          const float p0 = pair_bit3(gB[0], gB[1]), p1 = pair_bit3(gB[2], gB[3]);
-          const float p2 = pair_bit3(gC[0], gC[1]), p3 = pair_bit3(gC[2], gC[3]);
-          float r0 = pair_bit2(p0, p1), r1 = pair_bit2(p2, p3);
-          swap_rows(r0, r1);
-          float r = r0 + r1, r2 = r;
-          swap_halves(r, r2);
-          r += r2;
-          if (!(l & 32)) {
-            const int which = (l >> 4) & 1, n = 4 * ln.j + ((l >> 2) & 1) * 2 + ((l >> 3) & 1);
-            a.part_bc[((((int64_t)row * a.T + tok) * a.tiles + ln.tile) * NW + w) * 32 + which * 16 + n] = r;
-          }
-        }
-        float ty = quad_total4(sy[0], sy[1], sy[2], sy[3], ln.odd, ln.high);
-        float tB = quad_total4(sb[0], sb[1], sb[2], sb[3], ln.odd, ln.high);
-        float tA = quad_total4(sa[0], sa[1], sa[2], sa[3], ln.odd, ln.high);
-        auto finish = [&](float ypre, float sumB, float sumA) {
-          ypre = fmaf(Dc, uv[t], ypre);
-          dD = fmaf(Y, uv[t], dD);
-          const float ddt = fmaf(uv[t], sumB, sumA * 0.6931471806f);
-          const float dd = a.softplus && raw[t] <= 20.f ? ddt * sigmoid_full(raw[t]) : ddt;
-          if (ln.on) {
-            dbias += dd;
-            const int64_t at = out0 + (int64_t)tok * a.D_;
-            ((T*)a.du)[at] = from_f32<T>(fmaf(dt, sumB, Dc * Y));
-            ((T*)a.ddelta)[at] = from_f32<T>(dd);
-            if (a.z) ((T*)a.dz)[at] = from_f32<T>(gv[t] * ypre * (sz + zv[t] * sz * (1.f - sz)));
-          }
-        };
-        if constexpr (NW == 1) {
-          finish(ty, tB, tA);
+      };
+      for (int hi = ns, lo; hi > 0; hi = lo) {
+        lo = min(hi - 1, max(0, cur.s - ts));
+        if (ts + lo == cur.s) {
+          load_state(a, ln, a.init, cur.n, h);
+          if (sub == 0 && lo == 0 && tb > t0) fetch_kept(tb - kTok);
+        } else if (sub == 0) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[k][i] = h0[k][i];
+          // the next block's while the last two tokens of this one are walked: fetched with its rows it would need registers of its own
+          if (tb > t0) fetch_kept(tb - kTok);
         } else {
-          sS[turn][w][t][0][l] = ty;
-          sS[turn][w][t][1][l] = tB;
-          sS[turn][w][t][2][l] = tA;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const f32x4 v = sH[w][sub - 1][k][l];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[k][i] = v[i];
+          }
         }
-        if (tok == cur.s) {
-          if (a.d_init) ln.store(a, a.d_init + (int64_t)cur.n * a.D_ * a.N, carry);
+        if (hi - lo == kSub) walk(Whole{0, 0}, ts + hi == cur.e);
+        else walk(Part{lo, hi}, ts + hi == cur.e);
+        if (ts + lo == cur.s) {
+          if (a.d_init) store_state(a, ln, a.d_init, cur.n, carry);
           if (a.cu) {
-            int n = cur.n - 1;
-            for (; n >= 0 && a.cu[n] >= tok; --n)   // sequences without a token
-              if (a.d_init) {
-                float e[4][4] = {};
-                if (a.d_final) ln.load(a, a.d_final + (int64_t)n * a.D_ * a.N, e);
-                ln.store(a, a.d_init + (int64_t)n * a.D_ * a.N, e);
-              }
-            if (n >= 0) cur = {n, a.cu[n], tok};
+            const ScanSeq prev = prev_seq(a, cur);
+            hand_over(a, ln, a.d_final, a.d_init, prev.n + 1, cur.n);
+            cur = prev;
           }
         }
       }
@@ -694,37 +904,24 @@ __global__ __launch_bounds__(64 * NW) void scan_bwd_kernel(ScanArgs a) {
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < kSub; ++t) {
-          if (t % NW != w || t >= ns) continue;
+          if ((sub * kSub + t) % NW != w || t >= ns) continue;
           float s3[3];
 #pragma unroll
           for (int x = 0; x < 3; ++x) {
-            s3[x] = 0.f;
+            s3[x] = sS[turn][0][t][x][l];
 #pragma unroll
-            for (int k = 0; k < NW; ++k) s3[x] += sS[turn][k][t][x][l];
+            for (int k = 1; k < NW; ++k) s3[x] += sS[turn][k][t][x][l];
           }
-          const int tok = ts + t;
-          const float dt = sDt[w][sub * kSub + t][l];
-          const float sz = a.z ? sigmoid_full(zv[t]) : 0.f, Y = a.z ? gv[t] * zv[t] * sz : gv[t];
-          const float ypre = fmaf(Dc, uv[t], s3[0]);
-          dD = fmaf(Y, uv[t], dD);
-          const float ddt = fmaf(uv[t], s3[1], s3[2] * 0.6931471806f);
-          const float dd = a.softplus && raw[t] <= 20.f ? ddt * sigmoid_full(raw[t]) : ddt;
-          if (ln.on) {
-            dbias += dd;
-            const int64_t at = out0 + (int64_t)tok * a.D_;
-            ((T*)a.du)[at] = from_f32<T>(fmaf(dt, s3[1], Dc * Y));
-            ((T*)a.ddelta)[at] = from_f32<T>(dd);
-            if (a.z) ((T*)a.dz)[at] = from_f32<T>(gv[t] * ypre * (sz + zv[t] * sz * (1.f - sz)));
-          }
+          finish(t, sDt[sub * kSub + t][l], s3[0], s3[1], s3[2]);
         }
         turn ^= 1;
       }
     }
-    wave_lds_fence();
+    sync();
   }
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    ((f32x4*)a.part_a)[packed_at(slot, a, ln.tile, NW, w, k)] = (f32x4){dA[k][0], dA[k][1], dA[k][2], dA[k][3]};
+  take();
+  put(t0, min(kTok, t1 - t0));
+  store_packed(a.part_a, packed_at(slot, a, ln.tile, NW, w, 0), dA);
   float* pc = a.part_c + (((slot * a.tiles + ln.tile) * NW + w) * 64 + l) * 2;
   pc[0] = dD;
   pc[1] = dbias;
@@ -754,7 +951,7 @@ __global__ __launch_bounds__(256) void scan_bwd_params_kernel(ScanArgs a, int nw
   double t[4] = {0., 0., 0., 0.};
   if (z < 4) {
     for (int64_t i = v; i < slots; i += 4) {
-      const f32x4 x = ((const f32x4*)a.part_a)[packed_at(i, a, tile, nw, w, z)];
+      const f32x4 x = ((const f32x4*)a.part_a)[packed_at(i, a, tile, nw, w, z) + l];
 #pragma unroll
       for (int e = 0; e < 4; ++e) t[e] += x[e];
     }
@@ -792,7 +989,7 @@ __global__ __launch_bounds__(256) void scan_bwd_params_kernel(ScanArgs a, int nw
 static int check_scan(const PalScanDims* d) {
   if (!d) return PAL_E_NULL;
   if (d->batch <= 0 || d->seq_len <= 0 || d->n_seqs <= 0 || d->channels <= 0 || d->groups <= 0) return PAL_E_DIM;
-  if (d->batch > 65535 || d->channels > 1 << 20 || d->channels % d->groups) return PAL_E_DIM;
+  if (d->batch > 65535 || d->channels >= 1 << 24 || d->channels % d->groups) return PAL_E_DIM;
   if ((int64_t)d->batch * d->seq_len > (int64_t)1 << 30) return PAL_E_DIM;
   if (d->state < 1 || d->state > PAL_SCAN_MAX_STATE) return PAL_E_DIM;
   if (d->dtype != PAL_DTYPE_F32 && d->dtype != PAL_DTYPE_BF16) return PAL_E_DTYPE;
@@ -805,6 +1002,8 @@ static int check_scan(const PalScanDims* d) {
                              d->u_token, d->delta_token, d->z_token, d->B_token, d->C_token};
   for (int64_t s : strides)
     if (s < 0) return PAL_E_DIM;
+  for (int64_t s : {d->u_token, d->delta_token, d->z_token, d->B_token, d->C_token})
+    if (s >= 1 << 24) return PAL_E_DIM;
   return PAL_OK;
 }
 static int check_scan_tensors(const PalScanDims* d, const PalScanTensors* t) {
@@ -822,7 +1021,7 @@ static int64_t scan_tiles(const PalScanDims* d) { return (int64_t)d->groups * ((
 // Tokens per segment: enough segments for two waves on every SIMD, at least 64 tokens each
 static int scan_segment(const PalScanDims* d) {
   const int64_t waves = scan_tiles(d) * scan_waves(d) * d->batch;
-  int64_t segs = (2048 + waves - 1) / waves;
+  const int64_t segs = waves < 2048 ? 2048 / waves : 1;
   int64_t seg = (d->seq_len + segs - 1) / segs;
   seg = (seg + PAL_SCAN_BLOCK - 1) / PAL_SCAN_BLOCK * PAL_SCAN_BLOCK;
   if (seg < 64) seg = 64;
@@ -835,8 +1034,8 @@ static void scan_args(ScanArgs& a, const PalScanDims* d, const PalScanTensors* t
   a.tiles = a.G * a.tiles_g;
   a.softplus = d->softplus;
   a.vec = d->state % 4 == 0;
-  a.ub = d->u_batch; a.ut = d->u_token; a.db = d->delta_batch; a.dt = d->delta_token; a.zb = d->z_batch; a.zt = d->z_token;
-  a.Bb = d->B_batch; a.Bt = d->B_token; a.Cb = d->C_batch; a.Ct = d->C_token;
+  a.ub = d->u_batch; a.db = d->delta_batch; a.zb = d->z_batch; a.Bb = d->B_batch; a.Cb = d->C_batch;
+  a.ut = (int)d->u_token; a.dt = (int)d->delta_token; a.zt = (int)d->z_token; a.Bt = (int)d->B_token; a.Ct = (int)d->C_token;
   a.seg = scan_segment(d);
   a.segs = (a.T + a.seg - 1) / a.seg;
   a.ckpts = (a.T + PAL_SCAN_BLOCK - 1) / PAL_SCAN_BLOCK;

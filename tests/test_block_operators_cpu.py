@@ -148,7 +148,7 @@ def test_scan_entry_points_refuse(L):
     need = lib.pal_scan_fwd_workspace_bytes(_scan_dims(L, **long))
     assert need > 0 and lib.pal_scan_fwd_workspace_bytes(_scan_dims(L)) == 0
     assert fwd(_scan_dims(L, **long)) == L.PAL_E_WORKSPACE and fwd(_scan_dims(L, **long), P, need - 1) == L.PAL_E_WORKSPACE
-    assert lib.pal_scan_checkpoint_bytes(_scan_dims(L)) == 2 * 4096 and lib.pal_scan_checkpoint_bytes(_scan_dims(L, state=99)) == 0
+    assert lib.pal_scan_checkpoint_bytes(_scan_dims(L)) == 2 * 2 * 4096 and lib.pal_scan_checkpoint_bytes(_scan_dims(L, state=99)) == 0
     g = dict(dy=P, du=P, ddelta=P, dA=P, dB=P, dC=P)
     bwd = lambda g, ws=P, n=1 << 30, **kw: lib.pal_scan_bwd(_scan_dims(L), L.PalScanTensors(**{**t, "checkpoints": P, **kw}), L.PalScanGrads(**g), ws, n, None)  # noqa: E731
     assert bwd(g, checkpoints=None) == L.PAL_E_NULL and bwd({**g, "dA": None}) == L.PAL_E_NULL
