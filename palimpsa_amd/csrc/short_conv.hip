@@ -60,95 +60,127 @@ struct ConvRun {
   }
 };
 
-// VW neighbouring channels: pieces of eight for bf16 rows in the forward, of four elsewhere
+// VW neighbouring channels as fetched: eight of bf16 rows in the forward, four elsewhere (eight would leave the backward two
+// waves a SIMD), one where there are fewer channels than that.  The last piece of a row whose channels are no multiple of VW is moved back
+// to be whole: its first channels are computed twice, and written twice with the same values.
 template <typename T, int VW>
 struct Chans;
 template <typename T>
 struct Chans<T, 8> {
   Piece8<T> v;
-  __device__ __forceinline__ void load(const T* p, int n) { load_piece(v, p, n); }
+  __device__ __forceinline__ void load(const T* p) { v.load(p); }
   __device__ __forceinline__ float get(int e) const { return v.get(e); }
 };
 template <>
 struct Chans<bf16_t, 4> {
   typedef bf16x4 any __attribute__((aligned(2)));
   bf16x4 v;
-  __device__ __forceinline__ void load(const bf16_t* p, int n) {
-    if (n >= 4) {
-      v = *(const any*)p;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = e < n ? p[e] : (bf16_t)0.f;
-    }
-  }
+  __device__ __forceinline__ void load(const bf16_t* p) { v = *(const any*)p; }
   __device__ __forceinline__ float get(int e) const { return (float)v[e]; }
 };
 template <>
 struct Chans<float, 4> {
   f32x4 v;
-  __device__ __forceinline__ void load(const float* p, int n) {
-    if (n >= 4) {
-      v = *(const f32x4_any*)p;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = e < n ? p[e] : 0.f;
-    }
-  }
+  __device__ __forceinline__ void load(const float* p) { v = *(const f32x4_any*)p; }
   __device__ __forceinline__ float get(int e) const { return v[e]; }
 };
+template <typename T>
+struct Chans<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ float get(int) const { return to_f32(v); }
+};
 template <int VW>
-__device__ __forceinline__ void store_chans(bf16_t* p, const float* x, int n) {
+__device__ __forceinline__ void store_chans(bf16_t* p, const float* x) {
   if constexpr (VW == 8) {
-    store_piece(p, x, n);
-  } else if (n >= 4) {
+    store_piece(p, x, 8);
+  } else if constexpr (VW == 4) {
     typedef bf16x4 any __attribute__((aligned(2)));
     const bf16x2 a = pack2(x[0], x[1]), b = pack2(x[2], x[3]);
     const bf16x4 v = {a[0], a[1], b[0], b[1]};
     *(any*)p = v;
   } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < n) p[e] = (bf16_t)x[e];
+    *p = (bf16_t)x[0];
   }
 }
 template <int VW>
-__device__ __forceinline__ void store_chans(float* p, const float* x, int n) {
-  if (n >= 4) {
+__device__ __forceinline__ void store_chans(float* p, const float* x) {
+  if constexpr (VW == 4) {
     const f32x4 v = {x[0], x[1], x[2], x[3]};
     *(f32x4_any*)p = v;
   } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < n) p[e] = x[e];
+    *p = x[0];
   }
 }
 
-template <int W, int VW>
-__device__ __forceinline__ void load_taps(float (*w)[VW], float* bias, const ConvArgs& a, int c, int n) {
+// n consecutive parameters of either type; whichever it is, they are waited for in their branch (where the two meet, the compiler
+// would wait for everything in flight)
+template <int N>
+__device__ __forceinline__ void load_run(float* x, const void* p, int64_t i, int is_bf16) {
+  if (is_bf16) {
+    const bf16_t* q = (const bf16_t*)p + i;
+    if constexpr (N % 4 == 0) {
+      typedef bf16x4 any __attribute__((aligned(2)));
 #pragma unroll
-  for (int e = 0; e < VW; ++e) {
+      for (int k = 0; k < N; k += 4) {
+        const bf16x4 v = *(const any*)(q + k);
 #pragma unroll
-    for (int k = 0; k < W; ++k) w[k][e] = e < n ? load_rt(a.weight, (int64_t)(c + e) * W + k, a.weight_bf16) : 0.f;
-    bias[e] = a.bias && e < n ? load_rt(a.bias, c + e, a.weight_bf16) : 0.f;
-  }
-}
-// the W - 1 inputs before token t: rows of the sequence, or the state it starts with, or zero; h[0] the oldest
-template <typename T, int W, int VW>
-__device__ __forceinline__ void load_before(float (*h)[VW], const ConvArgs& a, const ConvRun& r, int64_t t, int c, int n) {
-#pragma unroll
-  for (int k = 0; k < W - 1; ++k) {
-    const int64_t tk = t - (W - 1) + k;
-    if (tk >= r.s0) {
-      Chans<T, VW> x;
-      x.load((const T*)a.x + r.at(a, tk) + c, n);
-#pragma unroll
-      for (int e = 0; e < VW; ++e) h[k][e] = x.get(e);
+        for (int e = 0; e < 4; ++e) x[k + e] = (float)v[e];
+      }
     } else {
-      const int slot = (int)(tk - r.s0) + W;   // 1 .. W - 1
 #pragma unroll
-      for (int e = 0; e < VW; ++e) h[k][e] = a.init && e < n ? to_f32(((const T*)a.init)[((int64_t)r.seq * a.D + c + e) * W + slot]) : 0.f;
+      for (int k = 0; k < N; ++k) x[k] = (float)q[k];
+    }
+  } else {
+    const float* q = (const float*)p + i;
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+      for (int k = 0; k < N; k += 4) {
+        const f32x4 v = *(const f32x4_any*)(q + k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[k + e] = v[e];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[k] = q[k];
     }
   }
+#pragma unroll
+  for (int k = 0; k < N; ++k) asm volatile("" : "+v"(x[k]));
+}
+template <int W, int VW>
+__device__ __forceinline__ void load_taps(float (*w)[VW], float* bias, const ConvArgs& a, int c) {
+  float x[VW * W];
+  load_run<VW * W>(x, a.weight, (int64_t)c * W, a.weight_bf16);
+#pragma unroll
+  for (int e = 0; e < VW; ++e) {
+    bias[e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) w[k][e] = x[e * W + k];
+  }
+  if (a.bias) load_run<VW>(bias, a.bias, c, a.weight_bf16);
+}
+// the W - 1 inputs before the run: rows of the sequence, or the state it starts with, or zero; h[0] the oldest
+template <typename T, int W, int VW>
+__device__ __forceinline__ void load_before(float (*h)[VW], const ConvArgs& a, const ConvRun& r, int c) {
+  if (r.t0 > r.s0) {       // (a run that is not the first has a whole run before it, at least 8 tokens)
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) {
+      Chans<T, VW> x;
+      x.load((const T*)a.x + r.at(a, r.t0 - (W - 1) + k) + c);
+#pragma unroll
+      for (int e = 0; e < VW; ++e) h[k][e] = x.get(e);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+      for (int e = 0; e < VW; ++e) h[k][e] = a.init ? to_f32(((const T*)a.init)[((int64_t)r.seq * a.D + c + e) * W + k + 1]) : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < W - 1; ++k)
+#pragma unroll
+    for (int e = 0; e < VW; ++e) asm volatile("" : "+v"(h[k][e]));
 }
 
 // final states: the last W inputs of a sequence, its old state moved up where it is shorter
@@ -174,7 +206,7 @@ __device__ __forceinline__ void conv_states(const ConvArgs& a, int W, int block)
   }
 }
 
-constexpr int kConvBatch = 4;   // rows fetched before the first of them is used
+constexpr int kConvBatch = 4;   // rows fetched together, one batch ahead
 
 template <typename T, int W, int VW>
 __global__ __launch_bounds__(256) void short_conv_fwd_kernel(ConvArgs a) {
@@ -183,49 +215,58 @@ __global__ __launch_bounds__(256) void short_conv_fwd_kernel(ConvArgs a) {
     return;
   }
   const unsigned idx = blockIdx.x * 256u + threadIdx.x;
-  const int run = idx / a.pieces, c = (int)(idx - (unsigned)run * a.pieces) * VW;
+  const int run = idx / a.pieces, c = min((int)(idx - (unsigned)run * a.pieces) * VW, a.D - VW);
   if (run >= a.runs) return;
   const ConvRun r(a, run);
   if (r.t0 >= r.t1) return;
-  const int n = a.D - c;
-  float w[W][VW], bias[VW], h[W][VW];
-  load_taps<W, VW>(w, bias, a, c, n);
-  load_before<T, W, VW>(h, a, r, r.t0, c, n);
+  const int len = (int)(r.t1 - r.t0);
   const T* px = (const T*)a.x + r.at(a, r.t0) + c;
   T* py = (T*)a.y + r.t0 * a.D + c;
-  const int len = (int)(r.t1 - r.t0);
-  for (int tb = 0; tb < len; tb += kConvBatch) {
-    Chans<T, VW> xb[kConvBatch];
+  Chans<T, VW> xb[kConvBatch];
 #pragma unroll
-    for (int u = 0; u < kConvBatch; ++u) xb[u].load(px + (int64_t)min(tb + u, len - 1) * a.xt, n);
+  for (int u = 0; u < kConvBatch; ++u) xb[u].load(px + (int64_t)min(u, len - 1) * a.xt);
+  float w[W][VW], bias[VW], h[W][VW];
+  load_taps<W, VW>(w, bias, a, c);
+  load_before<T, W, VW>(h, a, r, c);
+  auto one = [&](const Chans<T, VW>& x, T* to) {
+    float p[VW];
 #pragma unroll
-    for (int u = 0; u < kConvBatch; ++u) {
-      if (tb + u >= len) break;
-      float p[VW];
+    for (int e = 0; e < VW; ++e) {
+      h[W - 1][e] = x.get(e);
+      p[e] = bias[e];
 #pragma unroll
-      for (int e = 0; e < VW; ++e) {
-        h[W - 1][e] = xb[u].get(e);
-        p[e] = bias[e];
+      for (int k = 0; k < W; ++k) p[e] = fmaf(w[k][e], h[k][e], p[e]);
 #pragma unroll
-        for (int k = 0; k < W; ++k) p[e] = fmaf(w[k][e], h[k][e], p[e]);
-        if (a.silu) p[e] *= logistic(p[e]);
-#pragma unroll
-        for (int k = 0; k < W - 1; ++k) h[k][e] = h[k + 1][e];
-      }
-      store_chans<VW>(py + (int64_t)(tb + u) * a.D, p, n);
+      for (int k = 0; k < W - 1; ++k) h[k][e] = h[k + 1][e];
     }
+    if (a.silu)
+#pragma unroll
+      for (int e = 0; e < VW; ++e) p[e] *= logistic(p[e]);
+    store_chans<VW>(to, p);
+  };
+  int tb = 0;
+  for (; tb + kConvBatch <= len; tb += kConvBatch) {
+    Chans<T, VW> next[kConvBatch];
+#pragma unroll
+    for (int u = 0; u < kConvBatch; ++u) next[u].load(px + (int64_t)min(tb + kConvBatch + u, len - 1) * a.xt);
+#pragma unroll
+    for (int u = 0; u < kConvBatch; ++u) one(xb[u], py + (int64_t)(tb + u) * a.D);
+#pragma unroll
+    for (int u = 0; u < kConvBatch; ++u) xb[u] = next[u];
   }
+#pragma unroll
+  for (int u = 0; u < kConvBatch - 1; ++u)
+    if (tb + u < len) one(xb[u], py + (int64_t)(tb + u) * a.D);
 }
 
 // workgroups: (group of 4 runs, 64 pieces of channels), the pieces of a group next to each other; a wave walks one run, the
 // four waves' shares of dw and dbias meet in LDS
-template <typename T, int W>
+template <typename T, int W, int VW>
 __global__ __launch_bounds__(256) void short_conv_bwd_kernel(ConvArgs a) {
-  constexpr int VW = 4;
-  __shared__ float sW[4][W + 1][64 * VW + 4];
+  __shared__ __attribute__((aligned(16))) float sW[4][W + 1][64 * VW + 4];
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int spans = (a.pieces + 63) / 64, group = blockIdx.x / spans, span = blockIdx.x - group * spans;
-  const int c = (span * 64 + lane) * VW, n = a.D - c;
+  const int piece = span * 64 + lane, c = min(piece * VW, a.D - VW);
   const int run = group * 4 + wave;
   float dw[W][VW], db[VW];
 #pragma unroll
@@ -234,89 +275,127 @@ __global__ __launch_bounds__(256) void short_conv_bwd_kernel(ConvArgs a) {
 #pragma unroll
     for (int k = 0; k < W; ++k) dw[k][e] = 0.f;
   }
-  if (run < a.runs && n > 0) {
+  if (run < a.runs && piece < a.pieces) {
     const ConvRun r(a, run);
     if (r.t0 < r.t1) {
+      const T* px = (const T*)a.x + r.at(a, r.t0) + c;
+      const T* pg = (const T*)a.dy + r.t0 * a.D + c;
+      T* pd = (T*)a.dx + r.t0 * a.D + c;
+      const int len = (int)(r.t1 - r.t0), left = (int)min(r.s1 - r.t0, (int64_t)len + W - 1);   // tokens to walk, past the run
+      const bool first = r.t0 == r.s0;
+      struct Pair {
+        Chans<T, VW> x, g;
+      };
+      auto fetch = [&](Pair& b, int t) {
+        const int64_t at = min(t, left - 1);
+        b.x.load(px + at * a.xt);
+        b.g.load(pg + at * a.D);
+      };
+      Pair pb[W - 1], mb[kConvBatch];
+#pragma unroll
+      for (int u = 0; u < W - 1; ++u) fetch(pb[u], u);
+#pragma unroll
+      for (int u = 0; u < kConvBatch; ++u) fetch(mb[u], W - 1 + u);
       float w[W][VW], bias[VW], h[W][VW], dp[W][VW];   // dp[k]: token t - (W - 1) + k
-      load_taps<W, VW>(w, bias, a, c, n);
-      load_before<T, W, VW>(h, a, r, r.t0, c, n);
+      load_taps<W, VW>(w, bias, a, c);
+      load_before<T, W, VW>(h, a, r, c);
 #pragma unroll
       for (int e = 0; e < VW; ++e)
 #pragma unroll
         for (int k = 0; k < W; ++k) dp[k][e] = 0.f;
-      const T* px = (const T*)a.x + r.at(a, r.t0) + c;
-      const T* pg = (const T*)a.dy + r.t0 * a.D + c;
-      const int len = (int)(r.t1 - r.t0), left = (int)min(r.s1 - r.t0, (int64_t)len + W - 1);   // tokens to walk, past the run
-      const bool first = r.t0 == r.s0;
-      for (int tb = 0; tb < len + W - 1; tb += kConvBatch) {
-        Chans<T, VW> xb[kConvBatch], gb[kConvBatch];
+      // takes token t in; dx: the gradient of token t - (W - 1), which is whole now.  in: the token is one of the sequence; own: of the run
+      auto one = [&](const Pair& b, bool in, bool own, float* dx) {
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+          h[W - 1][e] = b.x.get(e);
+          float p = bias[e];
+#pragma unroll
+          for (int k = 0; k < W; ++k) p = fmaf(w[k][e], h[k][e], p);
+          float g = b.g.get(e);
+          if (a.silu) {
+            const float s = logistic(p);
+            g *= s + p * s * (1.f - s);
+          }
+          g = in ? g : 0.f;
+          dp[W - 1][e] = g;
+          dx[e] = 0.f;
+#pragma unroll
+          for (int k = 0; k < W; ++k) dx[e] = fmaf(w[W - 1 - k][e], dp[k][e], dx[e]);
+          const float go = own ? g : 0.f;
+          db[e] += go;
+#pragma unroll
+          for (int k = 0; k < W; ++k) dw[k][e] = own ? fmaf(go, h[k][e], dw[k][e]) : dw[k][e];
+#pragma unroll
+          for (int k = 0; k < W - 1; ++k) { h[k][e] = h[k + 1][e]; dp[k][e] = dp[k + 1][e]; }
+        }
+      };
+      // what came back through the final state, where token r.t0 + t is one of the last W
+      auto with_final = [&](int t, float* dx) {
+        const int64_t slot = r.t0 + t - r.s1 + W;
+        if (a.d_final && slot >= 0)
+#pragma unroll
+          for (int e = 0; e < VW; ++e) {
+            float d = to_f32(((const T*)a.d_final)[((int64_t)r.seq * a.D + c + e) * W + slot]);
+            asm volatile("" : "+v"(d));
+            dx[e] += d;
+          }
+      };
+      float dx[VW];
+#pragma unroll
+      for (int t = 0; t < W - 1; ++t) {
+        one(pb[t], t < left, t < len, dx);
+        if (first && a.d_init) {     // the gradient of the state's input t + 1 (the oldest, 0, meets no tap)
+          with_final(t - (W - 1), dx);
+#pragma unroll
+          for (int e = 0; e < VW; ++e) {
+            T* d = (T*)a.d_init + ((int64_t)r.seq * a.D + c + e) * W;
+            d[t + 1] = from_f32<T>(dx[e]);
+            if (t == 0) d[0] = (T)0.f;
+          }
+        }
+      }
+      int tb = W - 1;
+      for (; tb + kConvBatch <= len; tb += kConvBatch) {
+        Pair next[kConvBatch];
+#pragma unroll
+        for (int u = 0; u < kConvBatch; ++u) fetch(next[u], tb + kConvBatch + u);
 #pragma unroll
         for (int u = 0; u < kConvBatch; ++u) {
-          const int64_t t = min(tb + u, left - 1);
-          xb[u].load(px + t * a.xt, n);
-          gb[u].load(pg + t * a.D, n);
+          one(mb[u], true, true, dx);
+          with_final(tb + u - (W - 1), dx);
+          store_chans<VW>(pd + (int64_t)(tb + u - (W - 1)) * a.D, dx);
         }
+#pragma unroll
+        for (int u = 0; u < kConvBatch; ++u) mb[u] = next[u];
+      }
+      // the last tokens of the run, and the W - 1 behind it
+      for (; tb < len + W - 1; tb += kConvBatch) {
+        Pair next[kConvBatch];
+        if (tb + kConvBatch < len + W - 1)
+#pragma unroll
+          for (int u = 0; u < kConvBatch; ++u) fetch(next[u], tb + kConvBatch + u);
 #pragma unroll
         for (int u = 0; u < kConvBatch; ++u) {
           const int t = tb + u;
           if (t >= len + W - 1) break;
-          const bool in = t < left, own = t < len;
-          float dx[VW];
-#pragma unroll
-          for (int e = 0; e < VW; ++e) {
-            h[W - 1][e] = xb[u].get(e);
-            float p = bias[e];
-#pragma unroll
-            for (int k = 0; k < W; ++k) p = fmaf(w[k][e], h[k][e], p);
-            float g = in ? gb[u].get(e) : 0.f;
-            if (a.silu) {
-              const float s = logistic(p);
-              g = in ? g * (s + p * s * (1.f - s)) : 0.f;
-            }
-            dp[W - 1][e] = g;
-            dx[e] = 0.f;
-#pragma unroll
-            for (int k = 0; k < W; ++k) dx[e] = fmaf(w[W - 1 - k][e], dp[k][e], dx[e]);
-            if (own) {
-              db[e] += g;
-#pragma unroll
-              for (int k = 0; k < W; ++k) dw[k][e] = fmaf(g, h[k][e], dw[k][e]);
-            }
-#pragma unroll
-            for (int k = 0; k < W - 1; ++k) { h[k][e] = h[k + 1][e]; dp[k][e] = dp[k + 1][e]; }
-          }
-          const int64_t to = r.t0 + t - (W - 1);   // the token whose gradient is whole now
-          if (to < r.t0 && !(first && a.d_init)) continue;
-          const int64_t slot = to - r.s1 + W;      // its column of the final state, if it is there
-          if (a.d_final && slot >= 0)
-#pragma unroll
-            for (int e = 0; e < VW; ++e)
-              if (e < n) dx[e] += to_f32(((const T*)a.d_final)[((int64_t)r.seq * a.D + c + e) * W + slot]);
-          if (to >= r.t0) {
-            store_chans<VW>((T*)a.dx + to * a.D + c, dx, n);
-          } else {
-#pragma unroll
-            for (int e = 0; e < VW; ++e)
-              if (e < n) {
-                T* d = (T*)a.d_init + ((int64_t)r.seq * a.D + c + e) * W;
-                d[to - r.s0 + W] = from_f32<T>(dx[e]);
-                if (t == 0) d[0] = (T)0.f;         // the oldest input of the state meets no tap
-              }
-          }
+          one(mb[u], t < left, t < len, dx);
+          with_final(t - (W - 1), dx);
+          store_chans<VW>(pd + (int64_t)(t - (W - 1)) * a.D, dx);
         }
+#pragma unroll
+        for (int u = 0; u < kConvBatch; ++u) mb[u] = next[u];
       }
     }
   }
 #pragma unroll
-  for (int k = 0; k <= W; ++k) {
-    const f32x4 x = k < W ? (f32x4){dw[k < W ? k : 0][0], dw[k < W ? k : 0][1], dw[k < W ? k : 0][2], dw[k < W ? k : 0][3]}
-                          : (f32x4){db[0], db[1], db[2], db[3]};
-    *(f32x4*)&sW[wave][k][VW * lane] = x;
-  }
+  for (int k = 0; k <= W; ++k)
+#pragma unroll
+    for (int e = 0; e < VW; ++e) sW[wave][k][VW * lane + e] = k < W ? dw[k < W ? k : 0][e] : db[e];
   __syncthreads();
-  for (int i = threadIdx.x; i < (W + 1) * 256; i += 256) {
-    const int k = i >> 8, cc = i & 255, ch = span * 256 + cc;
-    if (ch < a.D) a.part[((int64_t)group * (W + 1) + k) * a.D + ch] = sW[0][k][cc] + sW[1][k][cc] + sW[2][k][cc] + sW[3][k][cc];
+  for (int i = threadIdx.x; i < (W + 1) * 64 * VW; i += 256) {
+    const int k = i / (64 * VW), cc = i - k * (64 * VW), pc = span * 64 + cc / VW;
+    if (pc < a.pieces)
+      a.part[((int64_t)group * (W + 1) + k) * a.D + min(pc * VW, a.D - VW) + cc % VW] = sW[0][k][cc] + sW[1][k][cc] + sW[2][k][cc] + sW[3][k][cc];
   }
 }
 
@@ -424,6 +503,11 @@ static void conv_runs(ConvArgs& a, const PalConvDims* d, int vw) {
   a.runs = a.per_tile * (a.cu ? a.chunks : d->batch);
 }
 
+// channels per thread
+static int conv_piece(const PalConvDims* d, bool bwd) {
+  const int vw = d->dtype == PAL_DTYPE_BF16 && !bwd ? 8 : 4;
+  return d->channels >= vw ? vw : 1;
+}
 template <typename T, int VW>
 static void conv_fwd_launch(const ConvArgs& a, int W, int grid, hipStream_t s) {
 #define PAL_CONV(W_)                                                                                                     \
@@ -433,10 +517,10 @@ static void conv_fwd_launch(const ConvArgs& a, int W, int grid, hipStream_t s) {
   switch (W) { PAL_CONV(2) PAL_CONV(3) PAL_CONV(4) PAL_CONV(5) PAL_CONV(6) PAL_CONV(7) PAL_CONV(8) }
 #undef PAL_CONV
 }
-template <typename T>
+template <typename T, int VW>
 static void conv_bwd_launch(const ConvArgs& a, int W, dim3 grid, hipStream_t s) {
 #define PAL_CONV(W_)                                                                                            \
-  case W_: PAL_TIMED_LAUNCH(kKernShortConvBwd, s, (short_conv_bwd_kernel<T, W_>), grid, dim3(256), 0, s, a); break;
+  case W_: PAL_TIMED_LAUNCH(kKernShortConvBwd, s, (short_conv_bwd_kernel<T, W_, VW>), grid, dim3(256), 0, s, a); break;
   switch (W) { PAL_CONV(2) PAL_CONV(3) PAL_CONV(4) PAL_CONV(5) PAL_CONV(6) PAL_CONV(7) PAL_CONV(8) }
 #undef PAL_CONV
 }
@@ -463,15 +547,15 @@ extern "C" int pal_short_conv_fwd(const PalConvDims* d, const PalConvTensors* t,
   if (int rc = check_conv_seqs(d, t)) return rc;
   if (((d->flags & PAL_FLAG_STORE_FINAL) != 0) != (t->final_ != nullptr)) return PAL_E_STATE;
   ConvArgs a = conv_args(d, t);
-  const int vw = d->dtype == PAL_DTYPE_BF16 ? 8 : 4;
+  const int vw = conv_piece(d, false);
   conv_runs(a, d, vw);
   const int64_t threads = (int64_t)a.runs * a.pieces;
   if (threads > (int64_t)1 << 31) return PAL_E_DIM;
   a.blocks = (int)((threads + 255) / 256);
   const int grid = a.blocks + (t->final_ ? conv_state_blocks(d) : 0);
   hipStream_t s = (hipStream_t)stream;
-  if (d->dtype == PAL_DTYPE_BF16) conv_fwd_launch<bf16_t, 8>(a, d->width, grid, s);
-  else conv_fwd_launch<float, 4>(a, d->width, grid, s);
+  if (d->dtype == PAL_DTYPE_BF16) vw == 8 ? conv_fwd_launch<bf16_t, 8>(a, d->width, grid, s) : conv_fwd_launch<bf16_t, 1>(a, d->width, grid, s);
+  else vw == 4 ? conv_fwd_launch<float, 4>(a, d->width, grid, s) : conv_fwd_launch<float, 1>(a, d->width, grid, s);
   PAL_HIP_LAUNCH_CHECK();
   return PAL_OK;
 }
@@ -483,7 +567,7 @@ extern "C" size_t pal_short_conv_bwd_workspace_bytes(const PalConvDims* d) {
   if (check_conv(d, &any) != PAL_OK) return 0;
   if (d->flags & PAL_FLAG_VARLEN) any.cu_seqlens = (const int32_t*)d;
   ConvArgs a = conv_args(d, &any);
-  conv_runs(a, d, 4);
+  conv_runs(a, d, conv_piece(d, true));
   return sizeof(float) * (size_t)conv_groups(a) * (d->width + 1) * d->channels;
 }
 
@@ -496,7 +580,8 @@ extern "C" int pal_short_conv_bwd(const PalConvDims* d, const PalConvTensors* t,
   if (gr->d_init && !t->init) return PAL_E_STATE;
   if (!workspace || workspace_bytes < pal_short_conv_bwd_workspace_bytes(d)) return PAL_E_WORKSPACE;
   ConvArgs a = conv_args(d, t);
-  conv_runs(a, d, 4);
+  const int vw = conv_piece(d, true);
+  conv_runs(a, d, vw);
   a.dy = gr->dy; a.dx = gr->dx; a.dweight = gr->dweight; a.dbias = gr->dbias; a.d_init = gr->d_init; a.d_final = gr->d_final;
   a.part = (float*)workspace;
   const int groups = conv_groups(a);
@@ -504,8 +589,8 @@ extern "C" int pal_short_conv_bwd(const PalConvDims* d, const PalConvTensors* t,
   if (blocks > (int64_t)1 << 31) return PAL_E_DIM;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)blocks);
-  if (d->dtype == PAL_DTYPE_BF16) conv_bwd_launch<bf16_t>(a, d->width, grid, s);
-  else conv_bwd_launch<float>(a, d->width, grid, s);
+  if (d->dtype == PAL_DTYPE_BF16) vw == 4 ? conv_bwd_launch<bf16_t, 4>(a, d->width, grid, s) : conv_bwd_launch<bf16_t, 1>(a, d->width, grid, s);
+  else vw == 4 ? conv_bwd_launch<float, 4>(a, d->width, grid, s) : conv_bwd_launch<float, 1>(a, d->width, grid, s);
   PAL_HIP_LAUNCH_CHECK();
   const int sums = (int)(((int64_t)(d->width + 1) * a.D + 63) / 64), more = a.cu && a.d_init ? conv_state_blocks(d) : 0;
   if (d->dtype == PAL_DTYPE_BF16)
