@@ -224,6 +224,9 @@ def _check_host(ext) -> None:
 
     want = (PAL_ABI_VERSION, C.sizeof(PalDims), C.sizeof(PalFwdTensors), C.sizeof(PalBwdTensors))
     have = tuple(getattr(ext, "abi", ()))
+    want += tuple(C.sizeof(t) for t in (PalNormDims, PalNormTensors, PalNormGrads, PalConvDims, PalConvTensors, PalConvGrads,
+                                        PalScanDims, PalScanTensors, PalScanGrads))
+    have += tuple(getattr(ext, "abi_block", ()))
     built = getattr(ext, "torch_version", None)
     if have != want or built != torch.__version__:
         raise ImportError(
@@ -250,7 +253,11 @@ def host():
 
 # the library's functions that the extension module calls, in the order of its table
 _HOST_FUNCTIONS = ("pal_recurrent_fwd", "pal_gla_recurrent_fwd", "pal_chunk_fwd", "pal_chunk_bwd",
-                   "pal_chunk_bwd_workspace_bytes", "pal_chunk_bwd_supported")
+                   "pal_chunk_bwd_workspace_bytes", "pal_chunk_bwd_supported",
+                   "pal_residual_norm_fwd", "pal_residual_norm_bwd", "pal_residual_norm_bwd_workspace_bytes",
+                   "pal_short_conv_fwd", "pal_short_conv_bwd", "pal_short_conv_bwd_workspace_bytes", "pal_short_conv_step",
+                   "pal_scan_fwd", "pal_scan_fwd_workspace_bytes", "pal_scan_checkpoint_bytes", "pal_scan_bwd",
+                   "pal_scan_bwd_workspace_bytes")
 
 
 # How the chunked entry points build the tile-start states (PAL_FLAG_STATES_* of the C ABI): 0 = chosen by shape,

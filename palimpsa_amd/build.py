@@ -104,7 +104,7 @@ def build_host(force: bool = False) -> str:
     """Compile the extension module of the native host path (host code only, against the installed torch)."""
     import torch
 
-    deps = [HOST_SRC, os.path.join(os.path.dirname(PKG_DIR), "include", "palimpsa_hip.h")]
+    deps = [HOST_SRC, os.path.join(CSRC, "host_block.h"), os.path.join(os.path.dirname(PKG_DIR), "include", "palimpsa_hip.h")]
     stamp = _host_stamp()
     if (not force and os.path.exists(HOST_PATH) and os.path.exists(HOST_STAMP) and open(HOST_STAMP).read() == stamp
             and os.path.getmtime(HOST_PATH) >= max(os.path.getmtime(p) for p in deps)):

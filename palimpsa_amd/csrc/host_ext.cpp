@@ -11,6 +11,7 @@
 #include <Python.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -33,6 +34,18 @@ struct Abi {
   int (*chunk_bwd)(const PalDims*, const PalFwdTensors*, const PalBwdTensors*, void*, size_t, void*);
   size_t (*chunk_bwd_workspace_bytes)(const PalDims*);
   int (*chunk_bwd_supported)(int32_t, int32_t, int32_t, uint32_t);
+  int (*residual_norm_fwd)(const PalNormDims*, const PalNormTensors*, void*);
+  int (*residual_norm_bwd)(const PalNormDims*, const PalNormTensors*, const PalNormGrads*, void*, size_t, void*);
+  size_t (*residual_norm_bwd_workspace_bytes)(const PalNormDims*);
+  int (*short_conv_fwd)(const PalConvDims*, const PalConvTensors*, void*);
+  int (*short_conv_bwd)(const PalConvDims*, const PalConvTensors*, const PalConvGrads*, void*, size_t, void*);
+  size_t (*short_conv_bwd_workspace_bytes)(const PalConvDims*);
+  int (*short_conv_step)(const PalConvDims*, const PalConvTensors*, void*);
+  int (*scan_fwd)(const PalScanDims*, const PalScanTensors*, void*, size_t, void*);
+  size_t (*scan_fwd_workspace_bytes)(const PalScanDims*);
+  size_t (*scan_checkpoint_bytes)(const PalScanDims*);
+  int (*scan_bwd)(const PalScanDims*, const PalScanTensors*, const PalScanGrads*, void*, size_t, void*);
+  size_t (*scan_bwd_workspace_bytes)(const PalScanDims*);
 } abi;
 py::handle raise_code;   // (code, where): raises what the Python routes raise for a code of the library
 
@@ -338,14 +351,24 @@ py::object chunk_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   return py::make_tuple(out.o, var ? py::cast(out.ov) : py::none(), out.fm, out.fI);
 }
 
+#include "host_block.h"
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
   // what this module was built from; the loader compares it before it binds the library
   m.attr("abi") = py::make_tuple(PAL_ABI_VERSION, sizeof(PalDims), sizeof(PalFwdTensors), sizeof(PalBwdTensors));
+  m.attr("abi_block") = py::make_tuple(sizeof(PalNormDims), sizeof(PalNormTensors), sizeof(PalNormGrads), sizeof(PalConvDims), sizeof(PalConvTensors),
+                                       sizeof(PalConvGrads), sizeof(PalScanDims), sizeof(PalScanTensors), sizeof(PalScanGrads));
   m.attr("torch_version") = PAL_TORCH_VERSION;
   m.def("bind", &bind);
   m.def("recurrent_fwd", &recurrent_fwd);
   m.def("gla_recurrent_fwd", &gla_recurrent_fwd);
   m.def("chunk_fwd", &chunk_fwd);
+  m.def("residual_norm", &block::residual_norm);
+  m.def("residual_norm_fp8", &block::residual_norm_fp8);
+  m.def("short_conv", &block::short_conv);
+  m.def("short_conv_step", &block::short_conv_step);
+  m.def("selective_scan", &block::selective_scan);
+  m.def("selective_scan_step", &block::selective_scan_step);
 }

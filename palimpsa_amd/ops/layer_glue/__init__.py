@@ -449,7 +449,6 @@ class ResidualRmsNorm(torch.autograd.Function):
         return dx.to(dt[0]), None if dt[1] is None else d_res.to(dt[1]), dw.to(dt[2]), None, None
 
 
-@cm.no_compile
 def residual_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-5,
                       residual_in_fp32: bool = False):
     """``s = x + residual``, ``y = s * rsqrt(mean(s ** 2) + eps) * weight``; returns ``(y, s)``: the block's input and the residual
@@ -457,17 +456,34 @@ def residual_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight:
 
     y has the type of x; s is bf16 where x and residual are bf16 and ``residual_in_fp32`` is not set, else fp32 (bf16 rows beside an
     fp32 stream are the usual choice for deep models).  The norm is that of s as it is handed on.  Gradients for x, residual and weight."""
+    if not torch.compiler.is_compiling() and x.is_cuda:
+        r = L.host().residual_norm(x, residual, weight, eps, residual_in_fp32)
+        if r is not None:
+            return r
+    return _residual_rms_norm(x, residual, weight, eps, residual_in_fp32)
+
+
+@cm.no_compile
+def _residual_rms_norm(x, residual, weight, eps, residual_in_fp32):
     cm._require_gpu(x, residual, weight)
     return ResidualRmsNorm.apply(x, residual, weight, eps, residual_in_fp32)
 
 
-@cm.no_compile
 def residual_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, eps: float = 1e-5,
                           group_size: Optional[int] = None, residual_in_fp32: bool = False):
     """``residual_rms_norm`` with y in 8 bits for a projection that takes such rows; returns ``(q, scales, s)`` with ``y = q * scales``:
     q ``[.., D]`` ``torch.float8_e4m3fn``, scales fp32 ``[.., D / group_size]``, one for each group of ``group_size`` entries (32, 64, 128
     or 256, a divisor of D), or ``[.., 1]``, one for the row (``group_size`` None).  A scale is the largest absolute y of its group (at least
     1e-12) over 448.  A row whose sum of squares is not a finite number has NaN scales.  No gradients: call it under ``torch.no_grad()``."""
+    if not torch.compiler.is_compiling() and x.is_cuda and group_size in (None, 32, 64, 128, 256):
+        r = L.host().residual_norm_fp8(x, residual, weight, eps, residual_in_fp32, group_size or 0)
+        if r is not None:
+            return r
+    return _residual_rms_norm_fp8(x, residual, weight, eps, group_size, residual_in_fp32)
+
+
+@cm.no_compile
+def _residual_rms_norm_fp8(x, residual, weight, eps, group_size, residual_in_fp32):
     cm._require_gpu(x, residual, weight)
     if cm.wants_grad(x, residual, weight):
         raise ValueError("residual_rms_norm_fp8 has no gradient: use residual_rms_norm, or torch.no_grad()")

@@ -279,7 +279,10 @@ def packed_batch(cu_seqlens: torch.Tensor, B: int, T: int, dev: torch.device):
 
 
 def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a derivative of a call on these would be asked for: backward, or forward by a tangent that one of them carries."""
+    from torch.autograd import forward_ad as fw
+    have = [t for t in tensors if t is not None]
+    return (torch.is_grad_enabled() and any(t.requires_grad for t in have)) or any(fw.unpack_dual(t).tangent is not None for t in have)
 
 
 def bump_version(x: torch.Tensor) -> None:

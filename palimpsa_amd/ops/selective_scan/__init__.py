@@ -139,16 +139,29 @@ def _grouped(t: torch.Tensor) -> torch.Tensor:
     return t.unsqueeze(-2) if t.dim() == 3 else t
 
 
-@cm.no_compile
 def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
                    D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None, delta_bias: Optional[torch.Tensor] = None,
                    delta_softplus: bool = True, initial_state: Optional[torch.Tensor] = None, output_final_state: bool = False,
                    cu_seqlens: Optional[torch.Tensor] = None):
     """Selective scan over prompts and training batches; returns ``(y, final_state | None)``.
 
-    u, delta, z ``[B, T, D]`` with at least one token, B, C ``[B, T, N]`` or, for ``G`` groups of channels, ``[B, T, G, N]`` (all bf16, or computed in fp32);
-    A ``[D, N]`` (negative for a decay; up to 64 entries), D, delta_bias ``[D]`` and states ``[N_seqs, D, N]`` in fp32.  Without ``delta_softplus`` the
-    time step is ``delta + delta_bias`` as it is.  ``cu_seqlens`` ``[N_seqs + 1]`` makes the batch one packed row of sequences, some of which may be empty."""
+    u, delta, z ``[B, T, D]`` with at least one token, B, C ``[B, T, N]`` or, for ``G`` groups of channels, ``[B, T, G, N]`` (all
+    bf16, or computed in fp32), slices of wider projections among them; A ``[D, N]`` (negative for a decay; up to 64 entries), D,
+    delta_bias ``[D]`` and states ``[N_seqs, D, N]`` in fp32.  Without ``delta_softplus`` the time step is ``delta + delta_bias`` as
+    it is.  ``cu_seqlens`` ``[N_seqs + 1]`` makes the batch one packed row of sequences, some of which may be empty: each starts
+    from its own state, and an empty one hands its state on.  Gradients for every tensor, through y and the final state."""
+    if not torch.compiler.is_compiling() and u.is_cuda and u.dim() == 3:
+        cu = None
+        if cu_seqlens is not None:
+            cu, _, _, _ = cm.packed_batch(cu_seqlens, u.shape[0], u.shape[1], u.device)
+        r = L.host().selective_scan(u, delta, A, B, C, D, z, delta_bias, bool(delta_softplus), initial_state, output_final_state, cu)
+        if r is not None:
+            return r
+    return _selective_scan(u, delta, A, B, C, D, z, delta_bias, delta_softplus, initial_state, output_final_state, cu_seqlens)
+
+
+@cm.no_compile
+def _selective_scan(u, delta, A, B, C, D, z, delta_bias, delta_softplus, initial_state, output_final_state, cu_seqlens):
     cm._require_gpu(u, delta, A, B, C, D, z, delta_bias, initial_state)
     if u.dim() != 3:
         raise ValueError(f"u must be [B, T, D], got {tuple(u.shape)}")
@@ -156,15 +169,23 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
                                output_final_state, cu_seqlens)
 
 
-@cm.no_compile
 def selective_scan_step(u: torch.Tensor, state: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor,
                         C: torch.Tensor, D: Optional[torch.Tensor] = None, z: Optional[torch.Tensor] = None,
                         delta_bias: Optional[torch.Tensor] = None, delta_softplus: bool = True) -> torch.Tensor:
-    """The next token (u, delta, z ``[B, D]``, B, C ``[B, N]`` or ``[B, G, N]``) or the next few (``[B, T, ..]``) of ``B`` generations;
-    returns y in the shape of u.
+    """The next token (u, delta, z ``[B, D]``, B, C ``[B, N]`` or ``[B, G, N]``) or the next few (``[B, T, ..]``) of ``B``
+    generations; returns y in the shape of u.
 
-    ``state`` ``[B, D, N]`` fp32, packed, is read and written in place.  Nothing but y is allocated, so a step can be
+    ``state`` ``[B, D, N]`` fp32, packed, is read and written in place.  Of one token nothing but y is allocated, so a step can be
     recorded into a HIP graph.  No gradients: call it under ``torch.no_grad()``, or ``selective_scan`` for training."""
+    if not torch.compiler.is_compiling() and u.is_cuda:
+        r = L.host().selective_scan_step(u, state, delta, A, B, C, D, z, delta_bias, bool(delta_softplus))
+        if r is not None:
+            return r
+    return _selective_scan_step(u, state, delta, A, B, C, D, z, delta_bias, delta_softplus)
+
+
+@cm.no_compile
+def _selective_scan_step(u, state, delta, A, B, C, D, z, delta_bias, delta_softplus):
     dev = cm._require_gpu(u, state, delta, A, B, C, D, z, delta_bias)
     if u.dim() not in (2, 3):
         raise ValueError(f"u must be [B, D] or [B, T, D], got {tuple(u.shape)}")

@@ -128,30 +128,50 @@ class ShortConv(torch.autograd.Function):
                 None if d_init is None else d_init.to(dt[3]), None, None)
 
 
-@cm.no_compile
 def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, activation: Optional[str] = "silu",
                initial_state: Optional[torch.Tensor] = None, output_final_state: bool = False,
                cu_seqlens: Optional[torch.Tensor] = None):
     """Causal convolution over time with one filter of ``W`` taps (2 to 8) per channel; returns ``(y, final_state | None)``.
 
-    x ``[B, T, D]`` with at least one token (bf16, or computed in fp32), a slice of a wider projection is read where it is;
-    weight ``[D, W]`` or ``[D, 1, W]``, the last tap meets the token itself; bias ``[D]``; ``activation`` "silu" (or "swish") or None.
-    ``initial_state`` ``[N, D, W]`` holds the ``W`` inputs before the first token, oldest first (the oldest meets no tap; it is
-    there because layers keep it); final states have the same form and the type of x.  ``cu_seqlens`` ``[N + 1]`` makes x one packed row of N sequences, some of which
-    may be empty: each starts from its own state, and an empty one hands its state on."""
+    x ``[B, T, D]`` with at least one token (bf16, or computed in fp32); a slice of a wider projection is read where it is.
+    weight ``[D, W]`` or ``[D, 1, W]``, the last tap meets the token itself; bias ``[D]``; ``activation`` "silu" (or "swish") or
+    None.  ``initial_state`` ``[N, D, W]`` holds the ``W`` inputs before the first token, oldest first (the oldest meets no tap;
+    it is there because layers keep it); final states have the same form and the type of x.  ``cu_seqlens`` ``[N + 1]`` makes x one
+    packed row of N sequences, some of which may be empty: each starts from its own state, and an empty one hands its state on.
+    Gradients for x, weight, bias and initial_state, through y and the final state."""
+    if not torch.compiler.is_compiling() and x.is_cuda and x.dim() == 3 and activation in (None, "silu", "swish"):
+        cu = table = None
+        if cu_seqlens is not None:
+            cu, table, _, _ = cm.packed_batch(cu_seqlens, x.shape[0], x.shape[1], x.device)
+        r = L.host().short_conv(x, weight, bias, activation is not None, initial_state, output_final_state, cu, table)
+        if r is not None:
+            return r
+    return _short_conv(x, weight, bias, activation, initial_state, output_final_state, cu_seqlens)
+
+
+@cm.no_compile
+def _short_conv(x, weight, bias, activation, initial_state, output_final_state, cu_seqlens):
     cm._require_gpu(x, weight, bias, initial_state)
     if x.dim() != 3:
         raise ValueError(f"x must be [B, T, D], got {tuple(x.shape)}")
     return ShortConv.apply(x, weight, bias, _silu(activation), initial_state, output_final_state, cu_seqlens)
 
 
-@cm.no_compile
 def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                     activation: Optional[str] = "silu") -> torch.Tensor:
     """The next token (x ``[B, D]``) or the next few (x ``[B, T, D]``) of ``B`` generations; returns y in the shape of x.
 
     ``state`` ``[B, D, W]``, packed and in the type of x (bf16 or fp32), is read and written in place.  Nothing but y is allocated,
     so a step can be recorded into a HIP graph.  No gradients: call it under ``torch.no_grad()``, or ``short_conv`` for training."""
+    if not torch.compiler.is_compiling() and x.is_cuda and activation in (None, "silu", "swish"):
+        r = L.host().short_conv_step(x, state, weight, bias, activation is not None)
+        if r is not None:
+            return r
+    return _short_conv_step(x, state, weight, bias, activation)
+
+
+@cm.no_compile
+def _short_conv_step(x, state, weight, bias, activation):
     silu = _silu(activation)
     dev = cm._require_gpu(x, state, weight, bias)
     if x.dim() not in (2, 3):
