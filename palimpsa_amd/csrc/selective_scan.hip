@@ -42,7 +42,7 @@ struct ScanArgs {
   const int32_t* cu;
   int64_t ub, db, zb, Bb, Cb;                        // strides between batch rows
   int32_t ut, dt, zt, Bt, Ct;                        // and between tokens (below 2^24)
-  int32_t rows, T, seqs, D_, N, G, per_group, tiles_g, tiles, softplus, vec;
+  int32_t rows, T, seqs, D_, N, G, per_group, tiles_g, tiles, softplus, vec, scalar;
   int32_t seg, segs, ckpts;                          // tokens per segment (a multiple of PAL_SCAN_BLOCK), segments and kept states per row
 };
 
@@ -54,17 +54,28 @@ __device__ __forceinline__ float exp_full(float x) {
   const float e = fast_exp2(t);
   return fmaf(e, r * 0.6931471806f, e);
 }
-// log(1 + e) for e >= 0: the rounding of 1 + e is made up for
+// exp2 of x log2(e): for rows in fp32 made up for as above; rows in bf16 are 2^-9 apart, where the rounding of the exponent
+// (1.3e-6 of the result at |x| = 20, less below) does not count
+template <typename T>
+__device__ __forceinline__ float exp_rows(float x) {
+  if constexpr (std::is_same<T, float>::value) return exp_full(x);
+  else return fast_exp2(x * kLog2e);
+}
+// log(1 + e) for e >= 0.  The rounding of s = 1 + e is made up for: log(1 + e) - log(s) is (e - (s - 1)) / s to first order.  Below s = 2
+// the division changes that by at most 2^-25, half a step of the sum behind it; above, all of it is below 2^-24 and the logarithm
+// above 0.69.  So the difference is taken as it is, and held to the 2^-24 that it has below s = 2.
 __device__ __forceinline__ float log1p_full(float e) {
   const float s = 1.f + e;
-  return fmaf(e - (s - 1.f), fast_rcp(s), __builtin_amdgcn_logf(s) * 0.6931471806f);
+  return fmaf(__builtin_amdgcn_logf(s), 0.6931471806f, __builtin_amdgcn_fmed3f(e - (s - 1.f), -0x1p-24f, 0x1p-24f));
 }
 // time step from the raw one (already with its bias); softplus is the identity above 20, as torch computes it (and for a NaN)
+template <typename T>
 __device__ __forceinline__ float time_step(float raw, int softplus) {
-  const float s = log1p_full(exp_full(raw));
+  const float s = log1p_full(exp_rows<T>(raw));
   return softplus && raw <= 20.f ? s : raw;
 }
-__device__ __forceinline__ float sigmoid_full(float x) { return fast_rcp(1.f + exp_full(-x)); }
+template <typename T>
+__device__ __forceinline__ float sigmoid_rows(float x) { return fast_rcp(1.f + exp_rows<T>(-x)); }
 
 // ------------------------------------------------------------------------------------------------ lanes
 // lane 4 q + j of a wave: channels 16 k + q (k = 0 .. 3) by entries 4 j + i (i = 0 .. 3) of the state; its own channel is 16 j + q
@@ -105,66 +116,100 @@ __device__ __forceinline__ int hidden_lane() {
   return l;
 }
 
-struct Lane {
-  int w, j, row, tile, group, base, end;   // wave, place in the quad, batch row, tile and its group, first channel of the tile, end of the group
-  unsigned own;                            // own channel
-  bool on, odd, high;
+// A wave's part of a tile of 64 channels: entries 16 w .. of their states.
+struct Tile {
+  int w, row, tile, group, base, end;      // wave, batch row, tile and its group, first channel of the tile, end of the group
   bool full;                               // all 64 channels of the tile are there
-  __device__ __forceinline__ Lane(const ScanArgs& a) {
-    const int l = threadIdx.x & 63;
+  __device__ __forceinline__ Tile(const ScanArgs& a) {
     w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    j = l & 3;
-    odd = j & 1; high = j & 2;
     tile = blockIdx.x;
     row = blockIdx.z;
     group = tile / a.tiles_g;
     base = group * a.per_group + (tile - group * a.tiles_g) * 64;
     end = (group + 1) * a.per_group;
     full = base + 64 <= end;
-    const int c = base + 16 * j + (l >> 2);
-    on = c < end;
-    own = min(c, end - 1);        // (lanes beyond the group compute its last channel again and store nothing)
   }
-  // The lane's 4 x 4 entries of a [.., channels, N] fp32 array, zero beyond N: where sequences start and end, not in the loops over tokens.
+};
+// Four consecutive entries of a state, zero beyond N.
+__device__ __forceinline__ void load4(const ScanArgs& a, const float* s, int n0, float* x) {
+  if (a.vec) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (n0 < a.N) v = *(const f32x4*)s;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = n0 + i < a.N ? s[i] : 0.f;
+  }
+}
+__device__ __forceinline__ void store4(const ScanArgs& a, float* d, int n0, const float* x) {
+  if (a.vec) {
+    if (n0 < a.N) *(f32x4*)d = (f32x4){x[0], x[1], x[2], x[3]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n0 + i < a.N) d[i] = x[i];
+  }
+}
+__device__ __forceinline__ void settle44(float (*x)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(x[k][i]));   // (see settle below)
+}
+// Lanes as columns: lane l has channel l of the tile, x[j][i] entry 4 j + i of the wave's sixteen.
+struct Column : Tile {
+  unsigned own;                            // own channel (lanes beyond the group compute its last channel again and store nothing)
+  bool on;
+  __device__ __forceinline__ Column(const ScanArgs& a) : Tile(a) {
+    const int c = base + (threadIdx.x & 63);
+    on = c < end;
+    own = min(c, end - 1);
+  }
+  // the lane's entries of a [.., channels, N] fp32 array: where sequences start and end, not in the loops over tokens
   __device__ __forceinline__ void load(const ScanArgs& a, const float* p, float (*x)[4]) const {
-    const int l = hidden_lane();
-    const int n0 = 16 * w + 4 * (l & 3);
+    const float* s = p + (int64_t)min(base + hidden_lane(), end - 1) * a.N + 16 * w;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float* s = p + (int64_t)min(base + 16 * k + (l >> 2), end - 1) * a.N + n0;
-      if (a.vec) {
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (n0 < a.N) v = *(const f32x4*)s;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[k][i] = v[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[k][i] = n0 + i < a.N ? s[i] : 0.f;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(x[k][i]));   // (see settle below)
+    for (int j = 0; j < 4; ++j) load4(a, s + 4 * j, 16 * w + 4 * j, x[j]);
+    settle44(x);
   }
   __device__ __forceinline__ void store(const ScanArgs& a, float* p, const float (*x)[4]) const {
-    const int l = hidden_lane();
-    const int n0 = 16 * w + 4 * (l & 3);
+    const int c = base + hidden_lane();
+    if (c >= end) return;
+    float* d = p + (int64_t)c * a.N + 16 * w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) store4(a, d + 4 * j, 16 * w + 4 * j, x[j]);
+  }
+  static __device__ __forceinline__ unsigned packed(int j) { return 64 * j + (threadIdx.x & 63); }
+};
+// Lanes as quads: x[k][i] is channel 16 k + q of the tile, entry 4 j + i of the wave's sixteen, for lane 4 q + j.
+struct Lane : Tile {
+  int j;                                   // place in the quad
+  unsigned own;                            // own channel
+  bool on, odd, high;
+  __device__ __forceinline__ Lane(const ScanArgs& a) : Tile(a) {
+    const int l = threadIdx.x & 63;
+    j = l & 3;
+    odd = j & 1; high = j & 2;
+    const int c = base + 16 * j + (l >> 2);
+    on = c < end;
+    own = min(c, end - 1);
+  }
+  __device__ __forceinline__ void load(const ScanArgs& a, const float* p, float (*x)[4]) const {
+    const int l = hidden_lane(), n0 = 16 * w + 4 * (l & 3);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) load4(a, p + (int64_t)min(base + 16 * k + (l >> 2), end - 1) * a.N + n0, n0, x[k]);
+    settle44(x);
+  }
+  __device__ __forceinline__ void store(const ScanArgs& a, float* p, const float (*x)[4]) const {
+    const int l = hidden_lane(), n0 = 16 * w + 4 * (l & 3);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int c = base + 16 * k + (l >> 2);
-      if (c >= end) continue;
-      float* d = p + (int64_t)c * a.N + n0;
-      if (a.vec) {
-        const f32x4 v = {x[k][0], x[k][1], x[k][2], x[k][3]};
-        if (n0 < a.N) *(f32x4*)d = v;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (n0 + i < a.N) d[i] = x[k][i];
-      }
+      if (c < end) store4(a, p + (int64_t)c * a.N + n0, n0, x[k]);
     }
   }
+  static __device__ __forceinline__ unsigned packed(int k) { return 64 * (threadIdx.x & 3) + 16 * k + ((threadIdx.x & 63) >> 2); }
 };
 // An element of a row: the row's address is the same for the whole wave, the lane adds 32 bits.  The empty assembly keeps the address
 // in scalar registers: left alone, the compiler adds the lane's part first and carries one 64-bit address per array and lane
@@ -216,23 +261,23 @@ struct Four {
     return n < a.N ? x : (f32x4){0.f, 0.f, 0.f, 0.f};
   }
 };
-// index of a wave's entries in an array of one float4 for each channel piece and lane of every wave and tile
-__device__ __forceinline__ int64_t packed_at(int64_t slot, const ScanArgs& a, int tile, int nw, int w, int k) {
-  return (((slot * a.tiles + tile) * nw + w) * 4 + k) * 64;
+// A wave's entries in scratch: a float4 for entries 4 j .. of every channel of the tile, j first
+__device__ __forceinline__ int64_t packed_at(int64_t slot, const ScanArgs& a, int tile, int nw, int w, int j) {
+  return (((slot * a.tiles + tile) * nw + w) * 4 + j) * 64;
 }
-__device__ __forceinline__ void load_packed(const float* p, int64_t at, float (*x)[4]) {
-  const unsigned l = threadIdx.x & 63;
+template <typename L>
+__device__ __forceinline__ void load_packed(const L&, const float* p, int64_t at, float (*x)[4]) {
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const f32x4 v = row_load((const f32x4*)p + at, 64 * k + l);
+    const f32x4 v = row_load((const f32x4*)p + at, L::packed(k));
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[k][i] = v[i];
   }
 }
-__device__ __forceinline__ void store_packed(float* p, int64_t at, const float (*x)[4]) {
-  const unsigned l = threadIdx.x & 63;
+template <typename L>
+__device__ __forceinline__ void store_packed(const L&, float* p, int64_t at, const float (*x)[4]) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) row_store((f32x4*)p + at, 64 * k + l, (f32x4){x[k][0], x[k][1], x[k][2], x[k][3]});
+  for (int k = 0; k < 4; ++k) row_store((f32x4*)p + at, L::packed(k), (f32x4){x[k][0], x[k][1], x[k][2], x[k][3]});
 }
 __device__ __forceinline__ void zero44(float (*x)[4]) {
 #pragma unroll
@@ -244,33 +289,24 @@ __device__ __forceinline__ void zero44(float (*x)[4]) {
 // the scheduler walks entry by entry to save registers, and the product, its exponential and what uses that wait for
 // each other.
 __device__ __forceinline__ void stage() { __builtin_amdgcn_sched_barrier(0); }
-// decays of a token, and its input to the states
-__device__ __forceinline__ void decays(float (*e)[4], const float* dk, const float (*A2)[4]) {
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) e[k][i] = dk[k] * A2[k][i];
-  stage();
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) e[k][i] = fast_exp2(e[k][i]);
-}
 __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 // a sequence's entries of a [seqs, channels, N] array, or zero where there is none
-__device__ __forceinline__ void load_state(const ScanArgs& a, const Lane& ln, const float* p, int seq, float (*h)[4]) {
+template <typename L>
+__device__ __forceinline__ void load_state(const ScanArgs& a, const L& ln, const float* p, int seq, float (*h)[4]) {
   if (p) ln.load(a, p + (int64_t)seq * a.D_ * a.N, h);
   else zero44(h);
 }
-__device__ __forceinline__ void store_state(const ScanArgs& a, const Lane& ln, float* p, int seq, const float (*h)[4]) {
+template <typename L>
+__device__ __forceinline__ void store_state(const ScanArgs& a, const L& ln, float* p, int seq, const float (*h)[4]) {
   ln.store(a, p + (int64_t)seq * a.D_ * a.N, h);
 }
 // sequences [n, end) have no token: what they start with is what they end with
-__device__ __forceinline__ void hand_over(const ScanArgs& a, const Lane& ln, const float* from, float* to, int n, int end) {
+template <typename L>
+__device__ __forceinline__ void hand_over(const ScanArgs& a, const L& ln, const float* from, float* to, int n, int end) {
   if (!to) return;
   for (; n < end; ++n) {
     float x[4][4];
@@ -309,7 +345,7 @@ template <typename T>
 struct BlockRows {
   Piece8<T> v;
   // row: the block's first token; left: tokens behind it
-  __device__ __forceinline__ void fetch(const Lane& ln, const T* row, int stride, int left) {
+  __device__ __forceinline__ void fetch(const Tile& ln, const T* row, int stride, int left) {
     const int l = threadIdx.x & 63;
     const unsigned at = __umul24(min(l >> 3, left), stride) + ln.base + 8 * (l & 7);
     if (ln.full) {
@@ -329,7 +365,7 @@ struct BlockRows {
     const int l = threadIdx.x & 63;
     v = *(const Piece8<T>*)&from[l >> 3][8 * (l & 7)];
   }
-  __device__ __forceinline__ void store(const Lane& ln, T* row, int stride, int nt) const {
+  __device__ __forceinline__ void store(const Tile& ln, T* row, int stride, int nt) const {
     const int l = threadIdx.x & 63;
     const unsigned at = __umul24(l >> 3, stride) + ln.base + 8 * (l & 7);
     if (ln.full && nt == kTok) {
@@ -347,16 +383,91 @@ struct BlockRows {
 // element of a block in LDS that belongs to a lane's own channel
 __device__ __forceinline__ int own_at() { return 16 * (threadIdx.x & 3) + ((threadIdx.x & 63) >> 2); }
 
+// Sixteen entries of B or C of one token, the same for every lane of the wave: in scalar registers, which a vector instruction takes
+// one of.  A row of them has to be whole and at a multiple of four bytes.  (volatile keeps the load where it is written, ahead of
+// the decays: others the compiler moves to their use.)
+typedef unsigned words8 __attribute__((ext_vector_type(8), aligned(4)));
+typedef unsigned words16 __attribute__((ext_vector_type(16), aligned(4)));
+template <typename T>
+struct Uniform16;
+template <>
+struct Uniform16<bf16_t> {
+  words8 v;
+  __device__ __forceinline__ void load(const bf16_t* p) { v = *(const volatile __attribute__((address_space(4))) words8*)(uint64_t)p; }
+  __device__ __forceinline__ float get(int n) const {
+    const unsigned x = v[n >> 1];
+    return __builtin_bit_cast(float, n & 1 ? x & 0xffff0000u : x << 16);
+  }
+};
+template <>
+struct Uniform16<float> {
+  words16 v;
+  __device__ __forceinline__ void load(const float* p) { v = *(const volatile __attribute__((address_space(4))) words16*)(uint64_t)p; }
+  __device__ __forceinline__ float get(int n) const {
+    const unsigned x = v[n];
+    return __builtin_bit_cast(float, x);
+  }
+};
+// B and C of a block of tokens: rows that Uniform16 takes are read as they are used, SC; others (N no multiple of 16, odd strides)
+// are fetched a block ahead by the lanes and read from LDS.
+template <typename T, bool SC, int M>
+struct TokenRows {
+  const T* p[M];
+  int stride[M];
+  Four<T> r[M];
+  __device__ __forceinline__ void fetch(const ScanArgs& a, int tb, int left, int w) {
+    if constexpr (!SC) {
+      const int l = threadIdx.x & 63, t = min((l >> 2) & 7, left);
+#pragma unroll
+      for (int m = 0; m < M; ++m) r[m].fetch(a, p[m] + (int64_t)tb * stride[m], __umul24(t, stride[m]) * (unsigned)sizeof(T), 16 * w + 4 * (l & 3));
+    }
+  }
+  __device__ __forceinline__ void to_lds(const ScanArgs& a, float (*s)[M][16], int w) const {
+    if constexpr (!SC) {
+      const int l = threadIdx.x & 63;
+#pragma unroll
+      for (int m = 0; m < M; ++m) *(f32x4*)&s[(l >> 2) & 7][m][4 * (l & 3)] = r[m].get(a, 16 * w + 4 * (l & 3));   // (the upper half holds the same)
+    }
+  }
+};
+template <typename T, bool SC>
+struct Entries {        // the sixteen of a token
+  Uniform16<T> u;
+  f32x4 v[SC ? 1 : 4];
+  __device__ __forceinline__ void take(const T* p, const float* lds) {
+    if constexpr (SC) {
+      u.load(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = ((const f32x4*)lds)[j];
+    }
+  }
+  __device__ __forceinline__ float get(int j, int i) const { return SC ? u.get(4 * j + i) : v[SC ? 0 : j][i]; }
+};
+// decays of a token: the products, then the exponentials (see stage)
+__device__ __forceinline__ void decays(float (*e)[4], float dt, const float (*A2)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[j][i] = dt * A2[j][i];
+  stage();
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[j][i] = fast_exp2(e[j][i]);
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 // OUT: the pass itself.  Otherwise the walk of a segment from zero: its last state, the sum of its dt, and whether a sequence starts in it.
-template <typename T, int NW, bool OUT>
+template <typename T, int NW, bool OUT, bool SC>
 __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs a) {
-  __shared__ float sBC[NW][kTok][2][16];
+  constexpr int M = OUT ? 2 : 1;
+  __shared__ __attribute__((aligned(16))) float sBC[SC ? 1 : NW][SC ? 1 : kTok][M][16];
   __shared__ __attribute__((aligned(16))) T sRow[NW][OUT ? 3 : 2][kTok][64];   // u, delta, z
   __shared__ __attribute__((aligned(16))) T sOut[OUT && NW == 1 ? kTok : 1][64];
   __shared__ float sY[NW > 1 && OUT ? 2 : 1][NW > 1 && OUT ? NW : 1][kTok][64];
-  const Lane ln(a);
-  const int l = threadIdx.x & 63, w = ln.w, row = ln.row, own = own_at();
+  const Column ln(a);
+  const int l = threadIdx.x & 63, w = ln.w, row = ln.row;
   const int t0 = blockIdx.y * a.seg, t1 = min(a.T, t0 + a.seg);
   const float bias = a.bias ? a.bias[ln.own] : 0.f, Dc = a.D ? a.D[ln.own] : 0.f;
   float A2[4][4], h[4][4], dt_sum = 0.f;
@@ -367,28 +478,28 @@ __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs a) {
     for (int i = 0; i < 4; ++i) A2[k][i] *= kLog2e;
   ScanSeq cur = seq_at(a, row, t0);
   int cut = 0;
-  if (OUT && t0 > 0 && cur.s != t0) load_packed(a.seg_h, packed_at((int64_t)row * a.segs + blockIdx.y, a, ln.tile, NW, w, 0), h);
+  if (OUT && t0 > 0 && cur.s != t0) load_packed(ln, a.seg_h, packed_at((int64_t)row * a.segs + blockIdx.y, a, ln.tile, NW, w, 0), h);
   else zero44(h);
   if (OUT && t0 == 0 && a.cu) hand_over(a, ln, a.init, a.final_, 0, cur.n);   // sequences without a token before the first one
   const T* pu = (const T*)a.u + row * a.ub;
   const T* pd = (const T*)a.delta + row * a.db;
   const T* pz = a.z ? (const T*)a.z + row * a.zb : nullptr;
   T* py = (T*)a.y + (int64_t)row * a.T * a.D_;
-
-  const T* pB = (const T*)a.Bm + row * a.Bb + (int64_t)ln.group * a.N;
-  const T* pC = (const T*)a.Cm + row * a.Cb + (int64_t)ln.group * a.N;
-  const int n4 = 16 * w + 4 * (l & 3);     // B and C: lane l takes these entries of token l / 4 (of the last token there is)
+  TokenRows<T, SC, M> bc;
+  bc.p[0] = (const T*)a.Bm + row * a.Bb + (int64_t)ln.group * a.N;
+  bc.stride[0] = a.Bt;
+  if constexpr (OUT) {
+    bc.p[1] = (const T*)a.Cm + row * a.Cb + (int64_t)ln.group * a.N;
+    bc.stride[1] = a.Ct;
+  }
 
   BlockRows<T> ru, rd, rz;
-  Four<T> rb, rc;
   auto fetch = [&](int tb) {
     const int left = min(kTok, t1 - tb) - 1;
     ru.fetch(ln, pu + (int64_t)tb * a.ut, a.ut, left);
     rd.fetch(ln, pd + (int64_t)tb * a.dt, a.dt, left);
     if (OUT && a.z) rz.fetch(ln, pz + (int64_t)tb * a.zt, a.zt, left);
-    const int t = min((l >> 2) & 7, left);
-    rb.fetch(a, pB + (int64_t)tb * a.Bt, __umul24(t, a.Bt) * (unsigned)sizeof(T), n4);
-    if (OUT) rc.fetch(a, pC + (int64_t)tb * a.Ct, __umul24(t, a.Ct) * (unsigned)sizeof(T), n4);
+    bc.fetch(a, tb, left, w);
   };
   fetch(t0);
   int turn = 0;
@@ -396,8 +507,7 @@ __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs a) {
     ru.to_lds(sRow[w][0]);
     rd.to_lds(sRow[w][1]);
     if (OUT && a.z) rz.to_lds(sRow[w][OUT ? 2 : 0]);
-    *(f32x4*)&sBC[w][(l >> 2) & 7][0][4 * (l & 3)] = rb.get(a, n4);     // (the upper half of the wave holds the same as the lower)
-    if (OUT) *(f32x4*)&sBC[w][(l >> 2) & 7][1][4 * (l & 3)] = rc.get(a, n4);
+    bc.to_lds(a, sBC[SC ? 0 : w], w);
     if constexpr (OUT && NW == 1) {
       if (tb > t0) {
         BlockRows<T> done;
@@ -405,50 +515,52 @@ __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs a) {
         done.store(ln, py + (int64_t)(tb - kTok) * a.D_, a.D_, kTok);
       }
     }
-    if (OUT && a.ckpt) store_packed(a.ckpt, packed_at((int64_t)row * a.ckpts + tb / kTok, a, ln.tile, NW, w, 0), h);
+    if (OUT && a.ckpt) store_packed(ln, a.ckpt, packed_at((int64_t)row * a.ckpts + tb / kTok, a, ln.tile, NW, w, 0), h);
     wave_lds_fence();
     if (tb + kTok < t1) fetch(tb + kTok);
     const int nt = min(kTok, t1 - tb);
     float dt[kTok], uv[kTok], gate[kTok];
 #pragma unroll
     for (int t = 0; t < kTok; ++t) {
-      uv[t] = to_f32(sRow[w][0][t][own]);
-      dt[t] = time_step(to_f32(sRow[w][1][t][own]) + bias, a.softplus);
+      uv[t] = to_f32(sRow[w][0][t][l]);
+      dt[t] = time_step<T>(to_f32(sRow[w][1][t][l]) + bias, a.softplus);
       gate[t] = 1.f;
     }
     if (OUT && a.z)
 #pragma unroll
       for (int t = 0; t < kTok; ++t) {
-        const float z = to_f32(sRow[w][OUT ? 2 : 0][t][own]);
-        gate[t] = z * sigmoid_full(z);
+        const float z = to_f32(sRow[w][OUT ? 2 : 0][t][l]);
+        gate[t] = z * sigmoid_rows<T>(z);
       }
+    const T *rowB = bc.p[0] + (int64_t)tb * bc.stride[0] + 16 * w, *rowC = OUT ? bc.p[M - 1] + (int64_t)tb * bc.stride[M - 1] + 16 * w : nullptr;
     auto walk = [&](auto r) {
+      const T *qB = rowB, *qC = rowC;
+      if (SC) asm volatile("" : "+s"(qB), "+s"(qC));     // (or the addresses of all tokens are computed before the walk, and spilled)
 #pragma unroll
-      for (int t = 0; t < kTok; ++t) {
+      for (int t = 0; t < kTok; ++t, qB += bc.stride[0], qC += bc.stride[M - 1]) {
         if (!walks(r, t)) continue;
-        const f32x4 Bv = *(const f32x4*)&sBC[w][t][0][4 * ln.j];
-        f32x4 Cv;
-        if (OUT) Cv = *(const f32x4*)&sBC[w][t][1][4 * ln.j];
-        const float x = dt[t] * uv[t];
-        const float dk[4] = {of_channel<0>(dt[t]), of_channel<1>(dt[t]), of_channel<2>(dt[t]), of_channel<3>(dt[t])};
-        const float xk[4] = {of_channel<0>(x), of_channel<1>(x), of_channel<2>(x), of_channel<3>(x)};
-        float e[4][4], s[4];
+        // B and C are on their way while the decays are computed
+        Entries<T, SC> B, C;
+        B.take(qB, sBC[SC ? 0 : w][SC ? 0 : t][0]);
+        if constexpr (OUT) C.take(qC, sBC[SC ? 0 : w][SC ? 0 : t][1]);
+        float dtt = dt[t], e[4][4], s[4];
+        settle(dtt);          // (the two walks have the same products, which the compiler would else compute before choosing between them)
+        const float x = dtt * uv[t];
         stage();
-        decays(e, dk, A2);
+        decays(e, dtt, A2);
         stage();
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) h[k][i] = fmaf(e[k][i], h[k][i], xk[k] * Bv[i]);
+          for (int i = 0; i < 4; ++i) h[j][i] = fmaf(e[j][i], h[j][i], x * B.get(j, i));
         stage();
-        if (OUT) {
+        if constexpr (OUT) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[k] = i ? fmaf(Cv[i], h[k][i], s[k]) : Cv[i] * h[k][i];
-
-          const float y = quad_total4(s[0], s[1], s[2], s[3], ln.odd, ln.high);
-          if constexpr (NW == 1) sOut[t][own] = from_f32<T>(fmaf(Dc, uv[t], y) * gate[t]);
+            for (int i = 0; i < 4; ++i) s[i] = j ? fmaf(C.get(j, i), h[j][i], s[i]) : C.get(j, i) * h[j][i];
+          const float y = (s[0] + s[1]) + (s[2] + s[3]);
+          if constexpr (NW == 1) sOut[t][l] = from_f32<T>(fmaf(Dc, uv[t], y) * gate[t]);
           else sY[turn][w][t][l] = y;
         } else {
           dt_sum += dt[t];
@@ -494,7 +606,7 @@ __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs a) {
   }
   if (!OUT) {
     const int64_t slot = (int64_t)row * a.segs + blockIdx.y;
-    store_packed(a.seg_h, packed_at(slot, a, ln.tile, NW, w, 0), h);
+    store_packed(ln, a.seg_h, packed_at(slot, a, ln.tile, NW, w, 0), h);
     if (w == 0) a.seg_dt[(slot * a.tiles + ln.tile) * 64 + l] = dt_sum;
     if (ln.tile == 0 && threadIdx.x == 0) a.seg_cut[slot] = cut;
   }
@@ -502,12 +614,12 @@ __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs a) {
 
 // What comes back over a segment from its end with nothing coming in: the backward's carry, g <- a (g + C Y) from the last
 // token to the first.
-template <typename T, int NW>
+template <typename T, int NW, bool SC>
 __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) {
-  __shared__ float sC[NW][kTok][16];
+  __shared__ __attribute__((aligned(16))) float sC[SC ? 1 : NW][SC ? 1 : kTok][1][16];
   __shared__ __attribute__((aligned(16))) T sRow[NW][3][kTok][64];   // dy, delta, z
-  const Lane ln(a);
-  const int l = threadIdx.x & 63, w = ln.w, row = ln.row, own = own_at();
+  const Column ln(a);
+  const int l = threadIdx.x & 63, w = ln.w, row = ln.row;
   const int t0 = blockIdx.y * a.seg, t1 = min(a.T, t0 + a.seg);
   const float bias = a.bias ? a.bias[ln.own] : 0.f;
   float A2[4][4], g[4][4], dt_sum = 0.f;
@@ -522,16 +634,16 @@ __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) 
   const T* pd = (const T*)a.delta + row * a.db;
   const T* pz = a.z ? (const T*)a.z + row * a.zb : nullptr;
   const T* pg = (const T*)a.dy + (int64_t)row * a.T * a.D_;
-  const T* pC = (const T*)a.Cm + row * a.Cb + (int64_t)ln.group * a.N;
-  const int n4 = 16 * w + 4 * (l & 3);
+  TokenRows<T, SC, 1> rc;
+  rc.p[0] = (const T*)a.Cm + row * a.Cb + (int64_t)ln.group * a.N;
+  rc.stride[0] = a.Ct;
   BlockRows<T> rg, rd, rz;
-  Four<T> rc;
   auto fetch = [&](int tb) {
     const int left = min(kTok, t1 - tb) - 1;
     rg.fetch(ln, pg + (int64_t)tb * a.D_, a.D_, left);
     rd.fetch(ln, pd + (int64_t)tb * a.dt, a.dt, left);
     if (a.z) rz.fetch(ln, pz + (int64_t)tb * a.zt, a.zt, left);
-    rc.fetch(a, pC + (int64_t)tb * a.Ct, __umul24(min((l >> 2) & 7, left), a.Ct) * (unsigned)sizeof(T), n4);
+    rc.fetch(a, tb, left, w);
   };
   const int last = t0 + (t1 - 1 - t0) / kTok * kTok;
   fetch(last);
@@ -539,41 +651,45 @@ __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) 
     rg.to_lds(sRow[w][0]);
     rd.to_lds(sRow[w][1]);
     if (a.z) rz.to_lds(sRow[w][2]);
-    *(f32x4*)&sC[w][(l >> 2) & 7][4 * (l & 3)] = rc.get(a, n4);
+    rc.to_lds(a, sC[SC ? 0 : w], w);
     wave_lds_fence();
     if (tb > t0) fetch(tb - kTok);
     const int nt = min(kTok, t1 - tb);
     float dt[kTok], Y[kTok];
 #pragma unroll
     for (int t = 0; t < kTok; ++t) {
-      dt[t] = time_step(to_f32(sRow[w][1][t][own]) + bias, a.softplus);
-      Y[t] = to_f32(sRow[w][0][t][own]);
+      dt[t] = time_step<T>(to_f32(sRow[w][1][t][l]) + bias, a.softplus);
+      Y[t] = to_f32(sRow[w][0][t][l]);
     }
     if (a.z)
 #pragma unroll
       for (int t = 0; t < kTok; ++t) {
-        const float z = to_f32(sRow[w][2][t][own]);
-        Y[t] *= z * sigmoid_full(z);
+        const float z = to_f32(sRow[w][2][t][l]);
+        Y[t] *= z * sigmoid_rows<T>(z);
       }
+    const T* rowC = rc.p[0] + (int64_t)(tb + kTok - 1) * rc.stride[0] + 16 * w;
     auto walk = [&](auto r) {
+      const T* qC = rowC;
+      if (SC) asm volatile("" : "+s"(qC));
 #pragma unroll
-      for (int t = kTok - 1; t >= 0; --t) {
+      for (int t = kTok - 1; t >= 0; --t, qC -= rc.stride[0]) {
         if (!walks(r, t)) continue;
-        const f32x4 Cv = *(const f32x4*)&sC[w][t][4 * ln.j];
-        const float dk[4] = {of_channel<0>(dt[t]), of_channel<1>(dt[t]), of_channel<2>(dt[t]), of_channel<3>(dt[t])};
-        const float Yk[4] = {of_channel<0>(Y[t]), of_channel<1>(Y[t]), of_channel<2>(Y[t]), of_channel<3>(Y[t])};
-        float e[4][4];
+        Entries<T, SC> C;
+        C.take(qC, sC[SC ? 0 : w][SC ? 0 : t][0]);
+        float dtt = dt[t], e[4][4];
+        settle(dtt);          // (as in the forward)
         stage();
-        decays(e, dk, A2);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) g[k][i] = fmaf(Cv[i], Yk[k], g[k][i]);
+        decays(e, dtt, A2);
         stage();
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) g[k][i] *= e[k][i];
+          for (int i = 0; i < 4; ++i) g[j][i] = fmaf(C.get(j, i), Y[t], g[j][i]);
+        stage();
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) g[j][i] *= e[j][i];
         dt_sum += dt[t];
       }
     };
@@ -591,7 +707,7 @@ __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) 
     wave_lds_fence();
   }
   const int64_t slot = (int64_t)row * a.segs + blockIdx.y;
-  store_packed(a.seg_h, packed_at(slot, a, ln.tile, NW, w, 0), g);
+  store_packed(ln, a.seg_h, packed_at(slot, a, ln.tile, NW, w, 0), g);
   if (w == 0) a.seg_dt[(slot * a.tiles + ln.tile) * 64 + l] = dt_sum;
   if (ln.tile == 0 && threadIdx.x == 0) a.seg_cut[slot] = cut;
 }
@@ -601,7 +717,7 @@ template <int NW, bool BACK>
 __global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs a) {
   const int l = threadIdx.x & 63, k = threadIdx.x >> 6, w = blockIdx.y, tile = blockIdx.x, row = blockIdx.z;
   const int group = tile / a.tiles_g, base = group * a.per_group + (tile - group * a.tiles_g) * 64;
-  const int chan = min(base + 16 * k + (l >> 2), (group + 1) * a.per_group - 1), n0 = 16 * w + 4 * (l & 3);
+  const int chan = min(base + l, (group + 1) * a.per_group - 1), n0 = 16 * w + 4 * k;
   float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 4; ++i) A2[i] = n0 + i < a.N ? a.A[(int64_t)chan * a.N + n0 + i] * kLog2e : 0.f;
@@ -616,7 +732,7 @@ __global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs a) {
       const int s = min(b + x, a.segs - 1);
       const int64_t slot = (int64_t)row * a.segs + (BACK ? a.segs - 1 - s : s);
       v[x] = H[packed_at(slot, a, tile, NW, w, k) + l];
-      d[x] = a.seg_dt[(slot * a.tiles + tile) * 64 + (l & ~3) + k];
+      d[x] = a.seg_dt[(slot * a.tiles + tile) * 64 + l];
       c[x] = a.seg_cut[slot];
     }
 #pragma unroll
@@ -659,7 +775,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
     for (int i = 0; i < 4; ++i) A2[k][i] *= kLog2e;
   zero44(dA);
   const int64_t slot = (int64_t)row * a.segs + blockIdx.y;
-  if (t1 < a.T) load_packed(a.seg_h, packed_at(slot, a, ln.tile, NW, w, 0), carry);
+  if (t1 < a.T) load_packed(ln, a.seg_h, packed_at(slot, a, ln.tile, NW, w, 0), carry);
   else zero44(carry);
   ScanSeq cur = seq_at(a, row, t1 - 1);
   if (t1 == a.T && a.cu) hand_over(a, ln, a.d_final, a.d_init, cur.n + 1, a.seqs);   // sequences without a token behind the last one
@@ -692,7 +808,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
     rb.fetch(a, pB + (int64_t)tb * a.Bt, __umul24(t, a.Bt) * (unsigned)sizeof(T), n4);
     rc.fetch(a, pC + (int64_t)tb * a.Ct, __umul24(t, a.Ct) * (unsigned)sizeof(T), n4);
   };
-  auto fetch_kept = [&](int tb) { load_packed(a.ckpt, packed_at((int64_t)row * a.ckpts + tb / kTok, a, ln.tile, NW, w, 0), h0); };
+  auto fetch_kept = [&](int tb) { load_packed(ln, a.ckpt, packed_at((int64_t)row * a.ckpts + tb / kTok, a, ln.tile, NW, w, 0), h0); };
   // results of a block: out of LDS, and on their way
   BlockRows<T> done[kOwn];
   f32x4 done_bc;
@@ -733,7 +849,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
     if (tb > t0) fetch(tb - kTok);
 #pragma unroll
     for (int t = 0; t < kTok; ++t)
-      if (t % NW == w) sDt[t][l] = time_step(to_f32(sRow[1][t][own]) + bias, a.softplus);
+      if (t % NW == w) sDt[t][l] = time_step<T>(to_f32(sRow[1][t][own]) + bias, a.softplus);
     sync();
     {
       float h[4][4];
@@ -778,7 +894,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
       float uv[kSub], Y[kSub], slope[kSub], gz[kSub];
 #pragma unroll
       for (int t = 0; t < kSub; ++t) {
-        const float raw = to_f32(sRow[1][sub * kSub + t][own]) + bias, sg = sigmoid_full(raw);
+        const float raw = to_f32(sRow[1][sub * kSub + t][own]) + bias, sg = sigmoid_rows<T>(raw);
         uv[t] = to_f32(sRow[0][sub * kSub + t][own]);
         Y[t] = to_f32(sRow[3][sub * kSub + t][own]);
         slope[t] = a.softplus && raw <= 20.f ? sg : 1.f;
@@ -787,7 +903,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
       if (a.z)
 #pragma unroll
         for (int t = 0; t < kSub; ++t) {
-          const float z = to_f32(sRow[2][sub * kSub + t][own]), sg = sigmoid_full(z);
+          const float z = to_f32(sRow[2][sub * kSub + t][own]), sg = sigmoid_rows<T>(z);
           gz[t] = Y[t] * (sg + z * sg * (1.f - sg));
           Y[t] *= z * sg;
         }
@@ -921,7 +1037,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
   }
   take();
   put(t0, min(kTok, t1 - t0));
-  store_packed(a.part_a, packed_at(slot, a, ln.tile, NW, w, 0), dA);
+  store_packed(ln, a.part_a, packed_at(slot, a, ln.tile, NW, w, 0), dA);
   float* pc = a.part_c + (((slot * a.tiles + ln.tile) * NW + w) * 64 + l) * 2;
   pc[0] = dD;
   pc[1] = dbias;
@@ -941,8 +1057,8 @@ __global__ __launch_bounds__(256) void scan_bwd_rows_kernel(ScanArgs a, int nw) 
   }
 }
 
-// dA, dD, ddelta_bias: the segments of all rows in their order, in 64 bits.  grid (tiles, waves of a tile, 5): z < 4 the channels
-// 16 z .. of dA, z = 4 dD and ddelta_bias; four waves take a quarter of the segments each.
+// dA, dD, ddelta_bias: the segments of all rows in their order, in 64 bits.  grid (tiles, waves of a tile, 5): z < 4 the entries
+// 4 z .. of dA, z = 4 dD and ddelta_bias; four waves take a quarter of the segments each.
 __global__ __launch_bounds__(256) void scan_bwd_params_kernel(ScanArgs a, int nw) {
   __shared__ double s[4][64][4];
   const int l = threadIdx.x & 63, v = threadIdx.x >> 6, tile = blockIdx.x, w = blockIdx.y, z = blockIdx.z;
@@ -969,15 +1085,14 @@ __global__ __launch_bounds__(256) void scan_bwd_params_kernel(ScanArgs a, int nw
   if (v) return;
 #pragma unroll
   for (int e = 0; e < 4; ++e) t[e] = s[0][l][e] + s[1][l][e] + s[2][l][e] + s[3][l][e];
-  const int q = l >> 2, j = l & 3;
   if (z < 4) {
-    const int c = base + 16 * z + q, n0 = 16 * w + 4 * j;
+    const int c = base + l, n0 = 16 * w + 4 * z;
     if (c < end)
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (n0 + e < a.N) a.dA[(int64_t)c * a.N + n0 + e] = (float)t[e];
   } else if (w == 0) {
-    const int c = base + 16 * j + q;
+    const int c = base + 16 * (l & 3) + (l >> 2);
     if (c < end) {
       if (a.dD) a.dD[c] = (float)t[0];
       if (a.dbias) a.dbias[c] = (float)t[1];
@@ -1018,16 +1133,17 @@ static int check_scan_tensors(const PalScanDims* d, const PalScanTensors* t) {
 static int scan_waves(const PalScanDims* d) { return (d->state + 15) / 16; }
 static int64_t scan_tiles(const PalScanDims* d) { return (int64_t)d->groups * ((d->channels / d->groups + 63) / 64); }
 
-// Tokens per segment: enough segments for two waves on every SIMD, at least 64 tokens each
-static int scan_segment(const PalScanDims* d) {
+// Tokens per segment: enough segments for `most` waves, at least 64 tokens each.  Forward three waves on every SIMD (1 x 16384 tokens of 1536
+// channels: 114 us with three, 131 with two, 116 with four), backward the two whose registers fit.
+static int scan_segment(const PalScanDims* d, int64_t most) {
   const int64_t waves = scan_tiles(d) * scan_waves(d) * d->batch;
-  const int64_t segs = waves < 2048 ? 2048 / waves : 1;
+  const int64_t segs = waves < most ? most / waves : 1;
   int64_t seg = (d->seq_len + segs - 1) / segs;
   seg = (seg + PAL_SCAN_BLOCK - 1) / PAL_SCAN_BLOCK * PAL_SCAN_BLOCK;
   if (seg < 64) seg = 64;
   return (int)(seg < d->seq_len ? seg : (d->seq_len + PAL_SCAN_BLOCK - 1) / PAL_SCAN_BLOCK * PAL_SCAN_BLOCK);
 }
-static void scan_args(ScanArgs& a, const PalScanDims* d, const PalScanTensors* t) {
+static void scan_args(ScanArgs& a, const PalScanDims* d, const PalScanTensors* t, bool back) {
   a.rows = d->batch; a.T = d->seq_len; a.seqs = d->n_seqs; a.D_ = d->channels; a.N = d->state; a.G = d->groups;
   a.per_group = d->channels / d->groups;
   a.tiles_g = (a.per_group + 63) / 64;
@@ -1036,12 +1152,17 @@ static void scan_args(ScanArgs& a, const PalScanDims* d, const PalScanTensors* t
   a.vec = d->state % 4 == 0;
   a.ub = d->u_batch; a.db = d->delta_batch; a.zb = d->z_batch; a.Bb = d->B_batch; a.Cb = d->C_batch;
   a.ut = (int)d->u_token; a.dt = (int)d->delta_token; a.zt = (int)d->z_token; a.Bt = (int)d->B_token; a.Ct = (int)d->C_token;
-  a.seg = scan_segment(d);
+  a.seg = scan_segment(d, back ? 2048 : 3072);
   a.segs = (a.T + a.seg - 1) / a.seg;
   a.ckpts = (a.T + PAL_SCAN_BLOCK - 1) / PAL_SCAN_BLOCK;
   if (!t) return;
   a.u = t->u; a.delta = t->delta; a.z = t->z; a.Bm = t->B; a.Cm = t->C;
   a.A = t->A; a.D = t->D; a.bias = t->delta_bias; a.init = t->init;
+  // rows of B and C that the scalar unit reads
+  auto words = [&](const void* p, int64_t batch, int64_t token) {
+    return d->dtype == PAL_DTYPE_F32 || ((uintptr_t)p % 4 == 0 && batch % 2 == 0 && token % 2 == 0);
+  };
+  a.scalar = d->state % 16 == 0 && words(t->B, d->B_batch, d->B_token) && words(t->C, d->C_batch, d->C_token);
   a.y = t->y; a.final_ = t->final_; a.ckpt = t->checkpoints; a.cu = t->cu_seqlens;
 }
 static size_t up256b(size_t x) { return (x + 255) / 256 * 256; }
@@ -1061,24 +1182,29 @@ static char* place_segments(ScanArgs& a, int nw, char* p) {
   return p + up256b((size_t)slots * 4);
 }
 
-template <typename T, int NW>
-static int scan_fwd_run(const ScanArgs& a, hipStream_t s) {
+template <typename T, int NW, bool SC>
+static int scan_fwd_launch(const ScanArgs& a, hipStream_t s) {
   const dim3 grid(a.tiles, a.segs, a.rows);
   if (a.segs > 1) {
-    PAL_TIMED_LAUNCH(kKernScanSegment, s, (scan_fwd_kernel<T, NW, false>), grid, dim3(64 * NW), 0, s, a);
+    PAL_TIMED_LAUNCH(kKernScanSegment, s, (scan_fwd_kernel<T, NW, false, SC>), grid, dim3(64 * NW), 0, s, a);
     PAL_HIP_LAUNCH_CHECK();
     PAL_TIMED_LAUNCH(kKernScanJoin, s, (scan_join_kernel<NW, false>), dim3(a.tiles, NW, a.rows), dim3(256), 0, s, a);
     PAL_HIP_LAUNCH_CHECK();
   }
-  PAL_TIMED_LAUNCH(kKernScanFwd, s, (scan_fwd_kernel<T, NW, true>), grid, dim3(64 * NW), 0, s, a);
+  PAL_TIMED_LAUNCH(kKernScanFwd, s, (scan_fwd_kernel<T, NW, true, SC>), grid, dim3(64 * NW), 0, s, a);
   PAL_HIP_LAUNCH_CHECK();
   return PAL_OK;
+}
+template <typename T, int NW>
+static int scan_fwd_run(const ScanArgs& a, hipStream_t s) {
+  return a.scalar ? scan_fwd_launch<T, NW, true>(a, s) : scan_fwd_launch<T, NW, false>(a, s);
 }
 template <typename T, int NW>
 static int scan_bwd_run(const ScanArgs& a, hipStream_t s) {
   const dim3 grid(a.tiles, a.segs, a.rows);
   if (a.segs > 1) {
-    PAL_TIMED_LAUNCH(kKernScanSegment, s, (scan_back_segment_kernel<T, NW>), grid, dim3(64 * NW), 0, s, a);
+    if (a.scalar) PAL_TIMED_LAUNCH(kKernScanSegment, s, (scan_back_segment_kernel<T, NW, true>), grid, dim3(64 * NW), 0, s, a);
+    else PAL_TIMED_LAUNCH(kKernScanSegment, s, (scan_back_segment_kernel<T, NW, false>), grid, dim3(64 * NW), 0, s, a);
     PAL_HIP_LAUNCH_CHECK();
     PAL_TIMED_LAUNCH(kKernScanJoin, s, (scan_join_kernel<NW, true>), dim3(a.tiles, NW, a.rows), dim3(256), 0, s, a);
     PAL_HIP_LAUNCH_CHECK();
@@ -1117,7 +1243,7 @@ extern "C" size_t pal_scan_checkpoint_bytes(const PalScanDims* d) {
   using namespace pal;
   if (check_scan(d) != PAL_OK) return 0;
   ScanArgs a{};
-  scan_args(a, d, nullptr);
+  scan_args(a, d, nullptr, false);
   return packed_bytes(a, scan_waves(d), (int64_t)a.rows * a.ckpts);
 }
 
@@ -1125,7 +1251,7 @@ extern "C" size_t pal_scan_fwd_workspace_bytes(const PalScanDims* d) {
   using namespace pal;
   if (check_scan(d) != PAL_OK) return 0;
   ScanArgs a{};
-  scan_args(a, d, nullptr);
+  scan_args(a, d, nullptr, false);
   return a.segs > 1 ? seg_bytes(a, scan_waves(d)) : 0;
 }
 
@@ -1136,7 +1262,7 @@ extern "C" int pal_scan_fwd(const PalScanDims* d, const PalScanTensors* t, void*
   if (!t->y) return PAL_E_NULL;
   if (((d->flags & PAL_FLAG_STORE_FINAL) != 0) != (t->final_ != nullptr)) return PAL_E_STATE;
   ScanArgs a{};
-  scan_args(a, d, t);
+  scan_args(a, d, t, false);
   const int nw = scan_waves(d);
   if (a.segs > 65535 || a.tiles > (1 << 24)) return PAL_E_DIM;
   if (a.segs > 1) {
@@ -1152,7 +1278,7 @@ extern "C" size_t pal_scan_bwd_workspace_bytes(const PalScanDims* d) {
   using namespace pal;
   if (check_scan(d) != PAL_OK) return 0;
   ScanArgs a{};
-  scan_args(a, d, nullptr);
+  scan_args(a, d, nullptr, true);
   const int nw = scan_waves(d);
   const int64_t slots = (int64_t)a.rows * a.segs;
   return (a.segs > 1 ? seg_bytes(a, nw) : 0) + up256b((size_t)a.rows * a.T * a.tiles * nw * 128) + packed_bytes(a, nw, slots) +
@@ -1173,7 +1299,7 @@ extern "C" int pal_scan_bwd(const PalScanDims* d, const PalScanTensors* t, const
   if (!workspace || workspace_bytes < pal_scan_bwd_workspace_bytes(d)) return PAL_E_WORKSPACE;
   if (!is_aligned16(workspace)) return PAL_E_ALIGN;
   ScanArgs a{};
-  scan_args(a, d, t);
+  scan_args(a, d, t, true);
   const int nw = scan_waves(d);
   if (a.segs > 65535 || a.tiles > (1 << 24)) return PAL_E_DIM;
   a.dy = gr->dy; a.d_final = gr->d_final; a.du = gr->du; a.ddelta = gr->ddelta; a.dA = gr->dA; a.dB = gr->dB; a.dC = gr->dC;
