@@ -42,7 +42,7 @@ struct ScanArgs {
   const int32_t* cu;
   int64_t ub, db, zb, Bb, Cb;                        // strides between batch rows
   int32_t ut, dt, zt, Bt, Ct;                        // and between tokens (below 2^24)
-  int32_t rows, T, seqs, D_, N, G, per_group, tiles_g, tiles, softplus, vec, scalar;
+  int32_t rows, T, seqs, D_, N, G, per_group, tiles_g, tiles, softplus, vec;
   int32_t seg, segs, ckpts;                          // tokens per segment (a multiple of PAL_SCAN_BLOCK), segments and kept states per row
 };
 
@@ -383,66 +383,23 @@ struct BlockRows {
 // element of a block in LDS that belongs to a lane's own channel
 __device__ __forceinline__ int own_at() { return 16 * (threadIdx.x & 3) + ((threadIdx.x & 63) >> 2); }
 
-// Sixteen entries of B or C of one token, the same for every lane of the wave: in scalar registers, which a vector instruction takes
-// one of.  A row of them has to be whole and at a multiple of four bytes.  (volatile keeps the load where it is written, ahead of
-// the decays: others the compiler moves to their use.)
-typedef unsigned words8 __attribute__((ext_vector_type(8), aligned(4)));
-typedef unsigned words16 __attribute__((ext_vector_type(16), aligned(4)));
-template <typename T>
-struct Uniform16;
-template <>
-struct Uniform16<bf16_t> {
-  words8 v;
-  __device__ __forceinline__ void load(const bf16_t* p) { v = *(const volatile __attribute__((address_space(4))) words8*)(uint64_t)p; }
-  __device__ __forceinline__ float get(int n) const {
-    const unsigned x = v[n >> 1];
-    return __builtin_bit_cast(float, n & 1 ? x & 0xffff0000u : x << 16);
-  }
-};
-template <>
-struct Uniform16<float> {
-  words16 v;
-  __device__ __forceinline__ void load(const float* p) { v = *(const volatile __attribute__((address_space(4))) words16*)(uint64_t)p; }
-  __device__ __forceinline__ float get(int n) const {
-    const unsigned x = v[n];
-    return __builtin_bit_cast(float, x);
-  }
-};
-// B and C of a block of tokens: rows that Uniform16 takes are read as they are used, SC; others (N no multiple of 16, odd strides)
-// are fetched a block ahead by the lanes and read from LDS.
-template <typename T, bool SC, int M>
+// B and C of a block of tokens, fetched a block ahead by the lanes and read from LDS by all at once.  (Read by the scalar unit and
+// taken from scalar registers they cost the same: 112 and 110 us of 16384 tokens of 1536 channels, and rows have to be whole and aligned.)
+template <typename T, int M>
 struct TokenRows {
   const T* p[M];
   int stride[M];
   Four<T> r[M];
   __device__ __forceinline__ void fetch(const ScanArgs& a, int tb, int left, int w) {
-    if constexpr (!SC) {
-      const int l = threadIdx.x & 63, t = min((l >> 2) & 7, left);
+    const int l = threadIdx.x & 63, t = min((l >> 2) & 7, left);   // lane l: four entries of token l / 4 (of the last token there is)
 #pragma unroll
-      for (int m = 0; m < M; ++m) r[m].fetch(a, p[m] + (int64_t)tb * stride[m], __umul24(t, stride[m]) * (unsigned)sizeof(T), 16 * w + 4 * (l & 3));
-    }
+    for (int m = 0; m < M; ++m) r[m].fetch(a, p[m] + (int64_t)tb * stride[m], __umul24(t, stride[m]) * (unsigned)sizeof(T), 16 * w + 4 * (l & 3));
   }
   __device__ __forceinline__ void to_lds(const ScanArgs& a, float (*s)[M][16], int w) const {
-    if constexpr (!SC) {
-      const int l = threadIdx.x & 63;
+    const int l = threadIdx.x & 63;
 #pragma unroll
-      for (int m = 0; m < M; ++m) *(f32x4*)&s[(l >> 2) & 7][m][4 * (l & 3)] = r[m].get(a, 16 * w + 4 * (l & 3));   // (the upper half holds the same)
-    }
+    for (int m = 0; m < M; ++m) *(f32x4*)&s[(l >> 2) & 7][m][4 * (l & 3)] = r[m].get(a, 16 * w + 4 * (l & 3));   // (the upper half holds the same)
   }
-};
-template <typename T, bool SC>
-struct Entries {        // the sixteen of a token
-  Uniform16<T> u;
-  f32x4 v[SC ? 1 : 4];
-  __device__ __forceinline__ void take(const T* p, const float* lds) {
-    if constexpr (SC) {
-      u.load(p);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = ((const f32x4*)lds)[j];
-    }
-  }
-  __device__ __forceinline__ float get(int j, int i) const { return SC ? u.get(4 * j + i) : v[SC ? 0 : j][i]; }
 };
 // decays of a token: the products, then the exponentials (see stage)
 __device__ __forceinline__ void decays(float (*e)[4], float dt, const float (*A2)[4]) {
@@ -459,10 +416,10 @@ __device__ __forceinline__ void decays(float (*e)[4], float dt, const float (*A2
 
 // ------------------------------------------------------------------------------------------------ forward
 // OUT: the pass itself.  Otherwise the walk of a segment from zero: its last state, the sum of its dt, and whether a sequence starts in it.
-template <typename T, int NW, bool OUT, bool SC>
-__global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs a) {
+template <typename T, int NW, bool OUT>
+__global__ __launch_bounds__(64 * NW, 3) void scan_fwd_kernel(ScanArgs a) {
   constexpr int M = OUT ? 2 : 1;
-  __shared__ __attribute__((aligned(16))) float sBC[SC ? 1 : NW][SC ? 1 : kTok][M][16];
+  __shared__ __attribute__((aligned(16))) float sBC[NW][kTok][M][16];
   __shared__ __attribute__((aligned(16))) T sRow[NW][OUT ? 3 : 2][kTok][64];   // u, delta, z
   __shared__ __attribute__((aligned(16))) T sOut[OUT && NW == 1 ? kTok : 1][64];
   __shared__ float sY[NW > 1 && OUT ? 2 : 1][NW > 1 && OUT ? NW : 1][kTok][64];
@@ -485,7 +442,7 @@ __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs a) {
   const T* pd = (const T*)a.delta + row * a.db;
   const T* pz = a.z ? (const T*)a.z + row * a.zb : nullptr;
   T* py = (T*)a.y + (int64_t)row * a.T * a.D_;
-  TokenRows<T, SC, M> bc;
+  TokenRows<T, M> bc;
   bc.p[0] = (const T*)a.Bm + row * a.Bb + (int64_t)ln.group * a.N;
   bc.stride[0] = a.Bt;
   if constexpr (OUT) {
@@ -507,7 +464,7 @@ __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs a) {
     ru.to_lds(sRow[w][0]);
     rd.to_lds(sRow[w][1]);
     if (OUT && a.z) rz.to_lds(sRow[w][OUT ? 2 : 0]);
-    bc.to_lds(a, sBC[SC ? 0 : w], w);
+    bc.to_lds(a, sBC[w], w);
     if constexpr (OUT && NW == 1) {
       if (tb > t0) {
         BlockRows<T> done;
@@ -532,33 +489,27 @@ __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs a) {
         const float z = to_f32(sRow[w][OUT ? 2 : 0][t][l]);
         gate[t] = z * sigmoid_rows<T>(z);
       }
-    const T *rowB = bc.p[0] + (int64_t)tb * bc.stride[0] + 16 * w, *rowC = OUT ? bc.p[M - 1] + (int64_t)tb * bc.stride[M - 1] + 16 * w : nullptr;
     auto walk = [&](auto r) {
-      const T *qB = rowB, *qC = rowC;
-      if (SC) asm volatile("" : "+s"(qB), "+s"(qC));     // (or the addresses of all tokens are computed before the walk, and spilled)
 #pragma unroll
-      for (int t = 0; t < kTok; ++t, qB += bc.stride[0], qC += bc.stride[M - 1]) {
+      for (int t = 0; t < kTok; ++t) {
         if (!walks(r, t)) continue;
-        // B and C are on their way while the decays are computed
-        Entries<T, SC> B, C;
-        B.take(qB, sBC[SC ? 0 : w][SC ? 0 : t][0]);
-        if constexpr (OUT) C.take(qC, sBC[SC ? 0 : w][SC ? 0 : t][1]);
         float dtt = dt[t], e[4][4], s[4];
         settle(dtt);          // (the two walks have the same products, which the compiler would else compute before choosing between them)
         const float x = dtt * uv[t];
+        const f32x4 *B = (const f32x4*)sBC[w][t][0], *C = (const f32x4*)sBC[w][t][M - 1];
         stage();
         decays(e, dtt, A2);
         stage();
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) h[j][i] = fmaf(e[j][i], h[j][i], x * B.get(j, i));
+          for (int i = 0; i < 4; ++i) h[j][i] = fmaf(e[j][i], h[j][i], x * B[j][i]);
         stage();
         if constexpr (OUT) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] = j ? fmaf(C.get(j, i), h[j][i], s[i]) : C.get(j, i) * h[j][i];
+            for (int i = 0; i < 4; ++i) s[i] = j ? fmaf(C[j][i], h[j][i], s[i]) : C[j][i] * h[j][i];
           const float y = (s[0] + s[1]) + (s[2] + s[3]);
           if constexpr (NW == 1) sOut[t][l] = from_f32<T>(fmaf(Dc, uv[t], y) * gate[t]);
           else sY[turn][w][t][l] = y;
@@ -612,11 +563,58 @@ __global__ __launch_bounds__(64 * NW) void scan_fwd_kernel(ScanArgs a) {
   }
 }
 
+// A few tokens: the state is all the traffic, and a wave of the kernel above would wait for one block of it at a time.  Thread = four
+// entries of the state of one channel, in the order of memory; LPC threads a channel add their sums.  256 x 1 tokens of 1536 channels, N 16:
+// 11 to 13 us, 4.1 to 4.8 TB/s (17.5 in the kernel above).
+constexpr int kStepTokens = 4;
+template <int LPC>
+__device__ __forceinline__ float channel_sum(float x) {
+  if constexpr (LPC > 1) x += in_quad<0xB1>(x);
+  if constexpr (LPC > 2) x += in_quad<0x4E>(x);
+  if constexpr (LPC > 4) x += in_quad<0x141>(x);   // row_half_mirror
+  if constexpr (LPC > 8) x += in_quad<0x140>(x);   // row_mirror
+  return x;
+}
+template <typename T, int LPC>
+__global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
+  constexpr int N = 4 * LPC;
+  const int c = blockIdx.x * (256 / LPC) + threadIdx.x / LPC, j = threadIdx.x % LPC, b = blockIdx.y;
+  if (c >= a.D_) return;
+  const int64_t at = ((int64_t)b * a.D_ + c) * N + 4 * j;
+  f32x4 h = {0.f, 0.f, 0.f, 0.f};
+  if (a.init) h = *(const f32x4*)(a.init + at);
+  const f32x4 A = *(const f32x4*)(a.A + (int64_t)c * N + 4 * j);
+  const float bias = a.bias ? a.bias[c] : 0.f, Dc = a.D ? a.D[c] : 0.f;
+  const int64_t bc = (int64_t)(c / a.per_group) * N + 4 * j;
+  typedef typename Raw4<T>::type any __attribute__((aligned(sizeof(T))));
+  for (int t = 0; t < a.T; ++t) {
+    const float u = to_f32(((const T*)a.u)[b * a.ub + (int64_t)t * a.ut + c]);
+    const float raw = to_f32(((const T*)a.delta)[b * a.db + (int64_t)t * a.dt + c]) + bias;
+    const any Bv = *(const any*)((const T*)a.Bm + b * a.Bb + (int64_t)t * a.Bt + bc);
+    const any Cv = *(const any*)((const T*)a.Cm + b * a.Cb + (int64_t)t * a.Ct + bc);
+    float gate = 1.f;
+    if (a.z) {
+      const float z = to_f32(((const T*)a.z)[b * a.zb + (int64_t)t * a.zt + c]);
+      gate = z * sigmoid_rows<T>(z);
+    }
+    const float dt = time_step<T>(raw, a.softplus), x = dt * u;
+    float y = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[i] = fmaf(fast_exp2(dt * (A[i] * kLog2e)), h[i], x * (float)Bv[i]);
+      y = fmaf((float)Cv[i], h[i], y);
+    }
+    y = channel_sum<LPC>(y);
+    if (j == 0) ((T*)a.y)[((int64_t)b * a.T + t) * a.D_ + c] = from_f32<T>(fmaf(Dc, u, y) * gate);
+  }
+  if (a.final_) *(f32x4*)(a.final_ + at) = h;
+}
+
 // What comes back over a segment from its end with nothing coming in: the backward's carry, g <- a (g + C Y) from the last
 // token to the first.
-template <typename T, int NW, bool SC>
+template <typename T, int NW>
 __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) {
-  __shared__ __attribute__((aligned(16))) float sC[SC ? 1 : NW][SC ? 1 : kTok][1][16];
+  __shared__ __attribute__((aligned(16))) float sC[NW][kTok][1][16];
   __shared__ __attribute__((aligned(16))) T sRow[NW][3][kTok][64];   // dy, delta, z
   const Column ln(a);
   const int l = threadIdx.x & 63, w = ln.w, row = ln.row;
@@ -634,7 +632,7 @@ __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) 
   const T* pd = (const T*)a.delta + row * a.db;
   const T* pz = a.z ? (const T*)a.z + row * a.zb : nullptr;
   const T* pg = (const T*)a.dy + (int64_t)row * a.T * a.D_;
-  TokenRows<T, SC, 1> rc;
+  TokenRows<T, 1> rc;
   rc.p[0] = (const T*)a.Cm + row * a.Cb + (int64_t)ln.group * a.N;
   rc.stride[0] = a.Ct;
   BlockRows<T> rg, rd, rz;
@@ -651,7 +649,7 @@ __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) 
     rg.to_lds(sRow[w][0]);
     rd.to_lds(sRow[w][1]);
     if (a.z) rz.to_lds(sRow[w][2]);
-    rc.to_lds(a, sC[SC ? 0 : w], w);
+    rc.to_lds(a, sC[w], w);
     wave_lds_fence();
     if (tb > t0) fetch(tb - kTok);
     const int nt = min(kTok, t1 - tb);
@@ -667,15 +665,11 @@ __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) 
         const float z = to_f32(sRow[w][2][t][l]);
         Y[t] *= z * sigmoid_rows<T>(z);
       }
-    const T* rowC = rc.p[0] + (int64_t)(tb + kTok - 1) * rc.stride[0] + 16 * w;
     auto walk = [&](auto r) {
-      const T* qC = rowC;
-      if (SC) asm volatile("" : "+s"(qC));
 #pragma unroll
-      for (int t = kTok - 1; t >= 0; --t, qC -= rc.stride[0]) {
+      for (int t = kTok - 1; t >= 0; --t) {
         if (!walks(r, t)) continue;
-        Entries<T, SC> C;
-        C.take(qC, sC[SC ? 0 : w][SC ? 0 : t][0]);
+        const f32x4* C = (const f32x4*)sC[w][t][0];
         float dtt = dt[t], e[4][4];
         settle(dtt);          // (as in the forward)
         stage();
@@ -684,7 +678,7 @@ __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) 
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) g[j][i] = fmaf(C.get(j, i), Y[t], g[j][i]);
+          for (int i = 0; i < 4; ++i) g[j][i] = fmaf(C[j][i], Y[t], g[j][i]);
         stage();
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -712,40 +706,72 @@ __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) 
   if (ln.tile == 0 && threadIdx.x == 0) a.seg_cut[slot] = cut;
 }
 
-// From what each segment gives by itself to what each segment starts with (BACK: ends with), in place.  Thread = one float4.
+// From what each segment gives by itself to what each segment starts with (BACK: ends with), in place.  A workgroup has one float4 of
+// every channel of a tile (entries 4 j ..); its waves (up to sixteen) take a run of the segments each: what a run gives by itself goes through
+// LDS, every wave adds up the runs in front of its own, and walks its run again with what it starts with.  One wave over all of the
+// 128 segments of 16384 tokens waited for sixteen batches of loads in turn: 27 us, so split 13.
+constexpr int kJoinWaves = 16, kJoinAhead = 8;
+__device__ __forceinline__ void join_step(float* h, const float* A2, float d, int cut, const f32x4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // (a state of zero stays zero whatever the decay over the segment has overflowed to)
+    const float through = cut || h[i] == 0.f ? 0.f : fast_exp2(A2[i] * d) * h[i];
+    h[i] = through + v[i];
+  }
+}
 template <int NW, bool BACK>
-__global__ __launch_bounds__(256) void scan_join_kernel(ScanArgs a) {
-  const int l = threadIdx.x & 63, k = threadIdx.x >> 6, w = blockIdx.y, tile = blockIdx.x, row = blockIdx.z;
+__global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanArgs a) {
+  __shared__ f32x4 sH[kJoinWaves][64];
+  __shared__ float sD[kJoinWaves][64];
+  __shared__ int sCut[kJoinWaves];
+  const int l = threadIdx.x & 63, v = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int tile = blockIdx.x, w = blockIdx.y >> 2, j = blockIdx.y & 3, row = blockIdx.z;
   const int group = tile / a.tiles_g, base = group * a.per_group + (tile - group * a.tiles_g) * 64;
-  const int chan = min(base + l, (group + 1) * a.per_group - 1), n0 = 16 * w + 4 * k;
-  float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
+  const int chan = min(base + l, (group + 1) * a.per_group - 1), n0 = 16 * w + 4 * j;
+  float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f}, d_sum = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) A2[i] = n0 + i < a.N ? a.A[(int64_t)chan * a.N + n0 + i] * kLog2e : 0.f;
   f32x4* H = (f32x4*)a.seg_h;
-  constexpr int kAhead = 8;
-  for (int b = 0; b < a.segs; b += kAhead) {
-    f32x4 v[kAhead];
-    float d[kAhead];
-    int c[kAhead];
+  const int waves = blockDim.x >> 6, per = (a.segs + waves - 1) / waves, s0 = min(v * per, a.segs), s1 = min(s0 + per, a.segs);
+  int any = 0;
+  constexpr int kAhead = kJoinAhead;
+  f32x4 x[kAhead];
+  float d[kAhead];
+  int c[kAhead];
+  auto slot_of = [&](int s) { return (int64_t)row * a.segs + (BACK ? a.segs - 1 - s : s); };
+  auto fetch = [&](int b) {
 #pragma unroll
-    for (int x = 0; x < kAhead; ++x) {
-      const int s = min(b + x, a.segs - 1);
-      const int64_t slot = (int64_t)row * a.segs + (BACK ? a.segs - 1 - s : s);
-      v[x] = H[packed_at(slot, a, tile, NW, w, k) + l];
-      d[x] = a.seg_dt[(slot * a.tiles + tile) * 64 + l];
-      c[x] = a.seg_cut[slot];
+    for (int y = 0; y < kAhead; ++y) {
+      const int64_t slot = slot_of(min(b + y, a.segs - 1));
+      x[y] = H[packed_at(slot, a, tile, NW, w, j) + l];
+      d[y] = a.seg_dt[(slot * a.tiles + tile) * 64 + l];
+      c[y] = a.seg_cut[slot];
     }
+  };
+  for (int b = s0; b < s1; b += kAhead) {
+    fetch(b);
 #pragma unroll
-    for (int x = 0; x < kAhead; ++x) {
-      if (b + x >= a.segs) break;
-      const int64_t slot = (int64_t)row * a.segs + (BACK ? a.segs - 1 - (b + x) : b + x);
-      H[packed_at(slot, a, tile, NW, w, k) + l] = (f32x4){h[0], h[1], h[2], h[3]};
+    for (int y = 0; y < kAhead; ++y) {
+      if (b + y >= s1) break;
+      join_step(h, A2, d[y], c[y], x[y]);
+      d_sum += d[y];
+      any |= c[y];
+    }
+  }
+  sH[v][l] = (f32x4){h[0], h[1], h[2], h[3]};
+  sD[v][l] = d_sum;
+  if (l == 0) sCut[v] = any;
+  __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // (a state of zero stays zero whatever the decay over the segment has overflowed to)
-        const float through = c[x] || h[i] == 0.f ? 0.f : fast_exp2(A2[i] * d[x]) * h[i];
-        h[i] = through + v[x][i];
-      }
+  for (int i = 0; i < 4; ++i) h[i] = 0.f;
+  for (int y = 0; y < v; ++y) join_step(h, A2, sD[y][l], sCut[y], sH[y][l]);
+  for (int b = s0; b < s1; b += kAhead) {
+    if (per > kAhead) fetch(b);       // (else they are still in registers)
+#pragma unroll
+    for (int y = 0; y < kAhead; ++y) {
+      if (b + y >= s1) break;
+      H[packed_at(slot_of(b + y), a, tile, NW, w, j) + l] = (f32x4){h[0], h[1], h[2], h[3]};
+      join_step(h, A2, d[y], c[y], x[y]);
     }
   }
 }
@@ -1043,36 +1069,47 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
   pc[1] = dbias;
 }
 
-// dB, dC [rows, T, G, N]: the tiles of a group in their order
+// dB, dC [rows, T, G, N]: the tiles of a group in their order.  Thread = four entries of a token.
 template <typename T>
 __global__ __launch_bounds__(256) void scan_bwd_rows_kernel(ScanArgs a, int nw) {
-  const int64_t per = 2 * (int64_t)a.G * a.N, total = (int64_t)a.rows * a.T * per;
+  const int64_t per = 2 * (int64_t)a.G * nw * 4, total = (int64_t)a.rows * a.T * per;
   for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < total; x += (int64_t)gridDim.x * 256) {
     const int64_t tok = x / per;
-    const int r = (int)(x - tok * per), which = r >= a.G * a.N, gn = r - which * a.G * a.N, g = gn / a.N, n = gn - g * a.N;
-    const float* p = a.part_bc + ((tok * a.tiles + (int64_t)g * a.tiles_g) * nw + (n >> 4)) * 32 + which * 16 + (n & 15);
-    float s = 0.f;
-    for (int i = 0; i < a.tiles_g; ++i) s += p[(int64_t)i * nw * 32];
-    ((T*)(which ? a.dC : a.dB))[tok * a.G * a.N + gn] = from_f32<T>(s);
+    const int r = (int)(x - tok * per), j = r & 3, which = (r >> 2) & 1, w = (r >> 3) % nw, g = (r >> 3) / nw, n = 16 * w + 4 * j;
+    const f32x4* p = (const f32x4*)(a.part_bc + ((tok * a.tiles + (int64_t)g * a.tiles_g) * nw + w) * 32 + which * 16 + 4 * j);
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < a.tiles_g; i0 += 8) {
+      f32x4 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = p[(int64_t)min(i0 + i, a.tiles_g - 1) * nw * 8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i0 + i < a.tiles_g) s += v[i];
+    }
+    T* out = (T*)(which ? a.dC : a.dB) + (tok * a.G + g) * a.N + n;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.N) out[i] = from_f32<T>(s[i]);
   }
 }
 
 // dA, dD, ddelta_bias: the segments of all rows in their order, in 64 bits.  grid (tiles, waves of a tile, 5): z < 4 the entries
-// 4 z .. of dA, z = 4 dD and ddelta_bias; four waves take a quarter of the segments each.
-__global__ __launch_bounds__(256) void scan_bwd_params_kernel(ScanArgs a, int nw) {
-  __shared__ double s[4][64][4];
+// 4 z .. of dA, z = 4 dD and ddelta_bias; sixteen waves take a share of the segments each.
+constexpr int kParamWaves = 16;
+__global__ __launch_bounds__(64 * kParamWaves) void scan_bwd_params_kernel(ScanArgs a, int nw) {
+  __shared__ double s[kParamWaves][64][4];
   const int l = threadIdx.x & 63, v = threadIdx.x >> 6, tile = blockIdx.x, w = blockIdx.y, z = blockIdx.z;
   const int64_t slots = (int64_t)a.rows * a.segs;
   const int group = tile / a.tiles_g, base = group * a.per_group + (tile - group * a.tiles_g) * 64, end = (group + 1) * a.per_group;
   double t[4] = {0., 0., 0., 0.};
   if (z < 4) {
-    for (int64_t i = v; i < slots; i += 4) {
+    for (int64_t i = v; i < slots; i += kParamWaves) {
       const f32x4 x = ((const f32x4*)a.part_a)[packed_at(i, a, tile, nw, w, z) + l];
 #pragma unroll
       for (int e = 0; e < 4; ++e) t[e] += x[e];
     }
   } else if (w == 0) {
-    for (int64_t i = v; i < slots; i += 4)
+    for (int64_t i = v; i < slots; i += kParamWaves)
       for (int k = 0; k < nw; ++k) {
         const float* p = a.part_c + (((i * a.tiles + tile) * nw + k) * 64 + l) * 2;
         t[0] += p[0];
@@ -1084,7 +1121,10 @@ __global__ __launch_bounds__(256) void scan_bwd_params_kernel(ScanArgs a, int nw
   __syncthreads();
   if (v) return;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) t[e] = s[0][l][e] + s[1][l][e] + s[2][l][e] + s[3][l][e];
+  for (int e = 0; e < 4; ++e) {
+    t[e] = 0.;
+    for (int x = 0; x < kParamWaves; ++x) t[e] += s[x][l][e];
+  }
   if (z < 4) {
     const int c = base + l, n0 = 16 * w + 4 * z;
     if (c < end)
@@ -1158,11 +1198,6 @@ static void scan_args(ScanArgs& a, const PalScanDims* d, const PalScanTensors* t
   if (!t) return;
   a.u = t->u; a.delta = t->delta; a.z = t->z; a.Bm = t->B; a.Cm = t->C;
   a.A = t->A; a.D = t->D; a.bias = t->delta_bias; a.init = t->init;
-  // rows of B and C that the scalar unit reads
-  auto words = [&](const void* p, int64_t batch, int64_t token) {
-    return d->dtype == PAL_DTYPE_F32 || ((uintptr_t)p % 4 == 0 && batch % 2 == 0 && token % 2 == 0);
-  };
-  a.scalar = d->state % 16 == 0 && words(t->B, d->B_batch, d->B_token) && words(t->C, d->C_batch, d->C_token);
   a.y = t->y; a.final_ = t->final_; a.ckpt = t->checkpoints; a.cu = t->cu_seqlens;
 }
 static size_t up256b(size_t x) { return (x + 255) / 256 * 256; }
@@ -1182,44 +1217,58 @@ static char* place_segments(ScanArgs& a, int nw, char* p) {
   return p + up256b((size_t)slots * 4);
 }
 
-template <typename T, int NW, bool SC>
-static int scan_fwd_launch(const ScanArgs& a, hipStream_t s) {
-  const dim3 grid(a.tiles, a.segs, a.rows);
-  if (a.segs > 1) {
-    PAL_TIMED_LAUNCH(kKernScanSegment, s, (scan_fwd_kernel<T, NW, false, SC>), grid, dim3(64 * NW), 0, s, a);
-    PAL_HIP_LAUNCH_CHECK();
-    PAL_TIMED_LAUNCH(kKernScanJoin, s, (scan_join_kernel<NW, false>), dim3(a.tiles, NW, a.rows), dim3(256), 0, s, a);
-    PAL_HIP_LAUNCH_CHECK();
-  }
-  PAL_TIMED_LAUNCH(kKernScanFwd, s, (scan_fwd_kernel<T, NW, true, SC>), grid, dim3(64 * NW), 0, s, a);
+// waves over the segments of a join: a batch of loads each, up to kJoinWaves
+static int join_waves(const ScanArgs& a) {
+  const int w = (a.segs + kJoinAhead - 1) / kJoinAhead;
+  return w < kJoinWaves ? w : kJoinWaves;
+}
+template <typename T, int LPC>
+static int scan_step_run(const ScanArgs& a, hipStream_t s) {
+  const int per = 256 / LPC;
+  PAL_TIMED_LAUNCH(kKernScanFwd, s, (scan_step_kernel<T, LPC>), dim3((a.D_ + per - 1) / per, a.rows), dim3(256), 0, s, a);
   PAL_HIP_LAUNCH_CHECK();
   return PAL_OK;
 }
 template <typename T, int NW>
 static int scan_fwd_run(const ScanArgs& a, hipStream_t s) {
-  return a.scalar ? scan_fwd_launch<T, NW, true>(a, s) : scan_fwd_launch<T, NW, false>(a, s);
+  const dim3 grid(a.tiles, a.segs, a.rows);
+  if (a.segs > 1) {
+    PAL_TIMED_LAUNCH(kKernScanSegment, s, (scan_fwd_kernel<T, NW, false>), grid, dim3(64 * NW), 0, s, a);
+    PAL_HIP_LAUNCH_CHECK();
+    PAL_TIMED_LAUNCH(kKernScanJoin, s, (scan_join_kernel<NW, false>), dim3(a.tiles, 4 * NW, a.rows), dim3(64 * join_waves(a)), 0, s, a);
+    PAL_HIP_LAUNCH_CHECK();
+  }
+  PAL_TIMED_LAUNCH(kKernScanFwd, s, (scan_fwd_kernel<T, NW, true>), grid, dim3(64 * NW), 0, s, a);
+  PAL_HIP_LAUNCH_CHECK();
+  return PAL_OK;
 }
 template <typename T, int NW>
 static int scan_bwd_run(const ScanArgs& a, hipStream_t s) {
   const dim3 grid(a.tiles, a.segs, a.rows);
   if (a.segs > 1) {
-    if (a.scalar) PAL_TIMED_LAUNCH(kKernScanSegment, s, (scan_back_segment_kernel<T, NW, true>), grid, dim3(64 * NW), 0, s, a);
-    else PAL_TIMED_LAUNCH(kKernScanSegment, s, (scan_back_segment_kernel<T, NW, false>), grid, dim3(64 * NW), 0, s, a);
+    PAL_TIMED_LAUNCH(kKernScanSegment, s, (scan_back_segment_kernel<T, NW>), grid, dim3(64 * NW), 0, s, a);
     PAL_HIP_LAUNCH_CHECK();
-    PAL_TIMED_LAUNCH(kKernScanJoin, s, (scan_join_kernel<NW, true>), dim3(a.tiles, NW, a.rows), dim3(256), 0, s, a);
+    PAL_TIMED_LAUNCH(kKernScanJoin, s, (scan_join_kernel<NW, true>), dim3(a.tiles, 4 * NW, a.rows), dim3(64 * join_waves(a)), 0, s, a);
     PAL_HIP_LAUNCH_CHECK();
   }
   PAL_TIMED_LAUNCH(kKernScanBwd, s, (scan_bwd_kernel<T, NW>), grid, dim3(64 * NW), 0, s, a);
   PAL_HIP_LAUNCH_CHECK();
-  const int64_t n = 2 * (int64_t)a.rows * a.T * a.G * a.N, blocks = (n + 255) / 256;
+  const int64_t n = 8 * (int64_t)a.rows * a.T * a.G * NW, blocks = (n + 255) / 256;
   PAL_TIMED_LAUNCH(kKernScanBwdRows, s, scan_bwd_rows_kernel<T>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, a, NW);
   PAL_HIP_LAUNCH_CHECK();
-  PAL_TIMED_LAUNCH(kKernScanBwdParams, s, scan_bwd_params_kernel, dim3(a.tiles, NW, 5), dim3(256), 0, s, a, NW);
+  PAL_TIMED_LAUNCH(kKernScanBwdParams, s, scan_bwd_params_kernel, dim3(a.tiles, NW, 5), dim3(64 * kParamWaves), 0, s, a, NW);
   PAL_HIP_LAUNCH_CHECK();
   return PAL_OK;
 }
 template <typename T>
 static int scan_fwd_waves(const ScanArgs& a, int nw, hipStream_t s) {
+  if (a.T <= kStepTokens && !a.cu && !a.ckpt) {
+    if (a.N == 4) return scan_step_run<T, 1>(a, s);
+    if (a.N == 8) return scan_step_run<T, 2>(a, s);
+    if (a.N == 16) return scan_step_run<T, 4>(a, s);
+    if (a.N == 32) return scan_step_run<T, 8>(a, s);
+    if (a.N == 64) return scan_step_run<T, 16>(a, s);
+  }
   switch (nw) {
     case 1: return scan_fwd_run<T, 1>(a, s);
     case 2: return scan_fwd_run<T, 2>(a, s);
@@ -1264,7 +1313,7 @@ extern "C" int pal_scan_fwd(const PalScanDims* d, const PalScanTensors* t, void*
   ScanArgs a{};
   scan_args(a, d, t, false);
   const int nw = scan_waves(d);
-  if (a.segs > 65535 || a.tiles > (1 << 24)) return PAL_E_DIM;
+  if (a.segs > 65535 || (int64_t)a.tiles * nw > 1 << 20) return PAL_E_DIM;   // (the second: 32-bit places in a block's shares)
   if (a.segs > 1) {
     if (!workspace || workspace_bytes < seg_bytes(a, nw)) return PAL_E_WORKSPACE;
     if (!is_aligned16(workspace)) return PAL_E_ALIGN;
@@ -1301,7 +1350,7 @@ extern "C" int pal_scan_bwd(const PalScanDims* d, const PalScanTensors* t, const
   ScanArgs a{};
   scan_args(a, d, t, true);
   const int nw = scan_waves(d);
-  if (a.segs > 65535 || a.tiles > (1 << 24)) return PAL_E_DIM;
+  if (a.segs > 65535 || (int64_t)a.tiles * nw > 1 << 20) return PAL_E_DIM;   // (the second: 32-bit places in a block's shares)
   a.dy = gr->dy; a.d_final = gr->d_final; a.du = gr->du; a.ddelta = gr->ddelta; a.dA = gr->dA; a.dB = gr->dB; a.dC = gr->dC;
   a.dD = gr->dD; a.dz = gr->dz; a.dbias = gr->ddelta_bias; a.d_init = gr->d_init;
   char* p = (char*)workspace;
