@@ -877,6 +877,10 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
     for (int t = 0; t < kTok; ++t)
       if (t % NW == w) sDt[t][l] = time_step<T>(to_f32(sRow[1][t][own]) + bias, a.softplus);
     sync();
+    // A whole block in which no sequence starts or ends is straight code: one path for the registers that are carried from block to
+    // block.  (Loops around it, over parts and over pairs of tokens, moved them, 16 states, 16 decays' gradients and the 16 states on
+    // their way from memory, between two sets on every round, and waited for the last.)
+    const bool plain = nt == kTok && cur.s < tb && cur.e > tb + kTok;
     {
       float h[4][4];
 #pragma unroll
@@ -901,20 +905,21 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
           }
         }
       };
-      const int most = min(nt, kTok - kSub);
-      ScanSeq fw = cur.s <= tb ? cur : seq_at(a, row, tb);
+      if (plain) walk(Whole{0, 0});
+      const int most = plain ? 0 : min(nt, kTok - kSub);
+      ScanSeq fw = plain || cur.s <= tb ? cur : seq_at(a, row, tb);
       for (int lo = 0, hi; lo < most; lo = hi) {
         if (tb + lo == fw.s) load_state(a, ln, a.init, fw.n, h);
         hi = max(lo + 1, min(most, fw.e - tb));
-        if (hi - lo == kTok - kSub) walk(Whole{0, 0});
-        else walk(Part{lo, hi});
+        walk(Part{lo, hi});
         if (hi < most) fw = next_seq(a, fw);
       }
     }
     wave_lds_fence();
     // ---- two tokens at a time from the end
-    for (int sub = (nt - 1) / kSub; sub >= 0; --sub) {
-      const int ts = tb + sub * kSub, ns = min(kSub, t1 - ts);
+    auto pair = [&](auto kind, int sub) __attribute__((always_inline)) {
+      constexpr bool whole = decltype(kind)::whole;
+      const int ts = tb + sub * kSub, ns = whole ? kSub : min(kSub, t1 - ts);
       // what the tokens take and, in the same place, what they give once they are done: Y -> du, slope (of the softplus) -> ddelta,
       // gz (dy silu'(z)) -> dz
       float uv[kSub], Y[kSub], slope[kSub], gz[kSub];
@@ -945,7 +950,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
         sRow[2][sub * kSub + t][own] = from_f32<T>(gz[t]);
       };
       float h[4][4];
-      auto walk = [&](auto r, bool ends) {
+      auto walk = [&](auto r, bool ends) __attribute__((always_inline)) {
         float av[kSub][4][4], ah[kSub][4][4];
 #pragma unroll
         for (int t = 0; t < kSub; ++t) {
@@ -963,7 +968,14 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
               h[k][i] = fmaf(xk[k], Bv[i], ah[t][k][i]);
             }
         }
-        if (ends) load_state(a, ln, a.d_final, cur.n, carry);
+        if constexpr (whole) {
+          if (sub == 0) {      // h0 is used up: the next block's (or the last one's again), while the last two tokens of this one are walked
+            stage();
+            fetch_kept(max(tb - kTok, t0));
+          }
+        } else if (ends) {
+          load_state(a, ln, a.d_final, cur.n, carry);
+        }
 #pragma unroll
         for (int t = kSub - 1; t >= 0; --t) {
           if (!walks(r, t)) continue;
@@ -1011,34 +1023,31 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
           }
         }
       };
-      for (int hi = ns, lo; hi > 0; hi = lo) {
-        lo = min(hi - 1, max(0, cur.s - ts));
-        if (ts + lo == cur.s) {
-          load_state(a, ln, a.init, cur.n, h);
-          if (sub == 0 && lo == 0 && tb > t0) fetch_kept(tb - kTok);
-        } else if (sub == 0) {
+      auto start = [&]() {      // the state before the pair
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < 4; ++k) {
+          const f32x4 v = sub ? sH[w][max(sub - 1, 0)][k][l] : (f32x4){h0[k][0], h0[k][1], h0[k][2], h0[k][3]};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[k][i] = h0[k][i];
-          // the next block's while the last two tokens of this one are walked: fetched with its rows it would need registers of its own
-          if (tb > t0) fetch_kept(tb - kTok);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const f32x4 v = sH[w][sub - 1][k][l];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) h[k][i] = v[i];
-          }
+          for (int i = 0; i < 4; ++i) h[k][i] = v[i];
         }
-        if (hi - lo == kSub) walk(Whole{0, 0}, ts + hi == cur.e);
-        else walk(Part{lo, hi}, ts + hi == cur.e);
-        if (ts + lo == cur.s) {
-          if (a.d_init) store_state(a, ln, a.d_init, cur.n, carry);
-          if (a.cu) {
-            const ScanSeq prev = prev_seq(a, cur);
-            hand_over(a, ln, a.d_final, a.d_init, prev.n + 1, cur.n);
-            cur = prev;
+      };
+      if constexpr (whole) {
+        start();
+        walk(kind, false);
+        settle44(dA);       // (or the sums of all pairs are put off to the last one, and what goes into them is kept)
+      } else {
+        for (int hi = ns, lo; hi > 0; hi = lo) {
+          lo = min(hi - 1, max(0, cur.s - ts));
+          if (ts + lo == cur.s) load_state(a, ln, a.init, cur.n, h);
+          else start();
+          walk(Part{lo, hi}, ts + hi == cur.e);
+          if (ts + lo == cur.s) {
+            if (a.d_init) store_state(a, ln, a.d_init, cur.n, carry);
+            if (a.cu) {
+              const ScanSeq prev = prev_seq(a, cur);
+              hand_over(a, ln, a.d_final, a.d_init, prev.n + 1, cur.n);
+              cur = prev;
+            }
           }
         }
       }
@@ -1058,6 +1067,13 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
         }
         turn ^= 1;
       }
+    };
+    if (plain) {
+#pragma unroll
+      for (int sub = kTok / kSub - 1; sub >= 0; --sub) pair(Whole{0, 0}, sub);
+    } else {
+      for (int sub = (nt - 1) / kSub; sub >= 0; --sub) pair(Part{0, 0}, sub);
+      fetch_kept(max(tb - kTok, t0));
     }
     sync();
   }
