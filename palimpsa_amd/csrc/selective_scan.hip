@@ -68,14 +68,46 @@ __device__ __forceinline__ float log1p_full(float e) {
   const float s = 1.f + e;
   return fmaf(__builtin_amdgcn_logf(s), 0.6931471806f, __builtin_amdgcn_fmed3f(e - (s - 1.f), -0x1p-24f, 0x1p-24f));
 }
-// time step from the raw one (already with its bias); softplus is the identity above 20, as torch computes it (and for a NaN)
-template <typename T>
-__device__ __forceinline__ float time_step(float raw, int softplus) {
-  const float s = log1p_full(exp_rows<T>(raw));
-  return softplus && raw <= 20.f ? s : raw;
+// Nothing is moved across by the scheduler.  Independent values go through each kind of operation together: left alone, the scheduler
+// walks value by value to save registers, and the product, its exponential and what uses that wait for each other.
+__device__ __forceinline__ void stage() { __builtin_amdgcn_sched_barrier(0); }
+template <typename T, int K>
+__device__ __forceinline__ void exp_rows(const float* x, float* e) {
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int i = 0; i < K; ++i) e[i] = exp_full(x[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < K; ++i) e[i] = x[i] * kLog2e;
+    stage();
+#pragma unroll
+    for (int i = 0; i < K; ++i) e[i] = fast_exp2(e[i]);
+  }
+  stage();
 }
-template <typename T>
-__device__ __forceinline__ float sigmoid_rows(float x) { return fast_rcp(1.f + exp_rows<T>(-x)); }
+// K time steps from the raw ones (with their bias); softplus is the identity above 20, as torch computes it (and for a NaN)
+template <typename T, int K>
+__device__ __forceinline__ void time_steps(const float* raw, float* dt, int softplus) {
+  float e[K];
+  exp_rows<T, K>(raw, e);
+#pragma unroll
+  for (int i = 0; i < K; ++i) e[i] = log1p_full(e[i]);
+#pragma unroll
+  for (int i = 0; i < K; ++i) dt[i] = softplus && raw[i] <= 20.f ? e[i] : raw[i];
+}
+// K logistic functions
+template <typename T, int K>
+__device__ __forceinline__ void sigmoids(const float* x, float* sg) {
+  float m[K], e[K];
+#pragma unroll
+  for (int i = 0; i < K; ++i) m[i] = -x[i];
+  exp_rows<T, K>(m, e);
+#pragma unroll
+  for (int i = 0; i < K; ++i) e[i] += 1.f;
+  stage();
+#pragma unroll
+  for (int i = 0; i < K; ++i) sg[i] = fast_rcp(e[i]);
+}
 
 // ------------------------------------------------------------------------------------------------ lanes
 // lane 4 q + j of a wave: channels 16 k + q (k = 0 .. 3) by entries 4 j + i (i = 0 .. 3) of the state; its own channel is 16 j + q
@@ -285,10 +317,6 @@ __device__ __forceinline__ void zero44(float (*x)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[k][i] = 0.f;
 }
-// Nothing is moved across by the scheduler.  The sixteen entries of a lane go through each kind of operation together: left alone,
-// the scheduler walks entry by entry to save registers, and the product, its exponential and what uses that wait for
-// each other.
-__device__ __forceinline__ void stage() { __builtin_amdgcn_sched_barrier(0); }
 __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -423,7 +451,8 @@ __global__ __launch_bounds__(64 * NW, 3) void scan_fwd_kernel(ScanArgs a) {
   __shared__ __attribute__((aligned(16))) T sRow[NW][OUT ? 3 : 2][kTok][64];   // u, delta, z
   __shared__ __attribute__((aligned(16))) T sOut[OUT && NW == 1 ? kTok : 1][64];
   __shared__ float sY[NW > 1 && OUT ? 2 : 1][NW > 1 && OUT ? NW : 1][kTok][64];
-  const Column ln(a);
+  Column ln(a);
+  if (NW == 1) ln.w = 0;      // (known to the compiler)
   const int l = threadIdx.x & 63, w = ln.w, row = ln.row;
   const int t0 = blockIdx.y * a.seg, t1 = min(a.T, t0 + a.seg);
   const float bias = a.bias ? a.bias[ln.own] : 0.f, Dc = a.D ? a.D[ln.own] : 0.f;
@@ -476,19 +505,23 @@ __global__ __launch_bounds__(64 * NW, 3) void scan_fwd_kernel(ScanArgs a) {
     wave_lds_fence();
     if (tb + kTok < t1) fetch(tb + kTok);
     const int nt = min(kTok, t1 - tb);
-    float dt[kTok], uv[kTok], gate[kTok];
+    float dt[kTok], uv[kTok], gate[kTok], raw[kTok];
 #pragma unroll
     for (int t = 0; t < kTok; ++t) {
       uv[t] = to_f32(sRow[w][0][t][l]);
-      dt[t] = time_step<T>(to_f32(sRow[w][1][t][l]) + bias, a.softplus);
+      raw[t] = to_f32(sRow[w][1][t][l]) + bias;
       gate[t] = 1.f;
     }
-    if (OUT && a.z)
+    stage();
+    time_steps<T, kTok>(raw, dt, a.softplus);
+    if (OUT && a.z) {
 #pragma unroll
-      for (int t = 0; t < kTok; ++t) {
-        const float z = to_f32(sRow[w][OUT ? 2 : 0][t][l]);
-        gate[t] = z * sigmoid_rows<T>(z);
-      }
+      for (int t = 0; t < kTok; ++t) raw[t] = to_f32(sRow[w][OUT ? 2 : 0][t][l]);
+      stage();
+      sigmoids<T, kTok>(raw, gate);
+#pragma unroll
+      for (int t = 0; t < kTok; ++t) gate[t] *= raw[t];
+    }
     auto walk = [&](auto r) {
 #pragma unroll
       for (int t = 0; t < kTok; ++t) {
@@ -595,9 +628,12 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
     float gate = 1.f;
     if (a.z) {
       const float z = to_f32(((const T*)a.z)[b * a.zb + (int64_t)t * a.zt + c]);
-      gate = z * sigmoid_rows<T>(z);
+      sigmoids<T, 1>(&z, &gate);
+      gate *= z;
     }
-    const float dt = time_step<T>(raw, a.softplus), x = dt * u;
+    float dt;
+    time_steps<T, 1>(&raw, &dt, a.softplus);
+    const float x = dt * u;
     float y = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -616,7 +652,8 @@ template <typename T, int NW>
 __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) {
   __shared__ __attribute__((aligned(16))) float sC[NW][kTok][1][16];
   __shared__ __attribute__((aligned(16))) T sRow[NW][3][kTok][64];   // dy, delta, z
-  const Column ln(a);
+  Column ln(a);
+  if (NW == 1) ln.w = 0;      // (known to the compiler)
   const int l = threadIdx.x & 63, w = ln.w, row = ln.row;
   const int t0 = blockIdx.y * a.seg, t1 = min(a.T, t0 + a.seg);
   const float bias = a.bias ? a.bias[ln.own] : 0.f;
@@ -653,18 +690,23 @@ __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) 
     wave_lds_fence();
     if (tb > t0) fetch(tb - kTok);
     const int nt = min(kTok, t1 - tb);
-    float dt[kTok], Y[kTok];
+    float dt[kTok], Y[kTok], raw[kTok];
 #pragma unroll
     for (int t = 0; t < kTok; ++t) {
-      dt[t] = time_step<T>(to_f32(sRow[w][1][t][l]) + bias, a.softplus);
+      raw[t] = to_f32(sRow[w][1][t][l]) + bias;
       Y[t] = to_f32(sRow[w][0][t][l]);
     }
-    if (a.z)
+    stage();
+    time_steps<T, kTok>(raw, dt, a.softplus);
+    if (a.z) {
+      float sg[kTok];
 #pragma unroll
-      for (int t = 0; t < kTok; ++t) {
-        const float z = to_f32(sRow[w][2][t][l]);
-        Y[t] *= z * sigmoid_rows<T>(z);
-      }
+      for (int t = 0; t < kTok; ++t) raw[t] = to_f32(sRow[w][2][t][l]);
+      stage();
+      sigmoids<T, kTok>(raw, sg);
+#pragma unroll
+      for (int t = 0; t < kTok; ++t) Y[t] *= raw[t] * sg[t];
+    }
     auto walk = [&](auto r) {
 #pragma unroll
       for (int t = kTok - 1; t >= 0; --t) {
@@ -788,7 +830,8 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
   __shared__ f32x4 sH[NW][kTok / kSub - 1][4][64];
   __shared__ __attribute__((aligned(16))) float sP[NW][kTok][32];   // the waves' shares of dB and dC
   __shared__ float sS[NW > 1 ? 2 : 1][NW > 1 ? NW : 1][kSub][3][64];
-  const Lane ln(a);
+  Lane ln(a);
+  if (NW == 1) ln.w = 0;      // (known to the compiler)
   const int l = threadIdx.x & 63, w = ln.w, row = ln.row, own = own_at();
   const int t0 = blockIdx.y * a.seg, t1 = min(a.T, t0 + a.seg);
   const float bias = a.bias ? a.bias[ln.own] : 0.f, Dc = a.D ? a.D[ln.own] : 0.f;
@@ -807,6 +850,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
   if (t1 == a.T && a.cu) hand_over(a, ln, a.d_final, a.d_init, cur.n + 1, a.seqs);   // sequences without a token behind the last one
   const int64_t out0 = (int64_t)row * a.T * a.D_;
   const int shares = ((l >> 4) & 1) * 16 + 4 * (l & 3) + ((l >> 2) & 1) * 2 + ((l >> 3) & 1);   // a lane's sum among dB and dC (below)
+  const bool has_z = a.z != nullptr;
   int turn = 0;
   auto sync = [&]() {
     if constexpr (NW == 1) wave_lds_fence();
@@ -869,19 +913,27 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
     }
     *(f32x4*)&sBC[w][(l >> 2) & 7][0][4 * (l & 3)] = rb.get(a, n4);
     *(f32x4*)&sBC[w][(l >> 2) & 7][1][4 * (l & 3)] = rc.get(a, n4);
+    settle44(h0);      // (older than the next fetch: waited for behind it, it would take that with it)
     sync();
     // (the stores after the wait for this block's rows and before the next fetch: they are never waited for by themselves)
     if (tb < last) put(tb + kTok, min(kTok, t1 - tb - kTok));
     if (tb > t0) fetch(tb - kTok);
+    {
+      constexpr int K = (kTok + NW - 1) / NW;      // tokens of a wave (the last one again where they do not share out)
+      float raw[K], dt[K];
 #pragma unroll
-    for (int t = 0; t < kTok; ++t)
-      if (t % NW == w) sDt[t][l] = time_step<T>(to_f32(sRow[1][t][own]) + bias, a.softplus);
+      for (int i = 0; i < K; ++i) raw[i] = to_f32(sRow[1][min(w + NW * i, kTok - 1)][own]) + bias;
+      stage();
+      time_steps<T, K>(raw, dt, a.softplus);
+#pragma unroll
+      for (int i = 0; i < K; ++i) sDt[min(w + NW * i, kTok - 1)][l] = dt[i];
+    }
     sync();
     // A whole block in which no sequence starts or ends is straight code: one path for the registers that are carried from block to
     // block.  (Loops around it, over parts and over pairs of tokens, moved them, 16 states, 16 decays' gradients and the 16 states on
     // their way from memory, between two sets on every round, and waited for the last.)
     const bool plain = nt == kTok && cur.s < tb && cur.e > tb + kTok;
-    {
+    auto states = [&](auto kind) __attribute__((always_inline)) {
       float h[4][4];
 #pragma unroll
       for (int k = 0; k < 4; ++k)
@@ -905,17 +957,19 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
           }
         }
       };
-      if (plain) walk(Whole{0, 0});
-      const int most = plain ? 0 : min(nt, kTok - kSub);
-      ScanSeq fw = plain || cur.s <= tb ? cur : seq_at(a, row, tb);
-      for (int lo = 0, hi; lo < most; lo = hi) {
-        if (tb + lo == fw.s) load_state(a, ln, a.init, fw.n, h);
-        hi = max(lo + 1, min(most, fw.e - tb));
-        walk(Part{lo, hi});
-        if (hi < most) fw = next_seq(a, fw);
+      if constexpr (decltype(kind)::whole) {
+        walk(kind);
+      } else {
+        const int most = min(nt, kTok - kSub);
+        ScanSeq fw = seq_at(a, row, tb);     // (`cur` where that is the one would put it into memory, for the choice between two addresses)
+        for (int lo = 0, hi; lo < most; lo = hi) {
+          if (tb + lo == fw.s) load_state(a, ln, a.init, fw.n, h);
+          hi = max(lo + 1, min(most, fw.e - tb));
+          walk(Part{lo, hi});
+          if (hi < most) fw = next_seq(a, fw);
+        }
       }
-    }
-    wave_lds_fence();
+    };
     // ---- two tokens at a time from the end
     auto pair = [&](auto kind, int sub) __attribute__((always_inline)) {
       constexpr bool whole = decltype(kind)::whole;
@@ -923,21 +977,23 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
       // what the tokens take and, in the same place, what they give once they are done: Y -> du, slope (of the softplus) -> ddelta,
       // gz (dy silu'(z)) -> dz
       float uv[kSub], Y[kSub], slope[kSub], gz[kSub];
+      float x2[2 * kSub], sg[2 * kSub];      // raw time steps and gates (without z: whatever is there, and not used)
 #pragma unroll
       for (int t = 0; t < kSub; ++t) {
-        const float raw = to_f32(sRow[1][sub * kSub + t][own]) + bias, sg = sigmoid_rows<T>(raw);
+        x2[t] = to_f32(sRow[1][sub * kSub + t][own]) + bias;
+        x2[kSub + t] = to_f32(sRow[2][sub * kSub + t][own]);
         uv[t] = to_f32(sRow[0][sub * kSub + t][own]);
         Y[t] = to_f32(sRow[3][sub * kSub + t][own]);
-        slope[t] = a.softplus && raw <= 20.f ? sg : 1.f;
-        gz[t] = 0.f;
       }
-      if (a.z)
+      stage();
+      sigmoids<T, 2 * kSub>(x2, sg);
 #pragma unroll
-        for (int t = 0; t < kSub; ++t) {
-          const float z = to_f32(sRow[2][sub * kSub + t][own]), sg = sigmoid_rows<T>(z);
-          gz[t] = Y[t] * (sg + z * sg * (1.f - sg));
-          Y[t] *= z * sg;
-        }
+      for (int t = 0; t < kSub; ++t) {
+        slope[t] = a.softplus && x2[t] <= 20.f ? sg[t] : 1.f;
+        const float z = x2[kSub + t], s = sg[kSub + t];
+        gz[t] = has_z ? Y[t] * (s + z * s * (1.f - s)) : 0.f;
+        Y[t] *= has_z ? z * s : 1.f;
+      }
       auto finish = [&](int t, float dt, float ypre, float sumB, float sumA) {
         const float ddt = fmaf(uv[t], sumB, sumA * 0.6931471806f);
         gz[t] *= fmaf(Dc, uv[t], ypre);
@@ -1069,9 +1125,13 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
       }
     };
     if (plain) {
+      states(Whole{0, 0});
+      wave_lds_fence();
 #pragma unroll
       for (int sub = kTok / kSub - 1; sub >= 0; --sub) pair(Whole{0, 0}, sub);
     } else {
+      states(Part{0, 0});
+      wave_lds_fence();
       for (int sub = (nt - 1) / kSub; sub >= 0; --sub) pair(Part{0, 0}, sub);
       fetch_kept(max(tb - kTok, t0));
     }
