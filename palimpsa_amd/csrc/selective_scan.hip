@@ -919,14 +919,15 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
     if (tb < last) put(tb + kTok, min(kTok, t1 - tb - kTok));
     if (tb > t0) fetch(tb - kTok);
     {
-      constexpr int K = (kTok + NW - 1) / NW;      // tokens of a wave (the last one again where they do not share out)
+      constexpr int K = (kTok + NW - 1) / NW;      // tokens of a wave (three waves: one token twice)
+      const int first = min(K * w, kTok - K);
       float raw[K], dt[K];
 #pragma unroll
-      for (int i = 0; i < K; ++i) raw[i] = to_f32(sRow[1][min(w + NW * i, kTok - 1)][own]) + bias;
+      for (int i = 0; i < K; ++i) raw[i] = to_f32(sRow[1][first + i][own]) + bias;
       stage();
       time_steps<T, K>(raw, dt, a.softplus);
 #pragma unroll
-      for (int i = 0; i < K; ++i) sDt[min(w + NW * i, kTok - 1)][l] = dt[i];
+      for (int i = 0; i < K; ++i) sDt[first + i][l] = dt[i];
     }
     sync();
     // A whole block in which no sequence starts or ends is straight code: one path for the registers that are carried from block to
@@ -1134,6 +1135,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
       wave_lds_fence();
       for (int sub = (nt - 1) / kSub; sub >= 0; --sub) pair(Part{0, 0}, sub);
       fetch_kept(max(tb - kTok, t0));
+      settle44(h0);
     }
     sync();
   }
