@@ -806,6 +806,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanArgs a) 
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = 0.f;
+#pragma unroll 4
   for (int y = 0; y < v; ++y) join_step(h, A2, sD[y][l], sCut[y], sH[y][l]);
   for (int b = s0; b < s1; b += kAhead) {
     if (per > kAhead) fetch(b);       // (else they are still in registers)
@@ -1251,14 +1252,15 @@ static int check_scan_tensors(const PalScanDims* d, const PalScanTensors* t) {
 static int scan_waves(const PalScanDims* d) { return (d->state + 15) / 16; }
 static int64_t scan_tiles(const PalScanDims* d) { return (int64_t)d->groups * ((d->channels / d->groups + 63) / 64); }
 
-// Tokens per segment: enough segments for `most` waves, at least 64 tokens each.  Forward three waves on every SIMD (1 x 16384 tokens of 1536
-// channels: 114 us with three, 131 with two, 116 with four), backward the two whose registers fit.
+// Tokens per segment: enough segments for `most` waves, at least 32 tokens each.  Forward three waves on every SIMD (1 x 16384 tokens of 1536
+// channels: 114 us with three, 131 with two, 116 with four), backward the two whose registers fit.  (4096 tokens of 384 channels in two
+// groups, all kernels of a forward and backward: segments of at least 64 tokens 270 us, of 32 183, of 16 181.)
 static int scan_segment(const PalScanDims* d, int64_t most) {
   const int64_t waves = scan_tiles(d) * scan_waves(d) * d->batch;
   const int64_t segs = waves < most ? most / waves : 1;
   int64_t seg = (d->seq_len + segs - 1) / segs;
   seg = (seg + PAL_SCAN_BLOCK - 1) / PAL_SCAN_BLOCK * PAL_SCAN_BLOCK;
-  if (seg < 64) seg = 64;
+  if (seg < 32) seg = 32;
   return (int)(seg < d->seq_len ? seg : (d->seq_len + PAL_SCAN_BLOCK - 1) / PAL_SCAN_BLOCK * PAL_SCAN_BLOCK);
 }
 static void scan_args(ScanArgs& a, const PalScanDims* d, const PalScanTensors* t, bool back) {
