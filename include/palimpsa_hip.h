@@ -476,7 +476,7 @@ typedef struct PalScanDims {
   int32_t dtype;          /* PAL_DTYPE_* of the rows: u, delta, B, C, z, y and their gradients */
   int32_t softplus;       /* 1: dt = softplus(delta + delta_bias); 0: their sum as it is */
   uint32_t flags;         /* PAL_FLAG_VARLEN, PAL_FLAG_HAS_INIT, PAL_FLAG_STORE_FINAL */
-  /* elements between batch rows and between tokens; y and all gradients are packed */
+  /* elements between batch rows and between tokens (those below 2^24); y and all gradients are packed */
   int64_t u_batch, u_token, delta_batch, delta_token, z_batch, z_token, B_batch, B_token, C_batch, C_token;
 } PalScanDims;
 
@@ -489,7 +489,7 @@ typedef struct PalScanTensors {
   const float *delta_bias;    /* fp32 [D] or NULL                               */
   void *y;                    /* dtype [B,T,D]                                  */
   const float *init;          /* fp32 [N_seqs,D,N] or NULL                      */
-  float *final_;              /* fp32 [N_seqs,D,N] or NULL; may be init where no gradient is wanted */
+  float *final_;              /* fp32 [N_seqs,D,N] or NULL; may be init where no gradient is wanted, but not with cu_seqlens (PAL_E_STATE) */
   const int32_t *cu_seqlens;  /* device int32 [n_seqs+1] or NULL                */
   float *checkpoints;         /* pal_scan_checkpoint_bytes(dims), for the backward, or NULL */
 } PalScanTensors;

@@ -90,6 +90,8 @@ bool row_stride(const Tensor& t, int64_t& stride) {
   return true;
 }
 
+constexpr int64_t kMaxNormRow = 16384;
+
 struct NormCall {
   bool ok = false;
   at::ScalarType rows, res;
@@ -104,7 +106,7 @@ struct NormCall {
     if (!row_stride(x, d.x_stride)) return;
     d.res_stride = x.size(-1);
     if (r.defined() && !row_stride(r, d.res_stride)) return;
-    if (x.size(-1) > INT32_MAX || !(eps >= 0)) return;
+    if (x.size(-1) > kMaxNormRow || !(eps >= 0)) return;
     d.dim = (int32_t)x.size(-1);
     d.rows = x.numel() / d.dim;
     d.dtype = pal_type(rows); d.res_dtype = pal_type(res); d.weight_dtype = pal_type(w.scalar_type());
@@ -211,8 +213,9 @@ struct ConvCall {
     B = x.size(0); T = x.size(1); D = x.size(2);
     if (!(w.dim() == 2 || (w.dim() == 3 && w.size(1) == 1)) || w.size(0) != D) return;
     W = w.size(-1);
+    if (W < 2 || W > PAL_CONV_MAX_WIDTH || D > 1 << 20 || B * T > (int64_t)1 << 30) return;
     if (b.defined() && (!packed(b, dev, w.scalar_type()) || b.dim() != 1 || b.size(0) != D)) return;
-    if (!token_strides(x, 1, d.x_batch_stride, d.x_token_stride) || B > INT32_MAX || T > INT32_MAX || D > INT32_MAX) return;
+    if (!token_strides(x, 1, d.x_batch_stride, d.x_token_stride)) return;
     N = B;
     if (cu.defined()) {
       if (B != 1 || !packed(cu, dev, at::kInt) || !packed(table, dev, at::kInt) || cu.dim() != 1 || cu.numel() < 2 || table.numel() % 4) return;
@@ -357,6 +360,8 @@ struct ScanCall {
         (i.z.defined() && !token_strides(i.z, 1, d.z_batch, d.z_token)) || !token_strides(i.B, inner, d.B_batch, d.B_token) ||
         !token_strides(i.C, inner, d.C_batch, d.C_token))
       return;
+    for (int64_t s : {d.u_token, d.delta_token, d.z_token, d.B_token, d.C_token})
+      if (s >= 1 << 24) return;
     seqs = bt;
     if (i.cu.defined()) {
       if (bt != 1 || !packed(i.cu, dev, at::kInt) || i.cu.dim() != 1 || i.cu.numel() < 2) return;
@@ -367,7 +372,8 @@ struct ScanCall {
       if (!packed(i.init, dev, at::kFloat) || i.init.dim() != 3 || i.init.size(0) != seqs || i.init.size(1) != ch || i.init.size(2) != N) return;
       d.flags |= PAL_FLAG_HAS_INIT;
     }
-    if (bt > INT32_MAX || T > INT32_MAX || ch > INT32_MAX || seqs > INT32_MAX || N > INT32_MAX) return;
+    if (bt > 65535 || bt * T > (int64_t)1 << 30 || ch >= 1 << 24 || seqs > INT32_MAX || N < 1 || N > PAL_SCAN_MAX_STATE) return;
+    if ((uintptr_t)ptr(i.A) % 16 || (uintptr_t)ptr(i.init) % 16) return;
     d.batch = (int32_t)bt; d.seq_len = (int32_t)T; d.n_seqs = (int32_t)seqs; d.channels = (int32_t)ch; d.state = (int32_t)N; d.groups = (int32_t)G;
     d.dtype = pal_type(rows); d.softplus = softplus;
     ok = true;
@@ -422,7 +428,8 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
     TORCH_CHECK_VALUE(c.ok && packed(kept, i.u.device(), at::kFloat) && kept.numel() == (int64_t)std::max<size_t>(abi.scan_checkpoint_bytes(&c.d) / 4, 4),
                       "selective_scan backward: a saved tensor came back in another shape, dtype, layout or device");
     const Tensor dy = gr[0].defined() ? gr[0].to(c.rows).contiguous() : at::zeros(i.u.sizes(), as(i.u, c.rows));
-    const Tensor df = gr.size() > 1 && gr[1].defined() ? gr[1].to(at::kFloat).contiguous() : Tensor();
+    Tensor df = gr.size() > 1 && gr[1].defined() ? gr[1].to(at::kFloat).contiguous() : Tensor();
+    if (df.defined() && (uintptr_t)ptr(df) % 16) df = df.clone();
     auto like = [&](const Tensor& t) { return t.defined() ? at::empty(t.sizes(), as(t, t.scalar_type())) : Tensor(); };
     Tensor du = like(i.u), dd = like(i.delta), dA = like(i.A), dB = like(i.B), dC = like(i.C), dD = like(i.D), dz = like(i.z), db = like(i.bias), di;
     if (ctx->saved_data["init_grad"].toBool()) di = like(i.init);

@@ -464,7 +464,9 @@ __global__ __launch_bounds__(64 * NW, 3) void scan_fwd_kernel(ScanArgs a) {
     for (int i = 0; i < 4; ++i) A2[k][i] *= kLog2e;
   ScanSeq cur = seq_at(a, row, t0);
   int cut = 0;
-  if (OUT && t0 > 0 && cur.s != t0) load_packed(ln, a.seg_h, packed_at((int64_t)row * a.segs + blockIdx.y, a, ln.tile, NW, w, 0), h);
+  // (of a dense batch in segments the join hands on the initial state too: the last segment may be writing the final state there already)
+  const bool joined = OUT && a.segs > 1 && !a.cu;
+  if (OUT && (joined || (t0 > 0 && cur.s != t0))) load_packed(ln, a.seg_h, packed_at((int64_t)row * a.segs + blockIdx.y, a, ln.tile, NW, w, 0), h);
   else zero44(h);
   if (OUT && t0 == 0 && a.cu) hand_over(a, ln, a.init, a.final_, 0, cur.n);   // sequences without a token before the first one
   const T* pu = (const T*)a.u + row * a.ub;
@@ -553,7 +555,7 @@ __global__ __launch_bounds__(64 * NW, 3) void scan_fwd_kernel(ScanArgs a) {
     };
     for (int lo = 0, hi; lo < nt; lo = hi) {   // the parts of the block that belong to one sequence each: one, nearly always
       if (tb + lo == cur.s) {
-        load_state(a, ln, a.init, cur.n, h);
+        if (!joined) load_state(a, ln, a.init, cur.n, h);
         cut = 1;
       }
       hi = max(lo + 1, min(nt, cur.e - tb));
@@ -806,6 +808,8 @@ __global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanArgs a) 
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = 0.f;
+  if (!BACK && v == 0 && a.init && !a.cu) load4(a, a.init + ((int64_t)row * a.D_ + chan) * a.N + n0, n0, h);   // (the first segment's own
+                                                                                      // state has it already, and lets nothing through)
 #pragma unroll 4
   for (int y = 0; y < v; ++y) join_step(h, A2, sD[y][l], sCut[y], sH[y][l]);
   for (int b = s0; b < s1; b += kAhead) {
@@ -1390,6 +1394,7 @@ extern "C" int pal_scan_fwd(const PalScanDims* d, const PalScanTensors* t, void*
   if (int rc = check_scan_tensors(d, t)) return rc;
   if (!t->y) return PAL_E_NULL;
   if (((d->flags & PAL_FLAG_STORE_FINAL) != 0) != (t->final_ != nullptr)) return PAL_E_STATE;
+  if (t->cu_seqlens && t->final_ && t->final_ == t->init) return PAL_E_STATE;   // read by one segment, written by another
   ScanArgs a{};
   scan_args(a, d, t, false);
   const int nw = scan_waves(d);

@@ -546,6 +546,7 @@ extern "C" int pal_short_conv_fwd(const PalConvDims* d, const PalConvTensors* t,
   if (int rc = check_conv(d, t)) return rc;
   if (int rc = check_conv_seqs(d, t)) return rc;
   if (((d->flags & PAL_FLAG_STORE_FINAL) != 0) != (t->final_ != nullptr)) return PAL_E_STATE;
+  if (t->final_ && t->final_ == t->init) return PAL_E_STATE;   // read by one workgroup, written by another
   ConvArgs a = conv_args(d, t);
   const int vw = conv_piece(d, false);
   conv_runs(a, d, vw);

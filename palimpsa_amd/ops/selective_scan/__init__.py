@@ -61,6 +61,19 @@ def _dims(u, delta, z, B, C_, N, G, seqs, cd, softplus, flags):
                          delta_token=dt, z_batch=zb, z_token=zt, B_batch=Bb, B_token=Bt, C_batch=Cb, C_token=Ct)
 
 
+def _rows(t, inner):
+    t = cm.token_rows(t, inner)
+    return t if cm.token_strides(t, inner)[1] < 1 << 24 else t.contiguous()   # (the kernels' limit)
+
+
+def _aligned(t):
+    """t in fp32, packed, from a multiple of 16 bytes on (parameters and states are read in pieces of that size)."""
+    if t is None:
+        return None
+    t = cm._plain(t, torch.float32)
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 class SelectiveScan(torch.autograd.Function):
     """forward(ctx, u, delta, A, B, C, D, z, delta_bias, softplus, initial_state, output_final_state, cu_seqlens) -> (y, final | None)
     on ``pal_scan_fwd`` / ``pal_scan_bwd``; B, C ``[B, T, G, N]``.  Gradients for every tensor; one that reaches the final state is taken."""
@@ -71,9 +84,9 @@ class SelectiveScan(torch.autograd.Function):
         ch, N, G = _check(u, delta, A, B, C_, D, z, delta_bias)
         bt, T = u.shape[:2]
         cd = torch.bfloat16 if all(t is None or t.dtype == torch.bfloat16 for t in (u, delta, B, C_, z)) else torch.float32
-        rows = lambda t, inner=1: None if t is None else cm.token_rows(t if t.dtype == cd else t.to(cd), inner)  # noqa: E731
+        rows = lambda t, inner=1: None if t is None else _rows(t if t.dtype == cd else t.to(cd), inner)  # noqa: E731
         uc, dc, zc, Bc, Cc = rows(u), rows(delta), rows(z), rows(B, 2), rows(C_, 2)
-        f32 = lambda t: None if t is None else cm._plain(t, torch.float32)  # noqa: E731
+        f32 = _aligned
         Ac, Dc, bc = f32(A), f32(D), f32(delta_bias)
         cu, seqs, flags = None, bt, 0
         if cu_seqlens is not None:
@@ -114,7 +127,7 @@ class SelectiveScan(torch.autograd.Function):
         m = ctx.meta
         dev, cd = u.device, m["cd"]
         dy = torch.zeros(u.shape, dtype=cd, device=dev) if dy is None else cm._plain(dy, cd)
-        d_final = None if d_final is None else cm._plain(d_final, torch.float32)
+        d_final = _aligned(d_final)
         like = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
         du, dd, dA, dB, dC, dD, dz, dbias = (like(t) for t in (u, delta, A, B, C_, D, z, bias))
         d_init = like(init) if init is not None and ctx.needs_input_grad[9] else None
@@ -175,8 +188,8 @@ def selective_scan_step(u: torch.Tensor, state: torch.Tensor, delta: torch.Tenso
     """The next token (u, delta, z ``[B, D]``, B, C ``[B, N]`` or ``[B, G, N]``) or the next few (``[B, T, ..]``) of ``B``
     generations; returns y in the shape of u.
 
-    ``state`` ``[B, D, N]`` fp32, packed, is read and written in place.  Of one token nothing but y is allocated, so a step can be
-    recorded into a HIP graph.  No gradients: call it under ``torch.no_grad()``, or ``selective_scan`` for training."""
+    ``state`` ``[B, D, N]`` fp32, packed, is read and written in place.  Of a few tokens nothing but y is allocated; a step
+    can be recorded into a HIP graph.  No gradients: call it under ``torch.no_grad()``, or ``selective_scan`` for training."""
     if not torch.compiler.is_compiling() and u.is_cuda:
         r = L.host().selective_scan_step(u, state, delta, A, B, C, D, z, delta_bias, bool(delta_softplus))
         if r is not None:
@@ -200,11 +213,13 @@ def _selective_scan_step(u, state, delta, A, B, C, D, z, delta_bias, delta_softp
     bt = u.shape[0]
     if tuple(state.shape) != (bt, ch, N) or state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError(f"state must be contiguous fp32 {(bt, ch, N)}, got {state.dtype} {tuple(state.shape)}")
+    if state.data_ptr() % 16:
+        raise ValueError("state must start at a multiple of 16 bytes")
     cd = torch.bfloat16 if all(t is None or t.dtype == torch.bfloat16 for t in (u, delta, B, C, z)) else torch.float32
     dtype = u.dtype
-    rows = lambda t, inner=1: None if t is None else cm.token_rows(t if t.dtype == cd else t.to(cd), inner)  # noqa: E731
+    rows = lambda t, inner=1: None if t is None else _rows(t if t.dtype == cd else t.to(cd), inner)  # noqa: E731
     u, delta, z, B, C = rows(u), rows(delta), rows(z), rows(B, 2), rows(C, 2)
-    f32 = lambda t: None if t is None else cm._plain(t, torch.float32)  # noqa: E731
+    f32 = _aligned
     A, D, delta_bias = f32(A), f32(D), f32(delta_bias)
     y = torch.empty(u.shape, dtype=cd, device=dev)
     dims = _dims(u, delta, z, B, C, N, G, bt, cd, delta_softplus, L.PAL_FLAG_HAS_INIT | L.PAL_FLAG_STORE_FINAL)

@@ -143,6 +143,10 @@ def test_scan_entry_points_refuse(L):
     assert fwd(_scan_dims(L, flags=L.PAL_FLAG_HAS_INIT)) == L.PAL_E_STATE and fwd(_scan_dims(L), init=P) == L.PAL_E_STATE
     assert fwd(_scan_dims(L), final_=P) == L.PAL_E_STATE
     assert fwd(_scan_dims(L), A=C.c_void_p(0x1008)) == L.PAL_E_ALIGN
+    both = L.PAL_FLAG_HAS_INIT | L.PAL_FLAG_STORE_FINAL      # of a packed batch one segment reads what another writes
+    assert fwd(_scan_dims(L, batch=1, flags=L.PAL_FLAG_VARLEN | both), cu_seqlens=P, init=P, final_=P) == L.PAL_E_STATE
+    assert fwd(_scan_dims(L, u_token=1 << 24)) == L.PAL_E_DIM
+    assert fwd(_scan_dims(L, channels=1 << 21, groups=1 << 21)) == L.PAL_E_DIM
     assert fwd(_scan_dims(L), y=None) == L.PAL_E_NULL and fwd(_scan_dims(L), C=None) == L.PAL_E_NULL
     long = dict(batch=1, n_seqs=1, seq_len=100000)
     need = lib.pal_scan_fwd_workspace_bytes(_scan_dims(L, **long))
