@@ -83,13 +83,13 @@ __device__ __forceinline__ void store_piece(float* p, const float* x, int n) {
   }
 }
 
-// per-channel parameters of either type, eight at a time
+// eight per-channel parameters of either type, those beyond n zero
 __device__ __forceinline__ void load_params(float* out, const void* p, int64_t i, int is_bf16, int n) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) out[e] = e < n ? load_rt(p, i + e, is_bf16) : 0.f;
 }
 
-// reciprocal to 1 ulp (one instruction; an IEEE division is ten), logistic function
+// logistic function by the one-instruction reciprocal (1 ulp; an IEEE division is ten instructions)
 __device__ __forceinline__ float logistic(float x) { return fast_rcp(1.f + __expf(-x)); }
 
 }  // namespace pal

@@ -6,11 +6,12 @@
 // with a = exp(dt A), h' the state before the token.  No two entries share a decay, so nothing here is a matrix product.
 //
 // Bound by the issue of vector instructions: an entry and token take an exponential and four multiplications or fused
-// multiply-adds forward (8.3 + 4 x 2.7 cycles a wave on this GPU), an exponential and fifteen backward.  The shape of a wave
-// follows from that: 64 channels by 16 state entries, a lane 4 by 4 of them.  Sums over n are then three quarters in registers
-// and the rest over the four lanes of a quad, sums over d (dB, dC) a quarter in registers and the rest over the sixteen quads; and
-// what is done once per channel and token (softplus, silu, their derivatives, loads and stores) is one channel for each lane, handed
-// to its quad by lane moves.  State sizes above 16 take one wave for each sixteen, which add their sums in LDS.
+// multiply-adds forward (13 + 4 x 2.9 cycles a wave in this mix on this GPU, whatever the order), an exponential and fourteen backward.  A
+// wave is 64 channels by 16 state entries.  Forward a lane has one channel and all sixteen: the sum over n stays in the lane, B and C come
+// from LDS to all lanes at once.  Backward a lane has 4 channels by 4 entries: sums over d (dB, dC) are then a quarter in registers and the
+// rest over sixteen quads, sums over n three quarters in registers and the rest over the four lanes of a quad, and what is done once
+// per channel and token (softplus, silu, their derivatives, loads and stores) is one channel for each lane, handed to its quad by lane
+// moves.  State sizes above 16 take one wave for each sixteen, which add their sums in LDS.
 //
 // Where the channels and sequences of a pass are too few waves, the tokens are cut into segments: a first kernel walks each
 // segment from zero and leaves its last state and the sum of its dt (the decay over the segment is exp(A sum dt)), a second
@@ -25,6 +26,9 @@
 //
 // For the backward the forward keeps the state before every 8th token in fp32; the backward computes the 8 tokens again, two
 // at a time, and keeps a and a h' of two tokens in registers.
+//
+// Measured (bf16, 1536 channels, N 16, z and D): 1 x 16384 tokens forward 183 us (pass 112, segments 80); 8 x 2048 forward and backward
+// 666 us (backward 375); a token of 256 sequences 11.8 us.
 #include "pal_common.h"
 #include "pal_host.h"
 #include "pal_profile.h"
