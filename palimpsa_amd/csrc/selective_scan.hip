@@ -757,14 +757,14 @@ __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) 
 // From what each segment gives by itself to what each segment starts with (BACK: ends with), in place.  A workgroup has one float4 of
 // every channel of a tile (entries 4 j ..); its waves (up to sixteen) take a run of the segments each: what a run gives by itself goes through
 // LDS, every wave adds up the runs in front of its own, and walks its run again with what it starts with.  One wave over all of the
-// 128 segments of 16384 tokens waited for sixteen batches of loads in turn: 27 us, so split 13.
+// 128 segments of 16384 tokens waited for sixteen batches of loads in turn: 27 us, so split 10.5.
 constexpr int kJoinWaves = 16, kJoinAhead = 8;
 __device__ __forceinline__ void join_step(float* h, const float* A2, float d, int cut, const f32x4 v) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     // (a state of zero stays zero whatever the decay over the segment has overflowed to)
-    const float through = cut || h[i] == 0.f ? 0.f : fast_exp2(A2[i] * d) * h[i];
-    h[i] = through + v[i];
+    const float through = fast_exp2(A2[i] * d) * h[i];
+    h[i] = ((cut != 0) | (h[i] == 0.f) ? 0.f : through) + v[i];
   }
 }
 template <int NW, bool BACK>
@@ -777,8 +777,9 @@ __global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanArgs a) 
   const int group = tile / a.tiles_g, base = group * a.per_group + (tile - group * a.tiles_g) * 64;
   const int chan = min(base + l, (group + 1) * a.per_group - 1), n0 = 16 * w + 4 * j;
   float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f}, d_sum = 0.f;
+  load4(a, a.A + (int64_t)chan * a.N + n0, n0, A2);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) A2[i] = n0 + i < a.N ? a.A[(int64_t)chan * a.N + n0 + i] * kLog2e : 0.f;
+  for (int i = 0; i < 4; ++i) A2[i] *= kLog2e;
   f32x4* H = (f32x4*)a.seg_h;
   const int waves = blockDim.x >> 6, per = (a.segs + waves - 1) / waves, s0 = min(v * per, a.segs), s1 = min(s0 + per, a.segs);
   int any = 0;
@@ -1190,18 +1191,20 @@ __global__ __launch_bounds__(64 * kParamWaves) void scan_bwd_params_kernel(ScanA
   const int group = tile / a.tiles_g, base = group * a.per_group + (tile - group * a.tiles_g) * 64, end = (group + 1) * a.per_group;
   double t[4] = {0., 0., 0., 0.};
   if (z < 4) {
+#pragma unroll 4
     for (int64_t i = v; i < slots; i += kParamWaves) {
       const f32x4 x = ((const f32x4*)a.part_a)[packed_at(i, a, tile, nw, w, z) + l];
 #pragma unroll
       for (int e = 0; e < 4; ++e) t[e] += x[e];
     }
   } else if (w == 0) {
-    for (int64_t i = v; i < slots; i += kParamWaves)
-      for (int k = 0; k < nw; ++k) {
-        const float* p = a.part_c + (((i * a.tiles + tile) * nw + k) * 64 + l) * 2;
-        t[0] += p[0];
-        t[1] += p[1];
-      }
+#pragma unroll 4
+    for (int64_t q = v; q < slots * nw; q += kParamWaves) {
+      const int64_t i = q / nw, k = q - i * nw;
+      const float* p = a.part_c + (((i * a.tiles + tile) * nw + k) * 64 + l) * 2;
+      t[0] += p[0];
+      t[1] += p[1];
+    }
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) s[v][l][e] = t[e];
