@@ -27,8 +27,8 @@
 // For the backward the forward keeps the state before every 8th token in fp32; the backward computes the 8 tokens again, two
 // at a time, and keeps a and a h' of two tokens in registers.
 //
-// Measured (bf16, 1536 channels, N 16, z and D): 1 x 16384 tokens forward 183 us (pass 112, segments 80); 8 x 2048 forward and backward
-// 666 us (backward 375); a token of 256 sequences 11.8 us.
+// Measured (bf16, 1536 channels, N 16, z and D): 1 x 16384 tokens forward 181 us (pass 111, segments 80); 8 x 2048 forward and backward
+// 664 us (backward 375); a token of 256 sequences 11.8 us.
 #include "pal_common.h"
 #include "pal_host.h"
 #include "pal_profile.h"
@@ -764,7 +764,7 @@ __device__ __forceinline__ void join_step(float* h, const float* A2, float d, in
   for (int i = 0; i < 4; ++i) {
     // (a state of zero stays zero whatever the decay over the segment has overflowed to)
     const float through = fast_exp2(A2[i] * d) * h[i];
-    h[i] = ((cut != 0) | (h[i] == 0.f) ? 0.f : through) + v[i];
+    h[i] = (((cut != 0) | (h[i] == 0.f)) ? 0.f : through) + v[i];
   }
 }
 template <int NW, bool BACK>
