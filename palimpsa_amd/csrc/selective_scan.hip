@@ -1266,6 +1266,7 @@ static int64_t scan_tiles(const PalScanDims* d) { return (int64_t)d->groups * ((
 // Tokens per segment: enough segments for `most` waves, at least 32 tokens each.  Forward three waves on every SIMD (1 x 16384 tokens of 1536
 // channels: 114 us with three, 131 with two, 116 with four), backward the two whose registers fit.  (4096 tokens of 384 channels in two
 // groups, all kernels of a forward and backward: segments of at least 64 tokens 270 us, of 32 183, of 16 181.)
+constexpr int64_t kSimds = 1024;   // of the GPU
 static int scan_segment(const PalScanDims* d, int64_t most) {
   const int64_t waves = scan_tiles(d) * scan_waves(d) * d->batch;
   const int64_t segs = waves < most ? most / waves : 1;
@@ -1283,7 +1284,7 @@ static void scan_args(ScanArgs& a, const PalScanDims* d, const PalScanTensors* t
   a.vec = d->state % 4 == 0;
   a.ub = d->u_batch; a.db = d->delta_batch; a.zb = d->z_batch; a.Bb = d->B_batch; a.Cb = d->C_batch;
   a.ut = (int)d->u_token; a.dt = (int)d->delta_token; a.zt = (int)d->z_token; a.Bt = (int)d->B_token; a.Ct = (int)d->C_token;
-  a.seg = scan_segment(d, back ? 2048 : 3072);
+  a.seg = scan_segment(d, (back ? 2 : 3) * kSimds);
   a.segs = (a.T + a.seg - 1) / a.seg;
   a.ckpts = (a.T + PAL_SCAN_BLOCK - 1) / PAL_SCAN_BLOCK;
   if (!t) return;
