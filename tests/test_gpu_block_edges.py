@@ -166,3 +166,36 @@ def test_types_that_are_converted_and_refusals_with_gradients(gpu_device):
                 lambda: residual_rms_norm(x, None, torch.ones(24, device=gpu_device), float("nan"))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,G,ch", [(16, 1, 70), (40, 2, 140), (64, 1, 12), (3, 5, 35)])
+def test_packs_of_ragged_sequences(gpu_device, N, G, ch, dt):
+    """Sequences of 0 to 70 tokens, their starts and ends anywhere in blocks, segments and pairs of tokens, with states in and out and all
+    gradients.  A term lives through its sequence's steps, at most 70 each way: k = (48 x 70 + 64 + N + ch) half steps."""
+    from palimpsa_amd.ops.selective_scan import selective_scan
+    gen = torch.Generator().manual_seed(N + ch)
+    lens = torch.randint(0, 71, (18,), generator=gen).tolist() + [0, 1, 1, 2, 0, 7, 8, 9, 16, 64, 0]
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    T, S = cu[-1], len(lens)
+    r = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    inp = dict(u=r(1, T, ch).to(dt), delta=(.5 * r(1, T, ch)).to(dt), A=-2 * torch.rand(ch, N, generator=gen), B=r(1, T, G, N).to(dt),
+               C=r(1, T, G, N).to(dt), D=r(ch), z=r(1, T, ch).to(dt), delta_bias=.3 * r(ch) - 1)
+    h0, dy, df = r(S, ch, N), r(1, T, ch).to(dt), r(S, ch, N)
+    lv = {n: t.to(gpu_device).requires_grad_(True) for n, t in inp.items()}
+    s0 = h0.to(gpu_device).requires_grad_(True)
+    y, f = selective_scan(**lv, initial_state=s0, output_final_state=True, cu_seqlens=torch.tensor(cu, device=gpu_device))
+    got = dict(zip([*("d" + n for n in lv), "d_init"], torch.autograd.grad((y, f), [*lv.values(), s0], (dy.to(gpu_device), df.to(gpu_device)))))
+    kw = dict(**inp, init=h0, cu=cu)
+    (yr, fr, _, _), (ym, fm, _, _) = bo.scan(**kw), bo.scan(**kw, mass=True)
+    want, mass = bo.scan_grads(dy, d_final=df, **kw), bo.scan_grads(dy, d_final=df, **kw, mass=True)
+    half = 2.0 ** -8 if dt == torch.bfloat16 else u32
+    k = (48 * 70 + 64 + N + ch) * u32
+    off = lambda t, ref: (t.detach().cpu().double() - ref).abs()  # noqa: E731
+    assert (off(y, yr) <= 1.01 * half * yr.abs() + k * ym).all() and (off(f, fr) <= k * fm).all()
+    for n, g in got.items():
+        own = half if n in ("du", "ddelta", "dB", "dC", "dz") else u32
+        chain = T if n in ("dA", "dD", "ddelta_bias") else 0
+        assert (off(g, want[n]) <= 1.01 * own * want[n].abs() + (k + chain * u32) * mass[n]).all(), n
