@@ -43,8 +43,7 @@ enum KernelId {
   kKernScanSegment,
   kKernScanJoin,
   kKernScanBwd,
-  kKernScanBwdRows,
-  kKernScanBwdParams,
+  kKernScanBwdSums,
   kKernCount
 };
 

@@ -57,7 +57,7 @@ static const char* kNames[kKernCount] = {
     "chunk_bwd_parts_sum_kernel", "recurrent_seg_kernel", "residual_norm_fwd_kernel", "residual_norm_bwd_kernel",
     "residual_norm_reduce_kernel", "short_conv_fwd_kernel", "short_conv_bwd_kernel", "short_conv_reduce_kernel",
     "short_conv_step_kernel", "scan_fwd_kernel", "scan_segment_kernel", "scan_join_kernel", "scan_bwd_kernel",
-    "scan_bwd_rows_kernel", "scan_bwd_params_kernel"};
+    "scan_bwd_sums_kernel"};
 
 }  // namespace pal
 

@@ -28,7 +28,7 @@
 // at a time, and keeps a and a h' of two tokens in registers.
 //
 // Measured (bf16, 1536 channels, N 16, z and D): 1 x 16384 tokens forward 181 us (pass 111, segments 80); 8 x 2048 forward and backward
-// 664 us (backward 375); a token of 256 sequences 11.8 us.
+// 660 us (backward 375); a token of 256 sequences 11.8 us.
 #include "pal_common.h"
 #include "pal_host.h"
 #include "pal_profile.h"
@@ -1159,9 +1159,9 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
 
 // dB, dC [rows, T, G, N]: the tiles of a group in their order.  Thread = four entries of a token.
 template <typename T>
-__global__ __launch_bounds__(256) void scan_bwd_rows_kernel(ScanArgs a, int nw) {
+__device__ __forceinline__ void sum_rows(const ScanArgs& a, int nw, int64_t first, int64_t step) {
   const int64_t per = 2 * (int64_t)a.G * nw * 4, total = (int64_t)a.rows * a.T * per;
-  for (int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x; x < total; x += (int64_t)gridDim.x * 256) {
+  for (int64_t x = first; x < total; x += step) {
     const int64_t tok = x / per;
     const int r = (int)(x - tok * per), j = r & 3, which = (r >> 2) & 1, w = (r >> 3) % nw, g = (r >> 3) / nw, n = 16 * w + 4 * j;
     const f32x4* p = (const f32x4*)(a.part_bc + ((tok * a.tiles + (int64_t)g * a.tiles_g) * nw + w) * 32 + which * 16 + 4 * j);
@@ -1181,25 +1181,32 @@ __global__ __launch_bounds__(256) void scan_bwd_rows_kernel(ScanArgs a, int nw) 
   }
 }
 
-// dA, dD, ddelta_bias: the segments of all rows in their order, in 64 bits.  grid (tiles, waves of a tile, 5): z < 4 the entries
-// 4 z .. of dA, z = 4 dD and ddelta_bias; sixteen waves take a share of the segments each.
-constexpr int kParamWaves = 16;
-__global__ __launch_bounds__(64 * kParamWaves) void scan_bwd_params_kernel(ScanArgs a, int nw) {
-  __shared__ double s[kParamWaves][64][4];
-  const int l = threadIdx.x & 63, v = threadIdx.x >> 6, tile = blockIdx.x, w = blockIdx.y, z = blockIdx.z;
+// dA, dD, ddelta_bias: the segments of all rows in their order, in 64 bits.  Workgroup = a tile, one of its waves and z: z < 4 the entries
+// 4 z .. of dA, z = 4 dD and ddelta_bias; sixteen waves take a share of the segments each.  Behind these workgroups those of dB and dC, in one
+// launch.
+constexpr int kSumWaves = 16;
+template <typename T>
+__global__ __launch_bounds__(64 * kSumWaves) void scan_bwd_sums_kernel(ScanArgs a, int nw) {
+  __shared__ double s[kSumWaves][64][4];
+  const int first = a.tiles * nw * 5;
+  if ((int)blockIdx.x >= first) {
+    sum_rows<T>(a, nw, (int64_t)(blockIdx.x - first) * (64 * kSumWaves) + threadIdx.x, (int64_t)(gridDim.x - first) * (64 * kSumWaves));
+    return;
+  }
+  const int l = threadIdx.x & 63, v = threadIdx.x >> 6, z = blockIdx.x % 5, tile = blockIdx.x / 5 / nw, w = blockIdx.x / 5 - tile * nw;
   const int64_t slots = (int64_t)a.rows * a.segs;
   const int group = tile / a.tiles_g, base = group * a.per_group + (tile - group * a.tiles_g) * 64, end = (group + 1) * a.per_group;
   double t[4] = {0., 0., 0., 0.};
   if (z < 4) {
 #pragma unroll 4
-    for (int64_t i = v; i < slots; i += kParamWaves) {
+    for (int64_t i = v; i < slots; i += kSumWaves) {
       const f32x4 x = ((const f32x4*)a.part_a)[packed_at(i, a, tile, nw, w, z) + l];
 #pragma unroll
       for (int e = 0; e < 4; ++e) t[e] += x[e];
     }
   } else if (w == 0) {
 #pragma unroll 4
-    for (int64_t q = v; q < slots * nw; q += kParamWaves) {
+    for (int64_t q = v; q < slots * nw; q += kSumWaves) {
       const int64_t i = q / nw, k = q - i * nw;
       const float* p = a.part_c + (((i * a.tiles + tile) * nw + k) * 64 + l) * 2;
       t[0] += p[0];
@@ -1213,7 +1220,7 @@ __global__ __launch_bounds__(64 * kParamWaves) void scan_bwd_params_kernel(ScanA
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     t[e] = 0.;
-    for (int x = 0; x < kParamWaves; ++x) t[e] += s[x][l][e];
+    for (int x = 0; x < kSumWaves; ++x) t[e] += s[x][l][e];
   }
   if (z < 4) {
     const int c = base + l, n0 = 16 * w + 4 * z;
@@ -1345,10 +1352,9 @@ static int scan_bwd_run(const ScanArgs& a, hipStream_t s) {
   }
   PAL_TIMED_LAUNCH(kKernScanBwd, s, (scan_bwd_kernel<T, NW>), grid, dim3(64 * NW), 0, s, a);
   PAL_HIP_LAUNCH_CHECK();
-  const int64_t n = 8 * (int64_t)a.rows * a.T * a.G * NW, blocks = (n + 255) / 256;
-  PAL_TIMED_LAUNCH(kKernScanBwdRows, s, scan_bwd_rows_kernel<T>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, s, a, NW);
-  PAL_HIP_LAUNCH_CHECK();
-  PAL_TIMED_LAUNCH(kKernScanBwdParams, s, scan_bwd_params_kernel, dim3(a.tiles, NW, 5), dim3(64 * kParamWaves), 0, s, a, NW);
+  const int64_t n = 8 * (int64_t)a.rows * a.T * a.G * NW, blocks = (n + 64 * kSumWaves - 1) / (64 * kSumWaves);
+  PAL_TIMED_LAUNCH(kKernScanBwdSums, s, scan_bwd_sums_kernel<T>, dim3(a.tiles * NW * 5 + (unsigned)(blocks < 2048 ? blocks : 2048)),
+                   dim3(64 * kSumWaves), 0, s, a, NW);
   PAL_HIP_LAUNCH_CHECK();
   return PAL_OK;
 }
