@@ -83,10 +83,25 @@ __device__ __forceinline__ void store_piece(float* p, const float* x, int n) {
   }
 }
 
-// eight per-channel parameters of either type, those beyond n zero
-__device__ __forceinline__ void load_params(float* out, const void* p, int64_t i, int is_bf16, int n) {
+// eight per-channel parameters of either type; whichever it is, they are waited for in their branch (where the two meet, the
+// compiler would wait for everything in flight)
+__device__ __forceinline__ void load_params(float* x, const void* p, int64_t i, int is_bf16) {
+  if (is_bf16) {
+    const bf16x8 v = *(const bf16x8_any*)((const bf16_t*)p + i);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) out[e] = e < n ? load_rt(p, i + e, is_bf16) : 0.f;
+    for (int e = 0; e < 8; ++e) x[e] = (float)v[e];
+  } else {
+    const f32x4 lo = *(const f32x4_any*)((const float*)p + i), hi = *(const f32x4_any*)((const float*)p + i + 4);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = e < 4 ? lo[e & 3] : hi[e & 3];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) asm volatile("" : "+v"(x[e]));
+}
+// the same of fewer: those beyond n zero
+__device__ __forceinline__ void load_few_params(float* x, const void* p, int is_bf16, int n) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = e < n ? load_rt(p, e, is_bf16) : 0.f;
 }
 
 // logistic function by the one-instruction reciprocal (1 ulp; an IEEE division is ten instructions)

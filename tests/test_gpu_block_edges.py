@@ -199,3 +199,40 @@ def test_packs_of_ragged_sequences(gpu_device, N, G, ch, dt):
         own = half if n in ("du", "ddelta", "dB", "dC", "dz") else u32
         chain = T if n in ("dA", "dD", "ddelta_bias") else 0
         assert (off(g, want[n]) <= 1.01 * own * want[n].abs() + (k + chain * u32) * mass[n]).all(), n
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [1, 5, 8, 9, 15, 504, 513, 1027, 2047, 2055, 5000, 10001])
+def test_norm_of_any_row_length(gpu_device, D, dt):
+    """Rows whose last piece is moved back, of less than a piece, of lanes and waves without a piece; and nothing behind the last row.
+
+    A lane adds at most 64 squares one after the other and the lanes 6 times more: r is off by 40 half steps, y by 64, dx by 128 of the
+    sizes of its terms, dw by those and one for each row, every result by the half step of its type."""
+    from palimpsa_amd.ops.layer_glue import residual_rms_norm, residual_rms_norm_fp8
+    gen = torch.Generator().manual_seed(D)
+    n = 5
+    x, res, dy, ds = (torch.randn(n, D, generator=gen).to(dt) for _ in range(4))
+    w = .5 + torch.rand(D, generator=gen)
+    lv = [t.to(gpu_device).requires_grad_(True) for t in (x, res, w)]
+    y, s = residual_rms_norm(*lv, 1e-5)
+    gx, gr, gw = torch.autograd.grad((y, s), lv, (dy.to(gpu_device), ds.to(gpu_device)))
+    half = 2.0 ** -8 if dt == torch.bfloat16 else u32
+    sd = s.detach().cpu().double()
+    assert ((sd - (x.double() + res.double())).abs() <= 1.01 * half * (x.double() + res.double()).abs()).all()
+    r = torch.rsqrt((sd * sd).mean(-1, keepdim=True) + 1e-5)
+    g, wd = dy.double(), w.double()
+    c = lambda t: t.detach().cpu().double()  # noqa: E731
+    yr = sd * r * wd
+    assert ((c(y) - yr).abs() <= (1.01 * half + 64 * u32) * yr.abs()).all()
+    dot, size = (g * wd * sd).sum(-1, keepdim=True), (g * wd * sd).abs().sum(-1, keepdim=True)
+    dr = r * g * wd - sd * r ** 3 * dot / D + ds.double()
+    mass = r * (g * wd).abs() + sd.abs() * r ** 3 * size / D + ds.double().abs()
+    for t in (gx, gr):
+        assert ((c(t) - dr).abs() <= 1.01 * half * dr.abs() + 128 * u32 * mass).all()
+    dw, mw = (g * sd * r).sum(0), (g * sd * r).abs().sum(0)
+    assert ((c(gw) - dw).abs() <= (64 + n) * u32 * mw).all()
+    with torch.no_grad():
+        q, scales, s8 = residual_rms_norm_fp8(lv[0], lv[1], lv[2], 1e-5)
+    top = yr.abs().amax(-1, keepdim=True).clamp(min=1e-12) / 448
+    assert torch.equal(s8, s) and ((c(scales) - top).abs() <= 70 * u32 * top).all()
+    assert ((q.float().cpu().double() * c(scales) - yr).abs() <= 2.0 ** -4 * 1.01 * yr.abs() + 2.0 ** -10 * 1.01 * top).all()
