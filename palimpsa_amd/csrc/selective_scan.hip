@@ -33,6 +33,7 @@
 #include "pal_host.h"
 #include "pal_profile.h"
 #include "rows8.h"
+#include "scan_seqs.h"
 
 namespace pal {
 
@@ -127,21 +128,6 @@ __device__ __forceinline__ float quad_total4(float p0, float p1, float p2, float
   const float a = (odd ? p1 : p0) + in_quad<0xB1>(odd ? p0 : p1);
   const float b = (odd ? p3 : p2) + in_quad<0xB1>(odd ? p2 : p3);
   return (high ? b : a) + in_quad<0x4E>(high ? a : b);
-}
-
-// a sequence: its number and its tokens [s, e) in the row
-struct ScanSeq {
-  int n, s, e;
-};
-__device__ __forceinline__ ScanSeq seq_at(const ScanArgs& a, int row, int t) {
-  if (!a.cu) return {row, 0, a.T};
-  int lo = 0, hi = a.seqs - 1;      // last sequence that starts at t or before: it holds t if any does
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (a.cu[mid] <= t) lo = mid;
-    else hi = mid - 1;
-  }
-  return {lo, a.cu[lo], a.cu[lo + 1]};
 }
 
 // The lane's number, hidden from the compiler: what rare paths compute from it stays in them instead of being kept in
@@ -345,17 +331,6 @@ __device__ __forceinline__ void hand_over(const ScanArgs& a, const L& ln, const 
     load_state(a, ln, from, n, x);
     store_state(a, ln, to, n, x);
   }
-}
-// the sequence after / before `s` that has a token (the last one / first one: itself)
-__device__ __forceinline__ ScanSeq next_seq(const ScanArgs& a, const ScanSeq& s) {
-  int n = s.n + 1;
-  while (n < a.seqs && a.cu[n + 1] <= s.e) ++n;
-  return n < a.seqs ? ScanSeq{n, s.e, a.cu[n + 1]} : ScanSeq{a.seqs, s.e, a.T + 1};
-}
-__device__ __forceinline__ ScanSeq prev_seq(const ScanArgs& a, const ScanSeq& s) {
-  int n = s.n - 1;
-  while (n >= 0 && a.cu[n] >= s.s) --n;
-  return n >= 0 ? ScanSeq{n, a.cu[n], s.s} : ScanSeq{-1, -1, s.s};
 }
 // the tokens of a block that are walked: all of them, known to the compiler, or [lo, hi)
 struct Whole {
