@@ -160,10 +160,12 @@ __device__ __forceinline__ void load_taps(float (*w)[VW], float* bias, const Con
   }
   if (a.bias) load_run<VW>(bias, a.bias, c, a.weight_bf16);
 }
-// the W - 1 inputs before the run: rows of the sequence, or the state it starts with, or zero; h[0] the oldest
+// the W - 1 inputs before the run: rows of the sequence, or the state it starts with, or zero; h[0] the oldest.  A run that is not the
+// first of its sequence has a whole run before it, at least 8 tokens; where a table that was not made from these bounds says otherwise, the rows
+// before the sequence (of the first one: before the tensor) are not read.
 template <typename T, int W, int VW>
 __device__ __forceinline__ void load_before(float (*h)[VW], const ConvArgs& a, const ConvRun& r, int c) {
-  if (r.t0 > r.s0) {       // (a run that is not the first has a whole run before it, at least 8 tokens)
+  if (r.t0 - r.s0 >= W - 1) {
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {
       Chans<T, VW> x;

@@ -44,3 +44,32 @@ def test_scan(gpu_device, values, N):
     rewrite(cu, [0, 10, 30, 60])
     again, _ = selective_scan(**lv, initial_state=init, cu_seqlens=cu)
     assert torch.equal(whole, again)
+
+
+@pytest.mark.parametrize("W", [2, 4, 8])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("moved", [[0, 2, 40], [0, 0, 40], [0, 1, 3], [0, 40, 40], [0, 39, 3], [0, 50, 60], [-7, 2, 90]])
+def test_convolution(gpu_device, W, dt, moved):
+    """The table of tiles still is that of the bounds that were checked: a tile may start inside a sequence, fewer tokens from its start than
+    the filter is long."""
+    from palimpsa_amd.ops.short_conv import short_conv
+
+    gen = torch.Generator().manual_seed(W)
+    T, D = 40, 24
+    x, dy = (inside(torch.randn(1, T, D, generator=gen).to(dt), gpu_device) for _ in range(2))
+    x.requires_grad_(True)
+    init, df = (inside(torch.randn(2, D, W, generator=gen).to(dt), gpu_device) for _ in range(2))
+    init.requires_grad_(True)
+    w, b = (torch.randn(*s, generator=gen).to(gpu_device).requires_grad_(True) for s in ((D, W), (D,)))
+    cu = torch.tensor([0, 3, 40], dtype=torch.int32, device=gpu_device)
+    whole, _ = short_conv(x, w, b, initial_state=init, cu_seqlens=cu)
+    rewrite(cu, moved)
+    y, fin = short_conv(x, w, b, initial_state=init, output_final_state=True, cu_seqlens=cu)
+    gx, gw, gb = torch.autograd.grad((y, fin), (x, w, b), (dy, df))
+    # rows that a tile of the old table and a sequence of the new bounds both hold are computed; the others are left as they are
+    first, last = min(max(moved[1], 0), T), min(max(moved[2], 0), T)
+    done = list(range(min(3, first))) + list(range(min(max(3, first), max(first, last)), max(first, last)))
+    assert torch.isfinite(y[0, done]).all() and torch.isfinite(gx[0, done]).all() and torch.isfinite(fin).all()
+    assert torch.isfinite(gw).all() and torch.isfinite(gb).all()
+    rewrite(cu, [0, 3, 40])
+    assert torch.equal(whole, short_conv(x, w, b, initial_state=init, cu_seqlens=cu)[0])
