@@ -202,6 +202,12 @@ struct Column : Tile {
 #pragma unroll
     for (int j = 0; j < 4; ++j) store4(a, d + 4 * j, 16 * w + 4 * j, x[j]);
   }
+  __device__ __forceinline__ void clear_beyond(const ScanArgs& a, float (*x)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[j][i] = 16 * w + 4 * j + i < a.N ? x[j][i] : 0.f;
+  }
   static __device__ __forceinline__ unsigned packed(int j) { return 64 * j + (threadIdx.x & 63); }
 };
 // Lanes as quads: x[k][i] is channel 16 k + q of the tile, entry 4 j + i of the wave's sixteen, for lane 4 q + j.
@@ -230,6 +236,14 @@ struct Lane : Tile {
       const int c = base + 16 * k + (l >> 2);
       if (c < end) store4(a, p + (int64_t)c * a.N + n0, n0, x[k]);
     }
+  }
+  __device__ __forceinline__ int entries(const ScanArgs& a) const { return a.N - 16 * w - 4 * (hidden_lane() & 3); }   // of the lane's four
+  __device__ __forceinline__ void clear_beyond(const ScanArgs& a, float (*x)[4]) const {
+    const int have = entries(a);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[k][i] = i < have ? x[k][i] : 0.f;
   }
   static __device__ __forceinline__ unsigned packed(int k) { return 64 * (threadIdx.x & 3) + 16 * k + ((threadIdx.x & 63) >> 2); }
 };
@@ -346,6 +360,14 @@ __device__ __forceinline__ bool walks(const R& r, int t) { return R::whole || (t
 
 constexpr int kTok = PAL_SCAN_BLOCK;   // tokens of a block
 
+// Entries beyond N have B = C = 0 and no decay, so they stay zero, unless a factor is infinite: inf x 0 is no number, and would get into the
+// sums over n.  A block in which one is takes the path that clears them; this looks for it in `most`, the largest of the factors.  (A factor
+// that is no number makes every entry of its channel one, until its sequence ends, and need not be looked for.)  In what a segment leaves they
+// are whatever they are: it is cleared where it is read.  Passes over states of a multiple of 16 entries are kernels of their own (FULL):
+// the second path and the looking take 1 to 3 % of a forward call, and 4 x 2048 tokens of 1536 channels forward and backward from 347 to 364 us
+// for N 8, from 695 to 743 for N 24 (bf16; 575 to 503 and 958 to 961 in fp32).
+__device__ __forceinline__ bool any_infinite(float most) { return __builtin_amdgcn_ballot_w64(most == INFINITY) != 0; }
+
 // A block of one array: lane l takes channels 8 (l % 8) .. of token l / 8 (of the last token where the block has fewer).  Whole tiles
 // without a branch; of the last tile of a group what is there, the channels beyond it are zero.
 template <typename T>
@@ -423,7 +445,7 @@ __device__ __forceinline__ void decays(float (*e)[4], float dt, const float (*A2
 
 // ------------------------------------------------------------------------------------------------ forward
 // OUT: the pass itself.  Otherwise the walk of a segment from zero: its last state, the sum of its dt, and whether a sequence starts in it.
-template <typename T, int NW, bool OUT>
+template <typename T, int NW, bool OUT, bool FULL>
 __global__ __launch_bounds__(64 * NW, 3) void scan_fwd_kernel(ScanArgs a) {
   constexpr int M = OUT ? 2 : 1;
   __shared__ __attribute__((aligned(16))) float sBC[NW][kTok][M][16];
@@ -441,12 +463,14 @@ __global__ __launch_bounds__(64 * NW, 3) void scan_fwd_kernel(ScanArgs a) {
   for (int k = 0; k < 4; ++k)
 #pragma unroll
     for (int i = 0; i < 4; ++i) A2[k][i] *= kLog2e;
+  const bool beyond = OUT && !FULL && 16 * (w + 1) > a.N;      // entries beyond N in this wave
   ScanSeq cur = seq_at(a, row, t0);
   int cut = 0;
   // (of a dense batch in segments the join hands on the initial state too: the last segment may be writing the final state there already)
   const bool joined = OUT && a.segs > 1 && !a.cu;
   if (OUT && (joined || (t0 > 0 && cur.s != t0))) load_packed(ln, a.seg_h, packed_at((int64_t)row * a.segs + blockIdx.y, a, ln.tile, NW, w, 0), h);
   else zero44(h);
+  if (beyond) ln.clear_beyond(a, h);
   if (OUT && t0 == 0 && a.cu) hand_over(a, ln, a.init, a.final_, 0, cur.n);   // sequences without a token before the first one
   const T* pu = (const T*)a.u + row * a.ub;
   const T* pd = (const T*)a.delta + row * a.db;
@@ -503,6 +527,13 @@ __global__ __launch_bounds__(64 * NW, 3) void scan_fwd_kernel(ScanArgs a) {
 #pragma unroll
       for (int t = 0; t < kTok; ++t) gate[t] *= raw[t];
     }
+    bool clear = false;
+    if (beyond) {
+      float most = 0.f;
+#pragma unroll
+      for (int t = 0; t < kTok; ++t) most = fmaxf(fmaxf(most, fabsf(dt[t])), fabsf(dt[t] * uv[t]));
+      clear = any_infinite(most);
+    }
     auto walk = [&](auto r) {
 #pragma unroll
       for (int t = 0; t < kTok; ++t) {
@@ -518,6 +549,7 @@ __global__ __launch_bounds__(64 * NW, 3) void scan_fwd_kernel(ScanArgs a) {
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i) h[j][i] = fmaf(e[j][i], h[j][i], x * B[j][i]);
+        if (beyond && !decltype(r)::whole && clear) ln.clear_beyond(a, h);
         stage();
         if constexpr (OUT) {
 #pragma unroll
@@ -537,7 +569,7 @@ __global__ __launch_bounds__(64 * NW, 3) void scan_fwd_kernel(ScanArgs a) {
         if (!joined) load_state(a, ln, a.init, cur.n, h);
         cut = 1;
       }
-      hi = max(lo + 1, min(nt, cur.e - tb));
+      hi = max(lo + 1, min(clear ? min(nt, kTok - 1) : nt, cur.e - tb));
       if (hi - lo == kTok) walk(Whole{0, 0});
       else walk(Part{lo, hi});
       if (tb + hi == cur.e) {
@@ -806,7 +838,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanArgs a) 
 // ------------------------------------------------------------------------------------------------ backward
 constexpr int kSub = 2;   // tokens whose decays and states are in registers
 
-template <typename T, int NW>
+template <typename T, int NW, bool FULL>
 __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
   constexpr int kOwn = (4 + NW - 1) / NW;   // arrays that a wave fetches for the workgroup
   __shared__ float sBC[NW][kTok][2][16];
@@ -828,9 +860,11 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) A2[k][i] *= kLog2e;
   zero44(dA);
+  const bool beyond = !FULL && 16 * (w + 1) > a.N;      // entries beyond N in this wave
   const int64_t slot = (int64_t)row * a.segs + blockIdx.y;
   if (t1 < a.T) load_packed(ln, a.seg_h, packed_at(slot, a, ln.tile, NW, w, 0), carry);
   else zero44(carry);
+  if (beyond) ln.clear_beyond(a, carry);
   ScanSeq cur = seq_at(a, row, t1 - 1);
   if (t1 == a.T && a.cu) hand_over(a, ln, a.d_final, a.d_init, cur.n + 1, a.seqs);   // sequences without a token behind the last one
   const int64_t out0 = (int64_t)row * a.T * a.D_;
@@ -918,7 +952,17 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
     // A whole block in which no sequence starts or ends is straight code: one path for the registers that are carried from block to
     // block.  (Loops around it, over parts and over pairs of tokens, moved them, 16 states, 16 decays' gradients and the 16 states on
     // their way from memory, between two sets on every round, and waited for the last.)
-    const bool plain = nt == kTok && cur.s < tb && cur.e > tb + kTok;
+    bool clear = false;
+    if (beyond) {
+      float most = 0.f;
+#pragma unroll
+      for (int t = 0; t < kTok; ++t) {
+        const float dt = sDt[t][l], gy = to_f32(sRow[3][t][own]) * (has_z ? to_f32(sRow[2][t][own]) : 1.f);   // (at least |dy silu(z)|)
+        most = fmaxf(fmaxf(fmaxf(most, fabsf(dt)), fabsf(dt * to_f32(sRow[0][t][own]))), fabsf(gy));
+      }
+      clear = any_infinite(most);
+    }
+    const bool plain = nt == kTok && cur.s < tb && cur.e > tb + kTok && !clear;
     auto states = [&](auto kind) __attribute__((always_inline)) {
       float h[4][4];
 #pragma unroll
@@ -936,7 +980,9 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) h[k][i] = fmaf(fast_exp2(dk[k] * A2[k][i]), h[k][i], xk[k] * Bv[i]);
+              for (int i = 0; i < 4; ++i) {
+                h[k][i] = fmaf(fast_exp2(dk[k] * A2[k][i]), h[k][i], xk[k] * Bv[i]);
+              }
             if (t % kSub == kSub - 1)
 #pragma unroll
               for (int k = 0; k < 4; ++k) sH[w][t / kSub][k][l] = (f32x4){h[k][0], h[k][1], h[k][2], h[k][3]};
@@ -994,6 +1040,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
       float h[4][4];
       auto walk = [&](auto r, bool ends) __attribute__((always_inline)) {
         float av[kSub][4][4], ah[kSub][4][4];
+        const int have = !FULL && !whole && clear ? ln.entries(a) : 4;      // entries that count in the sums over n
 #pragma unroll
         for (int t = 0; t < kSub; ++t) {
           if (!walks(r, t)) continue;
@@ -1032,15 +1079,16 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
           for (int k = 0; k < 4; ++k) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float hv = fmaf(xk[k], Bv[i], ah[t][k][i]);
-              const float g = fmaf(Cv[i], Yk[k], carry[k][i]), p = g * ah[t][k][i];
+              float hv = fmaf(xk[k], Bv[i], ah[t][k][i]), g = fmaf(Cv[i], Yk[k], carry[k][i]);
+              float p = g * ah[t][k][i];
+              carry[k][i] = g * av[t][k][i];
+              if (!FULL && !whole && i >= have) hv = g = p = 0.f;
               gC[i] = k ? fmaf(Yk[k], hv, gC[i]) : Yk[k] * hv;
               gB[i] = k ? fmaf(g, xk[k], gB[i]) : g * xk[k];
               sy[k] = i ? fmaf(Cv[i], hv, sy[k]) : Cv[i] * hv;
               sb[k] = i ? fmaf(g, Bv[i], sb[k]) : g * Bv[i];
               sa[k] = i ? fmaf(p, A2[k][i], sa[k]) : p * A2[k][i];
               dA[k][i] = fmaf(p, dk[k], dA[k][i]);
-              carry[k][i] = g * av[t][k][i];
             }
           }
           // dB, dC: eight sums over the sixteen quads; lane bits 3, 2, 4 choose among them, bit 5 holds the same twice
@@ -1119,6 +1167,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
       states(Part{0, 0});
       wave_lds_fence();
       for (int sub = (nt - 1) / kSub; sub >= 0; --sub) pair(Part{0, 0}, sub);
+      if (!FULL && clear) ln.clear_beyond(a, carry);
       fetch_kept(max(tb - kTok, t0));
       settle44(h0);
     }
@@ -1303,20 +1352,20 @@ static int scan_step_run(const ScanArgs& a, hipStream_t s) {
   PAL_HIP_LAUNCH_CHECK();
   return PAL_OK;
 }
-template <typename T, int NW>
+template <typename T, int NW, bool FULL>
 static int scan_fwd_run(const ScanArgs& a, hipStream_t s) {
   const dim3 grid(a.tiles, a.segs, a.rows);
   if (a.segs > 1) {
-    PAL_TIMED_LAUNCH(kKernScanSegment, s, (scan_fwd_kernel<T, NW, false>), grid, dim3(64 * NW), 0, s, a);
+    PAL_TIMED_LAUNCH(kKernScanSegment, s, (scan_fwd_kernel<T, NW, false, true>), grid, dim3(64 * NW), 0, s, a);
     PAL_HIP_LAUNCH_CHECK();
     PAL_TIMED_LAUNCH(kKernScanJoin, s, (scan_join_kernel<NW, false>), dim3(a.tiles, 4 * NW, a.rows), dim3(64 * join_waves(a)), 0, s, a);
     PAL_HIP_LAUNCH_CHECK();
   }
-  PAL_TIMED_LAUNCH(kKernScanFwd, s, (scan_fwd_kernel<T, NW, true>), grid, dim3(64 * NW), 0, s, a);
+  PAL_TIMED_LAUNCH(kKernScanFwd, s, (scan_fwd_kernel<T, NW, true, FULL>), grid, dim3(64 * NW), 0, s, a);
   PAL_HIP_LAUNCH_CHECK();
   return PAL_OK;
 }
-template <typename T, int NW>
+template <typename T, int NW, bool FULL>
 static int scan_bwd_run(const ScanArgs& a, hipStream_t s) {
   const dim3 grid(a.tiles, a.segs, a.rows);
   if (a.segs > 1) {
@@ -1325,7 +1374,7 @@ static int scan_bwd_run(const ScanArgs& a, hipStream_t s) {
     PAL_TIMED_LAUNCH(kKernScanJoin, s, (scan_join_kernel<NW, true>), dim3(a.tiles, 4 * NW, a.rows), dim3(64 * join_waves(a)), 0, s, a);
     PAL_HIP_LAUNCH_CHECK();
   }
-  PAL_TIMED_LAUNCH(kKernScanBwd, s, (scan_bwd_kernel<T, NW>), grid, dim3(64 * NW), 0, s, a);
+  PAL_TIMED_LAUNCH(kKernScanBwd, s, (scan_bwd_kernel<T, NW, FULL>), grid, dim3(64 * NW), 0, s, a);
   PAL_HIP_LAUNCH_CHECK();
   const int64_t n = 8 * (int64_t)a.rows * a.T * a.G * NW, blocks = (n + 64 * kSumWaves - 1) / (64 * kSumWaves);
   PAL_TIMED_LAUNCH(kKernScanBwdSums, s, scan_bwd_sums_kernel<T>, dim3(a.tiles * NW * 5 + (unsigned)(blocks < 2048 ? blocks : 2048)),
@@ -1343,19 +1392,19 @@ static int scan_fwd_waves(const ScanArgs& a, int nw, hipStream_t s) {
     if (a.N == 64) return scan_step_run<T, 16>(a, s);
   }
   switch (nw) {
-    case 1: return scan_fwd_run<T, 1>(a, s);
-    case 2: return scan_fwd_run<T, 2>(a, s);
-    case 3: return scan_fwd_run<T, 3>(a, s);
-    default: return scan_fwd_run<T, 4>(a, s);
+    case 1: return a.N % 16 ? scan_fwd_run<T, 1, false>(a, s) : scan_fwd_run<T, 1, true>(a, s);
+    case 2: return a.N % 16 ? scan_fwd_run<T, 2, false>(a, s) : scan_fwd_run<T, 2, true>(a, s);
+    case 3: return a.N % 16 ? scan_fwd_run<T, 3, false>(a, s) : scan_fwd_run<T, 3, true>(a, s);
+    default: return a.N % 16 ? scan_fwd_run<T, 4, false>(a, s) : scan_fwd_run<T, 4, true>(a, s);
   }
 }
 template <typename T>
 static int scan_bwd_waves(const ScanArgs& a, int nw, hipStream_t s) {
   switch (nw) {
-    case 1: return scan_bwd_run<T, 1>(a, s);
-    case 2: return scan_bwd_run<T, 2>(a, s);
-    case 3: return scan_bwd_run<T, 3>(a, s);
-    default: return scan_bwd_run<T, 4>(a, s);
+    case 1: return a.N % 16 ? scan_bwd_run<T, 1, false>(a, s) : scan_bwd_run<T, 1, true>(a, s);
+    case 2: return a.N % 16 ? scan_bwd_run<T, 2, false>(a, s) : scan_bwd_run<T, 2, true>(a, s);
+    case 3: return a.N % 16 ? scan_bwd_run<T, 3, false>(a, s) : scan_bwd_run<T, 3, true>(a, s);
+    default: return a.N % 16 ? scan_bwd_run<T, 4, false>(a, s) : scan_bwd_run<T, 4, true>(a, s);
   }
 }
 
