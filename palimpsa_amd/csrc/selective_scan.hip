@@ -181,7 +181,7 @@ __device__ __forceinline__ void settle44(float (*x)[4]) {
 }
 // Lanes as columns: lane l has channel l of the tile, x[j][i] entry 4 j + i of the wave's sixteen.
 struct Column : Tile {
-  unsigned own;                            // own channel (lanes beyond the group compute its last channel again and store nothing)
+  unsigned own;                            // own channel; lanes beyond the group have an empty one: rows, states and decays of zero
   bool on;
   __device__ __forceinline__ Column(const ScanArgs& a) : Tile(a) {
     const int c = base + (threadIdx.x & 63);
@@ -190,9 +190,10 @@ struct Column : Tile {
   }
   // the lane's entries of a [.., channels, N] fp32 array: where sequences start and end, not in the loops over tokens
   __device__ __forceinline__ void load(const ScanArgs& a, const float* p, float (*x)[4]) const {
-    const float* s = p + (int64_t)min(base + hidden_lane(), end - 1) * a.N + 16 * w;
+    const int c = base + hidden_lane();
+    const float* s = p + (int64_t)c * a.N + 16 * w;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) load4(a, s + 4 * j, 16 * w + 4 * j, x[j]);
+    for (int j = 0; j < 4; ++j) load4(a, s + 4 * j, c < end ? 16 * w + 4 * j : a.N, x[j]);
     settle44(x);
   }
   __device__ __forceinline__ void store(const ScanArgs& a, float* p, const float (*x)[4]) const {
@@ -226,7 +227,10 @@ struct Lane : Tile {
   __device__ __forceinline__ void load(const ScanArgs& a, const float* p, float (*x)[4]) const {
     const int l = hidden_lane(), n0 = 16 * w + 4 * (l & 3);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) load4(a, p + (int64_t)min(base + 16 * k + (l >> 2), end - 1) * a.N + n0, n0, x[k]);
+    for (int k = 0; k < 4; ++k) {
+      const int c = base + 16 * k + (l >> 2);
+      load4(a, p + (int64_t)c * a.N + n0, c < end ? n0 : a.N, x[k]);
+    }
     settle44(x);
   }
   __device__ __forceinline__ void store(const ScanArgs& a, float* p, const float (*x)[4]) const {
@@ -456,7 +460,7 @@ __global__ __launch_bounds__(64 * NW, 3) void scan_fwd_kernel(ScanArgs a) {
   if (NW == 1) ln.w = 0;      // (known to the compiler)
   const int l = threadIdx.x & 63, w = ln.w, row = ln.row;
   const int t0 = blockIdx.y * a.seg, t1 = min(a.T, t0 + a.seg);
-  const float bias = a.bias ? a.bias[ln.own] : 0.f, Dc = a.D ? a.D[ln.own] : 0.f;
+  const float bias = a.bias && ln.on ? a.bias[ln.own] : 0.f, Dc = a.D ? a.D[ln.own] : 0.f;
   float A2[4][4], h[4][4], dt_sum = 0.f;
   ln.load(a, a.A, A2);
 #pragma unroll
@@ -669,7 +673,7 @@ __global__ __launch_bounds__(64 * NW) void scan_back_segment_kernel(ScanArgs a) 
   if (NW == 1) ln.w = 0;      // (known to the compiler)
   const int l = threadIdx.x & 63, w = ln.w, row = ln.row;
   const int t0 = blockIdx.y * a.seg, t1 = min(a.T, t0 + a.seg);
-  const float bias = a.bias ? a.bias[ln.own] : 0.f;
+  const float bias = a.bias && ln.on ? a.bias[ln.own] : 0.f;
   float A2[4][4], g[4][4], dt_sum = 0.f;
   ln.load(a, a.A, A2);
 #pragma unroll
@@ -782,7 +786,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void scan_join_kernel(ScanArgs a) 
   const int l = threadIdx.x & 63, v = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int tile = blockIdx.x, w = blockIdx.y >> 2, j = blockIdx.y & 3, row = blockIdx.z;
   const int group = tile / a.tiles_g, base = group * a.per_group + (tile - group * a.tiles_g) * 64;
-  const int chan = min(base + l, (group + 1) * a.per_group - 1), n0 = 16 * w + 4 * j;
+  const int chan = base + l, n0 = chan < (group + 1) * a.per_group ? 16 * w + 4 * j : a.N;   // (lanes beyond the group: nothing)
   float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f}, d_sum = 0.f;
   load4(a, a.A + (int64_t)chan * a.N + n0, n0, A2);
 #pragma unroll
@@ -851,7 +855,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
   if (NW == 1) ln.w = 0;      // (known to the compiler)
   const int l = threadIdx.x & 63, w = ln.w, row = ln.row, own = own_at();
   const int t0 = blockIdx.y * a.seg, t1 = min(a.T, t0 + a.seg);
-  const float bias = a.bias ? a.bias[ln.own] : 0.f, Dc = a.D ? a.D[ln.own] : 0.f;
+  const float bias = a.bias && ln.on ? a.bias[ln.own] : 0.f, Dc = a.D ? a.D[ln.own] : 0.f;
   float A2[4][4], carry[4][4], dA[4][4];
   float dD = 0.f, dbias = 0.f;
   ln.load(a, a.A, A2);

@@ -59,3 +59,13 @@ def test_an_infinite_gradient(gpu_device, N, ch):
     inp["u"][0, 40, 1] = INF
     dy[0, 21, 0] = INF
     check(gpu_device, inp, init, dy, df)
+
+
+@pytest.mark.parametrize("N,ch", [(3, 3), (16, 70), (24, 5)])
+@pytest.mark.parametrize("where", ["init", "d_final", "delta_bias"])
+def test_the_last_channel_of_a_tile(gpu_device, N, ch, where):
+    """Lanes without a channel have nothing of the last channel's: sums over the channels (dB, dC) stay as they are."""
+    inp, init, dy, df = inputs(45, ch, N, 1, torch.float32, True)
+    inp["u"][0, 3, 0] = INF
+    {"init": init, "d_final": df, "delta_bias": inp["delta_bias"].view(1, ch)}[where][0, -1] = INF
+    check(gpu_device, inp, init, dy, df)
