@@ -69,3 +69,13 @@ def test_the_last_channel_of_a_tile(gpu_device, N, ch, where):
     inp["u"][0, 3, 0] = INF
     {"init": init, "d_final": df, "delta_bias": inp["delta_bias"].view(1, ch)}[where][0, -1] = INF
     check(gpu_device, inp, init, dy, df)
+
+
+def test_through_many_segments(gpu_device):
+    """3000 tokens of few channels run in 94 segments; the decay over a run of them is zero in fp32, and an infinite state stays infinite."""
+    inp, init, dy, df = inputs(3000, 40, 1, 1, torch.float32, False)
+    inp["u"][0, 5, 3], df[0, 7, 0] = INF, INF
+    check(gpu_device, inp, init, dy, df)
+    init, df = init.repeat(3, 1, 1), df.repeat(3, 1, 1)
+    df[1] = 1.0
+    check(gpu_device, inp, init, dy, df, [0, 1000, 1003, 3000])
