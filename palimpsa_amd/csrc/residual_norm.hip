@@ -3,7 +3,7 @@
 // with rows of y in the type of x, or in 8 bits (OCP e4m3) with one fp32 scale per row or per group of the row:
 //     scale = max(max |y|, 1e-12) / 448,   q = round(y / scale).
 // Backward, with dy and the gradient dres that comes back along the stream (both may be missing):
-//     ds = r (w dy - s r^2 mean(w dy s)) + dres  (the gradient of x and of residual),   dw = sum over rows of dy s r.
+//     ds = r (w dy - s r mean(w dy s r)) + dres  (the gradient of x and of residual),   dw = sum over rows of dy s r.
 // It reads s as the forward call handed it on and takes the mean square again, so nothing else is kept between the two.
 //
 // Bound by HBM: every row is read once and written once.  A row is held in registers by one wave (up to 2048 entries) or by
@@ -260,7 +260,8 @@ __global__ __launch_bounds__(256, WPR == 1 && NV <= 3 ? 2 : 1) void residual_nor
     ss = row_sum<WPR>(ss, sSum, turn);
     dot = row_sum<WPR>(dot, sDot, turn);
     const float r = rsqrtf(fmaf(ss, inv_d, A.eps));
-    const float c2 = has_dy ? r * r * r * dot * inv_d : 0.f;
+    // (never the cube of r by itself: it passes the range of fp32 for rows whose entries are beyond 1e13 or below 1e-13)
+    const float mean = has_dy ? r * dot * inv_d : 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const At p(lane, v, D);
@@ -268,7 +269,7 @@ __global__ __launch_bounds__(256, WPR == 1 && NV <= 3 ? 2 : 1) void residual_nor
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         dw[v][e] = fmaf(g[v][e] * r, s[v][e], dw[v][e]);
-        d[e] = fmaf(-s[v][e], c2, fmaf(g[v][e] * w[v][e], r, ex[v][e]));
+        d[e] = fmaf(r, fmaf(-s[v][e] * r, mean, g[v][e] * w[v][e]), ex[v][e]);
       }
       if (p.on) store_piece((TX*)A.dx + row * D + p.at, d, WHOLE ? 8 : D - p.at);
       if (p.on && A.dres_in) store_piece((TR*)A.dres_in + row * D + p.at, d, WHOLE ? 8 : D - p.at);

@@ -1,4 +1,4 @@
-"""residual_rms_norm where a workgroup's four waves walk several rows.
+"""residual_rms_norm where a workgroup's four waves walk several rows, and for rows of very small and very large entries.
 
 Bounds as in test_gpu_residual_norm.py: u = 2^-24, U = 2^-8; r is off by (D / 64 + 16) u, y by that and 4 roundings, ds by (D / 64 + 24) u of
 twice the sizes of its terms, dweight by (rows + D / 64 + 24) u of its, all behind the half step of the result's type; an 8-bit number by
@@ -61,3 +61,12 @@ def test_many_rows_of_four_waves_in_eight_bits(gpu_device, D, group):
     want = y * 448 / top.unsqueeze(-1)
     have = q.cpu().float().double().reshape(want.shape)
     assert ((have - want).abs() <= (2.0 ** -4 + 2 * k) * want.abs() + 2.0 ** -10 * (1 + k)).all()
+
+
+@pytest.mark.parametrize("size,eps", [(1e-15, 0.0), (1e-13, 0.0), (1e12, 1e-5), (1e15, 1e-5), (1e17, 1e-5)])
+@pytest.mark.parametrize("D,dt", [(5, torch.float32), (200, torch.float32), (200, torch.bfloat16), (2100, torch.float32)])
+def test_sizes_of_rows(gpu_device, size, eps, D, dt):
+    """The cube of 1 / rms passes the range of fp32 from 1e13 and 1e-13 on; the gradients, of size 1 / rms, do not."""
+    gen = torch.Generator().manual_seed(D)
+    n = lambda: torch.randn(9, D, generator=gen)  # noqa: E731
+    check(gpu_device, (n() * size).to(dt), None, 0.5 + torch.rand(D, generator=gen), n().to(dt), None, eps, dt)
