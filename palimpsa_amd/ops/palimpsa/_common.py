@@ -144,6 +144,9 @@ def prepare_inputs(q, k, v, b, gt, g, Ip, initial_mu_state, initial_I_state, cu_
 # table happen once per step instead of once per layer
 _chunk_meta_cache: dict = {}
 _CHUNK_META_CACHE_MAX = 8
+# what was handed to a call that was being captured into a graph: the graph reads it at every replay, so it stays for as long as its
+# cu_seqlens tensor (which the graph reads too), whatever happens to the entry above
+_captured_meta: dict = {}
 
 
 def chunk_meta(cu_seqlens: torch.Tensor, total_tokens: int, device: torch.device):
@@ -157,7 +160,23 @@ def chunk_meta(cu_seqlens: torch.Tensor, total_tokens: int, device: torch.device
     the copy taken when its entry was made (its memory may be shared with an array that a loader rewrites without
     torch noticing).  For a device tensor the entry relies on torch's version counter: a kernel or extension that
     writes through ``data_ptr()`` must call ``invalidate_chunk_meta()`` (or hand over a new tensor)."""
-    return _chunk_entry(cu_seqlens, total_tokens, device)[:2]
+    packed, total, _ = _chunk_entry(cu_seqlens, total_tokens, device)
+    if _capturing(device):
+        _keep_captured(cu_seqlens, packed)
+    return packed, total
+
+
+def _capturing(device: torch.device) -> bool:
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
+def _keep_captured(cu_seqlens: torch.Tensor, packed: torch.Tensor) -> None:
+    key = id(cu_seqlens)
+    kept = _captured_meta.get(key)
+    if kept is None:
+        kept = _captured_meta[key] = (weakref.ref(cu_seqlens, lambda _r, k=key: _captured_meta.pop(k, None)), [])
+    if not any(t is packed for t in kept[1]):
+        kept[1].append(packed)
 
 
 def longest_sequence(cu_seqlens: torch.Tensor, total_tokens: int, device: torch.device) -> int:
