@@ -507,6 +507,9 @@ static void conv_runs(ConvArgs& a, const PalConvDims* d, int vw) {
   a.runs = a.per_tile * (a.cu ? a.chunks : d->batch);
 }
 
+// workgroups of 256 that one launch holds: below 2^32 threads
+constexpr int64_t kConvMostBlocks = (int64_t)1 << 23;
+
 // channels per thread
 static int conv_piece(const PalConvDims* d, bool bwd) {
   const int vw = d->dtype == PAL_DTYPE_BF16 && !bwd ? 8 : 4;
@@ -554,9 +557,9 @@ extern "C" int pal_short_conv_fwd(const PalConvDims* d, const PalConvTensors* t,
   ConvArgs a = conv_args(d, t);
   const int vw = conv_piece(d, false);
   conv_runs(a, d, vw);
-  const int64_t threads = (int64_t)a.runs * a.pieces;
-  if (threads > (int64_t)1 << 31) return PAL_E_DIM;
-  a.blocks = (int)((threads + 255) / 256);
+  const int64_t blocks = ((int64_t)a.runs * a.pieces + 255) / 256;
+  if (blocks > kConvMostBlocks) return PAL_E_DIM;
+  a.blocks = (int)blocks;
   const int grid = a.blocks + (t->final_ ? conv_state_blocks(d) : 0);
   hipStream_t s = (hipStream_t)stream;
   if (d->dtype == PAL_DTYPE_BF16) vw == 8 ? conv_fwd_launch<bf16_t, 8>(a, d->width, grid, s) : conv_fwd_launch<bf16_t, 1>(a, d->width, grid, s);
@@ -591,7 +594,7 @@ extern "C" int pal_short_conv_bwd(const PalConvDims* d, const PalConvTensors* t,
   a.part = (float*)workspace;
   const int groups = conv_groups(a);
   const int64_t blocks = (int64_t)((a.pieces + 63) / 64) * groups;
-  if (blocks > (int64_t)1 << 31) return PAL_E_DIM;
+  if (blocks > kConvMostBlocks) return PAL_E_DIM;
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)blocks);
   if (d->dtype == PAL_DTYPE_BF16) vw == 4 ? conv_bwd_launch<bf16_t, 4>(a, d->width, grid, s) : conv_bwd_launch<bf16_t, 1>(a, d->width, grid, s);
@@ -612,6 +615,7 @@ extern "C" int pal_short_conv_step(const PalConvDims* d, const PalConvTensors* t
   if (d->flags & PAL_FLAG_VARLEN) return PAL_E_VARLEN_BATCH;
   if (d->n_seqs != d->batch) return PAL_E_DIM;
   if (!t->final_) return PAL_E_STATE;
+  if ((int64_t)d->n_seqs * d->channels > 256 * kConvMostBlocks) return PAL_E_DIM;
   ConvArgs a = conv_args(d, t);
   if (d->dtype == PAL_DTYPE_BF16) conv_step_launch<bf16_t>(a, d->width, (hipStream_t)stream);
   else conv_step_launch<float>(a, d->width, (hipStream_t)stream);

@@ -174,3 +174,15 @@ def test_entry_points_run_on_a_gpu_only():
                  lambda: residual_rms_norm_fp8(x, x, torch.ones(8))):
         with pytest.raises(RuntimeError, match="GPU only"):
             call()
+
+
+def test_conv_passes_of_more_threads_than_a_launch_holds_are_refused(L):
+    """2^32 threads: refused as a size, before a launch that the runtime would turn down."""
+    lib = L.load()
+    t = L.PalConvTensors(x=P, weight=P, y=P, final_=P)
+    step = _conv_dims(L, batch=1 << 22, n_seqs=1 << 22, seq_len=1, channels=1 << 10, x_token_stride=1 << 10, x_batch_stride=1 << 10)
+    assert lib.pal_short_conv_step(step, t, None) == L.PAL_E_DIM
+    many = _conv_dims(L, batch=1 << 27, n_seqs=1 << 27, seq_len=1, channels=4, x_token_stride=4, x_batch_stride=4)
+    t = L.PalConvTensors(x=P, weight=P, y=P)
+    need = lib.pal_short_conv_bwd_workspace_bytes(many)
+    assert lib.pal_short_conv_bwd(many, t, L.PalConvGrads(dy=P, dx=P, dweight=P), P, need, None) == L.PAL_E_DIM
