@@ -1466,7 +1466,7 @@ extern "C" int pal_scan_fwd(const PalScanDims* d, const PalScanTensors* t, void*
   ScanArgs a{};
   scan_args(a, d, t, false);
   const int nw = scan_waves(d);
-  if (a.segs > 65535 || (int64_t)a.tiles * nw > 1 << 20) return PAL_E_DIM;   // (the second: 32-bit places in a block's shares)
+  if (a.segs > 65535 || (int64_t)a.tiles * nw > 1 << 20) return PAL_E_DIM;   // (the second: the threads of a launch, and 32-bit places)
   if (a.segs > 1) {
     if (!workspace || workspace_bytes < seg_bytes(a, nw)) return PAL_E_WORKSPACE;
     if (!is_aligned16(workspace)) return PAL_E_ALIGN;
@@ -1503,7 +1503,8 @@ extern "C" int pal_scan_bwd(const PalScanDims* d, const PalScanTensors* t, const
   ScanArgs a{};
   scan_args(a, d, t, true);
   const int nw = scan_waves(d);
-  if (a.segs > 65535 || (int64_t)a.tiles * nw > 1 << 20) return PAL_E_DIM;   // (the second: 32-bit places in a block's shares)
+  // (the second: 32-bit places in a block's shares, and the threads of the sums, which have five workgroups of 1024 for each)
+  if (a.segs > 65535 || (int64_t)a.tiles * nw > 1 << 19) return PAL_E_DIM;
   a.dy = gr->dy; a.d_final = gr->d_final; a.du = gr->du; a.ddelta = gr->ddelta; a.dA = gr->dA; a.dB = gr->dB; a.dC = gr->dC;
   a.dD = gr->dD; a.dz = gr->dz; a.dbias = gr->ddelta_bias; a.d_init = gr->d_init;
   char* p = (char*)workspace;

@@ -186,3 +186,14 @@ def test_conv_passes_of_more_threads_than_a_launch_holds_are_refused(L):
     t = L.PalConvTensors(x=P, weight=P, y=P)
     need = lib.pal_short_conv_bwd_workspace_bytes(many)
     assert lib.pal_short_conv_bwd(many, t, L.PalConvGrads(dy=P, dx=P, dweight=P), P, need, None) == L.PAL_E_DIM
+
+
+def test_scan_backward_of_more_tiles_than_its_sums_hold_is_refused(L):
+    """A million groups of one channel: the last launch would have 5 x 2^30 threads."""
+    lib = L.load()
+    n = 1 << 20
+    d = L.PalScanDims(batch=1, seq_len=8, n_seqs=1, channels=n, state=8, groups=n, dtype=1, softplus=1, flags=0,
+                      **{x + "_batch": 0 for x in ("u", "delta", "z", "B", "C")}, u_token=n, delta_token=n, z_token=n, B_token=8 * n, C_token=8 * n)
+    t = L.PalScanTensors(u=P, delta=P, A=P, B=P, C=P, y=P, checkpoints=P)
+    g = L.PalScanGrads(dy=P, du=P, ddelta=P, dA=P, dB=P, dC=P)
+    assert lib.pal_scan_bwd(d, t, g, P, lib.pal_scan_bwd_workspace_bytes(d), None) == L.PAL_E_DIM
