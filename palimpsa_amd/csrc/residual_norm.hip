@@ -29,7 +29,7 @@ struct NormArgs {
   float *part, *dweight;  // [workgroups][dim]; [dim]
   int64_t rows;
   int64_t x_stride, res_stride;   // elements between rows of x and of residual (all other rows are packed)
-  int dim, weight_bf16, group, n_part;
+  int dim, weight_bf16, group;
   float eps;
 };
 

@@ -270,7 +270,6 @@ template <typename T>
 __device__ __forceinline__ void row_store(T* row, unsigned i, T x) { *row_element(row, i * (unsigned)sizeof(T)) = x; }
 // A load that only some paths make has to be waited for on those paths: where they meet the others again, the compiler would wait for
 // every load in flight on any of them, the next block's rows among them.  The empty assembly is a use of the value.
-__device__ __forceinline__ void settle(f32x4& x) { asm volatile("" : "+v"(x)); }
 __device__ __forceinline__ void settle(float& x) { asm volatile("" : "+v"(x)); }
 
 // Four entries of B or C, from entry n on (zero beyond N), as fetched.  p: the group's entries of the block's first token; the
