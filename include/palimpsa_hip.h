@@ -490,7 +490,7 @@ typedef struct PalScanTensors {
   void *y;                    /* dtype [B,T,D]                                  */
   const float *init;          /* fp32 [N_seqs,D,N] or NULL                      */
   float *final_;              /* fp32 [N_seqs,D,N] or NULL; may be init where no gradient is wanted, but not with cu_seqlens (PAL_E_STATE) */
-  const int32_t *cu_seqlens;  /* device int32 [n_seqs+1] or NULL                */
+  const int32_t *cu_seqlens;  /* device int32 [n_seqs+1], ascending from 0 to T (held to the tokens, as in pal_chunk_fwd), or NULL */
   float *checkpoints;         /* pal_scan_checkpoint_bytes(dims), for the backward, or NULL */
 } PalScanTensors;
 

@@ -27,8 +27,9 @@
 // For the backward the forward keeps the state before every 8th token in fp32; the backward computes the 8 tokens again, two
 // at a time, and keeps a and a h' of two tokens in registers.
 //
-// Measured (bf16, 1536 channels, N 16, z and D): 1 x 16384 tokens forward 181 us (pass 111, segments 80); 8 x 2048 forward and backward
-// 660 us (backward 375); a token of 256 sequences 11.8 us.
+// Measured (bf16, 1536 channels, N 16, z and D): a call of 1 x 16384 tokens forward 179 us, of 8 x 2048 forward and backward 661 us, of a token of
+// 256 sequences 11.7 us.  Under the profiler the first two take 208 and 716: 114 (pass) + 82 (segments) + 11 (join), and 374 (backward) +
+// 116 (pass) + 100 + 97 (segments) + 14 (sums) + 9 + 8 (joins).
 #include "pal_common.h"
 #include "pal_host.h"
 #include "pal_profile.h"
@@ -614,7 +615,8 @@ __global__ __launch_bounds__(64 * NW, 3) void scan_fwd_kernel(ScanArgs a) {
 
 // A few tokens: the state is all the traffic, and a wave of the kernel above would wait for one block of it at a time.  Thread = four
 // entries of the state of one channel, in the order of memory; LPC threads a channel add their sums.  256 x 1 tokens of 1536 channels, N 16:
-// 11 to 13 us, 4.1 to 4.8 TB/s (17.5 in the kernel above).
+// a call of 11.8 us, 4.5 TB/s (18.1 in the kernel above; at eight tokens the two are equal).  The sum over a channel's threads is by lane moves, which
+// takes a power of two of them: N 4, 8, 16, 32 and 64; the others go to the kernel above (N 12, 24, 48: 16, 28, 44 us; N 32, 64 here 20, 35).
 constexpr int kStepTokens = 4;
 template <int LPC>
 __device__ __forceinline__ float channel_sum(float x) {
