@@ -1011,9 +1011,7 @@ __global__ __launch_bounds__(64 * NW, 2) void scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                h[k][i] = fmaf(fast_exp2(dk[k] * A2[k][i]), h[k][i], xk[k] * Bv[i]);
-              }
+              for (int i = 0; i < 4; ++i) h[k][i] = fmaf(fast_exp2(dk[k] * A2[k][i]), h[k][i], xk[k] * Bv[i]);
             if (t % kSub == kSub - 1)
 #pragma unroll
               for (int k = 0; k < 4; ++k) sH[w][t / kSub][k][l] = (f32x4){h[k][0], h[k][1], h[k][2], h[k][3]};
