@@ -516,6 +516,105 @@ size_t pal_scan_bwd_workspace_bytes(const PalScanDims *dims);
 int pal_scan_bwd(const PalScanDims *dims, const PalScanTensors *t, const PalScanGrads *gr, void *workspace,
                  size_t workspace_bytes, void *stream);
 
+/* ----------------------------------------------- dropout, layer norm */
+
+/* Which entries a dropout keeps is a function of its seed and their place alone, nothing is stored: entry (row, column) of [rows,dim]
+ * takes word column % 4 of Philox4x32 with seven rounds (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", 2011) of the
+ * counter (column / 4, row mod 2^32, row / 2^32, site) and the key (seed mod 2^32, seed / 2^32), and is kept where the word is not below
+ * p 2^32 (rounded to a whole number, at most 2^32 - 1).  Kept entries are multiplied by 1 / (1 - p), the others are zero whatever they held. */
+typedef struct PalDropout {
+  double p;               /* 0 <= p < 1; 0: nothing is dropped, the rest is not looked at */
+  int64_t seed;           /* its 64 bits are the key                              */
+  const int64_t *seed_at; /* device: the seed is read from there (a captured graph can have a new one at every replay), or NULL */
+  uint32_t site;          /* number of the place in a model: sites share a seed    */
+} PalDropout;
+
+/* y = dropout(x) of `rows` rows of dim entries, those of x x_stride apart, those of y packed; dtype PAL_DTYPE_*; x and y may be the same.  The gradient is the
+ * same call on the gradient. */
+int pal_dropout(const PalDropout *drop, const void *x, void *y, int64_t rows, int64_t dim, int64_t x_stride, int32_t dtype, void *stream);
+
+/* Layer norm, alone or as the pre-norm between two blocks with the residual's addition and a dropout in front of it:
+ *   s = dropout(x) + residual, rounded to res_dtype and handed on;  y = (s - mean(s)) r * weight + bias,  r = 1 / sqrt(mean((s - mean(s))^2) + eps)
+ * Rows of any length up to 16384 at any element's address. */
+typedef struct PalLayerNormDims {
+  int64_t rows;
+  int64_t x_stride;     /* elements between rows of x (>= dim); every other row tensor is packed, but: */
+  int64_t res_stride;   /* elements between rows of residual (>= dim)           */
+  int32_t dim;          /* entries per row                                      */
+  int32_t dtype;        /* PAL_DTYPE_* of x, y, dy, dx                          */
+  int32_t res_dtype;    /* of residual, residual_out and their gradients: F32, or BF16 if dtype is BF16 */
+  int32_t weight_dtype; /* of weight and bias                                   */
+  float eps;
+  PalDropout drop;
+} PalLayerNormDims;
+
+typedef struct PalLayerNormTensors {
+  const void *x;        /* dtype [rows,dim]                                     */
+  const void *residual; /* res_dtype [rows,dim] or NULL                         */
+  const void *weight;   /* weight_dtype [dim]                                   */
+  const void *bias;     /* weight_dtype [dim] or NULL                           */
+  void *residual_out;   /* res_dtype [rows,dim]; NULL for the norm of x itself (no residual, no dropout, res_dtype == dtype) */
+  void *y;              /* dtype [rows,dim]                                     */
+  float *stats;         /* fp32 [rows,2]: mean(s) and r, for the backward, or NULL */
+} PalLayerNormTensors;
+
+typedef struct PalLayerNormGrads {
+  const void *dy;            /* dtype [rows,dim] or NULL (zero)                 */
+  const void *dresidual_out; /* res_dtype [rows,dim] or NULL (zero)             */
+  void *dx;                  /* dtype [rows,dim]                                */
+  void *dresidual;           /* res_dtype [rows,dim] or NULL (not wanted; without a dropout and of one type it is dx) */
+  float *dweight;            /* fp32 [dim]                                      */
+  float *dbias;              /* fp32 [dim], NULL iff bias is NULL               */
+} PalLayerNormGrads;
+
+int pal_layer_norm_fwd(const PalLayerNormDims *dims, const PalLayerNormTensors *t, void *stream);
+/* Backward: reads weight, stats, and s from residual_out as the forward call wrote it (NULL: from x); the other tensors are not touched. */
+size_t pal_layer_norm_bwd_workspace_bytes(const PalLayerNormDims *dims);
+int pal_layer_norm_bwd(const PalLayerNormDims *dims, const PalLayerNormTensors *t, const PalLayerNormGrads *gr,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------ gated feed-forward block */
+
+/* The second half of a block (fla.modules.GatedMLP of the reference's PalimpsaBlock, restated from its published behaviour):
+ *   g = x w_gate^T,  u = x w_up^T,  h = act(g) u,  y = h w_down^T
+ * Dims are multiples of 8 and every pointer is 16-byte aligned (callers with other sizes pad with zeros). */
+#define PAL_ACT_SILU 0       /* g sigmoid(g)                                     */
+#define PAL_ACT_GELU 1       /* g (1 + erf(g / sqrt 2)) / 2                      */
+#define PAL_ACT_GELU_TANH 2  /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 */
+#define PAL_ACT_RELU 3       /* max(g, 0)                                        */
+
+typedef struct PalMlpDims {
+  int64_t rows;         /* up to 2^30                                           */
+  int64_t x_stride;     /* elements between rows of x (>= dim, a multiple of 8, up to 2^20); every other tensor is packed */
+  int32_t dim;          /* entries of a row of x                                */
+  int32_t hidden;       /* of g, u and h                                        */
+  int32_t out_dim;      /* of y                                                 */
+  int32_t dtype;        /* PAL_DTYPE_* of every tensor                          */
+  int32_t activation;   /* PAL_ACT_*                                            */
+} PalMlpDims;
+
+typedef struct PalMlpTensors {
+  const void *x;               /* [rows,dim]                                    */
+  const void *w_gate, *w_up;   /* [hidden,dim]                                  */
+  const void *w_down;          /* [out_dim,hidden]                              */
+  void *y;                     /* [rows,out_dim]                                */
+  void *gate, *up;             /* [rows,hidden]: g and u, kept for the backward; both NULL where none follows */
+} PalMlpTensors;
+
+typedef struct PalMlpGrads {
+  const void *dy;              /* [rows,out_dim]                                */
+  void *dx;                    /* [rows,dim] or NULL (not wanted), as the others: */
+  void *dw_gate, *dw_up;       /* [hidden,dim]                                  */
+  void *dw_down;               /* [out_dim,hidden]                              */
+} PalMlpGrads;
+
+size_t pal_gated_mlp_fwd_workspace_bytes(const PalMlpDims *dims);
+int pal_gated_mlp_fwd(const PalMlpDims *dims, const PalMlpTensors *t, void *workspace, size_t workspace_bytes, void *stream);
+/* Backward: t as in the forward call, with gate and up as that call left them; t->y is not touched. */
+size_t pal_gated_mlp_bwd_workspace_bytes(const PalMlpDims *dims);
+int pal_gated_mlp_bwd(const PalMlpDims *dims, const PalMlpTensors *t, const PalMlpGrads *gr, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------------------ shape queries */
 
 /* 1 if the chunked entry points would build the tile-start states of this call (dims as handed to them,

@@ -120,6 +120,39 @@ class PalScanGrads(C.Structure):
                                           "d_init")]
 
 
+PAL_ACT = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
+
+
+class PalMlpDims(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("rows", "x_stride")] +
+                [(n, C.c_int32) for n in ("dim", "hidden", "out_dim", "dtype", "activation")])
+
+
+class PalMlpTensors(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "w_gate", "w_up", "w_down", "y", "gate", "up")]
+
+
+class PalMlpGrads(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("dy", "dx", "dw_gate", "dw_up", "dw_down")]
+
+
+class PalDropout(C.Structure):
+    _fields_ = [("p", C.c_double), ("seed", C.c_int64), ("seed_at", C.c_void_p), ("site", C.c_uint32)]
+
+
+class PalLayerNormDims(C.Structure):
+    _fields_ = ([(n, C.c_int64) for n in ("rows", "x_stride", "res_stride")] +
+                [(n, C.c_int32) for n in ("dim", "dtype", "res_dtype", "weight_dtype")] + [("eps", C.c_float), ("drop", PalDropout)])
+
+
+class PalLayerNormTensors(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "residual", "weight", "bias", "residual_out", "y", "stats")]
+
+
+class PalLayerNormGrads(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("dy", "dresidual_out", "dx", "dresidual", "dweight", "dbias")]
+
+
 class PalimpsaHipError(RuntimeError):
     def __init__(self, code: int, where: str, text: str):
         super().__init__(f"{where} failed with code {code}: {text}")
@@ -188,6 +221,20 @@ def load() -> C.CDLL:
     lib.pal_short_conv_step.restype = C.c_int
     lib.pal_short_conv_step.argtypes = [P(PalConvDims), P(PalConvTensors), C.c_void_p]
     lib.pal_scan_fwd.argtypes = [P(PalScanDims), P(PalScanTensors), C.c_void_p, C.c_size_t, C.c_void_p]
+    for name in ("pal_gated_mlp_fwd_workspace_bytes", "pal_gated_mlp_bwd_workspace_bytes"):
+        fn = getattr(lib, name)
+        fn.restype = C.c_size_t
+        fn.argtypes = [P(PalMlpDims)]
+    lib.pal_gated_mlp_fwd.restype = lib.pal_gated_mlp_bwd.restype = C.c_int
+    lib.pal_gated_mlp_fwd.argtypes = [P(PalMlpDims), P(PalMlpTensors), C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.pal_gated_mlp_bwd.argtypes = [P(PalMlpDims), P(PalMlpTensors), P(PalMlpGrads), C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.pal_layer_norm_fwd.restype = lib.pal_layer_norm_bwd.restype = lib.pal_dropout.restype = C.c_int
+    lib.pal_layer_norm_fwd.argtypes = [P(PalLayerNormDims), P(PalLayerNormTensors), C.c_void_p]
+    lib.pal_layer_norm_bwd.argtypes = [P(PalLayerNormDims), P(PalLayerNormTensors), P(PalLayerNormGrads), C.c_void_p, C.c_size_t,
+                                       C.c_void_p]
+    lib.pal_layer_norm_bwd_workspace_bytes.restype = C.c_size_t
+    lib.pal_layer_norm_bwd_workspace_bytes.argtypes = [P(PalLayerNormDims)]
+    lib.pal_dropout.argtypes = [P(PalDropout), C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int32, C.c_void_p]
     for name in ("pal_scan_fwd_workspace_bytes", "pal_scan_checkpoint_bytes"):
         fn = getattr(lib, name)
         fn.restype = C.c_size_t
@@ -225,7 +272,8 @@ def _check_host(ext) -> None:
     want = (PAL_ABI_VERSION, C.sizeof(PalDims), C.sizeof(PalFwdTensors), C.sizeof(PalBwdTensors))
     have = tuple(getattr(ext, "abi", ()))
     want += tuple(C.sizeof(t) for t in (PalNormDims, PalNormTensors, PalNormGrads, PalConvDims, PalConvTensors, PalConvGrads,
-                                        PalScanDims, PalScanTensors, PalScanGrads))
+                                        PalScanDims, PalScanTensors, PalScanGrads, PalDropout, PalLayerNormDims, PalLayerNormTensors,
+                                        PalLayerNormGrads, PalMlpDims, PalMlpTensors, PalMlpGrads))
     have += tuple(getattr(ext, "abi_block", ()))
     built = getattr(ext, "torch_version", None)
     if have != want or built != torch.__version__:
@@ -257,7 +305,9 @@ _HOST_FUNCTIONS = ("pal_recurrent_fwd", "pal_gla_recurrent_fwd", "pal_chunk_fwd"
                    "pal_residual_norm_fwd", "pal_residual_norm_bwd", "pal_residual_norm_bwd_workspace_bytes",
                    "pal_short_conv_fwd", "pal_short_conv_bwd", "pal_short_conv_bwd_workspace_bytes", "pal_short_conv_step",
                    "pal_scan_fwd", "pal_scan_fwd_workspace_bytes", "pal_scan_checkpoint_bytes", "pal_scan_bwd",
-                   "pal_scan_bwd_workspace_bytes")
+                   "pal_scan_bwd_workspace_bytes", "pal_dropout", "pal_layer_norm_fwd", "pal_layer_norm_bwd",
+                   "pal_layer_norm_bwd_workspace_bytes", "pal_gated_mlp_fwd", "pal_gated_mlp_fwd_workspace_bytes", "pal_gated_mlp_bwd",
+                   "pal_gated_mlp_bwd_workspace_bytes")
 
 
 # How the chunked entry points build the tile-start states (PAL_FLAG_STATES_* of the C ABI): 0 = chosen by shape,

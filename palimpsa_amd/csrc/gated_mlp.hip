@@ -1,0 +1,414 @@
+// Gated feed-forward block:  g = x Wg^T,  u = x Wu^T,  h = act(g) u,  y = h Wd^T,  and its gradients
+//     dh = dy Wd,  dg = dh u act'(g),  du = dh act(g),  dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h.
+//
+// Forward: two launches.  The first computes both products of a tile side by side and stores h (for training g and u too); the second
+// multiplies by Wd.  Backward: dh is never stored, the kernel that computes it turns it into dg and du and computes h again from g and u; the
+// gradient of x is one walk over both products, and the three of the weights are one launch (see tile_product.h).
+//
+// A call of few rows is bound by the weights, each of which is used once per 16 rows: few_rows_kernel has no tiles in LDS, the waves of a
+// workgroup walk over k side by side, each with a sixteenth of a line of the weights per lane straight from memory into the matrix units.
+//
+// Roundings to the type of the rows: g, u (kept, or only h without a gradient), h, dg and du, once each, half a step of the type; all sums are
+// in fp32.  Their errors in y and the gradients are of the size of the rounding of those results themselves.
+#include "pal_common.h"
+#include "pal_host.h"
+#include "pal_profile.h"
+#include "tile_product.h"
+
+namespace pal {
+
+constexpr int kFewRows = 64;
+
+// ------------------------------------------------------------------------------------------------------------ few rows
+struct FewArgs {
+  const void *x, *w, *w2;    // [rows][k] (x_ld), [n][k]; w2: second product (gated)
+  void *out, *gate_out, *up_out;   // [rows][n]
+  int64_t x_ld;              // elements
+  int32_t rows, n, k, act;
+};
+
+// W waves; R groups of sixteen rows of x
+template <typename T, bool GATED, int W, int R>
+__global__ __launch_bounds__(64 * W) void few_rows_kernel(FewArgs P) {
+  typedef TileType<T> E;
+  constexpr int kMats = GATED ? 2 : 1, kPiece = E::kPiece, kSpan = 8 * kPiece;   // 128 bytes of each row at a time
+  constexpr int kBatch = 4;
+  __shared__ f32x4 s[W][kMats * R][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int j = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
+  const int64_t wrow = (int64_t)min(n0 + j, P.n - 1) * P.k;
+  const T* w[2] = {(const T*)P.w + wrow, GATED ? (const T*)P.w2 + wrow : nullptr};
+  const T* x[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) x[r] = (const T*)P.x + min(16 * r + j, P.rows - 1) * P.x_ld;
+  f32x4 acc[kMats][R];
+#pragma unroll
+  for (int m = 0; m < kMats; ++m)
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = wave * kSpan; k0 < P.k; k0 += kBatch * W * kSpan) {
+    f32x4 wb[kBatch][2][kMats];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = k0 + b * W * kSpan + (2 * g + h) * kPiece;
+#pragma unroll
+        for (int m = 0; m < kMats; ++m) wb[b][h][m] = *(const f32x4*)(w[m] + min(k, P.k - kPiece));
+      }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (k0 + b * W * kSpan >= P.k) break;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = k0 + b * W * kSpan + (2 * g + h) * kPiece;
+        const bool in = k < P.k;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          f32x4 xb = *(const f32x4*)(x[r] + min(k, P.k - kPiece));
+          xb = in ? xb : zero;
+#pragma unroll
+          for (int m = 0; m < kMats; ++m) acc[m][r] = E::mma(in ? wb[b][h][m] : zero, xb, acc[m][r]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < kMats; ++m)
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[wave][m * R + r][lane] = acc[m][r];
+  __syncthreads();
+  // a thread: four neighbouring columns of one row
+  for (int i = threadIdx.x; i < R * 64; i += 64 * W) {
+    const int r = i >> 6, l = i & 63, row = 16 * r + (l & 15), n = n0 + 4 * (l >> 4);
+    f32x4 t[kMats];
+#pragma unroll
+    for (int m = 0; m < kMats; ++m) {
+      t[m] = s[0][m * R + r][l];
+#pragma unroll
+      for (int v = 1; v < W; ++v) t[m] += s[v][m * R + r][l];
+    }
+    if (row >= P.rows || n >= P.n) continue;
+    const int64_t at = (int64_t)row * P.n + n;
+    float c[4], none;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (GATED) {
+        activate<false>(P.act, t[0][e], c[e], none);
+        c[e] *= t[1][e];
+      } else {
+        c[e] = t[0][e];
+      }
+    }
+    store_vec<4>((T*)P.out + at, c);
+    if constexpr (GATED) {
+      if (P.gate_out) {
+        float a[4], b[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = t[0][e], b[e] = t[1][e];
+        store_vec<4>((T*)P.gate_out + at, a);
+        store_vec<4>((T*)P.up_out + at, b);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------- sums of k's shares
+struct JoinArgs {
+  const float* part[3];
+  void* out[3];
+  int64_t n[3];              // numbers of a share
+  int32_t splits;
+  const void *gate, *up;     // kTileGrad
+  void *h, *du;
+  int32_t act;
+};
+template <typename T, bool GRAD>
+__global__ __launch_bounds__(256) void tile_join_kernel(JoinArgs P) {
+  const int which = blockIdx.y;
+  const int64_t n = P.n[which];
+  for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; at < n; at += (int64_t)gridDim.x * 256 * 8) {
+    float c[8];
+    tile_load8(P.part[which] + at, c);
+#pragma unroll 4
+    for (int s = 1; s < P.splits; ++s) {
+      float b[8];
+      tile_load8(P.part[which] + s * n + at, b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) c[e] += b[e];
+    }
+    if constexpr (GRAD) {
+      float gt[8], up[8], du[8], h[8];
+      tile_load8((const T*)P.gate + at, gt);
+      tile_load8((const T*)P.up + at, up);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float a, d;
+        activate<true>(P.act, gt[e], a, d);
+        du[e] = c[e] * a;
+        c[e] = c[e] * up[e] * d;
+        h[e] = a * up[e];
+      }
+      tile_store8((T*)P.du + at, du);
+      if (P.h) tile_store8((T*)P.h + at, h);
+    }
+    tile_store8((T*)P.out[which] + at, c);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+struct TilePlan {
+  bool big;
+  int tiles, splits, split_steps;
+};
+constexpr int kBigTile = 256, kSmallTile = 128;
+
+// Tile size and shares of k: the cheapest by the time of a step of a tile (us), the launch's rounds over the chip and, for shares, their
+// way through memory.
+static TilePlan plan_tiles(const TileArgs& P, int kind, int dtype) {
+  TilePlan best{};
+  double least = 1e30;
+  const int one = (P.k + (dtype == PAL_DTYPE_BF16 ? 31 : 15)) / (dtype == PAL_DTYPE_BF16 ? 32 : 16);
+  const int steps = kind == kTileTwice ? 2 * one : one;
+  double numbers = 0;
+  for (int i = 0; i < P.n_prod; ++i) numbers += (double)P.prod[i].a.rows * P.prod[i].b.rows;
+  for (int big = 0; big < 2; ++big) {
+    const int t = big ? kBigTile : kSmallTile, tn = kind == kTileGated ? t / 2 : t, slots = big ? 256 : 512;
+    int64_t tiles = 0;
+    for (int i = 0; i < P.n_prod; ++i)
+      tiles += (int64_t)((P.prod[i].a.rows + t - 1) / t) * ((P.prod[i].b.rows + tn - 1) / tn);
+    if (tiles > 1 << 22) continue;   // threads of a launch
+    const double per_step = (big ? 0.6 : 0.42) * (dtype == PAL_DTYPE_BF16 ? 1 : 6);
+    for (int s = 1; s <= (kind == kTileGated ? 1 : 32) && s <= steps; ++s) {
+      const int share = (steps + s - 1) / s, splits = (steps + share - 1) / share;
+      if (splits != s || tiles * s > 1 << 22) continue;
+      const double rounds = (double)((tiles * s + slots - 1) / slots);
+      const double us = rounds * (share * per_step + 3) + (s > 1 ? 3 + numbers * s * 8 / 4e6 : 0);
+      if (us < least) {
+        least = us;
+        best = TilePlan{big != 0, (int)tiles, s, share};
+      }
+    }
+  }
+  return best;
+}
+
+template <typename T, int KIND, bool ACOLS, bool BCOLS, int WM, int WN, int NFM, int NFN>
+static int tile_launch(const TileArgs& P, int id, hipStream_t s) {
+  constexpr size_t lds = (size_t)kRing * 64 * 16 * (NFM * WM + NFN * WN);
+  const auto kernel = &tile_product_kernel<T, KIND, ACOLS, BCOLS, WM, WN, NFM, NFN>;
+  if (int rc = allow_lds((const void*)kernel, lds)) return rc;
+  PAL_TIMED_LAUNCH(id, s, (*kernel), dim3(P.tiles * P.splits), dim3(64 * WM * WN), lds, s, P);
+  PAL_HIP_LAUNCH_CHECK();
+  return PAL_OK;
+}
+
+static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
+static size_t part_bytes(const TileArgs& P, const TilePlan& plan) {
+  if (plan.splits < 2) return 0;
+  size_t n = 0;
+  for (int i = 0; i < P.n_prod; ++i) n += (size_t)P.prod[i].a.rows * P.prod[i].b.rows;
+  return round256(n * sizeof(float) * plan.splits);
+}
+
+// the launches of one set of products; `part`: part_bytes of them
+template <typename T, int KIND, bool ACOLS, bool BCOLS>
+static int tile_run(TileArgs P, const TilePlan& plan, float* part, int id, hipStream_t s) {
+  if (!plan.tiles) return PAL_E_DIM;
+  const int t = plan.big ? kBigTile : kSmallTile, tn = KIND == kTileGated ? t / 2 : t;
+  P.tiles = plan.tiles;
+  P.splits = plan.splits;
+  P.split_steps = plan.split_steps;
+  int first = 0;
+  JoinArgs J{};
+  int64_t most = 0;
+  for (int i = 0; i < P.n_prod; ++i) {
+    TileProduct& p = P.prod[i];
+    p.first = first;
+    p.tiles_n = (p.b.rows + tn - 1) / tn;
+    first += p.tiles_n * ((p.a.rows + t - 1) / t);
+    p.part = part;
+    J.part[i] = part;
+    J.out[i] = p.c;
+    J.n[i] = (int64_t)p.a.rows * p.b.rows;
+    most = J.n[i] > most ? J.n[i] : most;
+    if (part) part += J.n[i] * plan.splits;
+  }
+  const int rc = plan.big ? tile_launch<T, KIND, ACOLS, BCOLS, 2, 4, 8, 4>(P, id, s) : tile_launch<T, KIND, ACOLS, BCOLS, 2, 2, 4, 4>(P, id, s);
+  if (rc || plan.splits < 2) return rc;
+  J.splits = plan.splits; J.gate = P.gate; J.up = P.up; J.h = P.gate_out; J.du = P.up_out; J.act = P.act;
+  const int64_t blocks = (most + 2047) / 2048;
+  PAL_TIMED_LAUNCH(kKernTileJoin, s, (tile_join_kernel<T, KIND == kTileGrad>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), P.n_prod),
+                   dim3(256), 0, s, J);
+  PAL_HIP_LAUNCH_CHECK();
+  return PAL_OK;
+}
+
+template <typename T, bool GATED>
+static int few_launch(const FewArgs& P, hipStream_t s) {
+  const dim3 grid((P.n + 15) / 16);
+  const int id = GATED ? kKernMlpFewUp : kKernMlpFewDown;
+  constexpr int W = GATED ? 8 : 16;
+  if (P.rows <= 16) PAL_TIMED_LAUNCH(id, s, (few_rows_kernel<T, GATED, W, 1>), grid, dim3(64 * W), 0, s, P);
+  else if (P.rows <= 32) PAL_TIMED_LAUNCH(id, s, (few_rows_kernel<T, GATED, 8, 2>), grid, dim3(64 * 8), 0, s, P);
+  else PAL_TIMED_LAUNCH(id, s, (few_rows_kernel<T, GATED, 8, 4>), grid, dim3(64 * 8), 0, s, P);
+  PAL_HIP_LAUNCH_CHECK();
+  return PAL_OK;
+}
+
+static int check_mlp(const PalMlpDims* d) {
+  if (!d) return PAL_E_NULL;
+  if (d->dtype != PAL_DTYPE_F32 && d->dtype != PAL_DTYPE_BF16) return PAL_E_DTYPE;
+  if (d->activation < 0 || d->activation > PAL_ACT_RELU) return PAL_E_DIM;
+  for (int32_t n : {d->dim, d->hidden, d->out_dim})
+    if (n <= 0 || n % 8 || n > 1 << 20) return PAL_E_DIM;
+  if (d->rows <= 0 || d->rows > 1 << 30 || d->x_stride < d->dim || d->x_stride % 8) return PAL_E_DIM;
+  // a tile's rows are reached by offsets of 31 bits from its first
+  if (d->x_stride > (int64_t)1 << 20) return PAL_E_DIM;
+  return PAL_OK;
+}
+static size_t mlp_elem(const PalMlpDims* d) { return d->dtype == PAL_DTYPE_BF16 ? 2 : 4; }
+
+static TileOperand operand(const void* p, int64_t ld_elems, size_t es, int64_t rows, const void* p2 = nullptr) {
+  return TileOperand{(const char*)p, (const char*)p2, (int64_t)(ld_elems * es), (int32_t)rows};
+}
+
+struct MlpPlan {
+  TileArgs up{}, down{}, grad{}, dx{}, dw{};
+  TilePlan p_up{}, p_down{}, p_grad{}, p_dx{}, p_dw{};
+};
+static void plan_fwd(const PalMlpDims* d, const PalMlpTensors* t, const void* h, MlpPlan& m) {
+  const size_t es = mlp_elem(d);
+  m.up.n_prod = 1;
+  m.up.k = d->dim;
+  m.up.prod[0].a = operand(t->x, d->x_stride, es, d->rows);
+  m.up.prod[0].b = operand(t->w_gate, d->dim, es, d->hidden, t->w_up);
+  m.up.prod[0].c = (void*)h;
+  m.up.gate_out = t->gate;
+  m.up.up_out = t->up;
+  m.up.act = d->activation;
+  m.down.n_prod = 1;
+  m.down.k = d->hidden;
+  m.down.prod[0].a = operand(h, d->hidden, es, d->rows);
+  m.down.prod[0].b = operand(t->w_down, d->hidden, es, d->out_dim);
+  m.down.prod[0].c = t->y;
+  m.p_up = plan_tiles(m.up, kTileGated, d->dtype);
+  m.p_down = plan_tiles(m.down, kTilePlain, d->dtype);
+}
+static void plan_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrads* g, void* dg, void* du, void* h, MlpPlan& m) {
+  const size_t es = mlp_elem(d);
+  m.grad.n_prod = 1;
+  m.grad.k = d->out_dim;
+  m.grad.prod[0].a = operand(g->dy, d->out_dim, es, d->rows);
+  m.grad.prod[0].b = operand(t->w_down, d->hidden, es, d->hidden);
+  m.grad.prod[0].c = dg;
+  m.grad.gate = t->gate;
+  m.grad.up = t->up;
+  m.grad.up_out = du;
+  m.grad.gate_out = g->dw_down ? h : nullptr;
+  m.grad.act = d->activation;
+  m.p_grad = plan_tiles(m.grad, kTileGrad, d->dtype);
+  m.dx.n_prod = 1;
+  m.dx.k = d->hidden;
+  m.dx.prod[0].a = operand(dg, d->hidden, es, d->rows, du);
+  m.dx.prod[0].b = operand(t->w_gate, d->dim, es, d->dim, t->w_up);
+  m.dx.prod[0].c = g->dx;
+  m.p_dx = plan_tiles(m.dx, kTileTwice, d->dtype);
+  m.dw.k = (int32_t)d->rows;
+  auto add = [&](const TileOperand& a, const TileOperand& b, void* c) {
+    if (!c) return;
+    TileProduct& p = m.dw.prod[m.dw.n_prod++];
+    p.a = a;
+    p.b = b;
+    p.c = c;
+  };
+  add(operand(dg, d->hidden, es, d->hidden), operand(t->x, d->x_stride, es, d->dim), g->dw_gate);
+  add(operand(du, d->hidden, es, d->hidden), operand(t->x, d->x_stride, es, d->dim), g->dw_up);
+  add(operand(g->dy, d->out_dim, es, d->out_dim), operand(h, d->hidden, es, d->hidden), g->dw_down);
+  if (m.dw.n_prod) m.p_dw = plan_tiles(m.dw, kTilePlain, d->dtype);
+}
+static size_t most_of(size_t a, size_t b) { return a > b ? a : b; }
+static size_t rows_bytes(const PalMlpDims* d) { return round256((size_t)d->rows * d->hidden * mlp_elem(d)); }
+
+template <typename T>
+static int mlp_fwd(const PalMlpDims* d, const PalMlpTensors* t, char* ws, hipStream_t s) {
+  void* h = ws;
+  if (d->rows <= kFewRows) {
+    FewArgs up{t->x, t->w_gate, t->w_up, h, t->gate, t->up, d->x_stride, (int32_t)d->rows, d->hidden, d->dim, d->activation};
+    if (int rc = few_launch<T, true>(up, s)) return rc;
+    FewArgs down{h, t->w_down, nullptr, t->y, nullptr, nullptr, d->hidden, (int32_t)d->rows, d->out_dim, d->hidden, 0};
+    return few_launch<T, false>(down, s);
+  }
+  MlpPlan m;
+  plan_fwd(d, t, h, m);
+  if (int rc = tile_run<T, kTileGated, false, false>(m.up, m.p_up, nullptr, kKernMlpUp, s)) return rc;
+  return tile_run<T, kTilePlain, false, false>(m.down, m.p_down, (float*)(ws + rows_bytes(d)), kKernMlpDown, s);
+}
+template <typename T>
+static int mlp_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrads* g, char* ws, hipStream_t s) {
+  const size_t n = rows_bytes(d);
+  MlpPlan m;
+  plan_bwd(d, t, g, ws, ws + n, ws + 2 * n, m);
+  float* part = (float*)(ws + 3 * n);
+  if (int rc = tile_run<T, kTileGrad, false, true>(m.grad, m.p_grad, part, kKernMlpGrad, s)) return rc;
+  if (g->dx)
+    if (int rc = tile_run<T, kTileTwice, false, true>(m.dx, m.p_dx, part, kKernMlpDx, s)) return rc;
+  if (m.dw.n_prod) return tile_run<T, kTilePlain, true, true>(m.dw, m.p_dw, part, kKernMlpDw, s);
+  return PAL_OK;
+}
+
+}  // namespace pal
+
+extern "C" size_t pal_gated_mlp_fwd_workspace_bytes(const PalMlpDims* d) {
+  using namespace pal;
+  if (check_mlp(d) != PAL_OK) return 0;
+  if (d->rows <= kFewRows) return rows_bytes(d);
+  MlpPlan m;
+  PalMlpTensors t{};
+  plan_fwd(d, &t, nullptr, m);
+  return rows_bytes(d) + part_bytes(m.down, m.p_down);
+}
+extern "C" int pal_gated_mlp_fwd(const PalMlpDims* d, const PalMlpTensors* t, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace pal;
+  if (int rc = check_mlp(d)) return rc;
+  if (!t || !t->x || !t->w_gate || !t->w_up || !t->w_down || !t->y) return PAL_E_NULL;
+  if (!t->gate != !t->up) return PAL_E_STATE;
+  for (const void* p : {t->x, t->w_gate, t->w_up, t->w_down, (const void*)t->y, (const void*)t->gate, (const void*)t->up})
+    if (!is_aligned16(p)) return PAL_E_ALIGN;
+  if (!workspace || workspace_bytes < pal_gated_mlp_fwd_workspace_bytes(d)) return PAL_E_WORKSPACE;
+  if (!is_aligned16(workspace)) return PAL_E_ALIGN;
+  return d->dtype == PAL_DTYPE_BF16 ? mlp_fwd<bf16_t>(d, t, (char*)workspace, (hipStream_t)stream)
+                                    : mlp_fwd<float>(d, t, (char*)workspace, (hipStream_t)stream);
+}
+extern "C" size_t pal_gated_mlp_bwd_workspace_bytes(const PalMlpDims* d) {
+  using namespace pal;
+  if (check_mlp(d) != PAL_OK) return 0;
+  // enough for every choice of gradients
+  size_t part = 0;
+  for (int which = 0; which < 8; ++which) {
+    MlpPlan m;
+    PalMlpTensors t{};
+    PalMlpGrads g{};
+    char any;
+    g.dw_gate = which & 1 ? &any : nullptr;
+    g.dw_up = which & 2 ? &any : nullptr;
+    g.dw_down = which & 4 ? &any : nullptr;
+    plan_bwd(d, &t, &g, nullptr, nullptr, nullptr, m);
+    part = most_of(part, most_of(part_bytes(m.grad, m.p_grad), most_of(part_bytes(m.dx, m.p_dx), part_bytes(m.dw, m.p_dw))));
+  }
+  return 3 * rows_bytes(d) + part;
+}
+extern "C" int pal_gated_mlp_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrads* g, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  using namespace pal;
+  if (int rc = check_mlp(d)) return rc;
+  if (!t || !t->x || !t->w_gate || !t->w_up || !t->w_down || !t->gate || !t->up || !g || !g->dy) return PAL_E_NULL;
+  for (const void* p : {t->x, t->w_gate, t->w_up, t->w_down, (const void*)t->gate, (const void*)t->up, g->dy, (const void*)g->dx,
+                        (const void*)g->dw_gate, (const void*)g->dw_up, (const void*)g->dw_down})
+    if (!is_aligned16(p)) return PAL_E_ALIGN;
+  if (!workspace || workspace_bytes < pal_gated_mlp_bwd_workspace_bytes(d)) return PAL_E_WORKSPACE;
+  if (!is_aligned16(workspace)) return PAL_E_ALIGN;
+  return d->dtype == PAL_DTYPE_BF16 ? mlp_bwd<bf16_t>(d, t, g, (char*)workspace, (hipStream_t)stream)
+                                    : mlp_bwd<float>(d, t, g, (char*)workspace, (hipStream_t)stream);
+}

@@ -1,4 +1,4 @@
-// Native host path of the operators around the recurrences: residual norm, short convolution, selective scan.  Part of
+// Native host path of the operators around the recurrences: norms, dropout, short convolution, selective scan, feed-forward block.  Part of
 // host_ext.cpp, whose helpers it uses and whose rule it follows: a function serves the plain call (types that the kernels read, everything on
 // the current device, no tracer or mode listening) and returns None for any other before it does anything; the Python route then
 // converts, or raises the error that the call deserves.  It saves what that route takes in Python: 10 to 15 us of a forward, 50 of a
@@ -480,6 +480,274 @@ py::object selective_scan_step(const Tensor& u, const Tensor& state, const Tenso
   Tensor y = at::empty(u.sizes(), as(u, c.rows));
   if (c.run(i, y, (float*)state.mutable_data_ptr(), nullptr)) return py::none();
   written(state);
+  return py::cast(y);
+}
+
+// ------------------------------------------------------------------------------------------- dropout and layer norm
+// a seed on the device: one int64 number
+bool seed_ok(const Tensor& t, const c10::Device& dev) { return !t.defined() || (there(t, dev, at::kLong) && t.numel() == 1); }
+PalDropout drop_of(double p, int64_t seed, const Tensor& seed_t, int64_t site) {
+  return PalDropout{p, seed, (const int64_t*)ptr(seed_t), (uint32_t)site};
+}
+
+bool dropout_plain(const Tensor& x, const Tensor& seed_t, int64_t& stride) {
+  if (!x.defined() || x.device().type() != at::kCUDA || x.device().index() != c10::hip::current_device() || x.dim() < 1 || x.numel() == 0) return false;
+  return rows_type(x.scalar_type()) && there(x, x.device(), x.scalar_type()) && seed_ok(seed_t, x.device()) && row_stride(x, stride) && x.size(-1) <= 1 << 30;
+}
+int dropout_run(const Tensor& x, int64_t stride, double p, int64_t seed, const Tensor& seed_t, int64_t site, Tensor& y) {
+  const PalDropout d = drop_of(p, seed, seed_t, site);
+  const int64_t D = x.size(-1), rows = x.numel() / D;
+  void* out = y.mutable_data_ptr();
+  NoGil off;
+  return abi.dropout(&d, ptr(x), out, rows, D, stride, pal_type(x.scalar_type()), stream_of(x.device()));
+}
+struct DropoutNode : torch::autograd::Function<DropoutNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, double p, int64_t seed, const OptT& seed_, int64_t site) {
+    const Tensor seed_t = seed_.value_or(Tensor());
+    int64_t stride;
+    dropout_plain(x, seed_t, stride);
+    Tensor y = at::empty(x.sizes(), as(x, x.scalar_type()));
+    const int rc = dropout_run(x, stride, p, seed, seed_t, site, y);
+    if (rc) fail(rc, "pal_dropout");
+    ctx->save_for_backward({seed_t});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["site"] = site;
+    ctx->saved_data["type"] = (int64_t)x.scalar_type();
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gr) {
+    const Tensor seed_t = ctx->get_saved_variables()[0], none;
+    const c10::DeviceGuard guard(gr[0].device());
+    const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+    Tensor dy = gr[0].to(type);
+    int64_t stride;
+    if (!dropout_plain(dy, seed_t, stride)) dy = dy.contiguous();
+    TORCH_CHECK_VALUE(dropout_plain(dy, seed_t, stride), "dropout backward: the seed came back in another shape, dtype or device");
+    Tensor dx = at::empty(dy.sizes(), as(dy, type));
+    const int rc = dropout_run(dy, stride, ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(), seed_t, ctx->saved_data["site"].toInt(), dx);
+    if (rc) fail(rc, "pal_dropout");
+    return once({dx, none, none, none, none});
+  }
+};
+// y, or None
+py::object dropout(const Tensor& x, double p, int64_t seed, const OptT& seed_, int64_t site) {
+  const Tensor seed_t = seed_.value_or(Tensor());
+  if (observed_or_dual({&x})) return py::none();
+  int64_t stride;
+  if (!dropout_plain(x, seed_t, stride)) return py::none();
+  if (any_grad({&x})) return applied([&] { return py::cast(DropoutNode::apply(x, p, seed, seed_, site)); });
+  Tensor y = at::empty(x.sizes(), as(x, x.scalar_type()));
+  if (dropout_run(x, stride, p, seed, seed_t, site, y)) return py::none();
+  return py::cast(y);
+}
+
+struct LayerNormCall {
+  bool ok = false;
+  at::ScalarType rows, res;
+  PalLayerNormDims d{};
+  LayerNormCall(const Tensor& x, const Tensor& r, const Tensor& w, const Tensor& b, double eps, bool res_fp32, bool handed_on) {
+    if (!x.defined() || x.device().type() != at::kCUDA || x.device().index() != c10::hip::current_device() || x.dim() < 1 || x.numel() == 0) return;
+    const c10::Device dev = x.device();
+    rows = x.scalar_type();
+    if (!rows_type(rows) || !there(x, dev, rows) || !param_ok(w, dev) || w.dim() != 1 || w.size(0) != x.size(-1)) return;
+    if (b.defined() && (!packed(b, dev, w.scalar_type()) || b.sizes() != w.sizes())) return;
+    res = !handed_on ? rows : res_fp32 || rows == at::kFloat || (r.defined() && r.scalar_type() != at::kBFloat16) ? at::kFloat : at::kBFloat16;
+    if (r.defined() && (!there(r, dev, res) || r.sizes() != x.sizes())) return;
+    if (!row_stride(x, d.x_stride)) return;
+    d.res_stride = x.size(-1);
+    if (r.defined() && !row_stride(r, d.res_stride)) return;
+    if (x.size(-1) > kMaxNormRow || !(eps >= 0)) return;
+    d.dim = (int32_t)x.size(-1);
+    d.rows = x.numel() / d.dim;
+    d.dtype = pal_type(rows); d.res_dtype = pal_type(res); d.weight_dtype = pal_type(w.scalar_type());
+    d.eps = (float)eps;
+    ok = true;
+  }
+  int run(const Tensor& x, const Tensor& r, const Tensor& w, const Tensor& b, Tensor& s, Tensor& y, Tensor& stats) const {
+    PalLayerNormTensors t{};
+    t.x = ptr(x); t.residual = ptr(r); t.weight = ptr(w); t.bias = ptr(b);
+    t.residual_out = s.defined() ? s.mutable_data_ptr() : nullptr; t.y = y.mutable_data_ptr(); t.stats = fptr(stats);
+    NoGil off;
+    return abi.layer_norm_fwd(&d, &t, stream_of(x.device()));
+  }
+};
+
+struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptT& r_, const Tensor& w, const OptT& b_, double eps, bool res_fp32, bool handed_on,
+                               double p, int64_t seed, const OptT& seed_, int64_t site) {
+    const Tensor r = r_.value_or(Tensor()), b = b_.value_or(Tensor()), seed_t = seed_.value_or(Tensor());
+    LayerNormCall c(x, r, w, b, eps, res_fp32, handed_on);
+    c.d.drop = drop_of(p, seed, seed_t, site);
+    Tensor y = at::empty(x.sizes(), as(x, c.rows)), s, stats = at::empty({c.d.rows, 2}, as(x, at::kFloat));
+    if (handed_on) s = at::empty(x.sizes(), as(x, c.res));
+    const int rc = c.run(x, r, w, b, s, y, stats);
+    if (rc) fail(rc, "pal_layer_norm_fwd");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({handed_on ? s : x, w, stats, seed_t});
+    ctx->saved_data["rows"] = (int64_t)c.rows;
+    ctx->saved_data["handed_on"] = handed_on;
+    ctx->saved_data["has_res"] = r.defined();
+    ctx->saved_data["has_bias"] = b.defined();
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["site"] = site;
+    variable_list o{y};
+    if (handed_on) o.push_back(s);
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gr) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &s = saved[0], &w = saved[1], &stats = saved[2], &seed_t = saved[3], none;
+    if (!gr[0].defined() && (gr.size() < 2 || !gr[1].defined())) return variable_list(11);
+    const c10::DeviceGuard guard(s.device());
+    const auto rows = (at::ScalarType)ctx->saved_data["rows"].toInt();
+    const bool handed_on = ctx->saved_data["handed_on"].toBool(), has_res = ctx->saved_data["has_res"].toBool(), has_bias = ctx->saved_data["has_bias"].toBool();
+    const double p = ctx->saved_data["p"].toDouble();
+    PalLayerNormDims d{};
+    TORCH_CHECK_VALUE(s.dim() >= 1 && s.numel() > 0 && rows_type(s.scalar_type()) && there(s, s.device(), s.scalar_type()) && row_stride(s, d.x_stride) &&
+                          (!handed_on || s.is_contiguous()) && (handed_on || s.scalar_type() == rows) && param_ok(w, s.device()) && w.dim() == 1 &&
+                          w.size(0) == s.size(-1) && (rows == at::kBFloat16 || s.scalar_type() == at::kFloat) && packed(stats, s.device(), at::kFloat) &&
+                          stats.numel() == 2 * (s.numel() / s.size(-1)) && seed_ok(seed_t, s.device()),
+                      "layer_norm backward: a saved tensor came back in another shape, dtype, layout or device");
+    d.dim = (int32_t)s.size(-1);
+    d.rows = s.numel() / d.dim;
+    d.res_stride = d.dim;
+    d.dtype = pal_type(rows); d.res_dtype = pal_type(s.scalar_type()); d.weight_dtype = pal_type(w.scalar_type());
+    d.drop = drop_of(p, ctx->saved_data["seed"].toInt(), seed_t, ctx->saved_data["site"].toInt());
+    const Tensor dy = gr[0].defined() ? gr[0].to(rows).contiguous() : Tensor();
+    const Tensor dr = gr.size() > 1 && gr[1].defined() ? gr[1].to(s.scalar_type()).contiguous() : Tensor();
+    const bool apart = has_res && (p > 0.0 || rows != s.scalar_type());
+    Tensor dx = at::empty(s.sizes(), as(s, rows)), ds, dw = at::empty(w.sizes(), as(s, at::kFloat)), db;
+    if (apart) ds = at::empty(s.sizes(), as(s, s.scalar_type()));
+    if (has_bias) db = at::empty(w.sizes(), as(s, at::kFloat));
+    PalLayerNormTensors t{};
+    t.weight = ptr(w); t.bias = has_bias ? ptr(w) : nullptr; t.stats = (float*)ptr(stats);
+    if (handed_on) t.residual_out = (void*)ptr(s);
+    else t.x = ptr(s);
+    PalLayerNormGrads g{};
+    g.dy = ptr(dy); g.dresidual_out = ptr(dr); g.dx = dx.mutable_data_ptr(); g.dresidual = ds.defined() ? ds.mutable_data_ptr() : nullptr;
+    g.dweight = fptr(dw); g.dbias = fptr(db);
+    const size_t bytes = abi.layer_norm_bwd_workspace_bytes(&d);
+    Tensor ws = workspace(s, bytes);
+    int rc;
+    { NoGil off; rc = abi.layer_norm_bwd(&d, &t, &g, ws.mutable_data_ptr(), bytes, stream_of(s.device())); }
+    if (rc) fail(rc, "pal_layer_norm_bwd");
+    if (w.scalar_type() != at::kFloat) {
+      dw = dw.to(w.scalar_type());
+      if (db.defined()) db = db.to(w.scalar_type());
+    }
+    return once({dx, has_res ? (apart ? ds : dx) : none, dw, db, none, none, none, none, none, none, none});
+  }
+};
+
+// (y,) or (y, residual stream), or None
+py::object layer_norm(const Tensor& x, const OptT& r_, const Tensor& w, const OptT& b_, double eps, bool res_fp32, bool handed_on, double p, int64_t seed,
+                      const OptT& seed_, int64_t site) {
+  const Tensor r = r_.value_or(Tensor()), b = b_.value_or(Tensor()), seed_t = seed_.value_or(Tensor());
+  if (observed_or_dual({&x, &r, &w, &b})) return py::none();
+  LayerNormCall c(x, r, w, b, eps, res_fp32, handed_on);
+  if (!c.ok || !seed_ok(seed_t, x.device())) return py::none();
+  if (any_grad({&x, &r, &w, &b}))
+    return applied([&] {
+      auto o = LayerNormNode::apply(x, r_, w, b_, eps, res_fp32, handed_on, p, seed, seed_, site);
+      return handed_on ? py::make_tuple(o[0], o[1]) : py::make_tuple(o[0]);
+    });
+  c.d.drop = drop_of(p, seed, seed_t, site);
+  Tensor y = at::empty(x.sizes(), as(x, c.rows)), s, none;
+  if (handed_on) s = at::empty(x.sizes(), as(x, c.res));
+  if (c.run(x, r, w, b, s, y, none)) return py::none();   // nothing was launched: the Python route says what is wrong
+  return handed_on ? py::make_tuple(y, s) : py::make_tuple(y);
+}
+
+// --------------------------------------------------------------------------------------------- gated feed-forward block
+struct MlpCall {
+  bool ok = false;
+  at::ScalarType type;
+  PalMlpDims d{};
+  MlpCall(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t act) {
+    if (!x.defined() || x.device().type() != at::kCUDA || x.device().index() != c10::hip::current_device() || x.dim() < 1 || x.numel() == 0) return;
+    const c10::Device dev = x.device();
+    type = x.scalar_type();
+    if (!rows_type(type) || !there(x, dev, type)) return;
+    for (const Tensor* w : {&wg, &wu, &wd})
+      if (!packed(*w, dev, type) || w->dim() != 2 || (uintptr_t)ptr(*w) % 16) return;
+    const int64_t D = x.size(-1), F = wg.size(0), Do = wd.size(0), rows = x.numel() / D;
+    if (wg.size(1) != D || wu.sizes() != wg.sizes() || wd.size(1) != F) return;
+    if (D % 8 || F % 8 || Do % 8 || !F || !Do || D > 1 << 20 || F > 1 << 20 || Do > 1 << 20 || rows > 1 << 30) return;
+    if (!row_stride(x, d.x_stride) || d.x_stride % 8 || d.x_stride > 1 << 20 || (uintptr_t)ptr(x) % 16) return;
+    d.rows = rows; d.dim = (int32_t)D; d.hidden = (int32_t)F; d.out_dim = (int32_t)Do; d.dtype = pal_type(type); d.activation = (int32_t)act;
+    ok = true;
+  }
+  Tensor out(const Tensor& x) const {
+    auto shape = x.sizes().vec();
+    shape.back() = d.out_dim;
+    return at::empty(shape, as(x, type));
+  }
+  static PalMlpTensors fill(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd) {
+    PalMlpTensors t{};
+    t.x = ptr(x); t.w_gate = ptr(wg); t.w_up = ptr(wu); t.w_down = ptr(wd);
+    return t;
+  }
+  int run(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, Tensor& y, Tensor& gate, Tensor& up) const {
+    PalMlpTensors t = fill(x, wg, wu, wd);
+    t.y = y.mutable_data_ptr();
+    if (gate.defined()) { t.gate = gate.mutable_data_ptr(); t.up = up.mutable_data_ptr(); }
+    const size_t bytes = abi.gated_mlp_fwd_workspace_bytes(&d);
+    Tensor ws = workspace(x, bytes);
+    NoGil off;
+    return abi.gated_mlp_fwd(&d, &t, ws.mutable_data_ptr(), bytes, stream_of(x.device()));
+  }
+};
+
+struct MlpNode : torch::autograd::Function<MlpNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t act) {
+    MlpCall c(x, wg, wu, wd, act);
+    Tensor y = c.out(x), gate = at::empty({c.d.rows, c.d.hidden}, as(x, c.type)), up = at::empty({c.d.rows, c.d.hidden}, as(x, c.type));
+    const int rc = c.run(x, wg, wu, wd, y, gate, up);
+    if (rc) fail(rc, "pal_gated_mlp_fwd");
+    ctx->save_for_backward({x, wg, wu, wd, gate, up});
+    ctx->saved_data["act"] = act;
+    for (int i = 0; i < 4; ++i) {
+      const Tensor* t[] = {&x, &wg, &wu, &wd};
+      ctx->saved_data[std::string("need") + (char)('0' + i)] = t[i]->requires_grad();
+    }
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list gr) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &x = s[0], &gate = s[4], &up = s[5], none;
+    const c10::DeviceGuard guard(x.device());
+    MlpCall c(x, s[1], s[2], s[3], ctx->saved_data["act"].toInt());
+    TORCH_CHECK_VALUE(c.ok && packed(gate, x.device(), c.type) && packed(up, x.device(), c.type) && gate.numel() == c.d.rows * c.d.hidden &&
+                          up.numel() == gate.numel(),
+                      "gated_mlp backward: a saved tensor came back in another shape, dtype, layout or device");
+    Tensor dy = gr[0].to(c.type).contiguous();
+    if ((uintptr_t)ptr(dy) % 16) dy = dy.clone();
+    Tensor out[4];
+    for (int i = 0; i < 4; ++i)
+      if (ctx->saved_data[std::string("need") + (char)('0' + i)].toBool()) out[i] = at::empty(s[i].sizes(), as(x, c.type));
+    PalMlpTensors t = MlpCall::fill(x, s[1], s[2], s[3]);
+    t.gate = (void*)ptr(gate); t.up = (void*)ptr(up);
+    auto at_ = [](Tensor& o) { return o.defined() ? o.mutable_data_ptr() : nullptr; };
+    PalMlpGrads g{ptr(dy), at_(out[0]), at_(out[1]), at_(out[2]), at_(out[3])};
+    const size_t bytes = abi.gated_mlp_bwd_workspace_bytes(&c.d);
+    Tensor ws = workspace(x, bytes);
+    int rc;
+    { NoGil off; rc = abi.gated_mlp_bwd(&c.d, &t, &g, ws.mutable_data_ptr(), bytes, stream_of(x.device())); }
+    if (rc) fail(rc, "pal_gated_mlp_bwd");
+    return once({out[0], out[1], out[2], out[3], none});
+  }
+};
+
+// y, or None
+py::object gated_mlp(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t act) {
+  if (observed_or_dual({&x, &wg, &wu, &wd})) return py::none();
+  const MlpCall c(x, wg, wu, wd, act);
+  if (!c.ok) return py::none();
+  if (any_grad({&x, &wg, &wu, &wd})) return applied([&] { return py::cast(MlpNode::apply(x, wg, wu, wd, act)); });
+  Tensor y = c.out(x), none;
+  if (c.run(x, wg, wu, wd, y, none, none)) return py::none();
   return py::cast(y);
 }
 

@@ -46,6 +46,14 @@ struct Abi {
   size_t (*scan_checkpoint_bytes)(const PalScanDims*);
   int (*scan_bwd)(const PalScanDims*, const PalScanTensors*, const PalScanGrads*, void*, size_t, void*);
   size_t (*scan_bwd_workspace_bytes)(const PalScanDims*);
+  int (*dropout)(const PalDropout*, const void*, void*, int64_t, int64_t, int64_t, int32_t, void*);
+  int (*layer_norm_fwd)(const PalLayerNormDims*, const PalLayerNormTensors*, void*);
+  int (*layer_norm_bwd)(const PalLayerNormDims*, const PalLayerNormTensors*, const PalLayerNormGrads*, void*, size_t, void*);
+  size_t (*layer_norm_bwd_workspace_bytes)(const PalLayerNormDims*);
+  int (*gated_mlp_fwd)(const PalMlpDims*, const PalMlpTensors*, void*, size_t, void*);
+  size_t (*gated_mlp_fwd_workspace_bytes)(const PalMlpDims*);
+  int (*gated_mlp_bwd)(const PalMlpDims*, const PalMlpTensors*, const PalMlpGrads*, void*, size_t, void*);
+  size_t (*gated_mlp_bwd_workspace_bytes)(const PalMlpDims*);
 } abi;
 py::handle raise_code;   // (code, where): raises what the Python routes raise for a code of the library
 
@@ -359,7 +367,8 @@ PYBIND11_MODULE(_host, m) {
   // what this module was built from; the loader compares it before it binds the library
   m.attr("abi") = py::make_tuple(PAL_ABI_VERSION, sizeof(PalDims), sizeof(PalFwdTensors), sizeof(PalBwdTensors));
   m.attr("abi_block") = py::make_tuple(sizeof(PalNormDims), sizeof(PalNormTensors), sizeof(PalNormGrads), sizeof(PalConvDims), sizeof(PalConvTensors),
-                                       sizeof(PalConvGrads), sizeof(PalScanDims), sizeof(PalScanTensors), sizeof(PalScanGrads));
+                                       sizeof(PalConvGrads), sizeof(PalScanDims), sizeof(PalScanTensors), sizeof(PalScanGrads), sizeof(PalDropout), sizeof(PalLayerNormDims),
+                                       sizeof(PalLayerNormTensors), sizeof(PalLayerNormGrads), sizeof(PalMlpDims), sizeof(PalMlpTensors), sizeof(PalMlpGrads));
   m.attr("torch_version") = PAL_TORCH_VERSION;
   m.def("bind", &bind);
   m.def("recurrent_fwd", &recurrent_fwd);
@@ -371,4 +380,7 @@ PYBIND11_MODULE(_host, m) {
   m.def("short_conv_step", &block::short_conv_step);
   m.def("selective_scan", &block::selective_scan);
   m.def("selective_scan_step", &block::selective_scan_step);
+  m.def("dropout", &block::dropout);
+  m.def("layer_norm", &block::layer_norm);
+  m.def("gated_mlp", &block::gated_mlp);
 }

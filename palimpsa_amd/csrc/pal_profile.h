@@ -44,6 +44,18 @@ enum KernelId {
   kKernScanJoin,
   kKernScanBwd,
   kKernScanBwdSums,
+  kKernMlpUp,
+  kKernMlpDown,
+  kKernMlpGrad,
+  kKernMlpDx,
+  kKernMlpDw,
+  kKernMlpFewUp,
+  kKernMlpFewDown,
+  kKernTileJoin,
+  kKernLayerNormFwd,
+  kKernLayerNormBwd,
+  kKernLayerNormReduce,
+  kKernDropout,
   kKernCount
 };
 

@@ -57,7 +57,9 @@ static const char* kNames[kKernCount] = {
     "chunk_bwd_parts_sum_kernel", "recurrent_seg_kernel", "residual_norm_fwd_kernel", "residual_norm_bwd_kernel",
     "residual_norm_reduce_kernel", "short_conv_fwd_kernel", "short_conv_bwd_kernel", "short_conv_reduce_kernel",
     "short_conv_step_kernel", "scan_fwd_kernel", "scan_segment_kernel", "scan_join_kernel", "scan_bwd_kernel",
-    "scan_bwd_sums_kernel"};
+    "scan_bwd_sums_kernel", "mlp_up", "mlp_down", "mlp_grad",
+    "mlp_dx", "mlp_dw", "mlp_few_up", "mlp_few_down", "tile_join_kernel", "layer_norm_fwd_kernel",
+    "layer_norm_bwd_kernel", "layer_norm_reduce_kernel", "dropout_kernel"};
 
 }  // namespace pal
 

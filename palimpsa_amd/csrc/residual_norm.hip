@@ -13,12 +13,11 @@
 #include "pal_common.h"
 #include "pal_host.h"
 #include "pal_profile.h"
-#include "rows8.h"
+#include "norm_rows.h"
 
 namespace pal {
 
 constexpr float kFp8Max = 448.f, kFp8Least = 1e-12f;   // largest e4m3 number; |y| below the second counts as that much
-constexpr int kNormMaxRow = 16384;
 
 struct NormArgs {
   const void *x, *res, *weight;
@@ -33,18 +32,6 @@ struct NormArgs {
   float eps;
 };
 
-// sum over the waves of a row; `turn` alternates between two slots so that one barrier per sum is enough
-template <int WPR>
-__device__ __forceinline__ float row_sum(float x, float (*s)[4], int turn) {
-  x = wave_sum(x);
-  if constexpr (WPR > 1) {
-    const int w = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) s[turn][w] = x;
-    __syncthreads();
-    x = s[turn][0] + s[turn][1] + s[turn][2] + s[turn][3];
-  }
-  return x;
-}
 template <int WPR>
 __device__ __forceinline__ float row_max(float x, float (*s)[4], int turn) {
   x = wave_max(x);
@@ -72,28 +59,6 @@ __device__ __forceinline__ float group_max(float x, int lanes) {
     x = fmaxf(a, b);
   }
   return x;
-}
-
-// Piece v of a lane: eight entries from column `at` on.  Rows of eight entries or more, WHOLE: the last piece of a row whose length is no
-// multiple of eight, and those of lanes behind it, are moved back to be whole, so that no load waits on a branch; what is there twice has
-// the same values, is written twice and counts once in sums (entries from `from` on).  Shorter rows are read element by element.
-template <int NV, int WPR, bool WHOLE>
-struct NormPiece {
-  int at, from;
-  bool on;               // the lane has entries of its own
-  __device__ __forceinline__ NormPiece(int lane, int v, int D) {
-    const int c = 8 * (lane + 64 * WPR * v);
-    on = c < D;
-    at = WHOLE ? min(c, D - 8) : c;
-    from = c - at;
-  }
-  // (one wave a row: all pieces but the last are whole)
-  static constexpr bool masked(int v) { return WHOLE && (WPR > 1 || v == NV - 1); }
-};
-template <bool WHOLE, typename T>
-__device__ __forceinline__ void load_row_piece(Piece8<T>& d, const T* row, int at, int D) {
-  if constexpr (WHOLE) d.load(row + at);
-  else load_piece(d, row + at, D - at);
 }
 
 template <typename TX, typename TR, int NV, int WPR, bool FP8, bool WHOLE>

@@ -24,6 +24,12 @@ a residual; models/palimpsa/modeling_palimpsa.py:84-114), for training and, with
 
     y, residual = residual_rms_norm(x, residual, weight, eps)
     q, scales, residual = residual_rms_norm_fp8(x, residual, weight, eps, group_size=128)   # y = q * scales, e4m3
+
+Blocks with a layer norm in that place, and with a dropout of what is added to the stream, take
+
+    y, residual = residual_layer_norm(x, residual, weight, bias, eps, dropout_p=0.1, seed=seed, site=layer)
+    y = layer_norm(x, weight, bias, eps)
+    x = dropout(x, 0.1, seed, site)
 """
 from __future__ import annotations
 
@@ -38,7 +44,8 @@ from ..palimpsa import _common as cm
 
 __all__ = ["palimpsa_inputs", "palimpsa_output_norm", "PalimpsaInputs", "PalimpsaOutputNorm",
            "metamamba2_inputs", "metamamba2_output_norm", "MetaMamba2Inputs", "MetaMamba2OutputNorm",
-           "residual_rms_norm", "residual_rms_norm_fp8", "ResidualRmsNorm"]
+           "residual_rms_norm", "residual_rms_norm_fp8", "ResidualRmsNorm",
+           "layer_norm", "residual_layer_norm", "LayerNorm", "dropout", "Dropout"]
 
 
 def _rows_dtype(*tensors) -> torch.dtype:
@@ -498,6 +505,194 @@ def _residual_rms_norm_fp8(x, residual, weight, eps, group_size, residual_in_fp3
         rc = L.load().pal_residual_norm_fwd(dims, tens, cm.current_stream_ptr(dev))
     L.check(rc, "pal_residual_norm_fwd")
     return q, scales, res_out
+
+
+def _seed(seed, site, dev):
+    """(64 bits of the seed as a signed number, tensor | None, site) of a dropout."""
+    if not isinstance(site, int) or not 0 <= site < 1 << 32:
+        raise ValueError(f"site must be a whole number below 2^32, got {site!r}")
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.numel() != 1 or seed.device != dev:
+            raise ValueError(f"a seed tensor must be one int64 number on {dev}, got {seed.dtype} {tuple(seed.shape)} on {seed.device}")
+        return 0, seed, site
+    if not isinstance(seed, int) or not -(1 << 63) <= seed < 1 << 64:
+        raise ValueError(f"seed must be a whole number of 64 bits or an int64 tensor, got {seed!r}")
+    return ((seed + (1 << 63)) % (1 << 64)) - (1 << 63), None, site
+
+
+def _probability(p) -> float:
+    p = float(p)
+    if not 0.0 <= p < 1.0:
+        raise ValueError(f"the probability of being dropped must be at least 0 and below 1, got {p}")
+    return p
+
+
+def _drop_struct(p, seed, seed_t, site):
+    return L.PalDropout(p=p, seed=seed, seed_at=cm._ptr(seed_t), site=site)
+
+
+class Dropout(torch.autograd.Function):
+    """forward(ctx, x, p, seed, seed_t, site) -> y."""
+
+    @staticmethod
+    def _run(x, p, seed, seed_t, site):
+        cd = _rows_dtype(x)
+        y = torch.empty(x.shape, dtype=cd, device=x.device)
+        if x.numel():
+            xc, stride = _norm_rows(x if x.dim() else x.reshape(1), cd)
+            D = xc.shape[-1]
+            with torch.cuda.device(x.device):
+                rc = L.load().pal_dropout(_drop_struct(p, seed, seed_t, site), cm._ptr(xc), cm._ptr(y), x.numel() // D, D, stride,
+                                          cm._pal_dtype(cd), cm.current_stream_ptr(x.device))
+            L.check(rc, "pal_dropout")
+        return y if y.dtype == x.dtype else y.to(x.dtype)
+
+    @staticmethod
+    def forward(ctx, x, p, seed, seed_t, site):
+        ctx.meta = (p, seed, site)
+        ctx.save_for_backward(seed_t)
+        return Dropout._run(x, p, seed, seed_t, site)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        p, seed, site = ctx.meta
+        return Dropout._run(dy, p, seed, ctx.saved_tensors[0], site), None, None, None, None
+
+
+def dropout(x: torch.Tensor, p: float, seed, site: int = 0) -> torch.Tensor:
+    """Entries of x ``[.., D]`` are zero with probability p (0 <= p < 1), the others are multiplied by ``1 / (1 - p)``.
+
+    Which ones is a function of the seed (a whole number of 64 bits, or an int64 tensor of one element on the device, which a captured graph
+    reads at every replay) and of the entry's row and column alone: word ``column % 4`` of Philox4x32 with seven rounds of the counter
+    ``(column // 4, row, row >> 32, site)`` under the key ``seed``, kept where it is not below ``p * 2 ** 32``.  So nothing is stored for
+    the backward pass, the strides of x and the order of the work change nothing, and ``site`` numbers the places of a model that share a
+    step's seed.  A dropped entry is zero whatever it held.  A seed tensor must not be changed between the forward and the backward pass."""
+    if not torch.compiler.is_compiling() and x.is_cuda and isinstance(p, float) and 0.0 <= p < 1.0:
+        bits, seed_t, site = _seed(seed, site, x.device)
+        r = L.host().dropout(x, p, bits, seed_t, site)
+        if r is not None:
+            return r
+    return _dropout(x, p, seed, site)
+
+
+@cm.no_compile
+def _dropout(x, p, seed, site):
+    cm._require_gpu(x)
+    return Dropout.apply(x, _probability(p), *_seed(seed, site, x.device))
+
+
+class LayerNorm(torch.autograd.Function):
+    """forward(ctx, x, residual, weight, bias, eps, residual_in_fp32, handed_on, p, seed, seed_t, site) -> y, or (y, s) where the
+    stream is handed on."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps, residual_in_fp32, handed_on, p, seed, seed_t, site):
+        dev = cm._require_gpu(x, residual, weight, bias)
+        if x.dim() < 1 or x.numel() == 0:
+            raise ValueError(f"x must be [.., D] with at least one row, got {tuple(x.shape)}")
+        D = x.shape[-1]
+        if D > MAX_NORM_ROW:
+            raise ValueError(f"the norm serves rows of up to {MAX_NORM_ROW} entries, got {D}")
+        if residual is not None and residual.shape != x.shape:
+            raise ValueError(f"residual must have the shape of x, {tuple(x.shape)}, got {tuple(residual.shape)}")
+        if tuple(weight.shape) != (D,) or (bias is not None and tuple(bias.shape) != (D,)):
+            raise ValueError(f"weight and bias must be [{D}], got {tuple(weight.shape)} and {None if bias is None else tuple(bias.shape)}")
+        if not eps >= 0:
+            raise ValueError(f"eps must not be negative, got {eps}")
+        cd = _rows_dtype(x)
+        rd = cd
+        if handed_on and (residual_in_fp32 or _rows_dtype(x, residual) == torch.float32):
+            rd = torch.float32
+        xc, xs = _norm_rows(x, cd)
+        rc_, rs = (None, D) if residual is None else _norm_rows(residual, rd)
+        w, b = cm.param(weight), cm.param(bias)
+        if b is not None and b.dtype != w.dtype:
+            w, b = w.float(), b.float()
+        y = torch.empty(x.shape, dtype=cd, device=dev)
+        s = torch.empty(x.shape, dtype=rd, device=dev) if handed_on else None
+        rows = x.numel() // D
+        stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if any(ctx.needs_input_grad) else None
+        pt = cm._ptr
+        dims = L.PalLayerNormDims(rows=rows, x_stride=xs, res_stride=rs, dim=D, dtype=cm._pal_dtype(cd), res_dtype=cm._pal_dtype(rd),
+                                  weight_dtype=cm._pal_dtype(w.dtype), eps=float(eps), drop=_drop_struct(p, seed, seed_t, site))
+        tens = L.PalLayerNormTensors(x=pt(xc), residual=pt(rc_), weight=pt(w), bias=pt(b), residual_out=pt(s), y=pt(y), stats=pt(stats))
+        with torch.cuda.device(dev):
+            rc = L.load().pal_layer_norm_fwd(dims, tens, cm.current_stream_ptr(dev))
+        L.check(rc, "pal_layer_norm_fwd")
+        ctx.set_materialize_grads(False)
+        if stats is not None:
+            ctx.save_for_backward(s if handed_on else xc, w, stats, seed_t)
+            ctx.meta = dict(cd=cd, rd=rd, handed_on=handed_on, dims=dims, drop=(p, seed, site),
+                            dtypes=[None if t is None else t.dtype for t in (x, residual, weight, bias)])
+        y = y if y.dtype == x.dtype else y.to(x.dtype)
+        return (y, s) if handed_on else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dres=None):
+        rows, w, stats, seed_t = ctx.saved_tensors
+        m = ctx.meta
+        dev, cd, rd, dt = rows.device, m["cd"], m["rd"], m["dtypes"]
+        if dy is None and dres is None:
+            return (None,) * 11
+        dy = None if dy is None else cm._plain(dy, cd)
+        dres = None if dres is None else cm._plain(dres, rd)
+        dx = torch.empty(rows.shape, dtype=cd, device=dev)
+        p, seed, site = m["drop"]
+        apart = dt[1] is not None and (p > 0.0 or cd != rd)
+        ds = torch.empty(rows.shape, dtype=rd, device=dev) if apart else None
+        dw = torch.empty(w.shape, dtype=torch.float32, device=dev)
+        db = None if dt[3] is None else torch.empty_like(dw)
+        pt = cm._ptr
+        dims = L.PalLayerNormDims.from_buffer_copy(m["dims"])
+        dims.drop = _drop_struct(p, seed, seed_t, site)
+        tens = L.PalLayerNormTensors(weight=pt(w), bias=pt(w) if db is not None else None, stats=pt(stats),
+                                     **{"residual_out" if m["handed_on"] else "x": pt(rows)})
+        grads = L.PalLayerNormGrads(dy=pt(dy), dresidual_out=pt(dres), dx=pt(dx), dresidual=pt(ds), dweight=pt(dw), dbias=pt(db))
+        lib = L.load()
+        ws_bytes = int(lib.pal_layer_norm_bwd_workspace_bytes(dims))
+        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
+        with torch.cuda.device(dev):
+            rc = lib.pal_layer_norm_bwd(dims, tens, grads, C.c_void_p(ws.data_ptr()), ws_bytes, cm.current_stream_ptr(dev))
+        L.check(rc, "pal_layer_norm_bwd")
+        d_res = None if dt[1] is None else (ds if apart else dx).to(dt[1])
+        return (dx.to(dt[0]), d_res, dw.to(dt[2]), None if db is None else db.to(dt[3])) + (None,) * 7
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """``(x - mean(x)) * rsqrt(var(x) + eps) * weight + bias`` over the last dim of x ``[.., D]`` (D up to 16384; var the mean square around
+    the mean); weight, bias ``[D]`` in fp32 or bf16.  y has the type of x.  Gradients for x, weight and bias."""
+    if not torch.compiler.is_compiling() and x.is_cuda:
+        r = L.host().layer_norm(x, None, weight, bias, eps, False, False, 0.0, 0, None, 0)
+        if r is not None:
+            return r[0]
+    return _layer_norm(x, None, weight, bias, eps, False, False, 0.0, 0, None, 0)
+
+
+@cm.no_compile
+def _layer_norm(x, residual, weight, bias, *rest):
+    cm._require_gpu(x, residual, weight, bias)
+    return LayerNorm.apply(x, residual, weight, bias, *rest)
+
+
+def residual_layer_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                        eps: float = 1e-5, residual_in_fp32: bool = False, dropout_p: float = 0.0, seed=None, site: int = 0):
+    """``s = dropout(x) + residual``, ``y = layer_norm(s)``; returns ``(y, s)``: the block's input and the residual stream to hand on, as
+    ``residual_rms_norm`` does (types, rows and the missing residual of a first block are as there), with the bias of a layer norm and the
+    dropout of ``dropout(x, dropout_p, seed, site)`` in the same pass.  The norm is that of s as it is handed on.  Gradients for x, residual,
+    weight and bias."""
+    p = _probability(dropout_p)
+    bits, seed_t = 0, None
+    if p > 0.0:
+        if seed is None:
+            raise ValueError("a dropout needs a seed")
+        bits, seed_t, site = _seed(seed, site, x.device)
+    if not torch.compiler.is_compiling() and x.is_cuda:
+        r = L.host().layer_norm(x, residual, weight, bias, eps, residual_in_fp32, True, p, bits, seed_t, site)
+        if r is not None:
+            return r
+    return _layer_norm(x, residual, weight, bias, eps, residual_in_fp32, True, p, bits, seed_t, site)
 
 
 @cm.no_compile
