@@ -169,7 +169,7 @@ constexpr int kBigTile = 256, kSmallTile = 128;
 static TilePlan plan_tiles(const TileArgs& P, int kind, int dtype) {
   TilePlan best{};
   double least = 1e30;
-  const int one = (P.k + (dtype == PAL_DTYPE_BF16 ? 31 : 15)) / (dtype == PAL_DTYPE_BF16 ? 32 : 16);
+  const int one = (P.k + (dtype == PAL_DTYPE_BF16 ? 63 : 31)) / (dtype == PAL_DTYPE_BF16 ? 64 : 32);
   const int steps = kind == kTileTwice ? 2 * one : one;
   double numbers = 0;
   for (int i = 0; i < P.n_prod; ++i) numbers += (double)P.prod[i].a.rows * P.prod[i].b.rows;
@@ -179,7 +179,7 @@ static TilePlan plan_tiles(const TileArgs& P, int kind, int dtype) {
     for (int i = 0; i < P.n_prod; ++i)
       tiles += (int64_t)((P.prod[i].a.rows + t - 1) / t) * ((P.prod[i].b.rows + tn - 1) / tn);
     if (tiles > 1 << 22) continue;   // threads of a launch
-    const double per_step = (big ? 0.6 : 0.42) * (dtype == PAL_DTYPE_BF16 ? 1 : 6);
+    const double per_step = (big ? 1.2 : 0.84) * (dtype == PAL_DTYPE_BF16 ? 1 : 6);
     for (int s = 1; s <= (kind == kTileGated ? 1 : 32) && s <= steps; ++s) {
       const int share = (steps + s - 1) / s, splits = (steps + share - 1) / share;
       if (splits != s || tiles * s > 1 << 22) continue;
@@ -196,10 +196,11 @@ static TilePlan plan_tiles(const TileArgs& P, int kind, int dtype) {
 
 template <typename T, int KIND, bool ACOLS, bool BCOLS, int WM, int WN, int NFM, int NFN>
 static int tile_launch(const TileArgs& P, int id, hipStream_t s) {
-  constexpr size_t lds = (size_t)kRing * 64 * 16 * (NFM * WM + NFN * WN);
+  constexpr size_t lds = (size_t)2 * 128 * 16 * (NFM * WM + NFN * WN);
+  constexpr int slots = lds > kMaxLds / 2 ? 256 : 512;   // workgroups that the chip holds at a time
   const auto kernel = &tile_product_kernel<T, KIND, ACOLS, BCOLS, WM, WN, NFM, NFN>;
   if (int rc = allow_lds((const void*)kernel, lds)) return rc;
-  PAL_TIMED_LAUNCH(id, s, (*kernel), dim3(P.tiles * P.splits), dim3(64 * WM * WN), lds, s, P);
+  PAL_TIMED_LAUNCH(id, s, (*kernel), dim3(P.tiles * P.splits < slots ? P.tiles * P.splits : slots), dim3(64 * WM * WN), lds, s, P);
   PAL_HIP_LAUNCH_CHECK();
   return PAL_OK;
 }

@@ -4,23 +4,25 @@
 // products of a layer's forward pass (rows, rows), of the gradient of its input (rows, columns) and of its weight (columns, columns) all
 // read their operands as they lie in memory.
 //
-// A workgroup takes a tile of BM x BN.  64 bytes of k of both operands (32 bf16 or 16 fp32 numbers) are a step; a ring of four steps is
-// kept in LDS, filled by loads that write LDS directly (no registers, three steps ahead), and each wave reads its operands of the next
-// step into a second set of registers while the matrix units work on the present one.  A step needs one barrier: behind it the loads of the
-// next step have landed for all waves, and the present step's place in the ring, which all have read, is free.
+// A workgroup takes a tile of BM x BN.  128 bytes of k of both operands (64 bf16 or 32 fp32 numbers: a line of the caches) are a step; two
+// steps are kept in LDS, filled by loads that write LDS directly, without registers.  A wave goes through a step in four parts and reads the
+// operands of the next part while the matrix units work on one.  A step needs one barrier, before its last part: behind it the loads of
+// the next step have landed for all waves, and the present step's place, which all have read, is free for the one after.
 //
-// Layout of a step in LDS: pieces of 16 bytes, a row of an operand that lies in rows as four pieces, a k of one that lies in columns as
+// Layout of a step in LDS: pieces of 16 bytes, a row of an operand that lies in rows as eight pieces, a k of one that lies in columns as
 // BM / 8 (BM / 4) pieces, in either case with the piece's number changed by an exclusive or (`swizzle`) so that the sixteen lanes that
 // read at one time find sixteen different places among the banks.  (The direct loads write lane after lane, so the change is made to the
 // address that a lane reads from.)
 //
-// The 16 x 16 results are arranged so that a lane holds eight neighbouring columns of C of one row: matrix instruction (n, m) takes rows
-// 32 (f / 2) + 8 (j / 4) + 4 (f % 2) + j % 4, j < 16, of a wave's part of either operand as its fragment f, and B stands first, so that its index
-// runs along a lane's four numbers.  Two fragments together are 16-byte stores without a turn through LDS.
+// The 16 x 16 results are arranged so that a lane holds eight neighbouring columns of C of one row: a wave's fragment f of B is made of rows
+// 32 (f / 2) + 8 (j / 4) + 4 (f % 2) + j % 4, j < 16, of its part, and B stands first in the matrix instructions, so that its index runs
+// along a lane's four numbers.  Two fragments together are 16-byte stores without a turn through LDS.
 //
 // Whatever lies behind a matrix (rows behind the last one, k behind the end) is read as zero: by the bounds of the buffer for whole rows,
 // by an address beyond all bounds for the rest of a row.
 #pragma once
+#include <type_traits>
+
 #include "pal_common.h"
 
 namespace pal {
@@ -94,14 +96,14 @@ template <typename T>
 struct TileType;
 template <>
 struct TileType<bf16_t> {
-  static constexpr int kPiece = 8, kStep = 32;    // elements of 16 bytes; k of a step
+  static constexpr int kPiece = 8, kStep = 64;    // elements of 16 bytes; k of a step
   static __device__ __forceinline__ f32x4 mma(f32x4 a, f32x4 b, f32x4 c) {
     return mfma16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
   }
 };
 template <>
 struct TileType<float> {
-  static constexpr int kPiece = 4, kStep = 16;
+  static constexpr int kPiece = 4, kStep = 32;
   // each of the four instructions takes one k from each of the four lane groups' pieces
   static __device__ __forceinline__ f32x4 mma(f32x4 a, f32x4 b, f32x4 c) {
 #pragma unroll
@@ -130,64 +132,71 @@ __device__ __forceinline__ void tile_load8(const float* p, float* x) {
   for (int e = 0; e < 8; ++e) x[e] = e < 4 ? lo[e & 3] : hi[e & 3];
 }
 
-// row of a wave's part of an operand that entry j of fragment f stands for
-__device__ __forceinline__ constexpr int frag_row(int f, int j) { return 32 * (f >> 1) + 8 * (j >> 2) + 4 * (f & 1) + (j & 3); }
+// row of a wave's part of an operand that entry j of fragment f stands for; PAIRS: two fragments share 32 rows (see above)
+template <bool PAIRS>
+__device__ __forceinline__ constexpr int frag_row(int f, int j) {
+  return PAIRS ? 32 * (f >> 1) + 8 * (j >> 2) + 4 * (f & 1) + (j & 3) : 16 * f + j;
+}
+
+// a value that is the same in all lanes, in scalar registers whatever computed it (a division is done in vector registers, and a buffer's
+// description from there would be walked lane by lane)
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t scalar64(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)scalar((int)x) | (uint64_t)(uint32_t)scalar((int)(x >> 32)) << 32);
+}
 
 constexpr uint32_t kBeyond = 0x80000000u;   // an offset that no buffer's bounds reach
-constexpr int kRing = 4;
 
 // ------------------------------------------------------------------------------------------------------- an operand's way
 // ROWS rows of a step, loaded by WAVES waves, read in NF fragments by a wave whose part begins at row `base`; HALVES: every other 32 rows
 // come from the second matrix.
-template <typename T, bool COLS, int ROWS, int WAVES, int NF, bool HALVES>
+template <typename T, bool COLS, int ROWS, int WAVES, int NF, bool PAIRS, bool HALVES>
 struct OperandWay {
   typedef TileType<T> E;
-  static constexpr int kBytes = ROWS * 64;
+  static constexpr int kBytes = ROWS * 128;
   static constexpr int kLoads = kBytes / 1024 / WAVES;                   // of a wave: 64 lanes of 16 bytes
-  static constexpr int kLine = COLS ? ROWS * (int)sizeof(T) : 64;         // bytes of a row or a k
+  static constexpr int kLine = COLS ? ROWS * (int)sizeof(T) : 128;        // bytes of a row or a k
   static_assert(kBytes % (1024 * WAVES) == 0 && (!COLS || kLine >= 256), "tile");
 
+  // Lanes 0-3, 12-15, 20-23 and 24-27 of a 16-byte read meet in the banks, and so do the other half of 32 lanes; of an 8-byte transposing
+  // read all 32.  (Taken as sixteen neighbours, the reads of a step were 8 cycles each instead of 4.)
   static __device__ __forceinline__ int swizzle(int line) {
-    if constexpr (!COLS) return (line >> 3) & 3;
-    else if constexpr (sizeof(T) == 2) return 4 * (line & 3);
-    else return ((line >> 2) & 1) | ((line & 8));
+    if constexpr (!COLS) {
+      const int q = (PAIRS ? line >> 3 : line >> 2) & 3;
+      return (q >> 1) | ((q ^ (q >> 1)) & 1) << 1 | (line & 2) << 1;
+    } else if constexpr (sizeof(T) == 2) {
+      return PAIRS ? 4 * (line & 3) : 2 * ((line & 3) | ((line >> 3) & 1) << 2);
+    } else {
+      return PAIRS ? ((line >> 2) & 1) | (line & 8) : 4 * ((line >> 2) & 3);
+    }
   }
 
   uint32_t off[kLoads];   // of a lane's pieces from the step's beginning
-  int kpos[kLoads];       // rows: the piece's k in the step
+  int piece;              // rows: the piece's number in the step is this, changed by the swizzle of the load's first line
   const char* at;         // the step's beginning
   int64_t left;           // bytes from there to the end of the matrix
   int64_t advance;
 
-  __device__ __forceinline__ void begin(const TileOperand& o, int row0, int k0, int k, int wave, int lane) {
-    bool second = false;
+  __device__ __forceinline__ void begin(int64_t ld, int wave, int lane) {
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int instr = wave * kLoads + j, p = instr * 64 + lane;
-      const int line = p / (kLine / 16), piece = (p % (kLine / 16)) ^ swizzle(line);
-      if constexpr (COLS) {
-        off[j] = (uint32_t)(line * o.ld) + piece * 16;
-        kpos[j] = 0;
-      } else {
-        int row = line;
-        if constexpr (HALVES) {
-          static_assert(!HALVES || kLoads == 2, "a wave's loads are of one matrix");
-          second = wave & 1;
-          row = 32 * (line >> 6) + (line & 31);
-        }
-        off[j] = (uint32_t)(row * o.ld) + piece * 16;
-        kpos[j] = piece * E::kPiece;
+      const int line = p / (kLine / 16), pc = (p % (kLine / 16)) ^ swizzle(line);
+      int row = line;
+      if constexpr (HALVES) {
+        static_assert(!HALVES || (!COLS && kLoads == 4), "a wave's loads are of 32 rows, all of one matrix");
+        row = 32 * (line >> 6) + (line & 31);
       }
+      off[j] = (uint32_t)(row * ld) + pc * 16;
     }
-    const char* p = second ? o.p2 : o.p;
-    place(o, p, row0, k0, k);
-    advance = COLS ? E::kStep * o.ld : 64;
+    piece = (lane & 7) ^ swizzle(lane >> 3);
+    advance = COLS ? E::kStep * ld : 128;
   }
   __device__ __forceinline__ void place(const TileOperand& o, const char* p, int row0, int k0, int k) {
     const int64_t to = COLS ? k0 * o.ld + row0 * (int64_t)sizeof(T) : row0 * o.ld + k0 * (int64_t)sizeof(T);
     const int64_t end = COLS ? (k - 1) * o.ld + o.rows * (int64_t)sizeof(T) : (o.rows - 1) * o.ld + k * (int64_t)sizeof(T);
-    at = p + to;
-    left = end - to;
+    at = (const char*)scalar64((int64_t)(p + to));
+    left = scalar64(end - to);
   }
   // loads of a step into its place in LDS; k_left: numbers of k from the step's beginning on
   __device__ __forceinline__ void load(char* lds, int wave, int k_left) {
@@ -195,45 +204,51 @@ struct OperandWay {
     auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)at, 0, bound, 0x00027000);
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
+      const int instr = wave * kLoads + j;
       uint32_t o = off[j];
-      if constexpr (!COLS) o = kpos[j] < k_left ? o : kBeyond;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + (wave * kLoads + j) * 1024), 16, o, 0, 0, 0);
+      if constexpr (!COLS) o = (piece ^ swizzle(8 * instr)) * E::kPiece < k_left ? o : kBeyond;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)(lds + instr * 1024), 16, o, 0, 0, 0);
     }
     at += advance;
     left -= advance;
   }
+  static constexpr int kReads = NF * (!COLS ? 1 : sizeof(T) == 2 ? 2 : 4);   // of half a step, by a wave
 
   // places of a lane's fragments in a step
-  static constexpr int kPlaces = !COLS ? 1 : sizeof(T) == 2 ? NF / 2 : NF;
+  static constexpr int kPlaces = !COLS ? 2 : sizeof(T) == 2 && PAIRS ? NF / 2 : NF;
   uint32_t place_of[kPlaces];
   __device__ __forceinline__ void aim(int base, int lane) {
     const int j = lane & 15, g = lane >> 4;
     if constexpr (!COLS) {
-      const int row = base + frag_row(0, j);
-      place_of[0] = row * 64 + ((g ^ swizzle(row)) * 16);
+      const int row = base + frag_row<PAIRS>(0, j);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) place_of[h] = row * 128 + (((4 * h + g) ^ swizzle(row)) * 16);
     } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int f = 0; f < NF / 2; ++f) {
-        const int k = 8 * g + (j >> 2), col = base + 32 * f + 8 * (j & 3);
-        place_of[f] = k * kLine + (((col >> 3) ^ swizzle(k)) * 16);
+      for (int f = 0; f < kPlaces; ++f) {
+        const int k = 8 * g + (j >> 2), col = base + (PAIRS ? 32 * f + 8 * (j & 3) : 16 * f + 4 * (j & 3));
+        place_of[f] = k * kLine + (((col >> 3) ^ swizzle(k)) * 16) + (col & 7) * 2;
       }
     } else {
 #pragma unroll
       for (int f = 0; f < NF; ++f) {
-        const int k = 4 * g, col = base + frag_row(f, j);
+        const int k = 4 * g, col = base + frag_row<PAIRS>(f, j);
         place_of[f] = k * kLine + (((col >> 2) ^ swizzle(k)) * 16) + (col & 3) * 4;
       }
     }
   }
-  __device__ __forceinline__ f32x4 read(const char* step, int f) const {
+  __device__ __forceinline__ f32x4 read(const char* step, int half, int f) const {
     if constexpr (!COLS) {
-      return *(const f32x4*)(step + place_of[0] + (32 * (f >> 1) + 4 * (f & 1)) * 64);
-    } else if constexpr (sizeof(T) == 2) {
-      const char* p = step + place_of[f >> 1] + 8 * (f & 1);
-      return __builtin_bit_cast(f32x4, join(lds_read_tr((const bf16_t*)p), lds_read_tr((const bf16_t*)(p + 4 * kLine))));
+      return *(const f32x4*)(step + place_of[half] + frag_row<PAIRS>(f, 0) * 128);
     } else {
-      const char* p = step + place_of[f];
-      return f32x4{*(const float*)p, *(const float*)(p + kLine), *(const float*)(p + 2 * kLine), *(const float*)(p + 3 * kLine)};
+      const char* p = step + half * (E::kStep / 2) * kLine;
+      if constexpr (sizeof(T) == 2) {
+        p += PAIRS ? place_of[f >> 1] + 8 * (f & 1) : place_of[f];
+        return __builtin_bit_cast(f32x4, join(lds_read_tr((const bf16_t*)p), lds_read_tr((const bf16_t*)(p + 4 * kLine))));
+      } else {
+        p += place_of[f];
+        return f32x4{*(const float*)p, *(const float*)(p + kLine), *(const float*)(p + 2 * kLine), *(const float*)(p + 3 * kLine)};
+      }
     }
   }
 };
@@ -248,159 +263,224 @@ template <typename T, int KIND, bool ACOLS, bool BCOLS, int WM, int WN, int NFM,
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_product_kernel(TileArgs P) {
   typedef TileType<T> E;
   constexpr int W = WM * WN, BM = 16 * NFM * WM, BN = 16 * NFN * WN;
-  typedef OperandWay<T, ACOLS, BM, W, NFM, false> AWay;
-  typedef OperandWay<T, BCOLS, BN, W, NFN, KIND == kTileGated> BWay;
-  constexpr int kStepBytes = AWay::kBytes + BWay::kBytes, kLoads = AWay::kLoads + BWay::kLoads;
+  typedef OperandWay<T, ACOLS, BM, W, NFM, false, false> AWay;
+  typedef OperandWay<T, BCOLS, BN, W, NFN, true, KIND == kTileGated> BWay;
+  constexpr uint32_t kStepBytes = AWay::kBytes + BWay::kBytes;
+  constexpr int kLoads = AWay::kLoads + BWay::kLoads;
   extern __shared__ __attribute__((aligned(16))) char ring[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 
-  // tiles in order go to one die after the other: each gets a run of neighbouring ones, whose operands its cache then holds
-  const int all = P.tiles * P.splits, id = blockIdx.x, die = id & 7, q = all >> 3, r = all & 7;
-  const int place = die * q + min(die, r) + (id >> 3);
-  const int split = place / P.tiles, tile = place - split * P.tiles;
-  int which = 0;
-  if (P.n_prod > 1 && tile >= P.prod[1].first) which = 1;
-  if (P.n_prod > 2 && tile >= P.prod[2].first) which = 2;
-  const TileProduct& pr = P.prod[which];
-  const int M = pr.a.rows, N = pr.b.rows, tiles_m = (M + BM - 1) / BM;
-  // bands of eight tiles of m, in a band down the tiles of m first
-  const int in = tile - pr.first, band = in / (8 * pr.tiles_n), in_band = in - band * 8 * pr.tiles_n;
-  const int high = min(8, tiles_m - 8 * band), tn = in_band / high, tm = 8 * band + in_band - tn * high;
-  constexpr int kCols = KIND == kTileGated ? BN / 2 : BN;
-  const int m0 = tm * BM, n0 = tn * kCols;
-
-  int step = split * P.split_steps;
+  // Tiles in order go to the dies in eight runs, so that a die's cache holds the operands of neighbours; the workgroups of a die take
+  // its run's tiles in turn.
+  const int all = P.tiles * P.splits, die = blockIdx.x & 7;
+  const int run = (all >> 3) + (die < (all & 7)), run0 = die * (all >> 3) + min(die, all & 7);
+  const int takers = (gridDim.x >> 3) + (die < (int)(gridDim.x & 7)), mine = blockIdx.x >> 3;
   const int one = (P.k + E::kStep - 1) / E::kStep;         // steps of a matrix
-  const int end = min(KIND == kTileTwice ? 2 * one : one, step + P.split_steps);
-  const int steps = end - step;
+  constexpr int kCols = KIND == kTileGated ? BN / 2 : BN;
+  struct Place { int which, m0, n0, split, step, end; };
+  auto where = [&](int i) {
+    Place w;
+    const int place = run0 + i;
+    w.split = place / P.tiles;
+    const int tile = place - w.split * P.tiles;
+    w.which = 0;
+    if (P.n_prod > 1 && tile >= P.prod[1].first) w.which = 1;
+    if (P.n_prod > 2 && tile >= P.prod[2].first) w.which = 2;
+    const TileProduct& pr = P.prod[w.which];
+    // bands of eight tiles of m, in a band down the tiles of m first
+    const int tiles_m = (pr.a.rows + BM - 1) / BM, in = tile - pr.first, band = in / (8 * pr.tiles_n), in_band = in - band * 8 * pr.tiles_n;
+    const int high = min(8, tiles_m - 8 * band), tn = in_band / high, tm = 8 * band + in_band - tn * high;
+    w.m0 = scalar(tm * BM);
+    w.n0 = scalar(tn * kCols);
+    w.split = scalar(w.split);
+    w.which = scalar(w.which);
+    w.step = w.split * P.split_steps;
+    w.end = min(KIND == kTileTwice ? 2 * one : one, w.step + P.split_steps);
+    return w;
+  };
+
+  // Loads run two steps ahead of the products, over the ends of matrices and tiles: the next tile's first steps are on their way while
+  // this one's results are stored.
   AWay A;
   BWay B;
-  int k_left, to_second = 0;                                // steps until the second matrix
-  {
-    const bool second = KIND == kTileTwice && step >= one;
-    const int k0 = (second ? step - one : step) * E::kStep;
-    TileOperand oa = pr.a, ob = pr.b;
-    if (second) oa.p = oa.p2, ob.p = ob.p2;
-    A.begin(oa, m0, k0, P.k, wave, lane);
-    B.begin(ob, n0, k0, P.k, wave, lane);
+  int ahead = mine, which = -1, to_go = 0, k_left = 0;     // the tile that is loaded; steps left of its present matrix
+  uint32_t slot = 0;
+  Place next{};
+  auto second_of = [&](int w) { return KIND == kTileTwice && w >= one; };
+  auto go_on = [&]() {                                     // to the next matrix, the next tile, or nowhere
+    if (to_go) return;
+    if (next.step >= next.end) {
+      if (ahead >= run) {
+        A.left = B.left = 0;
+        k_left = 0;
+        to_go = -1;
+        return;
+      }
+      next = where(ahead);
+      ahead += takers;
+    }
+    const TileProduct& pr = P.prod[next.which];
+    if (next.which != which) {
+      which = next.which;
+      A.begin(pr.a.ld, wave, lane);
+      B.begin(pr.b.ld, wave, lane);
+    }
+    const bool second = second_of(next.step);
+    const int k0 = (second ? next.step - one : next.step) * E::kStep, end = KIND == kTileTwice && !second ? min(one, next.end) : next.end;
+    A.place(pr.a, second ? pr.a.p2 : pr.a.p, next.m0, k0, P.k);
+    B.place(pr.b, (KIND == kTileGated ? (wave & 1) != 0 : second) ? pr.b.p2 : pr.b.p, next.n0, k0, P.k);
     k_left = P.k - k0;
-    if (KIND == kTileTwice) to_second = second ? -1 : one - step;
-  }
+    to_go = end - next.step;
+    next.step = end;
+  };
+  auto issue = [&](uint32_t to) {
+    A.load(ring + to, wave, k_left);
+    B.load(ring + to + AWay::kBytes, wave, k_left);
+    k_left -= E::kStep;
+    --to_go;
+  };
   A.aim(wave / WN * 16 * NFM, lane);
   B.aim(wave % WN * 16 * NFN, lane);
-
-  int issued = 0;
-  auto issue = [&]() {
-    char* to = ring + (issued & (kRing - 1)) * kStepBytes;
-    const int k = issued < steps ? k_left : 0;
-    if (issued >= steps) A.left = 0, B.left = 0;            // nothing is read; the counts of loads in flight stay the same
-    A.load(to, wave, k);
-    B.load(to + AWay::kBytes, wave, k);
-    k_left -= E::kStep;
-    ++issued;
-    if (KIND == kTileTwice && issued == to_second) {
-      A.place(pr.a, pr.a.p2, m0, 0, P.k);
-      B.place(pr.b, pr.b.p2, n0, 0, P.k);
-      k_left = P.k;
-    }
-  };
-#pragma unroll
-  for (int s = 0; s < kRing; ++s) issue();
+  go_on();
+  issue(0);
+  go_on();
+  issue(kStepBytes);
+  go_on();
 
   f32x4 acc[NFM][NFN];
+  // A step in four parts: the half of k by the half of a wave's rows of A.  Operands of a part are read during the one before.
+  constexpr int HM = NFM / 2;
+  f32x4 a_low[HM], a_high[HM], b_first[NFN], b_second[NFN];
+  auto read_a = [&](f32x4 (&f)[HM], uint32_t at, int half, int m0) {
 #pragma unroll
-  for (int m = 0; m < NFM; ++m)
-#pragma unroll
-    for (int n = 0; n < NFN; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  struct Frags { f32x4 a[NFM], b[NFN]; } now, next;
-  auto read = [&](Frags& f, int s) {
-    const char* at = ring + (s & (kRing - 1)) * kStepBytes;
-#pragma unroll
-    for (int n = 0; n < NFN; ++n) f.b[n] = B.read(at + AWay::kBytes, n);
-#pragma unroll
-    for (int m = 0; m < NFM; ++m) f.a[m] = A.read(at, m);
+    for (int m = 0; m < HM; ++m) f[m] = A.read(ring + at, half, m0 + m);
   };
-  auto multiply = [&](const Frags& f) {
+  auto read_b = [&](f32x4 (&f)[NFN], uint32_t at, int half) {
+#pragma unroll
+    for (int n = 0; n < NFN; ++n) f[n] = B.read(ring + at + AWay::kBytes, half, n);
+  };
+  auto multiply = [&](const f32x4 (&a)[HM], const f32x4 (&b)[NFN], int m0) {
+#pragma unroll
+    for (int m = 0; m < HM; ++m)
+#pragma unroll
+      for (int n = 0; n < NFN; ++n) acc[m0 + m][n] = E::mma(b[n], a[m], acc[m0 + m][n]);
+  };
+  // the matrix units are fed without a pause: reads, then loads go out between their instructions
+  auto spread = [&](auto reads, auto loads) {
+    constexpr int kR = decltype(reads)::value, kL = decltype(loads)::value, kMma = HM * NFN * (sizeof(T) == 2 ? 1 : 4);
+    constexpr int kEach = kMma / (kR + kL) > 0 ? kMma / (kR + kL) : 1;
+#pragma unroll
+    for (int i = 0; i < kR; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kL; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  typedef std::integral_constant<int, 0> None;
+  typedef std::integral_constant<int, AWay::kReads / 2> ReadsA;
+  typedef std::integral_constant<int, AWay::kReads / 2 + BWay::kReads> ReadsAB;
+  typedef std::integral_constant<int, kLoads> Loads;
+
+  // a lane: row j of fragment m, columns 8 g .. of a pair of fragments n
+  auto store_tile = [&](const TileProduct& pr, const Place& at_tile) {
+    const int M = pr.a.rows, N = pr.b.rows, n0 = at_tile.n0, split = at_tile.split;
+    const int j = lane & 15, g = lane >> 4, mw = at_tile.m0 + wave / WN * 16 * NFM;
+#pragma unroll
+    for (int m = 0; m < NFM; ++m) {
+      const int row = mw + frag_row<false>(m, j);
+      if (row >= M) continue;
+      if constexpr (KIND == kTileGated) {
+#pragma unroll
+        for (int n = 0; n < NFN; n += 4) {
+          const int col = n0 + wave % WN * 8 * NFN + 8 * n + 8 * g;
+          if (col >= N) continue;
+          float gt[8], up[8], c[8], none;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) gt[e] = acc[m][n + (e >> 2)][e & 3], up[e] = acc[m][n + 2 + (e >> 2)][e & 3];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            activate<false>(P.act, gt[e], c[e], none);
+            c[e] *= up[e];
+          }
+          const int64_t at = (int64_t)row * N + col;
+          tile_store8((T*)pr.c + at, c);
+          if (P.gate_out) {
+            tile_store8((T*)P.gate_out + at, gt);
+            tile_store8((T*)P.up_out + at, up);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NFN; n += 2) {
+          const int col = n0 + wave % WN * 16 * NFN + 16 * n + 8 * g;
+          if (col >= N) continue;
+          float c[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) c[e] = acc[m][n + (e >> 2)][e & 3];
+          const int64_t at = (int64_t)row * N + col;
+          if (P.splits > 1) {
+            tile_store8(pr.part + (int64_t)split * M * N + at, c);
+          } else if constexpr (KIND == kTileGrad) {
+            float gt[8], up[8], dg[8], du[8], h[8];
+            tile_load8((const T*)P.gate + at, gt);
+            tile_load8((const T*)P.up + at, up);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float a, d;
+              activate<true>(P.act, gt[e], a, d);
+              dg[e] = c[e] * up[e] * d;
+              du[e] = c[e] * a;
+              h[e] = a * up[e];
+            }
+            tile_store8((T*)pr.c + at, dg);
+            tile_store8((T*)P.up_out + at, du);
+            if (P.gate_out) tile_store8((T*)P.gate_out + at, h);
+          } else {
+            tile_store8((T*)pr.c + at, c);
+          }
+        }
+      }
+    }
+  };
+  wait_loads_and_meet<kLoads>();
+  read_b(b_first, 0, 0);
+  read_a(a_low, 0, 0, 0);
+  for (int tile = mine; tile < run; tile += takers) {
+    const Place at = where(tile);
+    const TileProduct& pr = P.prod[at.which];
 #pragma unroll
     for (int m = 0; m < NFM; ++m)
 #pragma unroll
-      for (int n = 0; n < NFN; ++n) acc[m][n] = E::mma(f.b[n], f.a[m], acc[m][n]);
-  };
-  wait_loads_and_meet<(kRing - 1) * kLoads>();
-  read(now, 0);
-  // a step: the loads of the next one have landed, this one's place is free
-  auto turn = [&](Frags& f, Frags& g, int s) {
-    wait_loads_and_meet<(kRing - 2) * kLoads>();
-    issue();
-    read(g, s + 1);
-    multiply(f);
-  };
-  int s = 0;
-  for (; s + 2 <= steps; s += 2) {
-    turn(now, next, s);
-    turn(next, now, s + 1);
-  }
-  if (s < steps) multiply(now);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // loads into LDS do not outlive the workgroup
-
-  // a lane: row j of fragment m, columns 8 g .. of a pair of fragments n
-  const int j = lane & 15, g = lane >> 4, mw = m0 + wave / WN * 16 * NFM;
-#pragma unroll
-  for (int m = 0; m < NFM; ++m) {
-    const int row = mw + frag_row(m, j);
-    if (row >= M) continue;
-    if constexpr (KIND == kTileGated) {
-#pragma unroll
-      for (int n = 0; n < NFN; n += 4) {
-        const int col = n0 + wave % WN * 8 * NFN + 8 * n + 8 * g;
-        if (col >= N) continue;
-        float gt[8], up[8], c[8], none;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) gt[e] = acc[m][n + (e >> 2)][e & 3], up[e] = acc[m][n + 2 + (e >> 2)][e & 3];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          activate<false>(P.act, gt[e], c[e], none);
-          c[e] *= up[e];
-        }
-        const int64_t at = (int64_t)row * N + col;
-        tile_store8((T*)pr.c + at, c);
-        if (P.gate_out) {
-          tile_store8((T*)P.gate_out + at, gt);
-          tile_store8((T*)P.up_out + at, up);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < NFN; n += 2) {
-        const int col = n0 + wave % WN * 16 * NFN + 16 * n + 8 * g;
-        if (col >= N) continue;
-        float c[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = acc[m][n + (e >> 2)][e & 3];
-        const int64_t at = (int64_t)row * N + col;
-        if (P.splits > 1) {
-          tile_store8(pr.part + (int64_t)split * M * N + at, c);
-        } else if constexpr (KIND == kTileGrad) {
-          float gt[8], up[8], dg[8], du[8], h[8];
-          tile_load8((const T*)P.gate + at, gt);
-          tile_load8((const T*)P.up + at, up);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float a, d;
-            activate<true>(P.act, gt[e], a, d);
-            dg[e] = c[e] * up[e] * d;
-            du[e] = c[e] * a;
-            h[e] = a * up[e];
-          }
-          tile_store8((T*)pr.c + at, dg);
-          tile_store8((T*)P.up_out + at, du);
-          if (P.gate_out) tile_store8((T*)P.gate_out + at, h);
-        } else {
-          tile_store8((T*)pr.c + at, c);
-        }
-      }
+      for (int n = 0; n < NFN; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = at.step; s < at.end; ++s) {
+      read_a(a_high, slot, 0, HM);
+      multiply(a_low, b_first, 0);
+      spread(ReadsA(), None());
+      read_b(b_second, slot, 1);
+      read_a(a_low, slot, 1, 0);
+      multiply(a_high, b_first, HM);
+      spread(ReadsAB(), None());
+      read_a(a_high, slot, 1, HM);
+      multiply(a_low, b_second, 0);
+      spread(ReadsA(), None());
+      wait_loads_and_meet<0>();
+      __builtin_amdgcn_sched_barrier(0);
+      read_b(b_first, slot ^ kStepBytes, 0);
+      read_a(a_low, slot ^ kStepBytes, 0, 0);
+      issue(slot);
+      multiply(a_high, b_second, HM);
+      spread(ReadsAB(), Loads());
+      slot ^= kStepBytes;
+      go_on();
     }
+    store_tile(pr, at);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // loads into LDS do not outlive the workgroup
 }
 
 }  // namespace pal
