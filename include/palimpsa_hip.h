@@ -598,7 +598,7 @@ typedef struct PalMlpTensors {
   const void *w_gate, *w_up;   /* [hidden,dim]                                  */
   const void *w_down;          /* [out_dim,hidden]                              */
   void *y;                     /* [rows,out_dim]                                */
-  void *gate, *up;             /* [rows,hidden]: g and u, kept for the backward; both NULL where none follows */
+  void *kept;                  /* pal_gated_mlp_kept_bytes(dims): g, u and h for the backward, or NULL where none follows */
 } PalMlpTensors;
 
 typedef struct PalMlpGrads {
@@ -608,9 +608,10 @@ typedef struct PalMlpGrads {
   void *dw_down;               /* [out_dim,hidden]                              */
 } PalMlpGrads;
 
-size_t pal_gated_mlp_fwd_workspace_bytes(const PalMlpDims *dims);
+size_t pal_gated_mlp_kept_bytes(const PalMlpDims *dims);
+size_t pal_gated_mlp_fwd_workspace_bytes(const PalMlpDims *dims, int keeps); /* keeps: with t->kept */
 int pal_gated_mlp_fwd(const PalMlpDims *dims, const PalMlpTensors *t, void *workspace, size_t workspace_bytes, void *stream);
-/* Backward: t as in the forward call, with gate and up as that call left them; t->y is not touched. */
+/* Backward: t as in the forward call, with kept as that call left it; t->y is not touched. */
 size_t pal_gated_mlp_bwd_workspace_bytes(const PalMlpDims *dims);
 int pal_gated_mlp_bwd(const PalMlpDims *dims, const PalMlpTensors *t, const PalMlpGrads *gr, void *workspace,
                       size_t workspace_bytes, void *stream);

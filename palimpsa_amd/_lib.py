@@ -129,7 +129,7 @@ class PalMlpDims(C.Structure):
 
 
 class PalMlpTensors(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("x", "w_gate", "w_up", "w_down", "y", "gate", "up")]
+    _fields_ = [(n, C.c_void_p) for n in ("x", "w_gate", "w_up", "w_down", "y", "kept")]
 
 
 class PalMlpGrads(C.Structure):
@@ -221,10 +221,11 @@ def load() -> C.CDLL:
     lib.pal_short_conv_step.restype = C.c_int
     lib.pal_short_conv_step.argtypes = [P(PalConvDims), P(PalConvTensors), C.c_void_p]
     lib.pal_scan_fwd.argtypes = [P(PalScanDims), P(PalScanTensors), C.c_void_p, C.c_size_t, C.c_void_p]
-    for name in ("pal_gated_mlp_fwd_workspace_bytes", "pal_gated_mlp_bwd_workspace_bytes"):
+    for name in ("pal_gated_mlp_kept_bytes", "pal_gated_mlp_fwd_workspace_bytes", "pal_gated_mlp_bwd_workspace_bytes"):
         fn = getattr(lib, name)
         fn.restype = C.c_size_t
         fn.argtypes = [P(PalMlpDims)]
+    lib.pal_gated_mlp_fwd_workspace_bytes.argtypes = [P(PalMlpDims), C.c_int]
     lib.pal_gated_mlp_fwd.restype = lib.pal_gated_mlp_bwd.restype = C.c_int
     lib.pal_gated_mlp_fwd.argtypes = [P(PalMlpDims), P(PalMlpTensors), C.c_void_p, C.c_size_t, C.c_void_p]
     lib.pal_gated_mlp_bwd.argtypes = [P(PalMlpDims), P(PalMlpTensors), P(PalMlpGrads), C.c_void_p, C.c_size_t, C.c_void_p]
@@ -306,7 +307,7 @@ _HOST_FUNCTIONS = ("pal_recurrent_fwd", "pal_gla_recurrent_fwd", "pal_chunk_fwd"
                    "pal_short_conv_fwd", "pal_short_conv_bwd", "pal_short_conv_bwd_workspace_bytes", "pal_short_conv_step",
                    "pal_scan_fwd", "pal_scan_fwd_workspace_bytes", "pal_scan_checkpoint_bytes", "pal_scan_bwd",
                    "pal_scan_bwd_workspace_bytes", "pal_dropout", "pal_layer_norm_fwd", "pal_layer_norm_bwd",
-                   "pal_layer_norm_bwd_workspace_bytes", "pal_gated_mlp_fwd", "pal_gated_mlp_fwd_workspace_bytes", "pal_gated_mlp_bwd",
+                   "pal_layer_norm_bwd_workspace_bytes", "pal_gated_mlp_kept_bytes", "pal_gated_mlp_fwd", "pal_gated_mlp_fwd_workspace_bytes", "pal_gated_mlp_bwd",
                    "pal_gated_mlp_bwd_workspace_bytes")
 
 

@@ -2,14 +2,14 @@
 //     dh = dy Wd,  dg = dh u act'(g),  du = dh act(g),  dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x,  dWd = dy^T h.
 //
 // Forward: two launches.  The first computes both products of a tile side by side and stores h (for training g and u too); the second
-// multiplies by Wd.  Backward: dh is never stored, the kernel that computes it turns it into dg and du and computes h again from g and u; the
-// gradient of x is one walk over both products, and the three of the weights are one launch (see tile_product.h).
+// multiplies by Wd.  Backward: dh is never stored, the kernel that computes it turns it into dg and du; the gradient of x is one walk over
+// both products, and the three of the weights are one launch (see tile_product.h).
 //
 // A call of few rows is bound by the weights, each of which is used once per 16 rows: few_rows_kernel has no tiles in LDS, the waves of a
 // workgroup walk over k side by side, each with a sixteenth of a line of the weights per lane straight from memory into the matrix units.
 //
-// Roundings to the type of the rows: g, u (kept, or only h without a gradient), h, dg and du, once each, half a step of the type; all sums are
-// in fp32.  Their errors in y and the gradients are of the size of the rounding of those results themselves.
+// Roundings to the type of the rows: h, dg and du, once each, half a step of the type, as operands of the matrix units; g and u are kept more
+// exactly (Kept8); all sums are in fp32.  The errors in y and the gradients are then of the size of the rounding of those results themselves.
 #include "pal_common.h"
 #include "pal_host.h"
 #include "pal_profile.h"
@@ -22,8 +22,9 @@ constexpr int kFewRows = 64;
 // ------------------------------------------------------------------------------------------------------------ few rows
 struct FewArgs {
   const void *x, *w, *w2;    // [rows][k] (x_ld), [n][k]; w2: second product (gated)
-  void *out, *gate_out, *up_out;   // [rows][n]
-  int64_t x_ld;              // elements
+  void* out;                 // [rows][n]
+  Kept kept;
+  int64_t x_ld, out_ld;      // elements
   int32_t rows, n, k, act;
 };
 
@@ -79,37 +80,37 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(FewArgs P) {
 #pragma unroll
     for (int r = 0; r < R; ++r) s[wave][m * R + r][lane] = acc[m][r];
   __syncthreads();
-  // a thread: four neighbouring columns of one row
-  for (int i = threadIdx.x; i < R * 64; i += 64 * W) {
-    const int r = i >> 6, l = i & 63, row = 16 * r + (l & 15), n = n0 + 4 * (l >> 4);
-    f32x4 t[kMats];
+  // a thread: eight neighbouring columns of one row
+  for (int i = threadIdx.x; i < R * 32; i += 64 * W) {
+    const int r = i >> 5, l = (i & 15) | (i & 16) << 1, row = 16 * r + (l & 15), n = n0 + 4 * (l >> 4);
+    float t[kMats][8];
 #pragma unroll
     for (int m = 0; m < kMats; ++m) {
-      t[m] = s[0][m * R + r][l];
+      f32x4 lo = s[0][m * R + r][l], hi = s[0][m * R + r][l + 16];
 #pragma unroll
-      for (int v = 1; v < W; ++v) t[m] += s[v][m * R + r][l];
+      for (int v = 1; v < W; ++v) {
+        lo += s[v][m * R + r][l];
+        hi += s[v][m * R + r][l + 16];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t[m][e] = e < 4 ? lo[e & 3] : hi[e & 3];
     }
     if (row >= P.rows || n >= P.n) continue;
-    const int64_t at = (int64_t)row * P.n + n;
-    float c[4], none;
+    const int64_t at = row * P.out_ld + n;
+    if constexpr (GATED) {
+      float c[8], none;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (GATED) {
+      for (int e = 0; e < 8; ++e) {
         activate<false>(P.act, t[0][e], c[e], none);
         c[e] *= t[1][e];
-      } else {
-        c[e] = t[0][e];
       }
-    }
-    store_vec<4>((T*)P.out + at, c);
-    if constexpr (GATED) {
-      if (P.gate_out) {
-        float a[4], b[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = t[0][e], b[e] = t[1][e];
-        store_vec<4>((T*)P.gate_out + at, a);
-        store_vec<4>((T*)P.up_out + at, b);
+      tile_store8((T*)P.out + at, c);
+      if (P.kept.gate) {
+        Kept8<T>::store(P.kept.gate, at, t[0]);
+        Kept8<T>::store(P.kept.up, at, t[1]);
       }
+    } else {
+      tile_store8((T*)P.out + at, t[0]);
     }
   }
 }
@@ -118,76 +119,83 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(FewArgs P) {
 struct JoinArgs {
   const float* part[3];
   void* out[3];
+  int64_t ldc[3];
   int64_t n[3];              // numbers of a share
+  uint32_t row8[3];          // eighths of a row
   int32_t splits;
-  const void *gate, *up;     // kTileGrad
-  void *h, *du;
+  Kept kept;                 // kTileGrad
+  void* c2;
   int32_t act;
 };
 template <typename T, bool GRAD>
 __global__ __launch_bounds__(256) void tile_join_kernel(JoinArgs P) {
   const int which = blockIdx.y;
   const int64_t n = P.n[which];
-  for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; at < n; at += (int64_t)gridDim.x * 256 * 8) {
+  for (int64_t from = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; from < n; from += (int64_t)gridDim.x * 256 * 8) {
     float c[8];
-    tile_load8(P.part[which] + at, c);
+    tile_load8(P.part[which] + from, c);
 #pragma unroll 4
     for (int s = 1; s < P.splits; ++s) {
       float b[8];
-      tile_load8(P.part[which] + s * n + at, b);
+      tile_load8(P.part[which] + s * n + from, b);
 #pragma unroll
       for (int e = 0; e < 8; ++e) c[e] += b[e];
     }
+    const uint32_t piece = (uint32_t)(from >> 3), row = piece / P.row8[which];   // (the host joins no more than 2^32 pieces)
+    const int64_t at = row * P.ldc[which] + 8 * (int64_t)(piece - row * P.row8[which]);
     if constexpr (GRAD) {
-      float gt[8], up[8], du[8], h[8];
-      tile_load8((const T*)P.gate + at, gt);
-      tile_load8((const T*)P.up + at, up);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float a, d;
-        activate<true>(P.act, gt[e], a, d);
-        du[e] = c[e] * a;
-        c[e] = c[e] * up[e] * d;
-        h[e] = a * up[e];
-      }
-      tile_store8((T*)P.du + at, du);
-      if (P.h) tile_store8((T*)P.h + at, h);
+      Kept8<T> gate, up;
+      float dg[8], du[8];
+      gate.load(P.kept.gate, at);
+      up.load(P.kept.up, at);
+      gated_grad8(P.act, c, gate, up, dg, du);
+      tile_store8((T*)P.out[which] + at, dg);
+      tile_store8((T*)P.c2 + at, du);
+    } else {
+      tile_store8((T*)P.out[which] + at, c);
     }
-    tile_store8((T*)P.out[which] + at, c);
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
-struct TilePlan {
-  bool big;
-  int tiles, splits, split_steps;
+// Tiles that the products are made of: 256 x 256 and, for matrices whose columns fill the chip better so, 256 x 192 by eight waves, one
+// workgroup a compute unit; 128 x 128 by four, two of them, where there are few tiles.
+enum TileForm { kTileBig = 0, kTileNarrow, kTileSmall, kTileForms };
+struct TileShape {
+  int m, n, slots;   // of the chip
+  double step_us;    // time of a step of bf16 numbers while every slot has a tile
 };
-constexpr int kBigTile = 256, kSmallTile = 128;
+constexpr TileShape kTileShapes[kTileForms] = {{256, 256, 256, 1.65}, {256, 192, 256, 1.35}, {128, 128, 512, 1.0}};
+struct TilePlan {
+  int form, tiles, splits, split_steps;
+};
 
-// Tile size and shares of k: the cheapest by the time of a step of a tile (us), the launch's rounds over the chip and, for shares, their
-// way through memory.
+// Tile form and shares of k: the cheapest by the time of a step of a tile, the launch's rounds over the chip and, for shares, their way
+// through memory.
 static TilePlan plan_tiles(const TileArgs& P, int kind, int dtype) {
   TilePlan best{};
   double least = 1e30;
-  const int one = (P.k + (dtype == PAL_DTYPE_BF16 ? 63 : 31)) / (dtype == PAL_DTYPE_BF16 ? 64 : 32);
-  const int steps = kind == kTileTwice ? 2 * one : one;
+  const int per = dtype == PAL_DTYPE_BF16 ? 64 : 32, one = (P.k + per - 1) / per, steps = kind == kTileTwice ? 2 * one : one;
   double numbers = 0;
   for (int i = 0; i < P.n_prod; ++i) numbers += (double)P.prod[i].a.rows * P.prod[i].b.rows;
-  for (int big = 0; big < 2; ++big) {
-    const int t = big ? kBigTile : kSmallTile, tn = kind == kTileGated ? t / 2 : t, slots = big ? 256 : 512;
+  const int most = kind == kTileGated || numbers > 3e10 ? 1 : 32;   // shares: gated tiles have none, and the join counts pieces in 32 bits
+  for (int form = 0; form < kTileForms; ++form) {
+    if (form == kTileNarrow && kind == kTileGated) continue;
+    const TileShape& t = kTileShapes[form];
+    const int tn = kind == kTileGated ? t.n / 2 : t.n;
     int64_t tiles = 0;
     for (int i = 0; i < P.n_prod; ++i)
-      tiles += (int64_t)((P.prod[i].a.rows + t - 1) / t) * ((P.prod[i].b.rows + tn - 1) / tn);
-    if (tiles > 1 << 22) continue;   // threads of a launch
-    const double per_step = (big ? 1.2 : 0.84) * (dtype == PAL_DTYPE_BF16 ? 1 : 6);
-    for (int s = 1; s <= (kind == kTileGated ? 1 : 32) && s <= steps; ++s) {
+      tiles += (int64_t)((P.prod[i].a.rows + t.m - 1) / t.m) * ((P.prod[i].b.rows + tn - 1) / tn);
+    if (tiles > 1 << 24) continue;
+    const double step = t.step_us * (dtype == PAL_DTYPE_BF16 ? 1 : 5.5);
+    for (int s = 1; s <= most && s <= steps; ++s) {
       const int share = (steps + s - 1) / s, splits = (steps + share - 1) / share;
-      if (splits != s || tiles * s > 1 << 22) continue;
-      const double rounds = (double)((tiles * s + slots - 1) / slots);
-      const double us = rounds * (share * per_step + 3) + (s > 1 ? 3 + numbers * s * 8 / 4e6 : 0);
+      if (splits != s) continue;
+      const double rounds = (double)((tiles * s + t.slots - 1) / t.slots);
+      const double us = rounds * share * step + 3 + (s > 1 ? 4 + numbers * s * (4 / 3.5e6 + 4 / 1e7) : 0);
       if (us < least) {
         least = us;
-        best = TilePlan{big != 0, (int)tiles, s, share};
+        best = TilePlan{form, (int)tiles, s, share};
       }
     }
   }
@@ -217,7 +225,7 @@ static size_t part_bytes(const TileArgs& P, const TilePlan& plan) {
 template <typename T, int KIND, bool ACOLS, bool BCOLS>
 static int tile_run(TileArgs P, const TilePlan& plan, float* part, int id, hipStream_t s) {
   if (!plan.tiles) return PAL_E_DIM;
-  const int t = plan.big ? kBigTile : kSmallTile, tn = KIND == kTileGated ? t / 2 : t;
+  const int t = kTileShapes[plan.form].m, tn = KIND == kTileGated ? kTileShapes[plan.form].n / 2 : kTileShapes[plan.form].n;
   P.tiles = plan.tiles;
   P.splits = plan.splits;
   P.split_steps = plan.split_steps;
@@ -232,13 +240,18 @@ static int tile_run(TileArgs P, const TilePlan& plan, float* part, int id, hipSt
     p.part = part;
     J.part[i] = part;
     J.out[i] = p.c;
+    J.ldc[i] = p.ldc;
+    J.row8[i] = p.b.rows / 8;
     J.n[i] = (int64_t)p.a.rows * p.b.rows;
     most = J.n[i] > most ? J.n[i] : most;
     if (part) part += J.n[i] * plan.splits;
   }
-  const int rc = plan.big ? tile_launch<T, KIND, ACOLS, BCOLS, 2, 4, 8, 4>(P, id, s) : tile_launch<T, KIND, ACOLS, BCOLS, 2, 2, 4, 4>(P, id, s);
+  int rc = PAL_OK;
+  if (plan.form == kTileBig) rc = tile_launch<T, KIND, ACOLS, BCOLS, 2, 4, 8, 4>(P, id, s);
+  else if (plan.form == kTileSmall) rc = tile_launch<T, KIND, ACOLS, BCOLS, 2, 2, 4, 4>(P, id, s);
+  else if constexpr (KIND != kTileGated) rc = tile_launch<T, KIND, ACOLS, BCOLS, 4, 2, 4, 6>(P, id, s);
   if (rc || plan.splits < 2) return rc;
-  J.splits = plan.splits; J.gate = P.gate; J.up = P.up; J.h = P.gate_out; J.du = P.up_out; J.act = P.act;
+  J.splits = plan.splits; J.kept = P.kept; J.c2 = P.c2; J.act = P.act;
   const int64_t blocks = (most + 2047) / 2048;
   PAL_TIMED_LAUNCH(kKernTileJoin, s, (tile_join_kernel<T, KIND == kTileGrad>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), P.n_prod),
                    dim3(256), 0, s, J);
@@ -275,46 +288,60 @@ static TileOperand operand(const void* p, int64_t ld_elems, size_t es, int64_t r
   return TileOperand{(const char*)p, (const char*)p2, (int64_t)(ld_elems * es), (int32_t)rows};
 }
 
+// Rows of hidden numbers that the calls lay out themselves (h, dg, du, the kept factors) are an odd number of 128-byte lines apart: rows at a
+// multiple of 4096 bytes are in few of the caches' channels, and a tile reads or writes one piece of each of its rows at a time.
+static int64_t hidden_ld(const PalMlpDims* d) {
+  const int64_t line = 128 / (int64_t)mlp_elem(d), lines = (d->hidden + line - 1) / line;
+  return d->hidden < 8 * line ? d->hidden : (lines | 1) * line;
+}
+static size_t rows_bytes(const PalMlpDims* d) { return round256((size_t)d->rows * hidden_ld(d) * mlp_elem(d)); }
+// what the forward call keeps for the backward: the factors, and h
+static Kept kept_in(const PalMlpDims* d, void* kept) { return kept ? Kept{kept, (char*)kept + rows_bytes(d)} : Kept{}; }
+static void* kept_h(const PalMlpDims* d, void* kept) { return (char*)kept + 2 * rows_bytes(d); }
+
 struct MlpPlan {
   TileArgs up{}, down{}, grad{}, dx{}, dw{};
   TilePlan p_up{}, p_down{}, p_grad{}, p_dx{}, p_dw{};
 };
 static void plan_fwd(const PalMlpDims* d, const PalMlpTensors* t, const void* h, MlpPlan& m) {
   const size_t es = mlp_elem(d);
+  const int64_t ld = hidden_ld(d);
   m.up.n_prod = 1;
   m.up.k = d->dim;
   m.up.prod[0].a = operand(t->x, d->x_stride, es, d->rows);
   m.up.prod[0].b = operand(t->w_gate, d->dim, es, d->hidden, t->w_up);
   m.up.prod[0].c = (void*)h;
-  m.up.gate_out = t->gate;
-  m.up.up_out = t->up;
+  m.up.prod[0].ldc = ld;
+  m.up.kept = kept_in(d, t->kept);
   m.up.act = d->activation;
   m.down.n_prod = 1;
   m.down.k = d->hidden;
-  m.down.prod[0].a = operand(h, d->hidden, es, d->rows);
+  m.down.prod[0].a = operand(h, ld, es, d->rows);
   m.down.prod[0].b = operand(t->w_down, d->hidden, es, d->out_dim);
   m.down.prod[0].c = t->y;
+  m.down.prod[0].ldc = d->out_dim;
   m.p_up = plan_tiles(m.up, kTileGated, d->dtype);
   m.p_down = plan_tiles(m.down, kTilePlain, d->dtype);
 }
-static void plan_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrads* g, void* dg, void* du, void* h, MlpPlan& m) {
+static void plan_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrads* g, void* dg, void* du, MlpPlan& m) {
   const size_t es = mlp_elem(d);
+  const int64_t ld = hidden_ld(d);
   m.grad.n_prod = 1;
   m.grad.k = d->out_dim;
   m.grad.prod[0].a = operand(g->dy, d->out_dim, es, d->rows);
   m.grad.prod[0].b = operand(t->w_down, d->hidden, es, d->hidden);
   m.grad.prod[0].c = dg;
-  m.grad.gate = t->gate;
-  m.grad.up = t->up;
-  m.grad.up_out = du;
-  m.grad.gate_out = g->dw_down ? h : nullptr;
+  m.grad.prod[0].ldc = ld;
+  m.grad.kept = kept_in(d, t->kept);
+  m.grad.c2 = du;
   m.grad.act = d->activation;
   m.p_grad = plan_tiles(m.grad, kTileGrad, d->dtype);
   m.dx.n_prod = 1;
   m.dx.k = d->hidden;
-  m.dx.prod[0].a = operand(dg, d->hidden, es, d->rows, du);
+  m.dx.prod[0].a = operand(dg, ld, es, d->rows, du);
   m.dx.prod[0].b = operand(t->w_gate, d->dim, es, d->dim, t->w_up);
   m.dx.prod[0].c = g->dx;
+  m.dx.prod[0].ldc = d->dim;
   m.p_dx = plan_tiles(m.dx, kTileTwice, d->dtype);
   m.dw.k = (int32_t)d->rows;
   auto add = [&](const TileOperand& a, const TileOperand& b, void* c) {
@@ -323,35 +350,36 @@ static void plan_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGr
     p.a = a;
     p.b = b;
     p.c = c;
+    p.ldc = b.rows;
   };
-  add(operand(dg, d->hidden, es, d->hidden), operand(t->x, d->x_stride, es, d->dim), g->dw_gate);
-  add(operand(du, d->hidden, es, d->hidden), operand(t->x, d->x_stride, es, d->dim), g->dw_up);
-  add(operand(g->dy, d->out_dim, es, d->out_dim), operand(h, d->hidden, es, d->hidden), g->dw_down);
+  add(operand(dg, ld, es, d->hidden), operand(t->x, d->x_stride, es, d->dim), g->dw_gate);
+  add(operand(du, ld, es, d->hidden), operand(t->x, d->x_stride, es, d->dim), g->dw_up);
+  add(operand(g->dy, d->out_dim, es, d->out_dim), operand(kept_h(d, t->kept), ld, es, d->hidden), g->dw_down);
   if (m.dw.n_prod) m.p_dw = plan_tiles(m.dw, kTilePlain, d->dtype);
 }
 static size_t most_of(size_t a, size_t b) { return a > b ? a : b; }
-static size_t rows_bytes(const PalMlpDims* d) { return round256((size_t)d->rows * d->hidden * mlp_elem(d)); }
 
 template <typename T>
 static int mlp_fwd(const PalMlpDims* d, const PalMlpTensors* t, char* ws, hipStream_t s) {
-  void* h = ws;
+  void* h = t->kept ? kept_h(d, t->kept) : ws;
   if (d->rows <= kFewRows) {
-    FewArgs up{t->x, t->w_gate, t->w_up, h, t->gate, t->up, d->x_stride, (int32_t)d->rows, d->hidden, d->dim, d->activation};
+    const int64_t ld = hidden_ld(d);
+    FewArgs up{t->x, t->w_gate, t->w_up, h, kept_in(d, t->kept), d->x_stride, ld, (int32_t)d->rows, d->hidden, d->dim, d->activation};
     if (int rc = few_launch<T, true>(up, s)) return rc;
-    FewArgs down{h, t->w_down, nullptr, t->y, nullptr, nullptr, d->hidden, (int32_t)d->rows, d->out_dim, d->hidden, 0};
+    FewArgs down{h, t->w_down, nullptr, t->y, Kept{}, ld, d->out_dim, (int32_t)d->rows, d->out_dim, d->hidden, 0};
     return few_launch<T, false>(down, s);
   }
   MlpPlan m;
   plan_fwd(d, t, h, m);
   if (int rc = tile_run<T, kTileGated, false, false>(m.up, m.p_up, nullptr, kKernMlpUp, s)) return rc;
-  return tile_run<T, kTilePlain, false, false>(m.down, m.p_down, (float*)(ws + rows_bytes(d)), kKernMlpDown, s);
+  return tile_run<T, kTilePlain, false, false>(m.down, m.p_down, (float*)(t->kept ? ws : ws + rows_bytes(d)), kKernMlpDown, s);
 }
 template <typename T>
 static int mlp_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrads* g, char* ws, hipStream_t s) {
   const size_t n = rows_bytes(d);
   MlpPlan m;
-  plan_bwd(d, t, g, ws, ws + n, ws + 2 * n, m);
-  float* part = (float*)(ws + 3 * n);
+  plan_bwd(d, t, g, ws, ws + n, m);
+  float* part = (float*)(ws + 2 * n);
   if (int rc = tile_run<T, kTileGrad, false, true>(m.grad, m.p_grad, part, kKernMlpGrad, s)) return rc;
   if (g->dx)
     if (int rc = tile_run<T, kTileTwice, false, true>(m.dx, m.p_dx, part, kKernMlpDx, s)) return rc;
@@ -361,23 +389,28 @@ static int mlp_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrad
 
 }  // namespace pal
 
-extern "C" size_t pal_gated_mlp_fwd_workspace_bytes(const PalMlpDims* d) {
+extern "C" size_t pal_gated_mlp_kept_bytes(const PalMlpDims* d) {
+  using namespace pal;
+  return check_mlp(d) == PAL_OK ? 3 * rows_bytes(d) : 0;
+}
+extern "C" size_t pal_gated_mlp_fwd_workspace_bytes(const PalMlpDims* d, int keeps) {
   using namespace pal;
   if (check_mlp(d) != PAL_OK) return 0;
-  if (d->rows <= kFewRows) return rows_bytes(d);
+  const size_t h = keeps ? 0 : rows_bytes(d);
+  if (d->rows <= kFewRows) return h;
   MlpPlan m;
   PalMlpTensors t{};
   plan_fwd(d, &t, nullptr, m);
-  return rows_bytes(d) + part_bytes(m.down, m.p_down);
+  return h + part_bytes(m.down, m.p_down);
 }
 extern "C" int pal_gated_mlp_fwd(const PalMlpDims* d, const PalMlpTensors* t, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace pal;
   if (int rc = check_mlp(d)) return rc;
   if (!t || !t->x || !t->w_gate || !t->w_up || !t->w_down || !t->y) return PAL_E_NULL;
-  if (!t->gate != !t->up) return PAL_E_STATE;
-  for (const void* p : {t->x, t->w_gate, t->w_up, t->w_down, (const void*)t->y, (const void*)t->gate, (const void*)t->up})
+  for (const void* p : {t->x, t->w_gate, t->w_up, t->w_down, (const void*)t->y, (const void*)t->kept})
     if (!is_aligned16(p)) return PAL_E_ALIGN;
-  if (!workspace || workspace_bytes < pal_gated_mlp_fwd_workspace_bytes(d)) return PAL_E_WORKSPACE;
+  const size_t need = pal_gated_mlp_fwd_workspace_bytes(d, t->kept != nullptr);
+  if (need && (!workspace || workspace_bytes < need)) return PAL_E_WORKSPACE;
   if (!is_aligned16(workspace)) return PAL_E_ALIGN;
   return d->dtype == PAL_DTYPE_BF16 ? mlp_fwd<bf16_t>(d, t, (char*)workspace, (hipStream_t)stream)
                                     : mlp_fwd<float>(d, t, (char*)workspace, (hipStream_t)stream);
@@ -395,18 +428,18 @@ extern "C" size_t pal_gated_mlp_bwd_workspace_bytes(const PalMlpDims* d) {
     g.dw_gate = which & 1 ? &any : nullptr;
     g.dw_up = which & 2 ? &any : nullptr;
     g.dw_down = which & 4 ? &any : nullptr;
-    plan_bwd(d, &t, &g, nullptr, nullptr, nullptr, m);
+    plan_bwd(d, &t, &g, nullptr, nullptr, m);
     part = most_of(part, most_of(part_bytes(m.grad, m.p_grad), most_of(part_bytes(m.dx, m.p_dx), part_bytes(m.dw, m.p_dw))));
   }
-  return 3 * rows_bytes(d) + part;
+  return 2 * rows_bytes(d) + part;
 }
 extern "C" int pal_gated_mlp_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrads* g, void* workspace, size_t workspace_bytes,
                                  void* stream) {
   using namespace pal;
   if (int rc = check_mlp(d)) return rc;
-  if (!t || !t->x || !t->w_gate || !t->w_up || !t->w_down || !t->gate || !t->up || !g || !g->dy) return PAL_E_NULL;
-  for (const void* p : {t->x, t->w_gate, t->w_up, t->w_down, (const void*)t->gate, (const void*)t->up, g->dy, (const void*)g->dx,
-                        (const void*)g->dw_gate, (const void*)g->dw_up, (const void*)g->dw_down})
+  if (!t || !t->x || !t->w_gate || !t->w_up || !t->w_down || !t->kept || !g || !g->dy) return PAL_E_NULL;
+  for (const void* p : {t->x, t->w_gate, t->w_up, t->w_down, (const void*)t->kept, g->dy, (const void*)g->dx, (const void*)g->dw_gate,
+                        (const void*)g->dw_up, (const void*)g->dw_down})
     if (!is_aligned16(p)) return PAL_E_ALIGN;
   if (!workspace || workspace_bytes < pal_gated_mlp_bwd_workspace_bytes(d)) return PAL_E_WORKSPACE;
   if (!is_aligned16(workspace)) return PAL_E_ALIGN;

@@ -689,11 +689,11 @@ struct MlpCall {
     t.x = ptr(x); t.w_gate = ptr(wg); t.w_up = ptr(wu); t.w_down = ptr(wd);
     return t;
   }
-  int run(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, Tensor& y, Tensor& gate, Tensor& up) const {
+  int run(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, Tensor& y, Tensor& kept) const {
     PalMlpTensors t = fill(x, wg, wu, wd);
     t.y = y.mutable_data_ptr();
-    if (gate.defined()) { t.gate = gate.mutable_data_ptr(); t.up = up.mutable_data_ptr(); }
-    const size_t bytes = abi.gated_mlp_fwd_workspace_bytes(&d);
+    t.kept = kept.defined() ? kept.mutable_data_ptr() : nullptr;
+    const size_t bytes = abi.gated_mlp_fwd_workspace_bytes(&d, kept.defined());
     Tensor ws = workspace(x, bytes);
     NoGil off;
     return abi.gated_mlp_fwd(&d, &t, ws.mutable_data_ptr(), bytes, stream_of(x.device()));
@@ -703,10 +703,10 @@ struct MlpCall {
 struct MlpNode : torch::autograd::Function<MlpNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t act) {
     MlpCall c(x, wg, wu, wd, act);
-    Tensor y = c.out(x), gate = at::empty({c.d.rows, c.d.hidden}, as(x, c.type)), up = at::empty({c.d.rows, c.d.hidden}, as(x, c.type));
-    const int rc = c.run(x, wg, wu, wd, y, gate, up);
+    Tensor y = c.out(x), kept = workspace(x, abi.gated_mlp_kept_bytes(&c.d));
+    const int rc = c.run(x, wg, wu, wd, y, kept);
     if (rc) fail(rc, "pal_gated_mlp_fwd");
-    ctx->save_for_backward({x, wg, wu, wd, gate, up});
+    ctx->save_for_backward({x, wg, wu, wd, kept});
     ctx->saved_data["act"] = act;
     for (int i = 0; i < 4; ++i) {
       const Tensor* t[] = {&x, &wg, &wu, &wd};
@@ -716,11 +716,10 @@ struct MlpNode : torch::autograd::Function<MlpNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list gr) {
     const auto s = ctx->get_saved_variables();
-    const Tensor &x = s[0], &gate = s[4], &up = s[5], none;
+    const Tensor &x = s[0], &kept = s[4], none;
     const c10::DeviceGuard guard(x.device());
     MlpCall c(x, s[1], s[2], s[3], ctx->saved_data["act"].toInt());
-    TORCH_CHECK_VALUE(c.ok && packed(gate, x.device(), c.type) && packed(up, x.device(), c.type) && gate.numel() == c.d.rows * c.d.hidden &&
-                          up.numel() == gate.numel(),
+    TORCH_CHECK_VALUE(c.ok && packed(kept, x.device(), at::kByte) && kept.numel() == (int64_t)abi.gated_mlp_kept_bytes(&c.d),
                       "gated_mlp backward: a saved tensor came back in another shape, dtype, layout or device");
     Tensor dy = gr[0].to(c.type).contiguous();
     if ((uintptr_t)ptr(dy) % 16) dy = dy.clone();
@@ -728,7 +727,7 @@ struct MlpNode : torch::autograd::Function<MlpNode> {
     for (int i = 0; i < 4; ++i)
       if (ctx->saved_data[std::string("need") + (char)('0' + i)].toBool()) out[i] = at::empty(s[i].sizes(), as(x, c.type));
     PalMlpTensors t = MlpCall::fill(x, s[1], s[2], s[3]);
-    t.gate = (void*)ptr(gate); t.up = (void*)ptr(up);
+    t.kept = (void*)ptr(kept);
     auto at_ = [](Tensor& o) { return o.defined() ? o.mutable_data_ptr() : nullptr; };
     PalMlpGrads g{ptr(dy), at_(out[0]), at_(out[1]), at_(out[2]), at_(out[3])};
     const size_t bytes = abi.gated_mlp_bwd_workspace_bytes(&c.d);
@@ -747,7 +746,7 @@ py::object gated_mlp(const Tensor& x, const Tensor& wg, const Tensor& wu, const 
   if (!c.ok) return py::none();
   if (any_grad({&x, &wg, &wu, &wd})) return applied([&] { return py::cast(MlpNode::apply(x, wg, wu, wd, act)); });
   Tensor y = c.out(x), none;
-  if (c.run(x, wg, wu, wd, y, none, none)) return py::none();
+  if (c.run(x, wg, wu, wd, y, none)) return py::none();
   return py::cast(y);
 }
 

@@ -50,8 +50,9 @@ struct Abi {
   int (*layer_norm_fwd)(const PalLayerNormDims*, const PalLayerNormTensors*, void*);
   int (*layer_norm_bwd)(const PalLayerNormDims*, const PalLayerNormTensors*, const PalLayerNormGrads*, void*, size_t, void*);
   size_t (*layer_norm_bwd_workspace_bytes)(const PalLayerNormDims*);
+  size_t (*gated_mlp_kept_bytes)(const PalMlpDims*);
   int (*gated_mlp_fwd)(const PalMlpDims*, const PalMlpTensors*, void*, size_t, void*);
-  size_t (*gated_mlp_fwd_workspace_bytes)(const PalMlpDims*);
+  size_t (*gated_mlp_fwd_workspace_bytes)(const PalMlpDims*, int);
   int (*gated_mlp_bwd)(const PalMlpDims*, const PalMlpTensors*, const PalMlpGrads*, void*, size_t, void*);
   size_t (*gated_mlp_bwd_workspace_bytes)(const PalMlpDims*);
 } abi;

@@ -34,11 +34,18 @@ struct TileOperand {
   int32_t rows;        // m or n
 };
 
+// What a forward pass keeps of the two factors g and u of a gated product, [rows][ld] each: of fp32 rows the numbers, of bf16 rows 16 bits a
+// number as well, but more exactly than in bf16 (see Kept8).
+struct Kept {
+  void *gate, *up;           // NULL: not kept
+};
+
 // up to three products over the same k in one launch
 struct TileProduct {
   TileOperand a, b;
-  void* c;             // [m][n], packed
+  void* c;             // [m][n], rows ldc numbers apart
   float* part;         // [splits][m][n] where k is split
+  int64_t ldc;
   int32_t first;       // its first tile
   int32_t tiles_n;
 };
@@ -49,16 +56,16 @@ struct TileArgs {
   int32_t tiles;       // all products'
   int32_t splits;      // of k, each of a whole number of steps
   int32_t split_steps;
-  // for the feed-forward block's kinds: rows [m][n] beside C
-  const void *gate, *up;
-  void *gate_out, *up_out;
+  // for the feed-forward block's kinds
+  Kept kept;
+  void* c2;            // [m][n] beside C, rows as far apart
   int32_t act;
 };
 
 enum TileKind {
   kTilePlain = 0,
   kTileGated,   // b has two matrices, half of a tile's columns from each: C = act(A B^T) (A B2^T), both factors kept beside it if asked
-  kTileGrad,    // D = A B^T is the gradient of such a C: from its factors the gradients of both (c, up_out) and C itself (gate_out)
+  kTileGrad,    // D = A B^T is the gradient of such a C: from its kept factors the gradients of both (c, c2)
   kTileTwice,   // A B^T + A2 B2^T
 };
 
@@ -132,6 +139,84 @@ __device__ __forceinline__ void tile_load8(const float* p, float* x) {
   for (int e = 0; e < 8; ++e) x[e] = e < 4 ? lo[e & 3] : hi[e & 3];
 }
 
+// eight neighbouring numbers as they are kept, from fp32 and back
+template <typename T>
+struct Kept8;
+template <>
+struct Kept8<float> {
+  f32x4 lo, hi;
+  __device__ __forceinline__ void load(const void* p, int64_t at) {
+    lo = *(const f32x4*)((const float*)p + at);
+    hi = *(const f32x4*)((const float*)p + at + 4);
+  }
+  __device__ __forceinline__ void get(float* x) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = e < 4 ? lo[e & 3] : hi[e & 3];
+  }
+  static __device__ __forceinline__ void store(void* p, int64_t at, const float* x) { tile_store8((float*)p + at, x); }
+};
+// Of bf16 rows: whole numbers of 15 bits times a power of two that the eight share, its eight bits spread over their words' lowest bits.  An
+// error of at most 2^-14 (for the largest 2^-13) of the largest of the eight, where bf16 would have up to 2^-9 of each: those alone would be
+// as large in the gradients as all the other roundings together.  Eight with an infinity or a NaN among them are kept as the upper 15 bits
+// of the fp32 numbers.
+template <>
+struct Kept8<bf16_t> {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 w;
+  __device__ __forceinline__ void load(const void* p, int64_t at) { w = *(const u32x4*)((const uint16_t*)p + at); }
+  __device__ __forceinline__ void get(float* x) const {
+    // the lowest bits of word i (0 .. 7) of the eight are bit i of the power
+    const unsigned b = (w[0] & 0x10001u) | (w[1] & 0x10001u) << 2 | (w[2] & 0x10001u) << 4 | (w[3] & 0x10001u) << 6;
+    const int code = (b | b >> 15) & 0xff;
+    if (code == 255) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[e] = __builtin_bit_cast(float, (e & 1 ? w[e >> 1] >> 17 : w[e >> 1] << 15 >> 16) << 17);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int field = e & 1 ? (int)w[e >> 1] >> 17 : (int)(w[e >> 1] << 16) >> 17;
+        x[e] = __builtin_ldexpf((float)field, code - 140);
+      }
+    }
+  }
+  static __device__ __forceinline__ void store(void* p, int64_t at, const float* x) {
+    unsigned most = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = max(most, __builtin_bit_cast(unsigned, x[e]) & 0x7fffffffu);
+    const int code = max((int)(most >> 23), 1);    // the largest is below 2^(code - 126)
+    unsigned f[8];
+    if (code == 255) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        f[e] = __builtin_bit_cast(unsigned, x[e]) >> 17;
+        if (x[e] != x[e]) f[e] |= 1;               // (a NaN whose upper bits are an infinity's)
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = (unsigned)min((int)__builtin_rintf(__builtin_ldexpf(x[e], 140 - code)), 16383) & 0x7fffu;
+    }
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = f[2 * i] << 1 | f[2 * i + 1] << 17 | (code >> (2 * i) & 1) | (code >> (2 * i + 1) & 1) << 16;
+    *(u32x4*)((uint16_t*)p + at) = w;
+  }
+};
+// dg and du of eight numbers of the gradient of h
+template <typename T>
+__device__ __forceinline__ void gated_grad8(int act, const float* dh, const Kept8<T>& gate, const Kept8<T>& up, float* dg, float* du) {
+  float g[8], u[8];
+  gate.get(g);
+  up.get(u);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float a, d;
+    activate<true>(act, g[e], a, d);
+    dg[e] = dh[e] * u[e] * d;
+    du[e] = dh[e] * a;
+  }
+}
+
 // row of a wave's part of an operand that entry j of fragment f stands for; PAIRS: two fragments share 32 rows (see above)
 template <bool PAIRS>
 __device__ __forceinline__ constexpr int frag_row(int f, int j) {
@@ -156,7 +241,7 @@ struct OperandWay {
   static constexpr int kBytes = ROWS * 128;
   static constexpr int kLoads = kBytes / 1024 / WAVES;                   // of a wave: 64 lanes of 16 bytes
   static constexpr int kLine = COLS ? ROWS * (int)sizeof(T) : 128;        // bytes of a row or a k
-  static_assert(kBytes % (1024 * WAVES) == 0 && (!COLS || kLine >= 256), "tile");
+  static_assert(kBytes % (1024 * WAVES) == 0 && (!COLS || kLine >= 256) && (!COLS || kLine % 256 == 0 || (PAIRS && kLine == 384)), "tile");
 
   // Lanes 0-3, 12-15, 20-23 and 24-27 of a 16-byte read meet in the banks, and so do the other half of 32 lanes; of an 8-byte transposing
   // read all 32.  (Taken as sixteen neighbours, the reads of a step were 8 cycles each instead of 4.)
@@ -165,7 +250,8 @@ struct OperandWay {
       const int q = (PAIRS ? line >> 3 : line >> 2) & 3;
       return (q >> 1) | ((q ^ (q >> 1)) & 1) << 1 | (line & 2) << 1;
     } else if constexpr (sizeof(T) == 2) {
-      return PAIRS ? 4 * (line & 3) : 2 * ((line & 3) | ((line >> 3) & 1) << 2);
+      if constexpr (kLine % 256) return 2 * (line & 2);   // (192 rows: every second line begins in the other half of the banks)
+      else return PAIRS ? 4 * (line & 3) : 2 * ((line & 3) | ((line >> 3) & 1) << 2);
     } else {
       return PAIRS ? ((line >> 2) & 1) | (line & 8) : 4 * ((line >> 2) & 3);
     }
@@ -388,61 +474,74 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_product_kernel(TileArgs 
 
   // a lane: row j of fragment m, columns 8 g .. of a pair of fragments n
   auto store_tile = [&](const TileProduct& pr, const Place& at_tile) {
-    const int M = pr.a.rows, N = pr.b.rows, n0 = at_tile.n0, split = at_tile.split;
-    const int j = lane & 15, g = lane >> 4, mw = at_tile.m0 + wave / WN * 16 * NFM;
+    const int M = pr.a.rows, N = pr.b.rows, split = at_tile.split;
+    const int j = lane & 15, g = lane >> 4, m0 = at_tile.m0 + wave / WN * 16 * NFM;
+    const int n0 = at_tile.n0 + wave % WN * (kCols / WN) + 8 * g;
+    if constexpr (KIND == kTileGrad) {
+      if (P.splits == 1) {
+        // the factors are on their way a fragment ahead of their use
+        Kept8<T> gate[2][NFN / 2], up[2][NFN / 2];
+        auto fetch = [&](int m) {
+          const int row = min(m0 + frag_row<false>(m, j), M - 1);
+#pragma unroll
+          for (int n = 0; n < NFN / 2; ++n) {
+            const int64_t at = row * pr.ldc + min(n0 + 32 * n, N - 8);
+            gate[m & 1][n].load(P.kept.gate, at);
+            up[m & 1][n].load(P.kept.up, at);
+          }
+        };
+        fetch(0);
+#pragma unroll
+        for (int m = 0; m < NFM; ++m) {
+          if (m + 1 < NFM) fetch(m + 1);
+          const int row = m0 + frag_row<false>(m, j);
+#pragma unroll
+          for (int n = 0; n < NFN / 2; ++n) {
+            float c[8], dg[8], du[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) c[e] = acc[m][2 * n + (e >> 2)][e & 3];
+            gated_grad8(P.act, c, gate[m & 1][n], up[m & 1][n], dg, du);
+            if (row < M && n0 + 32 * n < N) {
+              const int64_t at = row * pr.ldc + n0 + 32 * n;
+              tile_store8((T*)pr.c + at, dg);
+              tile_store8((T*)P.c2 + at, du);
+            }
+          }
+        }
+        return;
+      }
+    }
 #pragma unroll
     for (int m = 0; m < NFM; ++m) {
-      const int row = mw + frag_row<false>(m, j);
+      const int row = m0 + frag_row<false>(m, j);
       if (row >= M) continue;
       if constexpr (KIND == kTileGated) {
+        static_assert(KIND != kTileGated || NFN == 4, "a wave has 32 columns of each matrix");
+        if (n0 >= N) continue;
+        float gt[8], up[8], c[8], none;
 #pragma unroll
-        for (int n = 0; n < NFN; n += 4) {
-          const int col = n0 + wave % WN * 8 * NFN + 8 * n + 8 * g;
-          if (col >= N) continue;
-          float gt[8], up[8], c[8], none;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) gt[e] = acc[m][n + (e >> 2)][e & 3], up[e] = acc[m][n + 2 + (e >> 2)][e & 3];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            activate<false>(P.act, gt[e], c[e], none);
-            c[e] *= up[e];
-          }
-          const int64_t at = (int64_t)row * N + col;
-          tile_store8((T*)pr.c + at, c);
-          if (P.gate_out) {
-            tile_store8((T*)P.gate_out + at, gt);
-            tile_store8((T*)P.up_out + at, up);
-          }
+        for (int e = 0; e < 8; ++e) {
+          gt[e] = acc[m][e >> 2][e & 3];
+          up[e] = acc[m][2 + (e >> 2)][e & 3];
+          activate<false>(P.act, gt[e], c[e], none);
+          c[e] *= up[e];
+        }
+        const int64_t at = row * pr.ldc + n0;
+        tile_store8((T*)pr.c + at, c);
+        if (P.kept.gate) {
+          Kept8<T>::store(P.kept.gate, at, gt);
+          Kept8<T>::store(P.kept.up, at, up);
         }
       } else {
 #pragma unroll
-        for (int n = 0; n < NFN; n += 2) {
-          const int col = n0 + wave % WN * 16 * NFN + 16 * n + 8 * g;
+        for (int n = 0; n < NFN / 2; ++n) {
+          const int col = n0 + 32 * n;
           if (col >= N) continue;
           float c[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) c[e] = acc[m][n + (e >> 2)][e & 3];
-          const int64_t at = (int64_t)row * N + col;
-          if (P.splits > 1) {
-            tile_store8(pr.part + (int64_t)split * M * N + at, c);
-          } else if constexpr (KIND == kTileGrad) {
-            float gt[8], up[8], dg[8], du[8], h[8];
-            tile_load8((const T*)P.gate + at, gt);
-            tile_load8((const T*)P.up + at, up);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              float a, d;
-              activate<true>(P.act, gt[e], a, d);
-              dg[e] = c[e] * up[e] * d;
-              du[e] = c[e] * a;
-              h[e] = a * up[e];
-            }
-            tile_store8((T*)pr.c + at, dg);
-            tile_store8((T*)P.up_out + at, du);
-            if (P.gate_out) tile_store8((T*)P.gate_out + at, h);
-          } else {
-            tile_store8((T*)pr.c + at, c);
-          }
+          for (int e = 0; e < 8; ++e) c[e] = acc[m][2 * n + (e >> 2)][e & 3];
+          if (P.splits > 1) tile_store8(pr.part + ((int64_t)split * M + row) * N + col, c);
+          else tile_store8((T*)pr.c + row * pr.ldc + col, c);
         }
       }
     }

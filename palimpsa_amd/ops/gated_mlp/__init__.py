@@ -79,19 +79,17 @@ class GatedMlp(torch.autograd.Function):
         dims = L.PalMlpDims(rows=rows, x_stride=xs, dim=_up8(D), hidden=_up8(Fh), out_dim=_up8(Do), dtype=cm._pal_dtype(cd),
                             activation=L.PAL_ACT[activation])
         y = torch.empty((rows, _up8(Do)), dtype=cd, device=dev)
-        gate = up = None
-        if any(ctx.needs_input_grad):
-            gate, up = (torch.empty((rows, _up8(Fh)), dtype=cd, device=dev) for _ in range(2))
-        pt = cm._ptr
-        tens = L.PalMlpTensors(x=pt(xc), w_gate=pt(wg), w_up=pt(wu), w_down=pt(wd), y=pt(y), gate=pt(gate), up=pt(up))
         lib = L.load()
-        ws_bytes = int(lib.pal_gated_mlp_fwd_workspace_bytes(dims))
+        kept = torch.empty(int(lib.pal_gated_mlp_kept_bytes(dims)), dtype=torch.uint8, device=dev) if any(ctx.needs_input_grad) else None
+        pt = cm._ptr
+        tens = L.PalMlpTensors(x=pt(xc), w_gate=pt(wg), w_up=pt(wu), w_down=pt(wd), y=pt(y), kept=pt(kept))
+        ws_bytes = int(lib.pal_gated_mlp_fwd_workspace_bytes(dims, kept is not None))
         ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
             rc = lib.pal_gated_mlp_fwd(dims, tens, C.c_void_p(ws.data_ptr()), ws_bytes, cm.current_stream_ptr(dev))
         L.check(rc, "pal_gated_mlp_fwd")
-        if gate is not None:
-            ctx.save_for_backward(xc, wg, wu, wd, gate, up)
+        if kept is not None:
+            ctx.save_for_backward(xc, wg, wu, wd, kept)
             ctx.dims = dims
         return cm.unpad_last(y, Do).reshape(x.shape[:-1] + (Do,)).to(x.dtype)
 
@@ -101,13 +99,13 @@ class GatedMlp(torch.autograd.Function):
         shapes, dtypes, need = ctx.shapes, ctx.dtypes, ctx.needs_input_grad
         if ctx.dims is None:
             return tuple(torch.zeros(s, dtype=t, device=dy.device) if n else None for s, t, n in zip(shapes, dtypes, need)) + (None,)
-        xc, wg, wu, wd, gate, up = ctx.saved_tensors
+        xc, wg, wu, wd, kept = ctx.saved_tensors
         dims, dev, cd = ctx.dims, xc.device, xc.dtype
         d, _ = _rows(dy.reshape(dims.rows, shapes[3][0]).to(cd).contiguous(), cd)
         out = [torch.empty(s, dtype=cd, device=dev) if n else None
                for s, n in zip(((dims.rows, dims.dim), wg.shape, wu.shape, wd.shape), need)]
         pt = cm._ptr
-        tens = L.PalMlpTensors(x=pt(xc), w_gate=pt(wg), w_up=pt(wu), w_down=pt(wd), gate=pt(gate), up=pt(up))
+        tens = L.PalMlpTensors(x=pt(xc), w_gate=pt(wg), w_up=pt(wu), w_down=pt(wd), kept=pt(kept))
         grads = L.PalMlpGrads(dy=pt(d), dx=pt(out[0]), dw_gate=pt(out[1]), dw_up=pt(out[2]), dw_down=pt(out[3]))
         lib = L.load()
         ws_bytes = int(lib.pal_gated_mlp_bwd_workspace_bytes(dims))
@@ -129,8 +127,8 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     w_up ``[F, D]``, w_down ``[D_out, F]``; returns y ``[.., D_out]`` in the type of x.  ``activation``: "silu" (the reference's), "gelu",
     "gelu_tanh" (its form by a tanh) or "relu".
 
-    Gradients for x and the weights.  The product of the two projections is rounded once to the type of the rows between the kernels, with
-    gradients also each projection and its gradient; sums are in fp32.  Rows and weights all in bf16, or everything is computed from fp32.
+    Gradients for x and the weights.  The product of the two projections is rounded once to the type of the rows between the kernels, and so
+    are the gradients of the projections; sums are in fp32.  For the backward pass six bytes per row and hidden entry are kept of bf16 rows.  Rows and weights all in bf16, or everything is computed from fp32.
     Dims that are no multiple of eight are padded by a copy.  Up to 64 rows without tiles, bound by the reading of the weights."""
     if not torch.compiler.is_compiling() and x.is_cuda and activation in L.PAL_ACT:
         r = L.host().gated_mlp(x, w_gate, w_up, w_down, L.PAL_ACT[activation])

@@ -33,13 +33,17 @@ def gated_mlp(x, wg, wu, wd, act, dtype, dy=None):
     dy = dy.detach().double()
     dh = dy @ wd
     edh = Do * E32 * (dy.abs() @ ad)
-    eg, eu = eg + r * g.abs(), eu + r * u.abs()                    # g and u are kept in the rows' type
+    if dtype == torch.bfloat16:                                     # g and u are kept in steps of the largest of eight
+        def step(t):
+            n = -t.shape[1] % 8
+            top = torch.nn.functional.pad(t.abs(), (0, n)).reshape(M, -1, 8).amax(2, keepdim=True)
+            return 2.0 ** -13 * top.expand(-1, -1, 8).reshape(M, -1)[:, :t.shape[1]]
+        eg, eu = eg + step(g), eu + step(u)
     ea = slope * eg + g.abs() * (g.abs() + 8) * 2 * E32
     bend = 0.8                                                     # the largest second derivative
     ed = bend * eg + (1 + g.abs()) * (g.abs() + 8) * 4 * E32
     if act == "relu":
         ed = ed + (g.abs() <= eg).double()                         # its derivative jumps at 0
-    eh = ea * u.abs() + a.abs() * eu + h.abs() * (r + 2 * E32)
     dg, du = dh * u * d, dh * a
     edg = edh * (u * d).abs() + dh.abs() * (eu * d.abs() + u.abs() * ed) + dg.abs() * (r + 4 * E32)
     edu = edh * a.abs() + dh.abs() * ea + du.abs() * (r + 2 * E32)
