@@ -14,9 +14,10 @@
 // read at one time find sixteen different places among the banks.  (The direct loads write lane after lane, so the change is made to the
 // address that a lane reads from.)
 //
-// The 16 x 16 results are arranged so that a lane holds eight neighbouring columns of C of one row: a wave's fragment f of B is made of rows
-// 32 (f / 2) + 8 (j / 4) + 4 (f % 2) + j % 4, j < 16, of its part, and B stands first in the matrix instructions, so that its index runs
-// along a lane's four numbers.  Two fragments together are 16-byte stores without a turn through LDS.
+// The 16 x 16 results are arranged so that a lane holds eight neighbouring columns of C of one row, and two fragments together are 16-byte stores
+// without a turn through LDS.  B stands first in the matrix instructions, so that its index runs along a lane's four numbers.  Where B lies
+// in rows, its fragment f is made of rows 32 (f / 2) + 8 (j / 4) + 4 (f % 2) + j % 4, j < 16, of a wave's part; where it lies in columns such
+// fragments would be read at half the rate (pieces of 8 bytes, 16 apart), and neighbouring ones' results change places at the end instead.
 //
 // Whatever lies behind a matrix (rows behind the last one, k behind the end) is read as zero: by the bounds of the buffer for whole rows,
 // by an address beyond all bounds for the rest of a row.
@@ -241,7 +242,7 @@ struct OperandWay {
   static constexpr int kBytes = ROWS * 128;
   static constexpr int kLoads = kBytes / 1024 / WAVES;                   // of a wave: 64 lanes of 16 bytes
   static constexpr int kLine = COLS ? ROWS * (int)sizeof(T) : 128;        // bytes of a row or a k
-  static_assert(kBytes % (1024 * WAVES) == 0 && (!COLS || kLine >= 256) && (!COLS || kLine % 256 == 0 || (PAIRS && kLine == 384)), "tile");
+  static_assert(kBytes % (1024 * WAVES) == 0 && (!COLS || kLine >= 256) && (!COLS || (!PAIRS && (kLine % 256 == 0 || kLine == 384))), "tile");
 
   // Lanes 0-3, 12-15, 20-23 and 24-27 of a 16-byte read meet in the banks, and so do the other half of 32 lanes; of an 8-byte transposing
   // read all 32.  (Taken as sixteen neighbours, the reads of a step were 8 cycles each instead of 4.)
@@ -250,10 +251,10 @@ struct OperandWay {
       const int q = (PAIRS ? line >> 3 : line >> 2) & 3;
       return (q >> 1) | ((q ^ (q >> 1)) & 1) << 1 | (line & 2) << 1;
     } else if constexpr (sizeof(T) == 2) {
-      if constexpr (kLine % 256) return 2 * (line & 2);   // (192 rows: every second line begins in the other half of the banks)
-      else return PAIRS ? 4 * (line & 3) : 2 * ((line & 3) | ((line >> 3) & 1) << 2);
+      if constexpr (kLine % 256) return (line & 2) | ((line >> 3) & 1) << 2;   // (192 rows: every second line begins in the other half of the banks)
+      else return 2 * ((line & 3) | ((line >> 3) & 1) << 2);
     } else {
-      return PAIRS ? ((line >> 2) & 1) | (line & 8) : 4 * ((line >> 2) & 3);
+      return 4 * ((line >> 2) & 3);
     }
   }
 
@@ -301,7 +302,7 @@ struct OperandWay {
   static constexpr int kReads = NF * (!COLS ? 1 : sizeof(T) == 2 ? 2 : 4);   // of half a step, by a wave
 
   // places of a lane's fragments in a step
-  static constexpr int kPlaces = !COLS ? 2 : sizeof(T) == 2 && PAIRS ? NF / 2 : NF;
+  static constexpr int kPlaces = !COLS ? 2 : NF;
   uint32_t place_of[kPlaces];
   __device__ __forceinline__ void aim(int base, int lane) {
     const int j = lane & 15, g = lane >> 4;
@@ -312,7 +313,7 @@ struct OperandWay {
     } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
       for (int f = 0; f < kPlaces; ++f) {
-        const int k = 8 * g + (j >> 2), col = base + (PAIRS ? 32 * f + 8 * (j & 3) : 16 * f + 4 * (j & 3));
+        const int k = 8 * g + (j >> 2), col = base + 16 * f + 4 * (j & 3);
         place_of[f] = k * kLine + (((col >> 3) ^ swizzle(k)) * 16) + (col & 7) * 2;
       }
     } else {
@@ -329,7 +330,7 @@ struct OperandWay {
     } else {
       const char* p = step + half * (E::kStep / 2) * kLine;
       if constexpr (sizeof(T) == 2) {
-        p += PAIRS ? place_of[f >> 1] + 8 * (f & 1) : place_of[f];
+        p += place_of[f];
         return __builtin_bit_cast(f32x4, join(lds_read_tr((const bf16_t*)p), lds_read_tr((const bf16_t*)(p + 4 * kLine))));
       } else {
         p += place_of[f];
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_product_kernel(TileArgs 
   typedef TileType<T> E;
   constexpr int W = WM * WN, BM = 16 * NFM * WM, BN = 16 * NFN * WN;
   typedef OperandWay<T, ACOLS, BM, W, NFM, false, false> AWay;
-  typedef OperandWay<T, BCOLS, BN, W, NFN, true, KIND == kTileGated> BWay;
+  typedef OperandWay<T, BCOLS, BN, W, NFN, !BCOLS, KIND == kTileGated> BWay;
   constexpr uint32_t kStepBytes = AWay::kBytes + BWay::kBytes;
   constexpr int kLoads = AWay::kLoads + BWay::kLoads;
   extern __shared__ __attribute__((aligned(16))) char ring[];
@@ -475,6 +476,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_product_kernel(TileArgs 
   // a lane: row j of fragment m, columns 8 g .. of a pair of fragments n
   auto store_tile = [&](const TileProduct& pr, const Place& at_tile) {
     const int M = pr.a.rows, N = pr.b.rows, split = at_tile.split;
+    if constexpr (BCOLS) {
+      asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");   // the last products' results, which the compiler does not see the swaps read
+#pragma unroll
+      for (int m = 0; m < NFM; ++m)
+#pragma unroll
+        for (int n = 0; n < NFN; n += 2)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float a = acc[m][n][e], b = acc[m][n + 1][e];
+            swap_halves(a, b);
+            swap_rows(a, b);
+            acc[m][n][e] = a;
+            acc[m][n + 1][e] = b;
+          }
+    }
     const int j = lane & 15, g = lane >> 4, m0 = at_tile.m0 + wave / WN * 16 * NFM;
     const int n0 = at_tile.n0 + wave % WN * (kCols / WN) + 8 * g;
     if constexpr (KIND == kTileGrad) {
