@@ -5,8 +5,9 @@
 // multiplies by Wd.  Backward: dh is never stored, the kernel that computes it turns it into dg and du; the gradient of x is one walk over
 // both products, and the three of the weights are one launch (see tile_product.h).
 //
-// A call of few rows is bound by the weights, each of which is used once per 16 rows: few_rows_kernel has no tiles in LDS, the waves of a
-// workgroup walk over k side by side, each with a sixteenth of a line of the weights per lane straight from memory into the matrix units.
+// A call of few rows is bound by the weights: few_rows_kernel has no tiles in LDS, the waves of a workgroup walk over k side by side, weights and
+// rows straight from memory into the matrix units.  Up to 32 rows: beyond, the rows, which every workgroup reads, are more traffic than the
+// weights (2048 -> 5632 -> 2048, both launches: 24 us for 1 row, 30 for 17, 45 for 48), and small tiles with k in shares are faster (36).
 //
 // Roundings to the type of the rows: h, dg and du, once each, half a step of the type, as operands of the matrix units; g and u are kept more
 // exactly (Kept8); all sums are in fp32.  The errors in y and the gradients are then of the size of the rounding of those results themselves.
@@ -17,7 +18,7 @@
 
 namespace pal {
 
-constexpr int kFewRows = 64;
+constexpr int kFewRows = 32;
 
 // ------------------------------------------------------------------------------------------------------------ few rows
 struct FewArgs {
@@ -28,14 +29,13 @@ struct FewArgs {
   int32_t rows, n, k, act;
 };
 
-// W waves; R groups of sixteen rows of x
-template <typename T, bool GATED, int W, int R>
-__global__ __launch_bounds__(64 * W) void few_rows_kernel(FewArgs P) {
+// R groups of sixteen rows of x.  The waves of a workgroup (as many as it has) take spans of 128 bytes of k in turn, B of them in one go.
+template <typename T, bool GATED, int R, int B>
+__global__ __launch_bounds__(GATED ? 512 : 1024) void few_rows_kernel(FewArgs P) {
   typedef TileType<T> E;
-  constexpr int kMats = GATED ? 2 : 1, kPiece = E::kPiece, kSpan = 8 * kPiece;   // 128 bytes of each row at a time
-  constexpr int kBatch = 4;
-  __shared__ f32x4 s[W][kMats * R][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  constexpr int kMats = GATED ? 2 : 1, kPiece = E::kPiece, kSpan = 8 * kPiece;
+  extern __shared__ f32x4 shares[];                    // [waves][kMats * R][64]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int j = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
   const int64_t wrow = (int64_t)min(n0 + j, P.n - 1) * P.k;
   const T* w[2] = {(const T*)P.w + wrow, GATED ? (const T*)P.w2 + wrow : nullptr};
@@ -48,49 +48,53 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(FewArgs P) {
 #pragma unroll
     for (int r = 0; r < R; ++r) acc[m][r] = f32x4{0.f, 0.f, 0.f, 0.f};
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  for (int k0 = wave * kSpan; k0 < P.k; k0 += kBatch * W * kSpan) {
-    f32x4 wb[kBatch][2][kMats];
+  const int turn = waves * kSpan;
+  for (int k0 = wave * kSpan; k0 < P.k; k0 += B * turn) {
+    // a span beyond the end is the last one once more, and counts as zero
+    auto at = [&](int b, int h) { return min(k0 + b * turn + (4 * h + g) * kPiece, P.k - kPiece); };
+    f32x4 wb[B][2][kMats], xb[B][2][R];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b)
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < R; ++r) xb[b][h][r] = *(const f32x4*)(x[r] + at(b, h));
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int m = 0; m < kMats; ++m) wb[b][h][m] = *(const f32x4*)(w[m] + at(b, h));
+    __builtin_amdgcn_sched_barrier(0);                 // all of these are on their way before the first is waited for
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int k = k0 + b * W * kSpan + (2 * g + h) * kPiece;
+        const bool in = k0 + b * turn + (4 * h + g) * kPiece < P.k;
 #pragma unroll
-        for (int m = 0; m < kMats; ++m) wb[b][h][m] = *(const f32x4*)(w[m] + min(k, P.k - kPiece));
-      }
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      if (k0 + b * W * kSpan >= P.k) break;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int k = k0 + b * W * kSpan + (2 * g + h) * kPiece;
-        const bool in = k < P.k;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          f32x4 xb = *(const f32x4*)(x[r] + min(k, P.k - kPiece));
-          xb = in ? xb : zero;
-#pragma unroll
-          for (int m = 0; m < kMats; ++m) acc[m][r] = E::mma(in ? wb[b][h][m] : zero, xb, acc[m][r]);
-        }
+          for (int m = 0; m < kMats; ++m) acc[m][r] = E::mma(in ? wb[b][h][m] : zero, in ? xb[b][h][r] : zero, acc[m][r]);
       }
     }
   }
 #pragma unroll
   for (int m = 0; m < kMats; ++m)
 #pragma unroll
-    for (int r = 0; r < R; ++r) s[wave][m * R + r][lane] = acc[m][r];
+    for (int r = 0; r < R; ++r) shares[(wave * kMats * R + m * R + r) * 64 + lane] = acc[m][r];
   __syncthreads();
   // a thread: eight neighbouring columns of one row
-  for (int i = threadIdx.x; i < R * 32; i += 64 * W) {
+  for (int i = threadIdx.x; i < R * 32; i += blockDim.x) {
     const int r = i >> 5, l = (i & 15) | (i & 16) << 1, row = 16 * r + (l & 15), n = n0 + 4 * (l >> 4);
     float t[kMats][8];
 #pragma unroll
     for (int m = 0; m < kMats; ++m) {
-      f32x4 lo = s[0][m * R + r][l], hi = s[0][m * R + r][l + 16];
-#pragma unroll
-      for (int v = 1; v < W; ++v) {
-        lo += s[v][m * R + r][l];
-        hi += s[v][m * R + r][l + 16];
+      f32x4 lo = zero, hi = zero;
+#pragma unroll 4
+      for (int v = 0; v < waves; ++v) {
+        const f32x4* s = shares + (v * kMats * R + m * R + r) * 64 + l;
+        lo += s[0];
+        hi += s[16];
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) t[m][e] = e < 4 ? lo[e & 3] : hi[e & 3];
@@ -98,12 +102,10 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(FewArgs P) {
     if (row >= P.rows || n >= P.n) continue;
     const int64_t at = row * P.out_ld + n;
     if constexpr (GATED) {
-      float c[8], none;
+      float c[8];
+      activate8<false>(P.act, t[0], c, nullptr);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        activate<false>(P.act, t[0][e], c[e], none);
-        c[e] *= t[1][e];
-      }
+      for (int e = 0; e < 8; ++e) c[e] *= t[1][e];
       tile_store8((T*)P.out + at, c);
       if (P.kept.gate) {
         Kept8<T>::store(P.kept.gate, at, t[0]);
@@ -127,32 +129,48 @@ struct JoinArgs {
   void* c2;
   int32_t act;
 };
-template <typename T, bool GRAD>
+template <typename T, int KIND>
 __global__ __launch_bounds__(256) void tile_join_kernel(JoinArgs P) {
+  constexpr int kMats = KIND == kTileGated ? 2 : 1;
   const int which = blockIdx.y;
   const int64_t n = P.n[which];
+  const uint32_t row8 = P.row8[which];
   for (int64_t from = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; from < n; from += (int64_t)gridDim.x * 256 * 8) {
-    float c[8];
-    tile_load8(P.part[which] + from, c);
-#pragma unroll 4
-    for (int s = 1; s < P.splits; ++s) {
-      float b[8];
-      tile_load8(P.part[which] + s * n + from, b);
+    const uint32_t piece = (uint32_t)(from >> 3), row = piece / row8, col = 8 * (piece - row * row8);   // (the host joins no more than 2^32 pieces)
+    float c[kMats][8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) c[e] += b[e];
+    for (int m = 0; m < kMats; ++m) {
+      const float* part = P.part[which] + from + (KIND == kTileGated ? ((int64_t)row + m) * (8 * (int64_t)row8) : 0);
+      tile_load8(part, c[m]);
+#pragma unroll 4
+      for (int s = 1; s < P.splits; ++s) {
+        float b[8];
+        tile_load8(part + s * kMats * n, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[m][e] += b[e];
+      }
     }
-    const uint32_t piece = (uint32_t)(from >> 3), row = piece / P.row8[which];   // (the host joins no more than 2^32 pieces)
-    const int64_t at = row * P.ldc[which] + 8 * (int64_t)(piece - row * P.row8[which]);
-    if constexpr (GRAD) {
+    const int64_t at = row * P.ldc[which] + col;
+    if constexpr (KIND == kTileGrad) {
       Kept8<T> gate, up;
       float dg[8], du[8];
       gate.load(P.kept.gate, at);
       up.load(P.kept.up, at);
-      gated_grad8(P.act, c, gate, up, dg, du);
+      gated_grad8(P.act, c[0], gate, up, dg, du);
       tile_store8((T*)P.out[which] + at, dg);
       tile_store8((T*)P.c2 + at, du);
+    } else if constexpr (KIND == kTileGated) {
+      float h[8];
+      activate8<false>(P.act, c[0], h, nullptr);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] *= c[1][e];
+      tile_store8((T*)P.out[which] + at, h);
+      if (P.kept.gate) {
+        Kept8<T>::store(P.kept.gate, at, c[0]);
+        Kept8<T>::store(P.kept.up, at, c[1]);
+      }
     } else {
-      tile_store8((T*)P.out[which] + at, c);
+      tile_store8((T*)P.out[which] + at, c[0]);
     }
   }
 }
@@ -163,9 +181,9 @@ __global__ __launch_bounds__(256) void tile_join_kernel(JoinArgs P) {
 enum TileForm { kTileBig = 0, kTileNarrow, kTileSmall, kTileForms };
 struct TileShape {
   int m, n, slots;   // of the chip
-  double step_us;    // time of a step of bf16 numbers while every slot has a tile
+  double bf16_us, fp32_us;   // time of a step while every slot has a tile
 };
-constexpr TileShape kTileShapes[kTileForms] = {{256, 256, 256, 1.65}, {256, 192, 256, 1.35}, {128, 128, 512, 1.0}};
+constexpr TileShape kTileShapes[kTileForms] = {{256, 256, 256, 1.65, 7.4}, {256, 192, 256, 1.35, 5.6}, {128, 128, 512, 1.0, 3.8}};
 struct TilePlan {
   int form, tiles, splits, split_steps;
 };
@@ -177,8 +195,8 @@ static TilePlan plan_tiles(const TileArgs& P, int kind, int dtype) {
   double least = 1e30;
   const int per = dtype == PAL_DTYPE_BF16 ? 64 : 32, one = (P.k + per - 1) / per, steps = kind == kTileTwice ? 2 * one : one;
   double numbers = 0;
-  for (int i = 0; i < P.n_prod; ++i) numbers += (double)P.prod[i].a.rows * P.prod[i].b.rows;
-  const int most = kind == kTileGated || numbers > 3e10 ? 1 : 32;   // shares: gated tiles have none, and the join counts pieces in 32 bits
+  for (int i = 0; i < P.n_prod; ++i) numbers += (double)P.prod[i].a.rows * P.prod[i].b.rows * (kind == kTileGated ? 2 : 1);
+  const int most = numbers > 3e10 ? 1 : 32;   // shares (the join counts pieces in 32 bits)
   for (int form = 0; form < kTileForms; ++form) {
     if (form == kTileNarrow && kind == kTileGated) continue;
     const TileShape& t = kTileShapes[form];
@@ -187,7 +205,7 @@ static TilePlan plan_tiles(const TileArgs& P, int kind, int dtype) {
     for (int i = 0; i < P.n_prod; ++i)
       tiles += (int64_t)((P.prod[i].a.rows + t.m - 1) / t.m) * ((P.prod[i].b.rows + tn - 1) / tn);
     if (tiles > 1 << 24) continue;
-    const double step = t.step_us * (dtype == PAL_DTYPE_BF16 ? 1 : 5.5);
+    const double step = dtype == PAL_DTYPE_BF16 ? t.bf16_us : t.fp32_us;
     for (int s = 1; s <= most && s <= steps; ++s) {
       const int share = (steps + s - 1) / s, splits = (steps + share - 1) / share;
       if (splits != s) continue;
@@ -214,11 +232,11 @@ static int tile_launch(const TileArgs& P, int id, hipStream_t s) {
 }
 
 static size_t round256(size_t n) { return (n + 255) & ~(size_t)255; }
-static size_t part_bytes(const TileArgs& P, const TilePlan& plan) {
+static size_t part_bytes(const TileArgs& P, const TilePlan& plan, int kind) {
   if (plan.splits < 2) return 0;
   size_t n = 0;
   for (int i = 0; i < P.n_prod; ++i) n += (size_t)P.prod[i].a.rows * P.prod[i].b.rows;
-  return round256(n * sizeof(float) * plan.splits);
+  return round256(n * sizeof(float) * plan.splits * (kind == kTileGated ? 2 : 1));
 }
 
 // the launches of one set of products; `part`: part_bytes of them
@@ -244,7 +262,7 @@ static int tile_run(TileArgs P, const TilePlan& plan, float* part, int id, hipSt
     J.row8[i] = p.b.rows / 8;
     J.n[i] = (int64_t)p.a.rows * p.b.rows;
     most = J.n[i] > most ? J.n[i] : most;
-    if (part) part += J.n[i] * plan.splits;
+    if (part) part += J.n[i] * plan.splits * (KIND == kTileGated ? 2 : 1);
   }
   int rc = PAL_OK;
   if (plan.form == kTileBig) rc = tile_launch<T, KIND, ACOLS, BCOLS, 2, 4, 8, 4>(P, id, s);
@@ -253,22 +271,30 @@ static int tile_run(TileArgs P, const TilePlan& plan, float* part, int id, hipSt
   if (rc || plan.splits < 2) return rc;
   J.splits = plan.splits; J.kept = P.kept; J.c2 = P.c2; J.act = P.act;
   const int64_t blocks = (most + 2047) / 2048;
-  PAL_TIMED_LAUNCH(kKernTileJoin, s, (tile_join_kernel<T, KIND == kTileGrad>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), P.n_prod),
+  PAL_TIMED_LAUNCH(kKernTileJoin, s, (tile_join_kernel<T, KIND>), dim3((unsigned)(blocks < 4096 ? blocks : 4096), P.n_prod),
                    dim3(256), 0, s, J);
   PAL_HIP_LAUNCH_CHECK();
   return PAL_OK;
 }
 
-template <typename T, bool GATED>
-static int few_launch(const FewArgs& P, hipStream_t s) {
-  const dim3 grid((P.n + 15) / 16);
+template <typename T, bool GATED, int R>
+static int few_launch_rows(const FewArgs& P, hipStream_t s) {
+  // spans that a wave takes in one go: 1, 2 or 4, so that the most waves that a workgroup may have take all of k if they can
+  constexpr int kMost = GATED ? 8 : 16;
+  const int spans = (P.k + 8 * TileType<T>::kPiece - 1) / (8 * TileType<T>::kPiece), each = (spans + kMost - 1) / kMost;
+  const int b = each <= 1 ? 1 : each <= 2 ? 2 : 4, rounds = (spans + b * kMost - 1) / (b * kMost), waves = (spans + b * rounds - 1) / (b * rounds);
+  const dim3 grid((P.n + 15) / 16), block(64 * waves);
+  const size_t lds = (size_t)waves * (GATED ? 2 : 1) * R * 64 * sizeof(f32x4);
   const int id = GATED ? kKernMlpFewUp : kKernMlpFewDown;
-  constexpr int W = GATED ? 8 : 16;
-  if (P.rows <= 16) PAL_TIMED_LAUNCH(id, s, (few_rows_kernel<T, GATED, W, 1>), grid, dim3(64 * W), 0, s, P);
-  else if (P.rows <= 32) PAL_TIMED_LAUNCH(id, s, (few_rows_kernel<T, GATED, 8, 2>), grid, dim3(64 * 8), 0, s, P);
-  else PAL_TIMED_LAUNCH(id, s, (few_rows_kernel<T, GATED, 8, 4>), grid, dim3(64 * 8), 0, s, P);
+  if (b == 1) PAL_TIMED_LAUNCH(id, s, (few_rows_kernel<T, GATED, R, 1>), grid, block, lds, s, P);
+  else if (b == 2) PAL_TIMED_LAUNCH(id, s, (few_rows_kernel<T, GATED, R, 2>), grid, block, lds, s, P);
+  else PAL_TIMED_LAUNCH(id, s, (few_rows_kernel<T, GATED, R, 4>), grid, block, lds, s, P);
   PAL_HIP_LAUNCH_CHECK();
   return PAL_OK;
+}
+template <typename T, bool GATED>
+static int few_launch(const FewArgs& P, hipStream_t s) {
+  return P.rows <= 16 ? few_launch_rows<T, GATED, 1>(P, s) : few_launch_rows<T, GATED, 2>(P, s);
 }
 
 static int check_mlp(const PalMlpDims* d) {
@@ -371,8 +397,9 @@ static int mlp_fwd(const PalMlpDims* d, const PalMlpTensors* t, char* ws, hipStr
   }
   MlpPlan m;
   plan_fwd(d, t, h, m);
-  if (int rc = tile_run<T, kTileGated, false, false>(m.up, m.p_up, nullptr, kKernMlpUp, s)) return rc;
-  return tile_run<T, kTilePlain, false, false>(m.down, m.p_down, (float*)(t->kept ? ws : ws + rows_bytes(d)), kKernMlpDown, s);
+  float* part = (float*)(t->kept ? ws : ws + rows_bytes(d));
+  if (int rc = tile_run<T, kTileGated, false, false>(m.up, m.p_up, part, kKernMlpUp, s)) return rc;
+  return tile_run<T, kTilePlain, false, false>(m.down, m.p_down, part, kKernMlpDown, s);
 }
 template <typename T>
 static int mlp_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrads* g, char* ws, hipStream_t s) {
@@ -401,7 +428,7 @@ extern "C" size_t pal_gated_mlp_fwd_workspace_bytes(const PalMlpDims* d, int kee
   MlpPlan m;
   PalMlpTensors t{};
   plan_fwd(d, &t, nullptr, m);
-  return h + part_bytes(m.down, m.p_down);
+  return h + most_of(part_bytes(m.up, m.p_up, kTileGated), part_bytes(m.down, m.p_down, kTilePlain));
 }
 extern "C" int pal_gated_mlp_fwd(const PalMlpDims* d, const PalMlpTensors* t, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace pal;
@@ -429,7 +456,7 @@ extern "C" size_t pal_gated_mlp_bwd_workspace_bytes(const PalMlpDims* d) {
     g.dw_up = which & 2 ? &any : nullptr;
     g.dw_down = which & 4 ? &any : nullptr;
     plan_bwd(d, &t, &g, nullptr, nullptr, m);
-    part = most_of(part, most_of(part_bytes(m.grad, m.p_grad), most_of(part_bytes(m.dx, m.p_dx), part_bytes(m.dw, m.p_dw))));
+    part = most_of(part, most_of(part_bytes(m.grad, m.p_grad, kTileGrad), most_of(part_bytes(m.dx, m.p_dx, kTileTwice), part_bytes(m.dw, m.p_dw, kTilePlain))));
   }
   return 2 * rows_bytes(d) + part;
 }

@@ -45,7 +45,7 @@ struct Kept {
 struct TileProduct {
   TileOperand a, b;
   void* c;             // [m][n], rows ldc numbers apart
-  float* part;         // [splits][m][n] where k is split
+  float* part;         // [splits][m][n] where k is split (kTileGated: [splits][m][2 n], the first matrix' columns and then the second's)
   int64_t ldc;
   int32_t first;       // its first tile
   int32_t tiles_n;
@@ -74,28 +74,57 @@ enum TileKind {
 enum { kActSilu = PAL_ACT_SILU, kActGelu = PAL_ACT_GELU, kActGeluTanh = PAL_ACT_GELU_TANH, kActRelu = PAL_ACT_RELU };
 
 __device__ __forceinline__ float act_logistic(float x) { return fast_rcp(1.f + __expf(-x)); }
-// a = act(g), d = act'(g)
 template <bool GRAD>
-__device__ __forceinline__ void activate(int act, float g, float& a, float& d) {
+__device__ __forceinline__ void act_silu(float g, float& a, float& d) {
+  const float f = act_logistic(g);
+  a = g * f;
+  if (GRAD) d = f * fmaf(g, 1.f - f, 1.f);
+}
+template <bool GRAD>
+__device__ __forceinline__ void act_gelu(float g, float& a, float& d) {
+  const float f = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+  a = g * f;
+  if (GRAD) d = fmaf(g * 0.39894228040143268f, __expf(-0.5f * g * g), f);
+}
+template <bool GRAD>
+__device__ __forceinline__ void act_gelu_tanh(float g, float& a, float& d) {
+  // (1 + tanh(z / 2)) / 2 is the logistic function of z
+  const float g2 = g * g, f = act_logistic(1.5957691216057308f * g * fmaf(0.044715f, g2, 1.f));
+  a = g * f;
+  if (GRAD) {
+    const float s = f * (1.f - f);
+    d = s > 0.f ? fmaf(1.5957691216057308f * g * s, fmaf(0.134145f, g2, 1.f), f) : f;   // (no 0 times infinity far out)
+  }
+}
+template <bool GRAD>
+__device__ __forceinline__ void act_relu(float g, float& a, float& d) {
+  a = g < 0.f ? 0.f : g;   // (a NaN stays)
+  if (GRAD) d = g > 0.f ? 1.f : 0.f;
+}
+// a = act(g), d = act'(g) of eight; one branch for all of them
+template <bool GRAD>
+__device__ __forceinline__ void activate8(int act, const float* g, float* a, float* d) {
   if (act == kActSilu) {
-    const float f = act_logistic(g);
-    a = g * f;
-    if (GRAD) d = f * fmaf(g, 1.f - f, 1.f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) act_silu<GRAD>(g[e], a[e], d[e]);
   } else if (act == kActGelu) {
-    const float f = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-    a = g * f;
-    if (GRAD) d = fmaf(g * 0.39894228040143268f, __expf(-0.5f * g * g), f);
-  } else if (act == kActGeluTanh) {
-    // (1 + tanh(z / 2)) / 2 is the logistic function of z
-    const float g2 = g * g, f = act_logistic(1.5957691216057308f * g * fmaf(0.044715f, g2, 1.f));
-    a = g * f;
-    if (GRAD) {
-      const float s = f * (1.f - f);
-      d = s > 0.f ? fmaf(1.5957691216057308f * g * s, fmaf(0.134145f, g2, 1.f), f) : f;   // (no 0 times infinity far out)
+#pragma unroll 1
+    for (int e = 0; e < 8; e += 4) {   // (erf is long)
+      float x[4], y[4], z[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[i] = e ? g[4 + i] : g[i];
+        act_gelu<GRAD>(x[i], y[i], z[i]);
+        (e ? a[4 + i] : a[i]) = y[i];
+        if (GRAD) (e ? d[4 + i] : d[i]) = z[i];
+      }
     }
+  } else if (act == kActGeluTanh) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) act_gelu_tanh<GRAD>(g[e], a[e], d[e]);
   } else {
-    a = g < 0.f ? 0.f : g;   // (a NaN stays)
-    if (GRAD) d = g > 0.f ? 1.f : 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) act_relu<GRAD>(g[e], a[e], d[e]);
   }
 }
 
@@ -156,50 +185,49 @@ struct Kept8<float> {
   }
   static __device__ __forceinline__ void store(void* p, int64_t at, const float* x) { tile_store8((float*)p + at, x); }
 };
-// Of bf16 rows: whole numbers of 15 bits times a power of two that the eight share, its eight bits spread over their words' lowest bits.  An
-// error of at most 2^-14 (for the largest 2^-13) of the largest of the eight, where bf16 would have up to 2^-9 of each: those alone would be
-// as large in the gradients as all the other roundings together.  Eight with an infinity or a NaN among them are kept as the upper 15 bits
-// of the fp32 numbers.
+// Of bf16 rows: whole numbers of 16 bits times a power of two that the eight share, whose eight bits stand in their lowest bits.  An error of at
+// most 2^-13 of the largest of the eight, where bf16 would have up to 2^-8 of each: those alone would be as large in the gradients as all
+// the other roundings together.  Eight with an infinity or a NaN among them are kept as the upper 15 bits of the fp32 numbers.
 template <>
 struct Kept8<bf16_t> {
   typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   u32x4 w;
   __device__ __forceinline__ void load(const void* p, int64_t at) { w = *(const u32x4*)((const uint16_t*)p + at); }
   __device__ __forceinline__ void get(float* x) const {
-    // the lowest bits of word i (0 .. 7) of the eight are bit i of the power
-    const unsigned b = (w[0] & 0x10001u) | (w[1] & 0x10001u) << 2 | (w[2] & 0x10001u) << 4 | (w[3] & 0x10001u) << 6;
-    const int code = (b | b >> 15) & 0xff;
+    // the lowest bits of numbers 2 i and 2 i + 1 are bits i and 4 + i of the power
+    const unsigned b = (w[0] & 0x10001u) | (w[1] & 0x10001u) << 1 | (w[2] & 0x10001u) << 2 | (w[3] & 0x10001u) << 3;
+    const int code = (b | b >> 12) & 0xff;
     if (code == 255) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        x[e] = __builtin_bit_cast(float, (e & 1 ? w[e >> 1] >> 17 : w[e >> 1] << 15 >> 16) << 17);
+        x[e] = __builtin_bit_cast(float, e & 1 ? w[e >> 1] & 0xfffe0000u : (w[e >> 1] & 0xfffeu) << 16);
     } else {
+      const float unit = __builtin_ldexpf(1.f / 32767.f, code - 126);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int field = e & 1 ? (int)w[e >> 1] >> 17 : (int)(w[e >> 1] << 16) >> 17;
-        x[e] = __builtin_ldexpf((float)field, code - 140);
-      }
+      for (int e = 0; e < 8; ++e) x[e] = (float)(e & 1 ? (int)w[e >> 1] >> 16 : (int)(short)w[e >> 1]) * unit;
     }
   }
   static __device__ __forceinline__ void store(void* p, int64_t at, const float* x) {
     unsigned most = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) most = max(most, __builtin_bit_cast(unsigned, x[e]) & 0x7fffffffu);
-    const int code = max((int)(most >> 23), 1);    // the largest is below 2^(code - 126)
-    unsigned f[8];
+    for (int e = 0; e < 8; ++e) most = max(most, __builtin_bit_cast(unsigned, x[e]) << 1);   // (a NaN is above an infinity)
+    const int code = max((int)(most >> 24), 1);    // the largest is below 2^(code - 126)
+    u32x4 w;
     if (code == 255) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        f[e] = __builtin_bit_cast(unsigned, x[e]) >> 17;
-        if (x[e] != x[e]) f[e] |= 1;               // (a NaN whose upper bits are an infinity's)
+      for (int i = 0; i < 4; ++i) {
+        unsigned a = __builtin_bit_cast(unsigned, x[2 * i]), b = __builtin_bit_cast(unsigned, x[2 * i + 1]);
+        if (x[2 * i] != x[2 * i]) a |= 0x20000u;    // (a NaN whose upper bits are an infinity's)
+        if (x[2 * i + 1] != x[2 * i + 1]) b |= 0x20000u;
+        w[i] = a >> 16 | (b & 0xffff0000u);
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = (unsigned)min((int)__builtin_rintf(__builtin_ldexpf(x[e], 140 - code)), 16383) & 0x7fffu;
+      for (int i = 0; i < 4; ++i)
+        w[i] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_i16(__builtin_ldexpf(x[2 * i], 126 - code), __builtin_ldexpf(x[2 * i + 1], 126 - code)));
     }
-    u32x4 w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = f[2 * i] << 1 | f[2 * i + 1] << 17 | (code >> (2 * i) & 1) | (code >> (2 * i + 1) & 1) << 16;
+    for (int i = 0; i < 4; ++i) w[i] = (w[i] & 0xfffefffeu) | (code >> i & 1) | (code >> (4 + i) & 1) << 16;
     *(u32x4*)((uint16_t*)p + at) = w;
   }
 };
@@ -209,12 +237,12 @@ __device__ __forceinline__ void gated_grad8(int act, const float* dh, const Kept
   float g[8], u[8];
   gate.get(g);
   up.get(u);
+  float a[8], d[8];
+  activate8<true>(act, g, a, d);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    float a, d;
-    activate<true>(act, g[e], a, d);
-    dg[e] = dh[e] * u[e] * d;
-    du[e] = dh[e] * a;
+    dg[e] = dh[e] * u[e] * d[e];
+    du[e] = dh[e] * a[e];
   }
 }
 
@@ -534,14 +562,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_product_kernel(TileArgs 
       if constexpr (KIND == kTileGated) {
         static_assert(KIND != kTileGated || NFN == 4, "a wave has 32 columns of each matrix");
         if (n0 >= N) continue;
-        float gt[8], up[8], c[8], none;
+        float gt[8], up[8], c[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           gt[e] = acc[m][e >> 2][e & 3];
           up[e] = acc[m][2 + (e >> 2)][e & 3];
-          activate<false>(P.act, gt[e], c[e], none);
-          c[e] *= up[e];
         }
+        if (P.splits > 1) {
+          float* part = pr.part + ((int64_t)split * M + row) * (2 * (int64_t)N) + n0;
+          tile_store8(part, gt);
+          tile_store8(part + N, up);
+          continue;
+        }
+        activate8<false>(P.act, gt, c, nullptr);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e] *= up[e];
         const int64_t at = row * pr.ldc + n0;
         tile_store8((T*)pr.c + at, c);
         if (P.kept.gate) {
