@@ -177,13 +177,18 @@ __global__ __launch_bounds__(256) void tile_join_kernel(JoinArgs P) {
 
 // ---------------------------------------------------------------------------------------------------------------- host
 // Tiles that the products are made of: 256 x 256 and, for matrices whose columns fill the chip better so, 256 x 192 by eight waves, one
-// workgroup a compute unit; 128 x 128 by four, two of them, where there are few tiles.
-enum TileForm { kTileBig = 0, kTileNarrow, kTileSmall, kTileForms };
+// workgroup a compute unit; 128 x 128 by four, two of them, where there are few tiles; of fp32 rows 64 x 64 (64 x 128 of gated products).
+// Products of bf16 rows are bound by the reads and writes of LDS, of which a large tile has less per number; those of fp32 rows by the matrix units,
+// whose share of a compute unit a tile of any size uses in full: they take the tiles that spread best, and a unit's tiles count one by one.
+enum TileForm { kTileBig = 0, kTileNarrow, kTileSmall, kTileTiny, kTileForms };
 struct TileShape {
-  int m, n, slots;   // of the chip
-  double bf16_us, fp32_us;   // time of a step while every slot has a tile
+  int m, n, slots;           // of the chip, bf16 rows
+  double bf16_us, fp32_us;   // time of a step: while every slot has a tile; of one tile that has a compute unit's matrix units
 };
-constexpr TileShape kTileShapes[kTileForms] = {{256, 256, 256, 1.65, 7.4}, {256, 192, 256, 1.35, 5.6}, {128, 128, 512, 1.0, 3.8}};
+constexpr TileShape kTileShapes[kTileForms] = {{256, 256, 256, 1.65, 7.4}, {256, 192, 256, 1.35, 5.6}, {128, 128, 512, 1.0, 1.95}, {64, 64, 0, 0, 0.52}};
+constexpr int tile_cols(int form, int kind) {   // of C
+  return kind == kTileGated ? (form == kTileTiny ? 64 : kTileShapes[form].n / 2) : kTileShapes[form].n;
+}
 struct TilePlan {
   int form, tiles, splits, split_steps;
 };
@@ -198,18 +203,18 @@ static TilePlan plan_tiles(const TileArgs& P, int kind, int dtype) {
   for (int i = 0; i < P.n_prod; ++i) numbers += (double)P.prod[i].a.rows * P.prod[i].b.rows * (kind == kTileGated ? 2 : 1);
   const int most = numbers > 3e10 ? 1 : 32;   // shares (the join counts pieces in 32 bits)
   for (int form = 0; form < kTileForms; ++form) {
-    if (form == kTileNarrow && kind == kTileGated) continue;
+    if ((form == kTileNarrow && kind == kTileGated) || (form == kTileTiny && dtype == PAL_DTYPE_BF16)) continue;
     const TileShape& t = kTileShapes[form];
-    const int tn = kind == kTileGated ? t.n / 2 : t.n;
+    const int tn = tile_cols(form, kind), slots = dtype == PAL_DTYPE_BF16 ? t.slots : 256;
     int64_t tiles = 0;
     for (int i = 0; i < P.n_prod; ++i)
       tiles += (int64_t)((P.prod[i].a.rows + t.m - 1) / t.m) * ((P.prod[i].b.rows + tn - 1) / tn);
     if (tiles > 1 << 24) continue;
-    const double step = dtype == PAL_DTYPE_BF16 ? t.bf16_us : t.fp32_us;
+    const double step = dtype == PAL_DTYPE_BF16 ? t.bf16_us : t.fp32_us * (kind == kTileGated && form == kTileTiny ? 2 : 1);
     for (int s = 1; s <= most && s <= steps; ++s) {
       const int share = (steps + s - 1) / s, splits = (steps + share - 1) / share;
       if (splits != s) continue;
-      const double rounds = (double)((tiles * s + t.slots - 1) / t.slots);
+      const double rounds = (double)((tiles * s + slots - 1) / slots);
       const double us = rounds * share * step + 3 + (s > 1 ? 4 + numbers * s * (4 / 3.5e6 + 4 / 1e7) : 0);
       if (us < least) {
         least = us;
@@ -223,7 +228,7 @@ static TilePlan plan_tiles(const TileArgs& P, int kind, int dtype) {
 template <typename T, int KIND, bool ACOLS, bool BCOLS, int WM, int WN, int NFM, int NFN>
 static int tile_launch(const TileArgs& P, int id, hipStream_t s) {
   constexpr size_t lds = (size_t)2 * 128 * 16 * (NFM * WM + NFN * WN);
-  constexpr int slots = lds > kMaxLds / 2 ? 256 : 512;   // workgroups that the chip holds at a time
+  constexpr int slots = 256 * (lds > kMaxLds / 2 ? 1 : lds > kMaxLds / 4 ? 2 : 4);   // workgroups that the chip holds at a time
   const auto kernel = &tile_product_kernel<T, KIND, ACOLS, BCOLS, WM, WN, NFM, NFN>;
   if (int rc = allow_lds((const void*)kernel, lds)) return rc;
   PAL_TIMED_LAUNCH(id, s, (*kernel), dim3(P.tiles * P.splits < slots ? P.tiles * P.splits : slots), dim3(64 * WM * WN), lds, s, P);
@@ -243,7 +248,7 @@ static size_t part_bytes(const TileArgs& P, const TilePlan& plan, int kind) {
 template <typename T, int KIND, bool ACOLS, bool BCOLS>
 static int tile_run(TileArgs P, const TilePlan& plan, float* part, int id, hipStream_t s) {
   if (!plan.tiles) return PAL_E_DIM;
-  const int t = kTileShapes[plan.form].m, tn = KIND == kTileGated ? kTileShapes[plan.form].n / 2 : kTileShapes[plan.form].n;
+  const int t = kTileShapes[plan.form].m, tn = tile_cols(plan.form, KIND);
   P.tiles = plan.tiles;
   P.splits = plan.splits;
   P.split_steps = plan.split_steps;
@@ -267,7 +272,11 @@ static int tile_run(TileArgs P, const TilePlan& plan, float* part, int id, hipSt
   int rc = PAL_OK;
   if (plan.form == kTileBig) rc = tile_launch<T, KIND, ACOLS, BCOLS, 2, 4, 8, 4>(P, id, s);
   else if (plan.form == kTileSmall) rc = tile_launch<T, KIND, ACOLS, BCOLS, 2, 2, 4, 4>(P, id, s);
-  else if constexpr (KIND != kTileGated) rc = tile_launch<T, KIND, ACOLS, BCOLS, 4, 2, 4, 6>(P, id, s);
+  else if (plan.form == kTileTiny) {
+    if constexpr (sizeof(T) == 4) rc = tile_launch<T, KIND, ACOLS, BCOLS, 2, 2, 2, KIND == kTileGated ? 4 : 2>(P, id, s);
+  } else if constexpr (KIND != kTileGated) {
+    rc = tile_launch<T, KIND, ACOLS, BCOLS, 4, 2, 4, 6>(P, id, s);
+  }
   if (rc || plan.splits < 2) return rc;
   J.splits = plan.splits; J.kept = P.kept; J.c2 = P.c2; J.act = P.act;
   const int64_t blocks = (most + 2047) / 2048;
