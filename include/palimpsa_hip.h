@@ -612,7 +612,7 @@ size_t pal_gated_mlp_kept_bytes(const PalMlpDims *dims);
 size_t pal_gated_mlp_fwd_workspace_bytes(const PalMlpDims *dims, int keeps); /* keeps: with t->kept */
 int pal_gated_mlp_fwd(const PalMlpDims *dims, const PalMlpTensors *t, void *workspace, size_t workspace_bytes, void *stream);
 /* Backward: t as in the forward call, with kept as that call left it; t->y is not touched. */
-size_t pal_gated_mlp_bwd_workspace_bytes(const PalMlpDims *dims);
+size_t pal_gated_mlp_bwd_workspace_bytes(const PalMlpDims *dims, const PalMlpGrads *gr); /* gr: as in the call (which gradients are wanted) */
 int pal_gated_mlp_bwd(const PalMlpDims *dims, const PalMlpTensors *t, const PalMlpGrads *gr, void *workspace,
                       size_t workspace_bytes, void *stream);
 

@@ -226,6 +226,7 @@ def load() -> C.CDLL:
         fn.restype = C.c_size_t
         fn.argtypes = [P(PalMlpDims)]
     lib.pal_gated_mlp_fwd_workspace_bytes.argtypes = [P(PalMlpDims), C.c_int]
+    lib.pal_gated_mlp_bwd_workspace_bytes.argtypes = [P(PalMlpDims), P(PalMlpGrads)]
     lib.pal_gated_mlp_fwd.restype = lib.pal_gated_mlp_bwd.restype = C.c_int
     lib.pal_gated_mlp_fwd.argtypes = [P(PalMlpDims), P(PalMlpTensors), C.c_void_p, C.c_size_t, C.c_void_p]
     lib.pal_gated_mlp_bwd.argtypes = [P(PalMlpDims), P(PalMlpTensors), P(PalMlpGrads), C.c_void_p, C.c_size_t, C.c_void_p]

@@ -211,7 +211,8 @@ static TilePlan plan_tiles(const TileArgs& P, int kind, int dtype) {
       tiles += (int64_t)((P.prod[i].a.rows + t.m - 1) / t.m) * ((P.prod[i].b.rows + tn - 1) / tn);
     if (tiles > 1 << 24) continue;
     const double step = dtype == PAL_DTYPE_BF16 ? t.bf16_us : t.fp32_us * (kind == kTileGated && form == kTileTiny ? 2 : 1);
-    for (int s = 1; s <= most && s <= steps; ++s) {
+    // (no more shares than fill the chip a few times)
+    for (int s = 1; s <= most && s <= steps && (s == 1 || tiles * s <= 8 * (int64_t)slots); ++s) {
       const int share = (steps + s - 1) / s, splits = (steps + share - 1) / share;
       if (splits != s) continue;
       const double rounds = (double)((tiles * s + slots - 1) / slots);
@@ -377,7 +378,7 @@ static void plan_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGr
   m.dx.prod[0].b = operand(t->w_gate, d->dim, es, d->dim, t->w_up);
   m.dx.prod[0].c = g->dx;
   m.dx.prod[0].ldc = d->dim;
-  m.p_dx = plan_tiles(m.dx, kTileTwice, d->dtype);
+  if (g->dx) m.p_dx = plan_tiles(m.dx, kTileTwice, d->dtype);
   m.dw.k = (int32_t)d->rows;
   auto add = [&](const TileOperand& a, const TileOperand& b, void* c) {
     if (!c) return;
@@ -451,23 +452,14 @@ extern "C" int pal_gated_mlp_fwd(const PalMlpDims* d, const PalMlpTensors* t, vo
   return d->dtype == PAL_DTYPE_BF16 ? mlp_fwd<bf16_t>(d, t, (char*)workspace, (hipStream_t)stream)
                                     : mlp_fwd<float>(d, t, (char*)workspace, (hipStream_t)stream);
 }
-extern "C" size_t pal_gated_mlp_bwd_workspace_bytes(const PalMlpDims* d) {
+extern "C" size_t pal_gated_mlp_bwd_workspace_bytes(const PalMlpDims* d, const PalMlpGrads* g) {
   using namespace pal;
-  if (check_mlp(d) != PAL_OK) return 0;
-  // enough for every choice of gradients
-  size_t part = 0;
-  for (int which = 0; which < 8; ++which) {
-    MlpPlan m;
-    PalMlpTensors t{};
-    PalMlpGrads g{};
-    char any;
-    g.dw_gate = which & 1 ? &any : nullptr;
-    g.dw_up = which & 2 ? &any : nullptr;
-    g.dw_down = which & 4 ? &any : nullptr;
-    plan_bwd(d, &t, &g, nullptr, nullptr, m);
-    part = most_of(part, most_of(part_bytes(m.grad, m.p_grad, kTileGrad), most_of(part_bytes(m.dx, m.p_dx, kTileTwice), part_bytes(m.dw, m.p_dw, kTilePlain))));
-  }
-  return 2 * rows_bytes(d) + part;
+  if (check_mlp(d) != PAL_OK || !g) return 0;
+  MlpPlan m;
+  PalMlpTensors t{};
+  plan_bwd(d, &t, g, nullptr, nullptr, m);
+  const size_t part = most_of(part_bytes(m.dx, m.p_dx, kTileTwice), part_bytes(m.dw, m.p_dw, kTilePlain));
+  return 2 * rows_bytes(d) + most_of(part_bytes(m.grad, m.p_grad, kTileGrad), part);
 }
 extern "C" int pal_gated_mlp_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrads* g, void* workspace, size_t workspace_bytes,
                                  void* stream) {
@@ -477,7 +469,7 @@ extern "C" int pal_gated_mlp_bwd(const PalMlpDims* d, const PalMlpTensors* t, co
   for (const void* p : {t->x, t->w_gate, t->w_up, t->w_down, (const void*)t->kept, g->dy, (const void*)g->dx, (const void*)g->dw_gate,
                         (const void*)g->dw_up, (const void*)g->dw_down})
     if (!is_aligned16(p)) return PAL_E_ALIGN;
-  if (!workspace || workspace_bytes < pal_gated_mlp_bwd_workspace_bytes(d)) return PAL_E_WORKSPACE;
+  if (!workspace || workspace_bytes < pal_gated_mlp_bwd_workspace_bytes(d, g)) return PAL_E_WORKSPACE;
   if (!is_aligned16(workspace)) return PAL_E_ALIGN;
   return d->dtype == PAL_DTYPE_BF16 ? mlp_bwd<bf16_t>(d, t, g, (char*)workspace, (hipStream_t)stream)
                                     : mlp_bwd<float>(d, t, g, (char*)workspace, (hipStream_t)stream);

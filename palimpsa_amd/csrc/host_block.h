@@ -730,7 +730,7 @@ struct MlpNode : torch::autograd::Function<MlpNode> {
     t.kept = (void*)ptr(kept);
     auto at_ = [](Tensor& o) { return o.defined() ? o.mutable_data_ptr() : nullptr; };
     PalMlpGrads g{ptr(dy), at_(out[0]), at_(out[1]), at_(out[2]), at_(out[3])};
-    const size_t bytes = abi.gated_mlp_bwd_workspace_bytes(&c.d);
+    const size_t bytes = abi.gated_mlp_bwd_workspace_bytes(&c.d, &g);
     Tensor ws = workspace(x, bytes);
     int rc;
     { NoGil off; rc = abi.gated_mlp_bwd(&c.d, &t, &g, ws.mutable_data_ptr(), bytes, stream_of(x.device())); }

@@ -54,7 +54,7 @@ struct Abi {
   int (*gated_mlp_fwd)(const PalMlpDims*, const PalMlpTensors*, void*, size_t, void*);
   size_t (*gated_mlp_fwd_workspace_bytes)(const PalMlpDims*, int);
   int (*gated_mlp_bwd)(const PalMlpDims*, const PalMlpTensors*, const PalMlpGrads*, void*, size_t, void*);
-  size_t (*gated_mlp_bwd_workspace_bytes)(const PalMlpDims*);
+  size_t (*gated_mlp_bwd_workspace_bytes)(const PalMlpDims*, const PalMlpGrads*);
 } abi;
 py::handle raise_code;   // (code, where): raises what the Python routes raise for a code of the library
 

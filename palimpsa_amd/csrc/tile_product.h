@@ -523,28 +523,30 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_product_kernel(TileArgs 
     const int n0 = at_tile.n0 + wave % WN * (kCols / WN) + 8 * g;
     if constexpr (KIND == kTileGrad) {
       if (P.splits == 1) {
-        // the factors are on their way a fragment ahead of their use
-        Kept8<T> gate[2][NFN / 2], up[2][NFN / 2];
+        // The factors are on their way kAhead fragments ahead of their use: a wait for them is one for the stores that went out before them.
+        constexpr int kAhead = sizeof(T) == 2 ? 2 : 1;
+        Kept8<T> gate[kAhead + 1][NFN / 2], up[kAhead + 1][NFN / 2];
         auto fetch = [&](int m) {
           const int row = min(m0 + frag_row<false>(m, j), M - 1);
 #pragma unroll
           for (int n = 0; n < NFN / 2; ++n) {
             const int64_t at = row * pr.ldc + min(n0 + 32 * n, N - 8);
-            gate[m & 1][n].load(P.kept.gate, at);
-            up[m & 1][n].load(P.kept.up, at);
+            gate[m % (kAhead + 1)][n].load(P.kept.gate, at);
+            up[m % (kAhead + 1)][n].load(P.kept.up, at);
           }
         };
-        fetch(0);
+#pragma unroll
+        for (int m = 0; m < kAhead && m < NFM; ++m) fetch(m);
 #pragma unroll
         for (int m = 0; m < NFM; ++m) {
-          if (m + 1 < NFM) fetch(m + 1);
+          if (m + kAhead < NFM) fetch(m + kAhead);
           const int row = m0 + frag_row<false>(m, j);
 #pragma unroll
           for (int n = 0; n < NFN / 2; ++n) {
             float c[8], dg[8], du[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) c[e] = acc[m][2 * n + (e >> 2)][e & 3];
-            gated_grad8(P.act, c, gate[m & 1][n], up[m & 1][n], dg, du);
+            gated_grad8(P.act, c, gate[m % (kAhead + 1)][n], up[m % (kAhead + 1)][n], dg, du);
             if (row < M && n0 + 32 * n < N) {
               const int64_t at = row * pr.ldc + n0 + 32 * n;
               tile_store8((T*)pr.c + at, dg);
@@ -629,6 +631,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_product_kernel(TileArgs 
       go_on();
     }
     store_tile(pr, at);
+    if constexpr (KIND == kTileGrad) {                   // (its registers are needed there: the operands are read again)
+      read_b(b_first, slot, 0);
+      read_a(a_low, slot, 0, 0);
+    }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // loads into LDS do not outlive the workgroup
 }

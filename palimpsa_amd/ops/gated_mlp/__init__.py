@@ -108,7 +108,7 @@ class GatedMlp(torch.autograd.Function):
         tens = L.PalMlpTensors(x=pt(xc), w_gate=pt(wg), w_up=pt(wu), w_down=pt(wd), kept=pt(kept))
         grads = L.PalMlpGrads(dy=pt(d), dx=pt(out[0]), dw_gate=pt(out[1]), dw_up=pt(out[2]), dw_down=pt(out[3]))
         lib = L.load()
-        ws_bytes = int(lib.pal_gated_mlp_bwd_workspace_bytes(dims))
+        ws_bytes = int(lib.pal_gated_mlp_bwd_workspace_bytes(dims, grads))
         ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
         with torch.cuda.device(dev):
             rc = lib.pal_gated_mlp_bwd(dims, tens, grads, C.c_void_p(ws.data_ptr()), ws_bytes, cm.current_stream_ptr(dev))

@@ -115,8 +115,10 @@ def test_gated_mlp_entry_points_refuse(L):
 
 def test_gated_mlp_sizes(L):
     lib = L.load()
-    for name in ("pal_gated_mlp_kept_bytes", "pal_gated_mlp_bwd_workspace_bytes"):
-        assert getattr(lib, name)(_mlp_dims(L)) > 0 and getattr(lib, name)(_mlp_dims(L, dim=5)) == 0
+    assert lib.pal_gated_mlp_kept_bytes(_mlp_dims(L)) > 0 and lib.pal_gated_mlp_kept_bytes(_mlp_dims(L, dim=5)) == 0
+    some = L.PalMlpGrads(dy=P, dw_up=P)
+    assert lib.pal_gated_mlp_bwd_workspace_bytes(_mlp_dims(L), some) >= 2 * 64 * 128 * 2 and lib.pal_gated_mlp_bwd_workspace_bytes(_mlp_dims(L, dim=5), some) == 0
+    assert lib.pal_gated_mlp_bwd_workspace_bytes(_mlp_dims(L), None) == 0
     assert lib.pal_gated_mlp_fwd_workspace_bytes(_mlp_dims(L, hidden=5), 0) == 0
     # rows of h an odd number of 128-byte lines apart, three arrays of them kept
     assert lib.pal_gated_mlp_kept_bytes(_mlp_dims(L, rows=16, hidden=2048)) == 3 * 16 * (4096 + 128)

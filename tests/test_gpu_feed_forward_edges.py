@@ -258,8 +258,8 @@ def test_nothing_is_written_around_the_results(gpu_device, dtype, rows, dim, hid
         n = lib.pal_gated_mlp_fwd_workspace_bytes(d, keep)
         t = L.PalMlpTensors(**base, y=room(rows * out * es), kept=kept if keep else None)
         assert lib.pal_gated_mlp_fwd(d, t, room(n), n, s) == 0
-    n = lib.pal_gated_mlp_bwd_workspace_bytes(d)
     g = L.PalMlpGrads(dy=cm._ptr(dy), dx=room(rows * dim * es), dw_gate=room(hidden * dim * es), dw_up=room(hidden * dim * es), dw_down=room(out * hidden * es))
+    n = lib.pal_gated_mlp_bwd_workspace_bytes(d, g)
     assert lib.pal_gated_mlp_bwd(d, L.PalMlpTensors(**base, kept=kept), g, room(n), n, s) == 0
     nd = L.PalLayerNormDims(rows=rows, x_stride=dim, res_stride=dim, dim=dim, dtype=dtype, res_dtype=0, weight_dtype=0, eps=1e-5, drop=L.PalDropout(p=0.5, seed=1))
     w = torch.ones(dim, device=dev)
