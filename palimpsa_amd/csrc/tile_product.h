@@ -185,12 +185,14 @@ struct Kept8<float> {
   }
   static __device__ __forceinline__ void store(void* p, int64_t at, const float* x) { tile_store8((float*)p + at, x); }
 };
-// Of bf16 rows: whole numbers of 16 bits times a power of two that the eight share, whose eight bits stand in their lowest bits.  An error of at
-// most 2^-13 of the largest of the eight, where bf16 would have up to 2^-8 of each: those alone would be as large in the gradients as all
-// the other roundings together.  Eight with an infinity or a NaN among them are kept as the upper 15 bits of the fp32 numbers.
+// Of bf16 rows: fp16 numbers, less their lowest bits, times a power of two that eight share, whose eight bits stand in those: the largest of the
+// eight is put just below 2^15.  An error of at most 2^-10 of a number, down to 2^-29 of the largest (there 2^-38 of it), where bf16 would have
+// up to 2^-8: those alone would be as large in the gradients as all the other roundings together.  Zero and the sign stay what they are (the derivative
+// at 0).  Eight with an infinity or a NaN among them are kept as the upper 15 bits of the fp32 numbers.
 template <>
 struct Kept8<bf16_t> {
   typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
   u32x4 w;
   __device__ __forceinline__ void load(const void* p, int64_t at) { w = *(const u32x4*)((const uint16_t*)p + at); }
   __device__ __forceinline__ void get(float* x) const {
@@ -202,9 +204,9 @@ struct Kept8<bf16_t> {
       for (int e = 0; e < 8; ++e)
         x[e] = __builtin_bit_cast(float, e & 1 ? w[e >> 1] & 0xfffe0000u : (w[e >> 1] & 0xfffeu) << 16);
     } else {
-      const float unit = __builtin_ldexpf(1.f / 32767.f, code - 126);
+      const float unit = __builtin_ldexpf(1.f, code - 141);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (float)(e & 1 ? (int)w[e >> 1] >> 16 : (int)(short)w[e >> 1]) * unit;
+      for (int e = 0; e < 8; ++e) x[e] = (float)__builtin_bit_cast(f16x2, w[e >> 1] & 0xfffefffeu)[e & 1] * unit;
     }
   }
   static __device__ __forceinline__ void store(void* p, int64_t at, const float* x) {
@@ -223,8 +225,8 @@ struct Kept8<bf16_t> {
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_i16(__builtin_ldexpf(x[2 * i], 126 - code), __builtin_ldexpf(x[2 * i + 1], 126 - code)));
+      for (int i = 0; i < 4; ++i)   // cut off at the lowest bit, and rounded at the one above it, away from zero halfway
+        w[i] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(__builtin_ldexpf(x[2 * i], 141 - code), __builtin_ldexpf(x[2 * i + 1], 141 - code))) + 0x10001u;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = (w[i] & 0xfffefffeu) | (code >> i & 1) | (code >> (4 + i) & 1) << 16;

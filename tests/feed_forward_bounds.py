@@ -33,11 +33,13 @@ def gated_mlp(x, wg, wu, wd, act, dtype, dy=None):
     dy = dy.detach().double()
     dh = dy @ wd
     edh = Do * E32 * (dy.abs() @ ad)
-    if dtype == torch.bfloat16:                                     # g and u are kept in steps of the largest of eight
+    # g and u are kept with nine bits after the leading one, rounded to the nearest: half a step is at most 2^-10 of the number; where that is
+    # below fp16's 2^-14, the largest of its eight being 2^14 or more, half a step is 2^-24, 2^-38 of the largest
+    if dtype == torch.bfloat16:
         def step(t):
             n = -t.shape[1] % 8
             top = torch.nn.functional.pad(t.abs(), (0, n)).reshape(M, -1, 8).amax(2, keepdim=True)
-            return 2.0 ** -13 * top.expand(-1, -1, 8).reshape(M, -1)[:, :t.shape[1]]
+            return 2.0 ** -10 * t.abs() + 2.0 ** -38 * top.expand(-1, -1, 8).reshape(M, -1)[:, :t.shape[1]]
         eg, eu = eg + step(g), eu + step(u)
     ea = slope * eg + g.abs() * (g.abs() + 8) * 2 * E32
     bend = 0.8                                                     # the largest second derivative

@@ -208,6 +208,44 @@ def test_a_hidden_entry_that_is_not_finite_keeps_its_neighbours_exact(gpu_device
     fb.within(dwu[rest], val["w_up"], tol["w_up"] + extra[rest], "dw_up")
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("M", [9, 200])
+def test_a_large_hidden_entry_keeps_its_neighbours_exact(gpu_device, dtype, M):
+    """Hidden entries thousands of times as large as those beside them: each entry's gradients stand in proportion to itself."""
+    from palimpsa_amd.ops.gated_mlp import gated_mlp
+    x, wg, wu, wd, dy = make(gpu_device, M, 64, 64, 64, dtype)
+    wg[3] *= 300
+    wu[3], wu[20], wu[21] = wu[3] * 5000, wu[20] * 2e6, wu[21] * 1e-6
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    grads = torch.autograd.grad(gated_mlp(*leaves), leaves, dy)
+    val, tol = fb.gated_mlp(x, wg, wu, wd, "silu", dtype, dy)
+    for got, name in zip(grads, ("x", "w_gate", "w_up", "w_down")):
+        fb.within(got, val[name], tol[name], name)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("M", [9, 200])
+def test_zero_factors_have_the_derivative_at_zero(gpu_device, dtype, M):
+    """Weights that begin as zeros, whole and in part: relu passes no gradient at zero, silu half of it."""
+    from palimpsa_amd.ops.gated_mlp import gated_mlp
+    x, wg, wu, wd, dy = make(gpu_device, M, 64, 96, 64, dtype)
+    for rows in (slice(0, 96), slice(5, 96, 2)):
+        wz = wg.clone()
+        wz[rows] = 0
+        for act in ("relu", "silu"):
+            leaves = [t.detach().clone().requires_grad_(True) for t in (x, wz, wu, wd)]
+            dx, dwg, dwu, dwd = torch.autograd.grad(gated_mlp(*leaves, act), leaves, dy)
+            assert not dwu[rows].any() and not dwd[:, rows].any()
+            if act == "relu":
+                assert not dwg[rows].any()
+                if rows == slice(0, 96):
+                    assert not dx.any()
+            val, tol = fb.gated_mlp(x, wz, wu, wd, act, dtype, dy)
+            for got, name in zip((dx, dwg, dwu, dwd), ("x", "w_gate", "w_up", "w_down")):
+                if act == "silu":          # (the bound takes relu's jump at zero for an error)
+                    fb.within(got, val[name], tol[name], name)
+
+
 def test_dropped_entries_are_zero_whatever_they_held(gpu_device):
     from palimpsa_amd.ops.layer_glue import dropout, residual_layer_norm
     x = _randn(gpu_device, 64, 96, dtype=BF)
