@@ -529,13 +529,13 @@ typedef struct PalDropout {
   uint32_t site;          /* number of the place in a model: sites share a seed    */
 } PalDropout;
 
-/* y = dropout(x) of `rows` rows of dim entries, those of x x_stride apart, those of y packed; dtype PAL_DTYPE_*; x and y may be the same.  The gradient is the
- * same call on the gradient. */
+/* y = dropout(x) of `rows` rows of dim entries (up to 2^30; 2^46 in all), those of x x_stride apart, those of y packed; dtype PAL_DTYPE_*.  x and y may be the
+ * same buffer if x is packed as well.  The gradient is the same call on the gradient. */
 int pal_dropout(const PalDropout *drop, const void *x, void *y, int64_t rows, int64_t dim, int64_t x_stride, int32_t dtype, void *stream);
 
 /* Layer norm, alone or as the pre-norm between two blocks with the residual's addition and a dropout in front of it:
  *   s = dropout(x) + residual, rounded to res_dtype and handed on;  y = (s - mean(s)) r * weight + bias,  r = 1 / sqrt(mean((s - mean(s))^2) + eps)
- * Rows of any length up to 16384 at any element's address. */
+ * Rows of any length up to 16384 at any element's address.  No result may overlap an operand or another result. */
 typedef struct PalLayerNormDims {
   int64_t rows;
   int64_t x_stride;     /* elements between rows of x (>= dim); every other row tensor is packed, but: */
@@ -577,7 +577,8 @@ int pal_layer_norm_bwd(const PalLayerNormDims *dims, const PalLayerNormTensors *
 
 /* The second half of a block (fla.modules.GatedMLP of the reference's PalimpsaBlock, restated from its published behaviour):
  *   g = x w_gate^T,  u = x w_up^T,  h = act(g) u,  y = h w_down^T
- * Dims are multiples of 8 and every pointer is 16-byte aligned (callers with other sizes pad with zeros). */
+ * Dims are multiples of 8 and every pointer is 16-byte aligned (callers with other sizes pad with zeros).  No result may overlap an operand or
+ * another result. */
 #define PAL_ACT_SILU 0       /* g sigmoid(g)                                     */
 #define PAL_ACT_GELU 1       /* g (1 + erf(g / sqrt 2)) / 2                      */
 #define PAL_ACT_GELU_TANH 2  /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 */

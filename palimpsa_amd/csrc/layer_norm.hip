@@ -428,15 +428,13 @@ extern "C" int pal_dropout(const PalDropout* drop, const void* x, void* y, int64
   if (int rc = drop_args(*drop, A.drop)) return rc;
   A.x = x; A.y = y; A.stride = x_stride; A.dim = (uint32_t)dim;
   A.per_row = (uint32_t)((dim + 7) / 8);
+  if (rows > ((int64_t)1 << 43) / A.per_row) return PAL_E_DIM;
   A.pieces = rows * A.per_row;
   A.magic = (uint32_t)((((uint64_t)1 << 32) + A.per_row - 1) / A.per_row);
   const int64_t each = A.pieces / (256 * 2048);
   A.turns = each < 1 ? 1 : each > 8 ? 8 : (int)each;
   const int64_t blocks = (A.pieces + 256 * A.turns - 1) / (256 * A.turns);
-  if (blocks > 1 << 23) {   // threads of a launch: more turns
-    A.turns = (int)((A.pieces + ((int64_t)256 << 23) - 1) / ((int64_t)256 << 23));
-    if (A.turns > 1 << 20) return PAL_E_DIM;
-  }
+  if (blocks > 1 << 23) A.turns = (int)((A.pieces + ((int64_t)256 << 23) - 1) / ((int64_t)256 << 23));   // threads of a launch: more turns
   const dim3 grid((unsigned)((A.pieces + (int64_t)256 * A.turns - 1) / ((int64_t)256 * A.turns)));
   if (dtype == PAL_DTYPE_BF16) PAL_TIMED_LAUNCH(kKernDropout, (hipStream_t)stream, dropout_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, A);
   else PAL_TIMED_LAUNCH(kKernDropout, (hipStream_t)stream, dropout_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, A);

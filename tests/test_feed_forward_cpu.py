@@ -170,6 +170,9 @@ def test_dropout_entry_point_refuses(L):
     assert call(x=None) == L.PAL_E_NULL and call(y=None) == L.PAL_E_NULL and call(dtype=2) == L.PAL_E_DTYPE
     for kw in (dict(rows=0), dict(dim=0), dict(dim=(1 << 30) + 1, stride=(1 << 30) + 1), dict(stride=7), dict(p=1.0), dict(p=-1e-9), dict(p=float("nan"))):
         assert call(**kw) == L.PAL_E_DIM, kw
+    # entries in all are counted in 64 bits
+    for rows, dim in ((1 << 40, 1 << 30), (1 << 37, 1 << 30), ((1 << 36) + 1, 1 << 10)):
+        assert call(rows=rows, dim=dim, stride=dim) == L.PAL_E_DIM, (rows, dim)
 
 
 # ------------------------------------------------------------------------------------------------ the Python boundary
