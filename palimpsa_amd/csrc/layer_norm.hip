@@ -9,7 +9,8 @@
 // Bound by HBM: every row is read once and written once, as in residual_norm.hip, whose division of the work this has: one wave holds a
 // row of up to 2048 entries, four one of up to 16384, the next row is fetched before the present one is summed.  The variance is
 // that of the row in registers around its mean, in a second sum: no difference of large squares.  Dropout's words are made from the place
-// (philox.h); pieces of rows whose length is no multiple of eight are then not moved back, so that four words belong to one piece.
+// (philox.h); pieces of rows whose length is no multiple of eight are then not moved back, so that four words belong to one piece.  16384 rows of
+// 1536, bf16 with a dropout beside an fp32 stream: forward 302 MB in 61 us, backward 403 MB in 77, its sum over the workgroups' shares 5.
 #include "norm_rows.h"
 #include "pal_common.h"
 #include "pal_host.h"
@@ -30,6 +31,25 @@ struct LayerNormArgs {
   float eps;
   DropArgs drop;
 };
+
+// A row's beginning in scalar registers, and a lane's place in it by 32 bits, which a load or store adds itself.  (As pointers of the lanes, 64 bits for
+// each piece of each tensor, they were the registers that the backward kernel lacked: read back from scratch memory between the loads of the next
+// row, they made each of these wait for the one before.)
+template <typename T>
+__device__ __forceinline__ T* row_at(T* p, int64_t entries) {
+  p += entries;
+  asm("" : "+s"(p));
+  return p;
+}
+template <typename T>
+__device__ __forceinline__ T* lane_at(T* row, int at) { return (T*)((char*)row + (uint32_t)at * (uint32_t)sizeof(T)); }
+template <typename T>
+__device__ __forceinline__ const T* lane_at(const T* row, int at) { return (const T*)((const char*)row + (uint32_t)at * (uint32_t)sizeof(T)); }
+template <bool WHOLE, typename T>
+__device__ __forceinline__ void fetch_piece(Piece8<T>& d, const T* row, int at, int D) {
+  if constexpr (WHOLE) d.load(lane_at(row, at));
+  else load_piece(d, lane_at(row, at), D - at);
+}
 
 // entry e of a piece is the row's own and counted here
 template <typename At, bool WHOLE>
@@ -70,16 +90,20 @@ __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(LayerNormArgs A) {
   Piece8<TR> rb[NV];
   const bool has_res = A.res != nullptr;
   auto fetch = [&](int64_t r) {
+    const TX* x_row = row_at((const TX*)A.x, r * A.x_stride);
+    const TR* res_row = row_at((const TR*)A.res, has_res ? r * A.res_stride : 0);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const At p(lane, v, D);
-      load_row_piece<WHOLE>(xb[v], (const TX*)A.x + r * A.x_stride, p.at, D);
-      if (has_res) load_row_piece<WHOLE>(rb[v], (const TR*)A.res + r * A.res_stride, p.at, D);
+      fetch_piece<WHOLE>(xb[v], x_row, p.at, D);
+      if (has_res) fetch_piece<WHOLE>(rb[v], res_row, p.at, D);
     }
   };
   fetch(row);
   for (int turn = 0; row < A.rows; row += step, turn ^= 1) {
     float s[NV][8], sum = 0.f;
+    TR* s_row = row_at((TR*)A.s, A.s ? row * D : 0);
+    TX* y_row = row_at((TX*)A.y, row * D);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const At p(lane, v, D);
@@ -89,7 +113,7 @@ __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(LayerNormArgs A) {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (has_res) s[v][e] += rb[v].get(e);
-      if (A.s && p.on) store_piece((TR*)A.s + row * D + p.at, s[v], WHOLE ? 8 : D - p.at);
+      if (A.s && p.on) store_piece(lane_at(s_row, p.at), s[v], WHOLE ? 8 : D - p.at);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         s[v][e] = to_f32(from_f32<TR>(s[v][e]));   // the norm is that of the stream as it is handed on
@@ -122,7 +146,7 @@ __global__ __launch_bounds__(256) void layer_norm_fwd_kernel(LayerNormArgs A) {
       float y[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = fmaf(s[v][e] * r, w[v][e], b[v][e]);
-      if (p.on) store_piece((TX*)A.y + row * D + p.at, y, WHOLE ? 8 : D - p.at);
+      if (p.on) store_piece(lane_at(y_row, p.at), y, WHOLE ? 8 : D - p.at);
     }
   }
 }
@@ -143,16 +167,21 @@ __global__ __launch_bounds__(256, WPR == 1 && NV <= 3 ? 2 : 1) void layer_norm_b
   const int64_t s_stride = A.s ? D : A.x_stride;
   const TR* s_rows = A.s ? (const TR*)A.s : (const TR*)A.x;
   const DropKey key(A.drop);
-  float w[NV][8], dw[NV][8], db[NV][8];
-#pragma unroll
-  for (int v = 0; v < NV; ++v) {
+  constexpr bool kWide = NV == 8;   // rows whose weights and whose next one would not fit the registers as well: both are read when they are used
+  float w[kWide ? 1 : NV][8], dw[NV][8], db[NV][8];
+  auto weights = [&](int v) {
     const At p(lane, v, D);
+    float (&o)[8] = w[kWide ? 0 : v];
     if constexpr (WHOLE) {
-      load_params(w[v], A.weight, p.at, A.weight_bf16);
+      load_params(o, A.weight, p.at, A.weight_bf16);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[v][e] = p.at + e < D ? load_rt(A.weight, p.at + e, A.weight_bf16) : 0.f;
+      for (int e = 0; e < 8; ++e) o[e] = p.at + e < D ? load_rt(A.weight, p.at + e, A.weight_bf16) : 0.f;
     }
+  };
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    if (!kWide) weights(v);
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[v][e] = db[v][e] = 0.f;
   }
@@ -161,49 +190,63 @@ __global__ __launch_bounds__(256, WPR == 1 && NV <= 3 ? 2 : 1) void layer_norm_b
   f32x2 st;
   auto fetch = [&](int64_t r) {
     st = *(const f32x2*)(A.stats + 2 * r);
+    const TR* s_row = row_at(s_rows, r * s_stride);
+    const TX* dy_row = row_at((const TX*)A.dy, has_dy ? r * D : 0);
+    const TR* dres_row = row_at((const TR*)A.dres, has_dres ? r * D : 0);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const At p(lane, v, D);
-      load_row_piece<WHOLE>(sb[v], s_rows + r * s_stride, p.at, D);
-      if (has_dy) load_row_piece<WHOLE>(gb[v], (const TX*)A.dy + r * D, p.at, D);
-      if (has_dres) load_row_piece<WHOLE>(eb[v], (const TR*)A.dres + r * D, p.at, D);
+      fetch_piece<WHOLE>(sb[v], s_row, p.at, D);
+      if (has_dy) fetch_piece<WHOLE>(gb[v], dy_row, p.at, D);
+      if (has_dres) fetch_piece<WHOLE>(eb[v], dres_row, p.at, D);
     }
   };
   int64_t row = (int64_t)blockIdx.x * kSlots + slot;
-  if (row < A.rows) fetch(row);
+  if (!kWide && row < A.rows) fetch(row);
   for (int turn = 0; row < A.rows; row += step, turn ^= 1) {
-    float h[NV][8], g[NV][8], ex[NV][8], sum = 0.f, dot = 0.f;
+    if constexpr (kWide) fetch(row);
+    float h[NV][8], sum = 0.f, dot = 0.f;
     const float mean = st[0], r = st[1];
+    Piece8<TX> gk[NV];       // (as they were read: half the registers of bf16 rows)
+    Piece8<TR> ek[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const At p(lane, v, D);
+      const float (&wv)[8] = w[kWide ? 0 : v];
+      if (kWide) weights(v);
+      gk[v] = gb[v];
+      ek[v] = eb[v];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         h[v][e] = (sb[v].get(e) - mean) * r;
-        g[v][e] = has_dy ? gb[v].get(e) : 0.f;
-        ex[v][e] = has_dres ? eb[v].get(e) : 0.f;
-        const float gw = g[v][e] * w[v][e], q = sum + gw, d = fmaf(gw, h[v][e], dot);
+        const float gw = (has_dy ? gk[v].get(e) : 0.f) * wv[e], q = sum + gw, d = fmaf(gw, h[v][e], dot);
         const bool out = (kAll || At::masked(v)) && !counts<At, WHOLE>(p, e, D);
         sum = out ? sum : q;
         dot = out ? dot : d;
       }
     }
-    if (row + step < A.rows) fetch(row + step);
+    if (!kWide && row + step < A.rows) fetch(row + step);
     sum = row_sum<WPR>(sum, sSum, turn) * inv_d;
     dot = row_sum<WPR>(dot, sDot, turn) * inv_d;
+    TR* ds_row = row_at((TR*)A.ds, A.ds ? row * D : 0);
+    TX* dx_row = row_at((TX*)A.dx, row * D);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const At p(lane, v, D);
       float d[8];
+      const float (&wv)[8] = w[kWide ? 0 : v];
+      if (kWide) weights(v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        dw[v][e] = fmaf(g[v][e], h[v][e], dw[v][e]);
-        db[v][e] += g[v][e];
-        d[e] = has_dy ? fmaf(r, fmaf(-h[v][e], dot, fmaf(g[v][e], w[v][e], -sum)), ex[v][e]) : ex[v][e];
+        const float g = has_dy ? gk[v].get(e) : 0.f, ex = has_dres ? ek[v].get(e) : 0.f;
+        dw[v][e] = fmaf(g, h[v][e], dw[v][e]);
+        db[v][e] += g;
+        d[e] = has_dy ? fmaf(r, fmaf(-h[v][e], dot, fmaf(g, wv[e], -sum)), ex) : ex;
       }
-      if (p.on && A.ds) store_piece((TR*)A.ds + row * D + p.at, d, WHOLE ? 8 : D - p.at);
+      if (p.on && A.ds) store_piece(lane_at(ds_row, p.at), d, WHOLE ? 8 : D - p.at);
       if constexpr (DROP) drop_piece(d, lane + kStep * v, row, A.drop, key);
-      if (p.on) store_piece((TX*)A.dx + row * D + p.at, d, WHOLE ? 8 : D - p.at);
+      if (p.on) store_piece(lane_at(dx_row, p.at), d, WHOLE ? 8 : D - p.at);
+      if constexpr (DROP || kWide) __builtin_amdgcn_sched_barrier(0);   // (one piece's words and weights at a time)
     }
   }
   // the parameters' gradients: the waves' shares in their order
@@ -264,7 +307,10 @@ __global__ __launch_bounds__(1024) void layer_norm_reduce_kernel(const float* pa
 
 static int layer_norm_blocks(int64_t rows, int dim, bool bwd) {
   const int slots = dim > 2048 ? 1 : 4;
-  const int64_t want = (rows + slots - 1) / slots, most = bwd ? 512 : 2048;
+  // Backward: as many as the chip holds at a time, by the registers that a row's pieces take: every further one is a share more of the parameters'
+  // gradients, and with fewer a compute unit waits (16384 rows of 2048: 48 us with 256, 54 with 512; of 1536 beside an fp32 stream 123 and 93).
+  const bool two = dim <= 1536 || (dim > 2048 && dim <= 4096);
+  const int64_t want = (rows + slots - 1) / slots, most = !bwd ? 2048 : dim <= 512 ? 1024 : two ? 512 : 256;
   return (int)(want < most ? want : most);
 }
 
@@ -337,8 +383,9 @@ struct DropoutArgs {
   DropArgs drop;
 };
 
-// A workgroup takes `turns` times 256 neighbouring pieces of eight entries; pieces are numbered over the rows.  Bound by HBM and by the random
-// words nearly alike.
+// A workgroup takes `turns` times 256 neighbouring pieces of eight entries; pieces are numbered over the rows.  Bound by HBM: 16384 rows of 2048 in
+// bf16 are 134 MB in 25.8 us (5.2 TB/s), the vector units at work for a half of it, most of that on the random words.  Two turns once they fill the
+// chip: 25.8 us, where one is 27.2, four 27.1 and sixteen 30.9.
 template <typename T>
 __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs A) {
   const DropKey key(A.drop);
@@ -432,7 +479,7 @@ extern "C" int pal_dropout(const PalDropout* drop, const void* x, void* y, int64
   A.pieces = rows * A.per_row;
   A.magic = (uint32_t)((((uint64_t)1 << 32) + A.per_row - 1) / A.per_row);
   const int64_t each = A.pieces / (256 * 2048);
-  A.turns = each < 1 ? 1 : each > 8 ? 8 : (int)each;
+  A.turns = each < 1 ? 1 : each > 2 ? 2 : (int)each;
   const int64_t blocks = (A.pieces + 256 * A.turns - 1) / (256 * A.turns);
   if (blocks > 1 << 23) A.turns = (int)((A.pieces + ((int64_t)256 << 23) - 1) / ((int64_t)256 << 23));   // threads of a launch: more turns
   const dim3 grid((unsigned)((A.pieces + (int64_t)256 * A.turns - 1) / ((int64_t)256 * A.turns)));
