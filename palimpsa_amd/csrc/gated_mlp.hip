@@ -10,7 +10,9 @@
 // weights (2048 -> 5632 -> 2048, both launches: 24 us for 1 row, 30 for 17, 45 for 48), and small tiles with k in shares are faster (36).
 //
 // Roundings to the type of the rows: h, dg and du, once each, half a step of the type, as operands of the matrix units; g and u are kept more
-// exactly (Kept8); all sums are in fp32.  The errors in y and the gradients are then of the size of the rounding of those results themselves.
+// exactly (Kept8); all sums are in fp32.  The errors in y and the gradients are then of the size of the rounding of those results themselves.  Up to
+// sixteen rows of bf16 have h as a sum of two bf16 numbers, whose second product the weights' traffic hides (2048 -> 5632 -> 2048, one row: 20.7
+// and 22.1 us; 32 rows, where it does not: 35.8 and 45.6).
 #include "pal_common.h"
 #include "pal_host.h"
 #include "pal_profile.h"
@@ -18,7 +20,7 @@
 
 namespace pal {
 
-constexpr int kFewRows = 32;
+constexpr int kFewRows = 32, kFewSpans = 4;
 
 // ------------------------------------------------------------------------------------------------------------ few rows
 struct FewArgs {
@@ -27,21 +29,31 @@ struct FewArgs {
   Kept kept;
   int64_t x_ld, out_ld;      // elements
   int32_t rows, n, k, act;
+  const void* x_low;         // bf16 rows of h: what its rounding left, to be added to x
+  void* out_low;
 };
 
-// R groups of sixteen rows of x.  The waves of a workgroup (as many as it has) take spans of 128 bytes of k in turn, B of them in one go.
-template <typename T, bool GATED, int R, int B>
+// R groups of sixteen rows of x.  The waves of a workgroup (as many as it has) take spans of 128 bytes of k in turn, four of them in one go (two of
+// two groups of rows, whose registers leave a compute unit two workgroups then): 768 -> 2048 -> 768 of one row, replayed, 8.5 us where one at
+// a time is 9.1, 2048 -> 5632 -> 2048 21.0 and 21.3.
+template <typename T, bool GATED, int R>
 __global__ __launch_bounds__(GATED ? 512 : 1024) void few_rows_kernel(FewArgs P) {
   typedef TileType<T> E;
+  constexpr int B = kFewSpans / R;
+  constexpr bool kSplits = sizeof(T) == 2 && R == 1, kLow = kSplits && !GATED;   // h in two parts
   constexpr int kMats = GATED ? 2 : 1, kPiece = E::kPiece, kSpan = 8 * kPiece;
   extern __shared__ f32x4 shares[];                    // [waves][kMats * R][64]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int j = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
   const int64_t wrow = (int64_t)min(n0 + j, P.n - 1) * P.k;
   const T* w[2] = {(const T*)P.w + wrow, GATED ? (const T*)P.w2 + wrow : nullptr};
-  const T* x[R];
+  const T *x[R], *x_low[R];
 #pragma unroll
-  for (int r = 0; r < R; ++r) x[r] = (const T*)P.x + min(16 * r + j, P.rows - 1) * P.x_ld;
+  for (int r = 0; r < R; ++r) {
+    const int64_t row = min(16 * r + j, P.rows - 1) * P.x_ld;
+    x[r] = (const T*)P.x + row;
+    if constexpr (kLow) x_low[r] = (const T*)P.x_low + row;
+  }
   f32x4 acc[kMats][R];
 #pragma unroll
   for (int m = 0; m < kMats; ++m)
@@ -52,13 +64,16 @@ __global__ __launch_bounds__(GATED ? 512 : 1024) void few_rows_kernel(FewArgs P)
   for (int k0 = wave * kSpan; k0 < P.k; k0 += B * turn) {
     // a span beyond the end is the last one once more, and counts as zero
     auto at = [&](int b, int h) { return min(k0 + b * turn + (4 * h + g) * kPiece, P.k - kPiece); };
-    f32x4 wb[B][2][kMats], xb[B][2][R];
+    f32x4 wb[B][2][kMats], xb[B][2][R], xl[B][2][kLow ? R : 1];
 #pragma unroll
     for (int b = 0; b < B; ++b)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int r = 0; r < R; ++r) xb[b][h][r] = *(const f32x4*)(x[r] + at(b, h));
+        for (int r = 0; r < R; ++r) {
+          xb[b][h][r] = *(const f32x4*)(x[r] + at(b, h));
+          if constexpr (kLow) xl[b][h][r] = *(const f32x4*)(x_low[r] + at(b, h));
+        }
 #pragma unroll
     for (int b = 0; b < B; ++b)
 #pragma unroll
@@ -74,7 +89,10 @@ __global__ __launch_bounds__(GATED ? 512 : 1024) void few_rows_kernel(FewArgs P)
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int m = 0; m < kMats; ++m) acc[m][r] = E::mma(in ? wb[b][h][m] : zero, in ? xb[b][h][r] : zero, acc[m][r]);
+          for (int m = 0; m < kMats; ++m) {
+            acc[m][r] = E::mma(in ? wb[b][h][m] : zero, in ? xb[b][h][r] : zero, acc[m][r]);
+            if constexpr (kLow) acc[m][r] = E::mma(in ? wb[b][h][m] : zero, in ? xl[b][h][r] : zero, acc[m][r]);
+          }
       }
     }
   }
@@ -107,6 +125,14 @@ __global__ __launch_bounds__(GATED ? 512 : 1024) void few_rows_kernel(FewArgs P)
 #pragma unroll
       for (int e = 0; e < 8; ++e) c[e] *= t[1][e];
       tile_store8((T*)P.out + at, c);
+      if constexpr (kSplits) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float high = to_f32(from_f32<T>(c[e]));
+          c[e] = __builtin_isfinite(high) ? c[e] - high : 0.f;
+        }
+        tile_store8((T*)P.out_low + at, c);
+      }
       if (P.kept.gate) {
         Kept8<T>::store(P.kept.gate, at, t[0]);
         Kept8<T>::store(P.kept.up, at, t[1]);
@@ -289,16 +315,13 @@ static int tile_run(TileArgs P, const TilePlan& plan, float* part, int id, hipSt
 
 template <typename T, bool GATED, int R>
 static int few_launch_rows(const FewArgs& P, hipStream_t s) {
-  // spans that a wave takes in one go: 1, 2 or 4, so that the most waves that a workgroup may have take all of k if they can
-  constexpr int kMost = GATED ? 8 : 16;
-  const int spans = (P.k + 8 * TileType<T>::kPiece - 1) / (8 * TileType<T>::kPiece), each = (spans + kMost - 1) / kMost;
-  const int b = each <= 1 ? 1 : each <= 2 ? 2 : 4, rounds = (spans + b * kMost - 1) / (b * kMost), waves = (spans + b * rounds - 1) / (b * rounds);
+  constexpr int kMost = GATED ? 8 : 16, kGo = kFewSpans / R;
+  const int spans = (P.k + 8 * TileType<T>::kPiece - 1) / (8 * TileType<T>::kPiece);
+  const int rounds = (spans + kGo * kMost - 1) / (kGo * kMost), waves = (spans + kGo * rounds - 1) / (kGo * rounds);
   const dim3 grid((P.n + 15) / 16), block(64 * waves);
   const size_t lds = (size_t)waves * (GATED ? 2 : 1) * R * 64 * sizeof(f32x4);
   const int id = GATED ? kKernMlpFewUp : kKernMlpFewDown;
-  if (b == 1) PAL_TIMED_LAUNCH(id, s, (few_rows_kernel<T, GATED, R, 1>), grid, block, lds, s, P);
-  else if (b == 2) PAL_TIMED_LAUNCH(id, s, (few_rows_kernel<T, GATED, R, 2>), grid, block, lds, s, P);
-  else PAL_TIMED_LAUNCH(id, s, (few_rows_kernel<T, GATED, R, 4>), grid, block, lds, s, P);
+  PAL_TIMED_LAUNCH(id, s, (few_rows_kernel<T, GATED, R>), grid, block, lds, s, P);
   PAL_HIP_LAUNCH_CHECK();
   return PAL_OK;
 }
@@ -400,9 +423,10 @@ static int mlp_fwd(const PalMlpDims* d, const PalMlpTensors* t, char* ws, hipStr
   void* h = t->kept ? kept_h(d, t->kept) : ws;
   if (d->rows <= kFewRows) {
     const int64_t ld = hidden_ld(d);
-    FewArgs up{t->x, t->w_gate, t->w_up, h, kept_in(d, t->kept), d->x_stride, ld, (int32_t)d->rows, d->hidden, d->dim, d->activation};
+    void* low = t->kept ? ws : ws + rows_bytes(d);
+    FewArgs up{t->x, t->w_gate, t->w_up, h, kept_in(d, t->kept), d->x_stride, ld, (int32_t)d->rows, d->hidden, d->dim, d->activation, nullptr, low};
     if (int rc = few_launch<T, true>(up, s)) return rc;
-    FewArgs down{h, t->w_down, nullptr, t->y, Kept{}, ld, d->out_dim, (int32_t)d->rows, d->out_dim, d->hidden, 0};
+    FewArgs down{h, t->w_down, nullptr, t->y, Kept{}, ld, d->out_dim, (int32_t)d->rows, d->out_dim, d->hidden, 0, low, nullptr};
     return few_launch<T, false>(down, s);
   }
   MlpPlan m;
@@ -434,7 +458,7 @@ extern "C" size_t pal_gated_mlp_fwd_workspace_bytes(const PalMlpDims* d, int kee
   using namespace pal;
   if (check_mlp(d) != PAL_OK) return 0;
   const size_t h = keeps ? 0 : rows_bytes(d);
-  if (d->rows <= kFewRows) return h;
+  if (d->rows <= kFewRows) return h + (d->dtype == PAL_DTYPE_BF16 && d->rows <= 16 ? rows_bytes(d) : 0);
   MlpPlan m;
   PalMlpTensors t{};
   plan_fwd(d, &t, nullptr, m);

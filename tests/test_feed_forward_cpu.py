@@ -122,8 +122,10 @@ def test_gated_mlp_sizes(L):
     assert lib.pal_gated_mlp_fwd_workspace_bytes(_mlp_dims(L, hidden=5), 0) == 0
     # rows of h an odd number of 128-byte lines apart, three arrays of them kept
     assert lib.pal_gated_mlp_kept_bytes(_mlp_dims(L, rows=16, hidden=2048)) == 3 * 16 * (4096 + 128)
-    assert lib.pal_gated_mlp_fwd_workspace_bytes(_mlp_dims(L, rows=16, hidden=2048), 0) == 16 * (4096 + 128)
-    assert lib.pal_gated_mlp_fwd_workspace_bytes(_mlp_dims(L, rows=16, hidden=2048), 1) == 0      # h is kept
+    # up to sixteen rows of bf16 have h in two parts, of which the first is kept
+    for dtype, keeps, n in ((1, 0, 2), (1, 1, 1), (0, 0, 1), (0, 1, 0)):
+        line = 2048 * (2 if dtype else 4) + 128
+        assert lib.pal_gated_mlp_fwd_workspace_bytes(_mlp_dims(L, rows=16, hidden=2048, dtype=dtype), keeps) == n * 16 * line
 
 
 def _norm_dims(L, drop=None, **kw):
