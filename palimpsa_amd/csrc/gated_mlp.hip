@@ -6,8 +6,8 @@
 // both products, and the three of the weights are one launch (see tile_product.h).
 //
 // A call of few rows is bound by the weights: few_rows_kernel has no tiles in LDS, the waves of a workgroup walk over k side by side, weights and
-// rows straight from memory into the matrix units.  Up to 32 rows: beyond, the rows, which every workgroup reads, are more traffic than the
-// weights (2048 -> 5632 -> 2048, both launches: 24 us for 1 row, 30 for 17, 45 for 48), and small tiles with k in shares are faster (36).
+// rows straight from memory into the matrix units.  Up to 16 rows, and up to 64 where the rows, which every workgroup reads, are not more traffic
+// than small tiles with k in shares take (plan_few).
 //
 // Roundings to the type of the rows: h, dg and du, once each, half a step of the type, as operands of the matrix units; g and u are kept more
 // exactly (Kept8); all sums are in fp32.  The errors in y and the gradients are then of the size of the rounding of those results themselves.  Up to
@@ -20,7 +20,7 @@
 
 namespace pal {
 
-constexpr int kFewRows = 32, kFewSpans = 4;
+constexpr int kFewRows = 64, kFewSpans = 4;
 
 // ------------------------------------------------------------------------------------------------------------ few rows
 struct FewArgs {
@@ -34,12 +34,12 @@ struct FewArgs {
 };
 
 // R groups of sixteen rows of x.  The waves of a workgroup (as many as it has) take spans of 128 bytes of k in turn, four of them in one go (two of
-// two groups of rows, whose registers leave a compute unit two workgroups then): 768 -> 2048 -> 768 of one row, replayed, 8.5 us where one at
+// more groups of rows, whose registers leave a compute unit two workgroups then): 768 -> 2048 -> 768 of one row, replayed, 8.5 us where one at
 // a time is 9.1, 2048 -> 5632 -> 2048 21.0 and 21.3.
 template <typename T, bool GATED, int R>
 __global__ __launch_bounds__(GATED ? 512 : 1024) void few_rows_kernel(FewArgs P) {
   typedef TileType<T> E;
-  constexpr int B = kFewSpans / R;
+  constexpr int B = R == 1 ? kFewSpans : kFewSpans / 2;
   constexpr bool kSplits = sizeof(T) == 2 && R == 1, kLow = kSplits && !GATED;   // h in two parts
   constexpr int kMats = GATED ? 2 : 1, kPiece = E::kPiece, kSpan = 8 * kPiece;
   extern __shared__ f32x4 shares[];                    // [waves][kMats * R][64]
@@ -221,6 +221,7 @@ constexpr int tile_cols(int form, int kind) {   // of C
 }
 struct TilePlan {
   int form, tiles, splits, split_steps;
+  double us;
 };
 
 // Tile form and shares of k: the cheapest by the time of a step of a tile, the launch's rounds over the chip and, for shares, their way
@@ -249,7 +250,7 @@ static TilePlan plan_tiles(const TileArgs& P, int kind, int dtype) {
       const double us = rounds * share * step + 3 + (s > 1 ? 4 + numbers * s * (4 / 3.5e6 + 4 / 1e7) : 0);
       if (us < least) {
         least = us;
-        best = TilePlan{form, (int)tiles, s, share};
+        best = TilePlan{form, (int)tiles, s, share, us};
       }
     }
   }
@@ -319,7 +320,7 @@ static int tile_run(TileArgs P, const TilePlan& plan, float* part, int id, hipSt
 
 template <typename T, bool GATED, int R>
 static int few_launch_rows(const FewArgs& P, hipStream_t s) {
-  constexpr int kMost = GATED ? 8 : 16, kGo = kFewSpans / R;
+  constexpr int kMost = GATED ? 8 : 16, kGo = R == 1 ? kFewSpans : kFewSpans / 2;
   const int spans = (P.k + 8 * TileType<T>::kPiece - 1) / (8 * TileType<T>::kPiece);
   const int rounds = (spans + kGo * kMost - 1) / (kGo * kMost), waves = (spans + kGo * rounds - 1) / (kGo * rounds);
   const dim3 grid((P.n + 15) / 16), block(64 * waves);
@@ -331,7 +332,11 @@ static int few_launch_rows(const FewArgs& P, hipStream_t s) {
 }
 template <typename T, bool GATED>
 static int few_launch(const FewArgs& P, hipStream_t s) {
-  return P.rows <= 16 ? few_launch_rows<T, GATED, 1>(P, s) : few_launch_rows<T, GATED, 2>(P, s);
+  const int groups = (P.rows + 15) / 16;
+  return groups == 1   ? few_launch_rows<T, GATED, 1>(P, s)
+         : groups == 2 ? few_launch_rows<T, GATED, 2>(P, s)
+         : groups == 3 ? few_launch_rows<T, GATED, 3>(P, s)
+                       : few_launch_rows<T, GATED, 4>(P, s);
 }
 
 static int check_mlp(const PalMlpDims* d) {
@@ -422,10 +427,23 @@ static void plan_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGr
 }
 static size_t most_of(size_t a, size_t b) { return a > b ? a : b; }
 
+// Plans a forward call; true: it takes the kernel of few rows.  Beyond 16 rows that goes by its time, fitted to 17 to 64 rows of six sizes (256 -> 704 -> 256 to 2048 -> 5632 -> 2048; within
+// a sixth), against that of the tiles' plan, which is up to a quarter too low there.  bf16, 33 rows: 768 -> 2048 -> 768 14.0 us and 22.4 by tiles, 1536 -> 4096 23.7 and 31.6, 2048 -> 5632 38.1 and
+// 32.5; fp32, 32 rows: 512 -> 1408 16.9 and 22.1, 1024 -> 2816 30.5 and 29.5.
+static bool plan_few(const PalMlpDims* d, const PalMlpTensors* t, const void* h, MlpPlan& m) {
+  if (d->rows <= 16) return true;
+  plan_fwd(d, t, h, m);
+  if (d->rows > kFewRows) return false;
+  auto rounds = [](int n) { return (double)((n + 16 * 256 - 1) / (16 * 256)); };   // of workgroups of sixteen columns over the compute units
+  const double k_bytes = (rounds(d->hidden) * d->dim + rounds(d->out_dim) * d->hidden) * (double)mlp_elem(d);
+  return 5 + k_bytes * (0.00086 + 0.00003 * (double)d->rows) < 1.25 * (m.p_up.us + m.p_down.us);
+}
+
 template <typename T>
 static int mlp_fwd(const PalMlpDims* d, const PalMlpTensors* t, char* ws, hipStream_t s) {
   void* h = t->kept ? kept_h(d, t->kept) : ws;
-  if (d->rows <= kFewRows) {
+  MlpPlan m;
+  if (plan_few(d, t, h, m)) {
     const int64_t ld = hidden_ld(d);
     void* low = t->kept ? ws : ws + rows_bytes(d);
     FewArgs up{t->x, t->w_gate, t->w_up, h, kept_in(d, t->kept), d->x_stride, ld, (int32_t)d->rows, d->hidden, d->dim, d->activation, nullptr, low};
@@ -433,8 +451,6 @@ static int mlp_fwd(const PalMlpDims* d, const PalMlpTensors* t, char* ws, hipStr
     FewArgs down{h, t->w_down, nullptr, t->y, Kept{}, ld, d->out_dim, (int32_t)d->rows, d->out_dim, d->hidden, 0, low, nullptr};
     return few_launch<T, false>(down, s);
   }
-  MlpPlan m;
-  plan_fwd(d, t, h, m);
   float* part = (float*)(t->kept ? ws : ws + rows_bytes(d));
   if (int rc = tile_run<T, kTileGated, false, false>(m.up, m.p_up, part, kKernMlpUp, s)) return rc;
   return tile_run<T, kTilePlain, false, false>(m.down, m.p_down, part, kKernMlpDown, s);
@@ -462,10 +478,9 @@ extern "C" size_t pal_gated_mlp_fwd_workspace_bytes(const PalMlpDims* d, int kee
   using namespace pal;
   if (check_mlp(d) != PAL_OK) return 0;
   const size_t h = keeps ? 0 : rows_bytes(d);
-  if (d->rows <= kFewRows) return h + (d->dtype == PAL_DTYPE_BF16 && d->rows <= 16 ? rows_bytes(d) : 0);
   MlpPlan m;
   PalMlpTensors t{};
-  plan_fwd(d, &t, nullptr, m);
+  if (plan_few(d, &t, nullptr, m)) return h + (d->dtype == PAL_DTYPE_BF16 && d->rows <= 16 ? rows_bytes(d) : 0);
   return h + most_of(part_bytes(m.up, m.p_up, kTileGated), part_bytes(m.down, m.p_down, kTilePlain));
 }
 extern "C" int pal_gated_mlp_fwd(const PalMlpDims* d, const PalMlpTensors* t, void* workspace, size_t workspace_bytes, void* stream) {

@@ -40,6 +40,13 @@ def test_against_the_form_in_64_bits(gpu_device, M, D, F, Do, dtype):
     check(gpu_device, M, D, F, Do, dtype, "silu")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M", [31, 32, 33, 48, 49, 64, 65])
+@pytest.mark.parametrize("D,F,Do", [(256, 704, 256), (136, 4104, 72), (2048, 1408, 2048)])
+def test_rows_about_the_kernels_of_few_rows(gpu_device, M, D, F, Do, dtype):
+    check(gpu_device, M, D, F, Do, dtype, "silu")
+
+
 @pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "relu"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("M", [5, 130])
