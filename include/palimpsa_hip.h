@@ -609,6 +609,17 @@ typedef struct PalMlpGrads {
   void *dw_down;               /* [out_dim,hidden]                              */
 } PalMlpGrads;
 
+/* For callers with other sizes: dst [dst_rows,dst_cols] = src [rows,cols] with zeros behind its rows and columns; rows src_ld and dst_ld elements
+ * apart, at any element's address.  Up to 8 matrices of one dtype in a launch, none of which may overlap another. */
+typedef struct PalMatrixCopy {
+  const void *src;
+  void *dst;
+  int64_t src_ld, dst_ld;     /* >= cols, >= dst_cols                          */
+  int64_t rows, cols;         /* up to dst_rows, dst_cols                      */
+  int64_t dst_rows, dst_cols; /* up to 2^30                                    */
+} PalMatrixCopy;
+int pal_copy_matrices(const PalMatrixCopy *m, int32_t n, int32_t dtype, void *stream);
+
 size_t pal_gated_mlp_kept_bytes(const PalMlpDims *dims);
 size_t pal_gated_mlp_fwd_workspace_bytes(const PalMlpDims *dims, int keeps); /* keeps: with t->kept */
 int pal_gated_mlp_fwd(const PalMlpDims *dims, const PalMlpTensors *t, void *workspace, size_t workspace_bytes, void *stream);

@@ -136,6 +136,10 @@ class PalMlpGrads(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("dy", "dx", "dw_gate", "dw_up", "dw_down")]
 
 
+class PalMatrixCopy(C.Structure):
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p)] + [(n, C.c_int64) for n in ("src_ld", "dst_ld", "rows", "cols", "dst_rows", "dst_cols")]
+
+
 class PalDropout(C.Structure):
     _fields_ = [("p", C.c_double), ("seed", C.c_int64), ("seed_at", C.c_void_p), ("site", C.c_uint32)]
 
@@ -230,6 +234,8 @@ def load() -> C.CDLL:
     lib.pal_gated_mlp_fwd.restype = lib.pal_gated_mlp_bwd.restype = C.c_int
     lib.pal_gated_mlp_fwd.argtypes = [P(PalMlpDims), P(PalMlpTensors), C.c_void_p, C.c_size_t, C.c_void_p]
     lib.pal_gated_mlp_bwd.argtypes = [P(PalMlpDims), P(PalMlpTensors), P(PalMlpGrads), C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.pal_copy_matrices.restype = C.c_int
+    lib.pal_copy_matrices.argtypes = [P(PalMatrixCopy), C.c_int32, C.c_int32, C.c_void_p]
     lib.pal_layer_norm_fwd.restype = lib.pal_layer_norm_bwd.restype = lib.pal_dropout.restype = C.c_int
     lib.pal_layer_norm_fwd.argtypes = [P(PalLayerNormDims), P(PalLayerNormTensors), C.c_void_p]
     lib.pal_layer_norm_bwd.argtypes = [P(PalLayerNormDims), P(PalLayerNormTensors), P(PalLayerNormGrads), C.c_void_p, C.c_size_t,
@@ -275,7 +281,7 @@ def _check_host(ext) -> None:
     have = tuple(getattr(ext, "abi", ()))
     want += tuple(C.sizeof(t) for t in (PalNormDims, PalNormTensors, PalNormGrads, PalConvDims, PalConvTensors, PalConvGrads,
                                         PalScanDims, PalScanTensors, PalScanGrads, PalDropout, PalLayerNormDims, PalLayerNormTensors,
-                                        PalLayerNormGrads, PalMlpDims, PalMlpTensors, PalMlpGrads))
+                                        PalLayerNormGrads, PalMlpDims, PalMlpTensors, PalMlpGrads, PalMatrixCopy))
     have += tuple(getattr(ext, "abi_block", ()))
     built = getattr(ext, "torch_version", None)
     if have != want or built != torch.__version__:
@@ -309,7 +315,7 @@ _HOST_FUNCTIONS = ("pal_recurrent_fwd", "pal_gla_recurrent_fwd", "pal_chunk_fwd"
                    "pal_scan_fwd", "pal_scan_fwd_workspace_bytes", "pal_scan_checkpoint_bytes", "pal_scan_bwd",
                    "pal_scan_bwd_workspace_bytes", "pal_dropout", "pal_layer_norm_fwd", "pal_layer_norm_bwd",
                    "pal_layer_norm_bwd_workspace_bytes", "pal_gated_mlp_kept_bytes", "pal_gated_mlp_fwd", "pal_gated_mlp_fwd_workspace_bytes", "pal_gated_mlp_bwd",
-                   "pal_gated_mlp_bwd_workspace_bytes")
+                   "pal_gated_mlp_bwd_workspace_bytes", "pal_copy_matrices")
 
 
 # How the chunked entry points build the tile-start states (PAL_FLAG_STATES_* of the C ABI): 0 = chosen by shape,

@@ -16,6 +16,7 @@
 #include "pal_common.h"
 #include "pal_host.h"
 #include "pal_profile.h"
+#include "rows8.h"
 #include "tile_product.h"
 
 namespace pal {
@@ -197,6 +198,35 @@ __global__ __launch_bounds__(256) void tile_join_kernel(JoinArgs P) {
       }
     } else {
       tile_store8((T*)P.out[which] + at, c[0]);
+    }
+  }
+}
+
+// -------------------------------------------------------------------------------------------------------------- copies
+// A wave takes a row, or as many neighbouring ones as it has lanes for, by pieces of eight entries: a call with dims that are no multiple of
+// eight has one such launch before and one behind its kernels (1503 x 771 and three weights of 771 x 2058 in fp32: 24 MB in and as much out).
+struct CopyArgs {
+  PalMatrixCopy m[8];
+};
+template <typename T>
+__global__ __launch_bounds__(256) void copy_matrices_kernel(CopyArgs A) {
+  const PalMatrixCopy& m = A.m[blockIdx.y];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, across = (int)min((m.dst_cols + 7) / 8, (int64_t)64), rows = 64 / across;
+  const int in_row = lane % across, in_wave = lane / across;
+  if (in_wave >= rows) return;
+  for (int64_t row = ((int64_t)blockIdx.x * 4 + wave) * rows + in_wave; row < m.dst_rows; row += (int64_t)gridDim.x * 4 * rows) {
+    const T* src = (const T*)m.src + row * m.src_ld;
+    T* dst = (T*)m.dst + row * m.dst_ld;
+    for (int64_t c = 8 * in_row; c < m.dst_cols; c += 8 * across) {
+      Piece8<T> b;
+      load_piece(b, src + c, row < m.rows ? (int)min(m.cols - c, (int64_t)8) : 0);
+      if (c + 8 <= m.dst_cols) {
+        b.store(dst + c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (c + e < m.dst_cols) dst[c + e] = b.at(e);
+      }
     }
   }
 }
@@ -469,6 +499,30 @@ static int mlp_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrad
 }
 
 }  // namespace pal
+
+extern "C" int pal_copy_matrices(const PalMatrixCopy* m, int32_t n, int32_t dtype, void* stream) {
+  using namespace pal;
+  if (!m) return PAL_E_NULL;
+  if (dtype != PAL_DTYPE_F32 && dtype != PAL_DTYPE_BF16) return PAL_E_DTYPE;
+  if (n < 1 || n > 8) return PAL_E_DIM;
+  CopyArgs A{};
+  int64_t most = 0;
+  for (int i = 0; i < n; ++i) {
+    A.m[i] = m[i];
+    if (!m[i].src || !m[i].dst) return PAL_E_NULL;
+    if (m[i].rows < 1 || m[i].cols < 1 || m[i].rows > m[i].dst_rows || m[i].cols > m[i].dst_cols || m[i].dst_rows > 1 << 30 || m[i].dst_cols > 1 << 30 ||
+        m[i].src_ld < m[i].cols || m[i].dst_ld < m[i].dst_cols)
+      return PAL_E_DIM;
+    const int64_t across = (m[i].dst_cols + 7) / 8 < 64 ? (m[i].dst_cols + 7) / 8 : 64, per = 4 * (64 / across), blocks = (m[i].dst_rows + per - 1) / per;
+    most = blocks > most ? blocks : most;
+  }
+  const dim3 grid((unsigned)(most < 2048 ? most : 2048), n);
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == PAL_DTYPE_BF16) PAL_TIMED_LAUNCH(kKernCopyMatrices, s, copy_matrices_kernel<bf16_t>, grid, dim3(256), 0, s, A);
+  else PAL_TIMED_LAUNCH(kKernCopyMatrices, s, copy_matrices_kernel<float>, grid, dim3(256), 0, s, A);
+  PAL_HIP_LAUNCH_CHECK();
+  return PAL_OK;
+}
 
 extern "C" size_t pal_gated_mlp_kept_bytes(const PalMlpDims* d) {
   using namespace pal;

@@ -661,42 +661,98 @@ py::object layer_norm(const Tensor& x, const OptT& r_, const Tensor& w, const Op
 }
 
 // --------------------------------------------------------------------------------------------- gated feed-forward block
+// Matrices that the kernels cannot read or write where they lie (dims that are no multiple of eight, addresses or strides off 16 bytes): copies of
+// them in one buffer, made by one launch, and results taken out of it by another.
+struct MlpCopies {
+  PalMatrixCopy in[5], out[5];
+  int n_in = 0, n_out = 0;
+  size_t bytes = 0;
+  const size_t es;
+  Tensor buffer;
+  explicit MlpCopies(size_t es) : es(es) {}
+  static int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+  // (places are offsets until the buffer is there)
+  void add(bool result, const void* p, int64_t ld, int64_t rows, int64_t cols, bool pad_rows) {
+    const int64_t r8 = pad_rows ? up8(rows) : rows, c8 = up8(cols);
+    if (result) out[n_out++] = PalMatrixCopy{(const void*)bytes, (void*)p, c8, ld, rows, cols, rows, cols};
+    else in[n_in++] = PalMatrixCopy{p, (void*)bytes, ld, c8, rows, cols, r8, c8};
+    bytes += ((size_t)(r8 * c8) * es + 255) & ~(size_t)255;
+  }
+  int make(const Tensor& like, int32_t dtype) {
+    if (!bytes) return 0;
+    buffer = workspace(like, bytes);
+    char* base = (char*)buffer.mutable_data_ptr();
+    for (int i = 0; i < n_in; ++i) in[i].dst = base + (size_t)in[i].dst;
+    for (int i = 0; i < n_out; ++i) out[i].src = base + (size_t)out[i].src;
+    return n_in ? abi.copy_matrices(in, n_in, dtype, stream_of(like.device())) : 0;
+  }
+  int take(const Tensor& like, int32_t dtype) { return n_out ? abi.copy_matrices(out, n_out, dtype, stream_of(like.device())) : 0; }
+};
+
 struct MlpCall {
   bool ok = false;
   at::ScalarType type;
-  PalMlpDims d{};
+  PalMlpDims d{};                    // multiples of eight
+  int64_t D, F, Do, x_ld;            // as they are
+  bool copied[4];                    // x, w_gate, w_up, w_down
   MlpCall(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t act) {
     if (!x.defined() || x.device().type() != at::kCUDA || x.device().index() != c10::hip::current_device() || x.dim() < 1 || x.numel() == 0) return;
     const c10::Device dev = x.device();
     type = x.scalar_type();
     if (!rows_type(type) || !there(x, dev, type)) return;
     for (const Tensor* w : {&wg, &wu, &wd})
-      if (!packed(*w, dev, type) || w->dim() != 2 || (uintptr_t)ptr(*w) % 16) return;
-    const int64_t D = x.size(-1), F = wg.size(0), Do = wd.size(0), rows = x.numel() / D;
+      if (!packed(*w, dev, type) || w->dim() != 2) return;
+    D = x.size(-1);
+    F = wg.size(0);
+    Do = wd.size(0);
+    const int64_t rows = x.numel() / D;
     if (wg.size(1) != D || wu.sizes() != wg.sizes() || wd.size(1) != F) return;
-    if (D % 8 || F % 8 || Do % 8 || !F || !Do || D > 1 << 20 || F > 1 << 20 || Do > 1 << 20 || rows > 1 << 30) return;
-    if (!row_stride(x, d.x_stride) || d.x_stride % 8 || d.x_stride > 1 << 20 || (uintptr_t)ptr(x) % 16) return;
-    d.rows = rows; d.dim = (int32_t)D; d.hidden = (int32_t)F; d.out_dim = (int32_t)Do; d.dtype = pal_type(type); d.activation = (int32_t)act;
+    if (!F || !Do || D > 1 << 20 || F > 1 << 20 || Do > 1 << 20 || rows > 1 << 30) return;
+    if (!row_stride(x, x_ld)) return;
+    const Tensor* t[] = {&x, &wg, &wu, &wd};
+    for (int i = 0; i < 4; ++i) copied[i] = (uintptr_t)ptr(*t[i]) % 16 || (i == 0 ? D % 8 || x_ld % 8 || x_ld > 1 << 20 : odd(i));
+    d.rows = rows;
+    d.x_stride = copied[0] ? MlpCopies::up8(D) : x_ld;
+    d.dim = (int32_t)MlpCopies::up8(D); d.hidden = (int32_t)MlpCopies::up8(F); d.out_dim = (int32_t)MlpCopies::up8(Do);
+    d.dtype = pal_type(type); d.activation = (int32_t)act;
     ok = true;
   }
+  // rows and columns of x (0), of the weights
+  int64_t high(int i) const { return i == 0 ? d.rows : i < 3 ? F : Do; }
+  int64_t wide(int i) const { return i == 0 || i < 3 ? D : F; }
+  bool odd(int i) const { return wide(i) % 8 || (i && high(i) % 8); }
+  size_t es() const { return type == at::kFloat ? 4 : 2; }
   Tensor out(const Tensor& x) const {
     auto shape = x.sizes().vec();
-    shape.back() = d.out_dim;
+    shape.back() = Do;
     return at::empty(shape, as(x, type));
   }
-  static PalMlpTensors fill(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd) {
-    PalMlpTensors t{};
-    t.x = ptr(x); t.w_gate = ptr(wg); t.w_up = ptr(wu); t.w_down = ptr(wd);
-    return t;
+  // operands, copied if need be; their copies are the first ones
+  void operands(MlpCopies& c, const Tensor* const* t) const {
+    for (int i = 0; i < 4; ++i)
+      if (copied[i]) c.add(false, ptr(*t[i]), i == 0 ? x_ld : wide(i), high(i), wide(i), i != 0);
+  }
+  PalMlpTensors fill(const MlpCopies& c, const Tensor* const* t) const {
+    const void* p[4];
+    for (int i = 0, n = 0; i < 4; ++i) p[i] = copied[i] ? c.in[n++].dst : ptr(*t[i]);
+    PalMlpTensors r{};
+    r.x = p[0]; r.w_gate = p[1]; r.w_up = p[2]; r.w_down = p[3];
+    return r;
   }
   int run(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, Tensor& y, Tensor& kept) const {
-    PalMlpTensors t = fill(x, wg, wu, wd);
-    t.y = y.mutable_data_ptr();
-    t.kept = kept.defined() ? kept.mutable_data_ptr() : nullptr;
+    const Tensor* t[] = {&x, &wg, &wu, &wd};
+    MlpCopies c(es());
+    operands(c, t);
+    if (Do % 8) c.add(true, y.mutable_data_ptr(), Do, d.rows, Do, false);
+    if (int rc = c.make(x, d.dtype)) return rc;
+    PalMlpTensors r = fill(c, t);
+    r.y = Do % 8 ? (void*)c.out[0].src : y.mutable_data_ptr();
+    r.kept = kept.defined() ? kept.mutable_data_ptr() : nullptr;
     const size_t bytes = abi.gated_mlp_fwd_workspace_bytes(&d, kept.defined());
     Tensor ws = workspace(x, bytes);
     NoGil off;
-    return abi.gated_mlp_fwd(&d, &t, ws.mutable_data_ptr(), bytes, stream_of(x.device()));
+    const int rc = abi.gated_mlp_fwd(&d, &r, ws.mutable_data_ptr(), bytes, stream_of(x.device()));
+    return rc ? rc : c.take(x, d.dtype);
   }
 };
 
@@ -721,19 +777,34 @@ struct MlpNode : torch::autograd::Function<MlpNode> {
     MlpCall c(x, s[1], s[2], s[3], ctx->saved_data["act"].toInt());
     TORCH_CHECK_VALUE(c.ok && packed(kept, x.device(), at::kByte) && kept.numel() == (int64_t)abi.gated_mlp_kept_bytes(&c.d),
                       "gated_mlp backward: a saved tensor came back in another shape, dtype, layout or device");
-    Tensor dy = gr[0].to(c.type).contiguous();
-    if ((uintptr_t)ptr(dy) % 16) dy = dy.clone();
+    const Tensor dy = gr[0].to(c.type).contiguous();
+    const Tensor* t[] = {&x, &s[1], &s[2], &s[3]};
+    MlpCopies m(c.es());
+    c.operands(m, t);
+    const bool dy_copied = c.Do % 8 || (uintptr_t)ptr(dy) % 16;
+    if (dy_copied) m.add(false, ptr(dy), c.Do, c.d.rows, c.Do, false);
     Tensor out[4];
-    for (int i = 0; i < 4; ++i)
-      if (ctx->saved_data[std::string("need") + (char)('0' + i)].toBool()) out[i] = at::empty(s[i].sizes(), as(x, c.type));
-    PalMlpTensors t = MlpCall::fill(x, s[1], s[2], s[3]);
-    t.kept = (void*)ptr(kept);
-    auto at_ = [](Tensor& o) { return o.defined() ? o.mutable_data_ptr() : nullptr; };
-    PalMlpGrads g{ptr(dy), at_(out[0]), at_(out[1]), at_(out[2]), at_(out[3])};
+    void* to[4] = {};
+    for (int i = 0; i < 4; ++i) {
+      if (!ctx->saved_data[std::string("need") + (char)('0' + i)].toBool()) continue;
+      out[i] = at::empty(s[i].sizes(), as(x, c.type));
+      to[i] = out[i].mutable_data_ptr();
+      if (c.odd(i)) m.add(true, to[i], c.wide(i), c.high(i), c.wide(i), i != 0);
+    }
+    int rc = m.make(x, c.d.dtype);
+    if (rc) fail(rc, "pal_copy_matrices");
+    PalMlpTensors r = c.fill(m, t);
+    r.kept = (void*)ptr(kept);
+    for (int i = 0, n = 0; i < 4; ++i)
+      if (to[i] && c.odd(i)) to[i] = (void*)m.out[n++].src;
+    PalMlpGrads g{dy_copied ? m.in[m.n_in - 1].dst : ptr(dy), to[0], to[1], to[2], to[3]};
     const size_t bytes = abi.gated_mlp_bwd_workspace_bytes(&c.d, &g);
     Tensor ws = workspace(x, bytes);
-    int rc;
-    { NoGil off; rc = abi.gated_mlp_bwd(&c.d, &t, &g, ws.mutable_data_ptr(), bytes, stream_of(x.device())); }
+    {
+      NoGil off;
+      rc = abi.gated_mlp_bwd(&c.d, &r, &g, ws.mutable_data_ptr(), bytes, stream_of(x.device()));
+      if (!rc) rc = m.take(x, c.d.dtype);
+    }
     if (rc) fail(rc, "pal_gated_mlp_bwd");
     return once({out[0], out[1], out[2], out[3], none});
   }

@@ -55,6 +55,7 @@ struct Abi {
   size_t (*gated_mlp_fwd_workspace_bytes)(const PalMlpDims*, int);
   int (*gated_mlp_bwd)(const PalMlpDims*, const PalMlpTensors*, const PalMlpGrads*, void*, size_t, void*);
   size_t (*gated_mlp_bwd_workspace_bytes)(const PalMlpDims*, const PalMlpGrads*);
+  int (*copy_matrices)(const PalMatrixCopy*, int32_t, int32_t, void*);
 } abi;
 py::handle raise_code;   // (code, where): raises what the Python routes raise for a code of the library
 
@@ -369,7 +370,7 @@ PYBIND11_MODULE(_host, m) {
   m.attr("abi") = py::make_tuple(PAL_ABI_VERSION, sizeof(PalDims), sizeof(PalFwdTensors), sizeof(PalBwdTensors));
   m.attr("abi_block") = py::make_tuple(sizeof(PalNormDims), sizeof(PalNormTensors), sizeof(PalNormGrads), sizeof(PalConvDims), sizeof(PalConvTensors),
                                        sizeof(PalConvGrads), sizeof(PalScanDims), sizeof(PalScanTensors), sizeof(PalScanGrads), sizeof(PalDropout), sizeof(PalLayerNormDims),
-                                       sizeof(PalLayerNormTensors), sizeof(PalLayerNormGrads), sizeof(PalMlpDims), sizeof(PalMlpTensors), sizeof(PalMlpGrads));
+                                       sizeof(PalLayerNormTensors), sizeof(PalLayerNormGrads), sizeof(PalMlpDims), sizeof(PalMlpTensors), sizeof(PalMlpGrads), sizeof(PalMatrixCopy));
   m.attr("torch_version") = PAL_TORCH_VERSION;
   m.def("bind", &bind);
   m.def("recurrent_fwd", &recurrent_fwd);

@@ -56,6 +56,7 @@ enum KernelId {
   kKernLayerNormBwd,
   kKernLayerNormReduce,
   kKernDropout,
+  kKernCopyMatrices,
   kKernCount
 };
 

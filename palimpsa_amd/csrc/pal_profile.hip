@@ -59,7 +59,7 @@ static const char* kNames[kKernCount] = {
     "short_conv_step_kernel", "scan_fwd_kernel", "scan_segment_kernel", "scan_join_kernel", "scan_bwd_kernel",
     "scan_bwd_sums_kernel", "mlp_up", "mlp_down", "mlp_grad",
     "mlp_dx", "mlp_dw", "mlp_few_up", "mlp_few_down", "tile_join_kernel", "layer_norm_fwd_kernel",
-    "layer_norm_bwd_kernel", "layer_norm_reduce_kernel", "dropout_kernel"};
+    "layer_norm_bwd_kernel", "layer_norm_reduce_kernel", "dropout_kernel", "copy_matrices_kernel"};
 
 }  // namespace pal
 

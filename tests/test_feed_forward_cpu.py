@@ -177,6 +177,24 @@ def test_dropout_entry_point_refuses(L):
         assert call(rows=rows, dim=dim, stride=dim) == L.PAL_E_DIM, (rows, dim)
 
 
+def test_copy_entry_point_refuses(L):
+    lib = L.load()
+    ok = dict(src=P, dst=P, src_ld=9, dst_ld=16, rows=3, cols=9, dst_rows=8, dst_cols=16)
+
+    def call(n=1, dtype=1, **kw):
+        m = (L.PalMatrixCopy * 9)(*[L.PalMatrixCopy(**ok)] * 8)
+        m[max(min(n, 8) - 1, 0)] = L.PalMatrixCopy(**{**ok, **kw})
+        return lib.pal_copy_matrices(m, n, dtype, None)
+
+    assert lib.pal_copy_matrices(None, 1, 1, None) == L.PAL_E_NULL
+    for n in (1, 3, 8):
+        assert call(n, src=None) == L.PAL_E_NULL and call(n, dst=None) == L.PAL_E_NULL
+        for kw in (dict(rows=0), dict(cols=0), dict(rows=9), dict(cols=17), dict(src_ld=8), dict(dst_ld=15), dict(dst_rows=(1 << 30) + 1),
+                   dict(dst_cols=(1 << 30) + 1, dst_ld=1 << 31)):
+            assert call(n, **kw) == L.PAL_E_DIM, kw
+    assert call(0) == L.PAL_E_DIM and call(9) == L.PAL_E_DIM and call(dtype=2) == L.PAL_E_DTYPE
+
+
 # ------------------------------------------------------------------------------------------------ the Python boundary
 def test_calls_that_are_refused():
     from palimpsa_amd.ops.gated_mlp import gated_mlp

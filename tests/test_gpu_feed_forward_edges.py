@@ -53,6 +53,54 @@ def test_layouts_of_the_block_give_the_same_bits(gpu_device, dtype, M):
         assert torch.equal(got.reshape(ref.shape), ref)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("M,D,Fh,Do", [(7, 61, 97, 3), (200, 64, 97, 64), (130, 61, 96, 72), (1, 8, 9, 5), (70, 515, 40, 1027)])
+def test_odd_layouts_of_the_block_give_the_same_bits(gpu_device, dtype, M, D, Fh, Do):
+    from palimpsa_amd import _lib as L
+    from palimpsa_amd.ops.gated_mlp import _gated_mlp, gated_mlp
+    x, wg, wu, wd, dy = make(gpu_device, M, D, Fh, Do, dtype)
+
+    def run(f, *a):
+        leaves = [t.detach().requires_grad_(True) for t in a]
+        y = f(*leaves, "silu")
+        with torch.no_grad():
+            assert torch.equal(f(*leaves, "silu"), y)
+        one = torch.autograd.grad(f(*leaves, "silu"), leaves[2:3], dy)[0]      # a part of the gradients
+        grads = torch.autograd.grad(y, leaves, dy)
+        assert torch.equal(one, grads[2])
+        return [y] + list(grads)
+
+    with torch.no_grad():
+        assert L.host().gated_mlp(x, wg, wu, wd, 0) is not None
+    want = run(_gated_mlp, x, wg, wu, wd)
+    wide = _randn(gpu_device, M, D + 13, seed=9, dtype=dtype)
+    wide[:, 5:5 + D] = x
+    off = lambda t: torch.empty(t.numel() + 3, dtype=dtype, device=t.device)[3:].view(t.shape).copy_(t)  # noqa: E731
+    for a in ((x, wg, wu, wd), (wide[:, 5:5 + D], wg, wu, wd), (off(x), off(wg), off(wu), off(wd))):
+        for got, ref in zip(run(gated_mlp, *a), want):
+            assert got.shape == ref.shape and torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_copies_of_matrices(gpu_device, dtype):
+    """Several at a time, rows and columns behind them zero, at odd addresses; nothing around them is written."""
+    from palimpsa_amd import _lib as L
+    sizes = [(1, 1, 1, 1), (3, 5, 8, 8), (130, 771, 136, 776), (9, 8, 9, 8), (1000, 17, 1000, 19), (2, 5000, 2, 5000)]
+    src = [_randn(gpu_device, r, c + 3, seed=i, dtype=dtype) for i, (r, c, _, _) in enumerate(sizes)]
+    room = [torch.full((r8 * (c8 + 2) + 6,), 7.0, dtype=dtype, device=gpu_device) for _, _, r8, c8 in sizes]
+    es = src[0].element_size()
+    m = (L.PalMatrixCopy * len(sizes))(*[
+        L.PalMatrixCopy(src=s.data_ptr() + es, dst=d.data_ptr() + 3 * es, src_ld=c + 3, dst_ld=c8 + 2, rows=r, cols=c, dst_rows=r8, dst_cols=c8)
+        for s, d, (r, c, r8, c8) in zip(src, room, sizes)])
+    assert L.load().pal_copy_matrices(m, len(sizes), int(dtype == BF), C.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    for s, d, (r, c, r8, c8) in zip(src, room, sizes):
+        want = torch.full_like(d, 7.0)
+        inner = want[3:3 + r8 * (c8 + 2)].view(r8, c8 + 2)
+        inner[:, :c8] = 0
+        inner[:r, :c] = s[:, 1:1 + c]
+        assert torch.equal(d, want)
+
+
 def test_layouts_of_the_norm_and_dropout_give_the_same_bits(gpu_device):
     from palimpsa_amd.ops.layer_glue import _dropout, _layer_norm, dropout, layer_norm, residual_layer_norm
     x, res, w, b, dy, dr = (_randn(gpu_device, *s, seed=i, dtype=BF) for i, s in enumerate(((6, 5, 100), (6, 5, 100), (100,), (100,), (6, 5, 100), (6, 5, 100))))
