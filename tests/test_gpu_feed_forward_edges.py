@@ -167,6 +167,33 @@ def test_gradients_that_are_not_wanted(gpu_device):
             assert (g.float() - r.float()).abs().max() <= 2 ** -7 * r.float().abs().max()
 
 
+@pytest.mark.parametrize("M,D,F", [(9, 64, 64), (130, 61, 61)])
+def test_one_tensor_in_two_places(gpu_device, M, D, F):
+    """Gate and up projection shared, down tied to both, and a stream that is added to itself: gradients are sums over the places."""
+    from palimpsa_amd.ops.gated_mlp import gated_mlp
+    from palimpsa_amd.ops.layer_glue import residual_layer_norm
+    x, w, _, _, dy = make(gpu_device, M, D, F, D, F32)
+    leaf = w.clone().requires_grad_(True)
+    apart = [w.clone().requires_grad_(True) for _ in range(3)]
+    y = gated_mlp(x, leaf, leaf, leaf)
+    z = gated_mlp(x, *apart)
+    assert torch.equal(y, z)
+    (g,) = torch.autograd.grad(y, [leaf], dy)
+    parts = torch.autograd.grad(z, apart, dy)
+    want = sum(t.double() for t in parts)
+    assert ((g - want).abs() <= 3 * 2.0 ** -24 * sum(t.double().abs() for t in parts)).all()      # two additions in fp32, in any order
+    nw = _randn(gpu_device, D, seed=3)
+    for p in (0.0, 0.5):
+        leaf = x.clone().requires_grad_(True)
+        two = [x.clone().requires_grad_(True) for _ in range(2)]
+        a = residual_layer_norm(leaf, leaf, nw, dropout_p=p, seed=4)
+        b = residual_layer_norm(*two, nw, dropout_p=p, seed=4)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        (g,) = torch.autograd.grad(a, [leaf], (dy, dy))
+        d = torch.autograd.grad(b, two, (dy, dy))
+        assert torch.equal(g, d[0] + d[1])
+
+
 def test_no_rows_and_refusals(gpu_device):
     from palimpsa_amd.ops.gated_mlp import gated_mlp
     from palimpsa_amd.ops.layer_glue import dropout, layer_norm, residual_layer_norm
@@ -428,8 +455,8 @@ def test_a_captured_block_takes_a_new_seed_at_every_replay(gpu_device):
         assert torch.equal(seen[0], seen[3]) and not torch.equal(seen[0], seen[1])
 
 
-def test_a_captured_training_step(gpu_device):
-    D, F, M = 128, 256, 300
+@pytest.mark.parametrize("D,F,M", [(128, 256, 300), (61, 99, 70), (61, 99, 20)])
+def test_a_captured_training_step(gpu_device, D, F, M):
     p = [[t.requires_grad_(True) for t in layer] for layer in _params(gpu_device, D, F, BF)]
     leaves = [t for layer in p for t in layer]
     x, res, dy = _randn(gpu_device, M, D, seed=70, dtype=BF), _randn(gpu_device, M, D, seed=71), _randn(gpu_device, M, D, seed=72, dtype=BF)
