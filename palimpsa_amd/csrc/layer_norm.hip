@@ -37,9 +37,9 @@ struct LayerNormArgs {
 // row, they made each of these wait for the one before.)
 template <typename T>
 __device__ __forceinline__ T* row_at(T* p, int64_t entries) {
-  p += entries;
-  asm("" : "+s"(p));
-  return p;
+  auto row = (__attribute__((address_space(1))) T*)(p + entries);
+  asm("" : "+s"(row));
+  return (T*)row;
 }
 template <typename T>
 __device__ __forceinline__ T* lane_at(T* row, int at) { return (T*)((char*)row + (uint32_t)at * (uint32_t)sizeof(T)); }
