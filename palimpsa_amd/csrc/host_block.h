@@ -608,7 +608,8 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     TORCH_CHECK_VALUE(s.dim() >= 1 && s.numel() > 0 && rows_type(s.scalar_type()) && there(s, s.device(), s.scalar_type()) && row_stride(s, d.x_stride) &&
                           (!handed_on || s.is_contiguous()) && (handed_on || s.scalar_type() == rows) && param_ok(w, s.device()) && w.dim() == 1 &&
                           w.size(0) == s.size(-1) && (rows == at::kBFloat16 || s.scalar_type() == at::kFloat) && packed(stats, s.device(), at::kFloat) &&
-                          stats.numel() == 2 * (s.numel() / s.size(-1)) && seed_ok(seed_t, s.device()),
+                          stats.numel() == 2 * (s.numel() / s.size(-1)) && seed_ok(seed_t, s.device()) && (!gr[0].defined() || gr[0].sizes() == s.sizes()) &&
+                          (gr.size() < 2 || !gr[1].defined() || gr[1].sizes() == s.sizes()),
                       "layer_norm backward: a saved tensor came back in another shape, dtype, layout or device");
     d.dim = (int32_t)s.size(-1);
     d.rows = s.numel() / d.dim;
@@ -775,7 +776,9 @@ struct MlpNode : torch::autograd::Function<MlpNode> {
     const Tensor &x = s[0], &kept = s[4], none;
     const c10::DeviceGuard guard(x.device());
     MlpCall c(x, s[1], s[2], s[3], ctx->saved_data["act"].toInt());
-    TORCH_CHECK_VALUE(c.ok && packed(kept, x.device(), at::kByte) && kept.numel() == (int64_t)abi.gated_mlp_kept_bytes(&c.d),
+    // (dy has the shape of y, whatever came back)
+    TORCH_CHECK_VALUE(c.ok && packed(kept, x.device(), at::kByte) && kept.numel() == (int64_t)abi.gated_mlp_kept_bytes(&c.d) &&
+                          gr[0].sizes().slice(0, gr[0].dim() - 1) == x.sizes().slice(0, x.dim() - 1) && gr[0].size(-1) == c.Do,
                       "gated_mlp backward: a saved tensor came back in another shape, dtype, layout or device");
     const Tensor dy = gr[0].to(c.type).contiguous();
     const Tensor* t[] = {&x, &s[1], &s[2], &s[3]};

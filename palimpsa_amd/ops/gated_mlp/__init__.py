@@ -91,6 +91,7 @@ class GatedMlp(torch.autograd.Function):
         if kept is not None:
             ctx.save_for_backward(xc, wg, wu, wd, kept)
             ctx.dims = dims
+            ctx.form = cm.saved_form(xc, wg, wu, wd, kept)
         return cm.unpad_last(y, Do).reshape(x.shape[:-1] + (Do,)).to(x.dtype)
 
     @staticmethod
@@ -99,8 +100,13 @@ class GatedMlp(torch.autograd.Function):
         shapes, dtypes, need = ctx.shapes, ctx.dtypes, ctx.needs_input_grad
         if ctx.dims is None:
             return tuple(torch.zeros(s, dtype=t, device=dy.device) if n else None for s, t, n in zip(shapes, dtypes, need)) + (None,)
-        xc, wg, wu, wd, kept = ctx.saved_tensors
-        dims, dev, cd = ctx.dims, xc.device, xc.dtype
+        saved = ctx.saved_tensors
+        cm.check_saved(saved, ctx.form, "gated_mlp")
+        dev, cd = saved[0].device, saved[0].dtype
+        dims = L.PalMlpDims.from_buffer_copy(ctx.dims)
+        xc, dims.x_stride = _rows(saved[0], cd)
+        wg, wu, wd = (_matrix(w, cd) for w in saved[1:4])
+        kept = saved[4].contiguous()
         d, _ = _rows(dy.reshape(dims.rows, shapes[3][0]).to(cd).contiguous(), cd)
         out = [torch.empty(s, dtype=cd, device=dev) if n else None
                for s, n in zip(((dims.rows, dims.dim), wg.shape, wu.shape, wd.shape), need)]

@@ -551,12 +551,14 @@ class Dropout(torch.autograd.Function):
     def forward(ctx, x, p, seed, seed_t, site):
         ctx.meta = (p, seed, site)
         ctx.save_for_backward(seed_t)
+        ctx.form = cm.saved_form(seed_t)
         return Dropout._run(x, p, seed, seed_t, site)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         p, seed, site = ctx.meta
+        cm.check_saved(ctx.saved_tensors, ctx.form, "dropout")
         return Dropout._run(dy, p, seed, ctx.saved_tensors[0], site), None, None, None, None
 
 
@@ -623,6 +625,7 @@ class LayerNorm(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         if stats is not None:
             ctx.save_for_backward(s if handed_on else xc, w, stats, seed_t)
+            ctx.form = cm.saved_form(s if handed_on else xc, w, stats, seed_t)
             ctx.meta = dict(cd=cd, rd=rd, handed_on=handed_on, dims=dims, drop=(p, seed, site),
                             dtypes=[None if t is None else t.dtype for t in (x, residual, weight, bias)])
         y = y if y.dtype == x.dtype else y.to(x.dtype)
@@ -631,8 +634,11 @@ class LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dres=None):
+        cm.check_saved(ctx.saved_tensors, ctx.form, "layer_norm")
         rows, w, stats, seed_t = ctx.saved_tensors
         m = ctx.meta
+        w, stats = w.contiguous(), stats.contiguous()
+        rows, stride = _norm_rows(rows.contiguous() if m["handed_on"] else rows, rows.dtype)
         dev, cd, rd, dt = rows.device, m["cd"], m["rd"], m["dtypes"]
         if dy is None and dres is None:
             return (None,) * 11
@@ -647,6 +653,7 @@ class LayerNorm(torch.autograd.Function):
         pt = cm._ptr
         dims = L.PalLayerNormDims.from_buffer_copy(m["dims"])
         dims.drop = _drop_struct(p, seed, seed_t, site)
+        dims.x_stride = stride
         tens = L.PalLayerNormTensors(weight=pt(w), bias=pt(w) if db is not None else None, stats=pt(stats),
                                      **{"residual_out" if m["handed_on"] else "x": pt(rows)})
         grads = L.PalLayerNormGrads(dy=pt(dy), dresidual_out=pt(dres), dx=pt(dx), dresidual=pt(ds), dweight=pt(dw), dbias=pt(db))

@@ -316,6 +316,18 @@ def unpad_state(x: Optional[torch.Tensor], p: Prepared):
     return x[:, :, :p.dv, :p.dk].contiguous()
 
 
+def saved_form(*tensors):
+    """What a backward pass relies on of the tensors that it saves; see ``check_saved``."""
+    return [None if t is None else (t.shape, t.dtype, t.device) for t in tensors]
+
+
+def check_saved(tensors, form, where: str) -> None:
+    """Saved tensors come back through whatever hooks the caller has set (``torch.autograd.graph``): the kernels read as much as they had when they were
+    saved.  Strides are not looked at: a tensor that was on the host in between comes back packed."""
+    if saved_form(*tensors) != form:
+        raise ValueError(f"{where} backward: a saved tensor came back in another shape, dtype or device")
+
+
 def unpad_last(x: Optional[torch.Tensor], n: int):
     if x is None or x.shape[-1] == n:
         return x
