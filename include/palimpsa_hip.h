@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define PAL_ABI_VERSION 4
+#define PAL_ABI_VERSION 5
 
 /* element types of tensors handed over the boundary */
 #define PAL_DTYPE_F32 0
@@ -577,7 +577,7 @@ int pal_layer_norm_bwd(const PalLayerNormDims *dims, const PalLayerNormTensors *
 
 /* The second half of a block (fla.modules.GatedMLP of the reference's PalimpsaBlock, restated from its published behaviour):
  *   g = x w_gate^T,  u = x w_up^T,  h = act(g) u,  y = h w_down^T
- * Dims are multiples of 8 and every pointer is 16-byte aligned (callers with other sizes pad with zeros).  No result may overlap an operand or
+ * Dims are multiples of 8 and every pointer is 16-byte aligned (callers with other sizes pad with zeros and say so in hidden_pad).  No result may overlap an operand or
  * another result. */
 #define PAL_ACT_SILU 0       /* g sigmoid(g)                                     */
 #define PAL_ACT_GELU 1       /* g (1 + erf(g / sqrt 2)) / 2                      */
@@ -592,6 +592,7 @@ typedef struct PalMlpDims {
   int32_t out_dim;      /* of y                                                 */
   int32_t dtype;        /* PAL_DTYPE_* of every tensor                          */
   int32_t activation;   /* PAL_ACT_*                                            */
+  int32_t hidden_pad;   /* 0 to 7: the last ones of hidden are padding, whose columns of g, u, h and their gradients are zero even beside an infinity */
 } PalMlpDims;
 
 typedef struct PalMlpTensors {

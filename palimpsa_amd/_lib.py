@@ -12,7 +12,7 @@ from typing import Optional
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "lib", "libpalimpsa_hip.so")
 
-PAL_ABI_VERSION = 4
+PAL_ABI_VERSION = 5
 PAL_DTYPE_F32, PAL_DTYPE_BF16 = 0, 1
 PAL_FLAG_VARLEN, PAL_FLAG_HAS_INIT, PAL_FLAG_STORE_FINAL, PAL_FLAG_HAS_VAR = 1, 2, 4, 8
 PAL_FLAG_STATES_TWO_KERNELS, PAL_FLAG_STATES_ONE_PASS, PAL_FLAG_FP32_FAST = 256, 512, 1024
@@ -125,7 +125,7 @@ PAL_ACT = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 
 class PalMlpDims(C.Structure):
     _fields_ = ([(n, C.c_int64) for n in ("rows", "x_stride")] +
-                [(n, C.c_int32) for n in ("dim", "hidden", "out_dim", "dtype", "activation")])
+                [(n, C.c_int32) for n in ("dim", "hidden", "out_dim", "dtype", "activation", "hidden_pad")])
 
 
 class PalMlpTensors(C.Structure):

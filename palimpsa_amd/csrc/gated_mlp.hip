@@ -32,6 +32,7 @@ struct FewArgs {
   int32_t rows, n, k, act;
   const void* x_low;         // bf16 rows of h: what its rounding left, to be added to x
   void* out_low;
+  int32_t used;              // gated: see TileArgs
 };
 
 // R groups of sixteen rows of x.  The waves of a workgroup (as many as it has) take spans of 128 bytes of k in turn, four of them in one go (two of
@@ -122,6 +123,13 @@ __global__ __launch_bounds__(GATED ? 512 : 1024) void few_rows_kernel(FewArgs P)
     const int64_t at = row * P.out_ld + n;
     if constexpr (GATED) {
       float c[8];
+      if (n + 8 > P.used) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          t[0][e] = n + e < P.used ? t[0][e] : 0.f;
+          t[1][e] = n + e < P.used ? t[1][e] : 0.f;
+        }
+      }
       activate8<false>(P.act, t[0], c, nullptr);
 #pragma unroll
       for (int e = 0; e < 8; ++e) c[e] *= t[1][e];
@@ -376,6 +384,7 @@ static int check_mlp(const PalMlpDims* d) {
   if (d->activation < 0 || d->activation > PAL_ACT_RELU) return PAL_E_DIM;
   for (int32_t n : {d->dim, d->hidden, d->out_dim})
     if (n <= 0 || n % 8 || n > 1 << 20) return PAL_E_DIM;
+  if (d->hidden_pad < 0 || d->hidden_pad > 7) return PAL_E_DIM;
   if (d->rows <= 0 || d->rows > 1 << 30 || d->x_stride < d->dim || d->x_stride % 8) return PAL_E_DIM;
   // a tile's rows are reached by offsets of 31 bits from its first
   if (d->x_stride > (int64_t)1 << 20) return PAL_E_DIM;
@@ -413,6 +422,7 @@ static void plan_fwd(const PalMlpDims* d, const PalMlpTensors* t, const void* h,
   m.up.prod[0].ldc = ld;
   m.up.kept = kept_in(d, t->kept);
   m.up.act = d->activation;
+  m.up.used = d->hidden - d->hidden_pad;
   m.down.n_prod = 1;
   m.down.k = d->hidden;
   m.down.prod[0].a = operand(h, ld, es, d->rows);
@@ -434,6 +444,7 @@ static void plan_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGr
   m.grad.kept = kept_in(d, t->kept);
   m.grad.c2 = du;
   m.grad.act = d->activation;
+  m.grad.used = d->hidden - d->hidden_pad;
   m.p_grad = plan_tiles(m.grad, kTileGrad, d->dtype);
   m.dx.n_prod = 1;
   m.dx.k = d->hidden;
@@ -477,9 +488,10 @@ static int mlp_fwd(const PalMlpDims* d, const PalMlpTensors* t, char* ws, hipStr
   if (plan_few(d, t, h, m)) {
     const int64_t ld = hidden_ld(d);
     void* low = t->kept ? ws : ws + rows_bytes(d);
-    FewArgs up{t->x, t->w_gate, t->w_up, h, kept_in(d, t->kept), d->x_stride, ld, (int32_t)d->rows, d->hidden, d->dim, d->activation, nullptr, low};
+    FewArgs up{t->x, t->w_gate, t->w_up, h, kept_in(d, t->kept), d->x_stride, ld, (int32_t)d->rows, d->hidden, d->dim, d->activation, nullptr, low,
+               d->hidden - d->hidden_pad};
     if (int rc = few_launch<T, true>(up, s)) return rc;
-    FewArgs down{h, t->w_down, nullptr, t->y, Kept{}, ld, d->out_dim, (int32_t)d->rows, d->out_dim, d->hidden, 0, low, nullptr};
+    FewArgs down{h, t->w_down, nullptr, t->y, Kept{}, ld, d->out_dim, (int32_t)d->rows, d->out_dim, d->hidden, 0, low, nullptr, 0};
     return few_launch<T, false>(down, s);
   }
   float* part = (float*)(t->kept ? ws : ws + rows_bytes(d));

@@ -716,6 +716,7 @@ struct MlpCall {
     d.x_stride = copied[0] ? MlpCopies::up8(D) : x_ld;
     d.dim = (int32_t)MlpCopies::up8(D); d.hidden = (int32_t)MlpCopies::up8(F); d.out_dim = (int32_t)MlpCopies::up8(Do);
     d.dtype = pal_type(type); d.activation = (int32_t)act;
+    d.hidden_pad = d.hidden - (int32_t)F;
     ok = true;
   }
   // rows and columns of x (0), of the weights

@@ -66,6 +66,7 @@ struct TileArgs {
   Kept kept;
   void* c2;            // [m][n] beside C, rows as far apart
   int32_t act;
+  int32_t used;        // columns of C from here on are padding
 };
 
 enum TileKind {
@@ -528,6 +529,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_product_kernel(TileArgs 
     }
     const int j = lane & 15, g = lane >> 4, m0 = at_tile.m0 + wave / WN * 16 * NFM;
     const int n0 = at_tile.n0 + wave % WN * (kCols / WN) + 8 * g;
+    if constexpr (KIND == kTileGated || KIND == kTileGrad) {
+      // Columns of padding are zero whatever the product is: the weights are zero there, but beside an infinity in a row of x or dy it is a NaN, which
+      // the next product, over these columns, would spread over the whole row.
+      if (P.used < N && at_tile.n0 + kCols > P.used) {
+#pragma unroll
+        for (int n = 0; n < NFN; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool own = n0 + (KIND == kTileGated ? 0 : 32 * (n >> 1)) + 4 * (n & 1) + e < P.used;
+#pragma unroll
+            for (int m = 0; m < NFM; ++m) acc[m][n][e] = own ? acc[m][n][e] : 0.f;
+          }
+      }
+    }
     if constexpr (KIND == kTileGrad) {
       if (P.splits == 1) {
         // The factors are on their way kAhead fragments ahead of their use: a wait for them is one for the stores that went out before them.

@@ -77,7 +77,7 @@ class GatedMlp(torch.autograd.Function):
         xc, xs = _rows(x, cd)
         wg, wu, wd = (_matrix(w, cd) for w in (w_gate, w_up, w_down))
         dims = L.PalMlpDims(rows=rows, x_stride=xs, dim=_up8(D), hidden=_up8(Fh), out_dim=_up8(Do), dtype=cm._pal_dtype(cd),
-                            activation=L.PAL_ACT[activation])
+                            activation=L.PAL_ACT[activation], hidden_pad=_up8(Fh) - Fh)
         y = torch.empty((rows, _up8(Do)), dtype=cd, device=dev)
         lib = L.load()
         kept = torch.empty(int(lib.pal_gated_mlp_kept_bytes(dims)), dtype=torch.uint8, device=dev) if any(ctx.needs_input_grad) else None
