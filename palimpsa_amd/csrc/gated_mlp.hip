@@ -432,6 +432,8 @@ static void plan_fwd(const PalMlpDims* d, const PalMlpTensors* t, const void* h,
   m.p_up = plan_tiles(m.up, kTileGated, d->dtype);
   m.p_down = plan_tiles(m.down, kTilePlain, d->dtype);
 }
+// the gradient of h, and dg and du with it, is for these; that of w_down takes h alone
+static bool wants_dh(const PalMlpGrads* g) { return g->dx || g->dw_gate || g->dw_up; }
 static void plan_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrads* g, void* dg, void* du, MlpPlan& m) {
   const size_t es = mlp_elem(d);
   const int64_t ld = hidden_ld(d);
@@ -445,7 +447,7 @@ static void plan_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGr
   m.grad.c2 = du;
   m.grad.act = d->activation;
   m.grad.used = d->hidden - d->hidden_pad;
-  m.p_grad = plan_tiles(m.grad, kTileGrad, d->dtype);
+  if (wants_dh(g)) m.p_grad = plan_tiles(m.grad, kTileGrad, d->dtype);
   m.dx.n_prod = 1;
   m.dx.k = d->hidden;
   m.dx.prod[0].a = operand(dg, ld, es, d->rows, du);
@@ -500,11 +502,12 @@ static int mlp_fwd(const PalMlpDims* d, const PalMlpTensors* t, char* ws, hipStr
 }
 template <typename T>
 static int mlp_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrads* g, char* ws, hipStream_t s) {
-  const size_t n = rows_bytes(d);
+  const size_t n = wants_dh(g) ? rows_bytes(d) : 0;
   MlpPlan m;
   plan_bwd(d, t, g, ws, ws + n, m);
   float* part = (float*)(ws + 2 * n);
-  if (int rc = tile_run<T, kTileGrad, false, true>(m.grad, m.p_grad, part, kKernMlpGrad, s)) return rc;
+  if (wants_dh(g))
+    if (int rc = tile_run<T, kTileGrad, false, true>(m.grad, m.p_grad, part, kKernMlpGrad, s)) return rc;
   if (g->dx)
     if (int rc = tile_run<T, kTileTwice, false, true>(m.dx, m.p_dx, part, kKernMlpDx, s)) return rc;
   if (m.dw.n_prod) return tile_run<T, kTilePlain, true, true>(m.dw, m.p_dw, part, kKernMlpDw, s);
@@ -569,7 +572,7 @@ extern "C" size_t pal_gated_mlp_bwd_workspace_bytes(const PalMlpDims* d, const P
   PalMlpTensors t{};
   plan_bwd(d, &t, g, nullptr, nullptr, m);
   const size_t part = most_of(part_bytes(m.dx, m.p_dx, kTileTwice), part_bytes(m.dw, m.p_dw, kTilePlain));
-  return 2 * rows_bytes(d) + most_of(part_bytes(m.grad, m.p_grad, kTileGrad), part);
+  return (wants_dh(g) ? 2 * rows_bytes(d) : 0) + most_of(part_bytes(m.grad, m.p_grad, kTileGrad), part);
 }
 extern "C" int pal_gated_mlp_bwd(const PalMlpDims* d, const PalMlpTensors* t, const PalMlpGrads* g, void* workspace, size_t workspace_bytes,
                                  void* stream) {
@@ -579,7 +582,8 @@ extern "C" int pal_gated_mlp_bwd(const PalMlpDims* d, const PalMlpTensors* t, co
   for (const void* p : {t->x, t->w_gate, t->w_up, t->w_down, (const void*)t->kept, g->dy, (const void*)g->dx, (const void*)g->dw_gate,
                         (const void*)g->dw_up, (const void*)g->dw_down})
     if (!is_aligned16(p)) return PAL_E_ALIGN;
-  if (!workspace || workspace_bytes < pal_gated_mlp_bwd_workspace_bytes(d, g)) return PAL_E_WORKSPACE;
+  const size_t need = pal_gated_mlp_bwd_workspace_bytes(d, g);
+  if (need && (!workspace || workspace_bytes < need)) return PAL_E_WORKSPACE;
   if (!is_aligned16(workspace)) return PAL_E_ALIGN;
   return d->dtype == PAL_DTYPE_BF16 ? mlp_bwd<bf16_t>(d, t, g, (char*)workspace, (hipStream_t)stream)
                                     : mlp_bwd<float>(d, t, g, (char*)workspace, (hipStream_t)stream);
