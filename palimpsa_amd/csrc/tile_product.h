@@ -88,7 +88,7 @@ __device__ __forceinline__ void act_silu(float g, float& a, float& d) {
 }
 template <bool GRAD>
 __device__ __forceinline__ void act_gelu(float g, float& a, float& d) {
-  const float f = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+  const float f = 0.5f * erfcf(g * -0.70710678118654752f);   // (1 + erf(-x) has no bits left from x = 4 on; the fp32 training step of 1503 rows, 771 -> 2058: 512 us with it, 516 so)
   a = g * f;
   if (GRAD) d = fmaf(g * 0.39894228040143268f, __expf(-0.5f * g * g), f);
 }
