@@ -621,6 +621,13 @@ typedef struct PalMatrixCopy {
 } PalMatrixCopy;
 int pal_copy_matrices(const PalMatrixCopy *m, int32_t n, int32_t dtype, void *stream);
 
+/* Which tiles the products of a call take, for tests and measurements: of up, down, the gradients of h, of x and of the weights the rows and columns of a
+ * tile, the shares of k and the tiles in all.  Zeros for a product that is not made, and for up and down of a call by the kernels of few rows. */
+typedef struct PalMlpForms {
+  int32_t tile_rows[5], tile_cols[5], shares[5], tiles[5];
+} PalMlpForms;
+int pal_gated_mlp_forms(const PalMlpDims *dims, const PalMlpGrads *gr, PalMlpForms *forms); /* gr: which gradients are wanted, or NULL for a forward alone */
+
 size_t pal_gated_mlp_kept_bytes(const PalMlpDims *dims);
 size_t pal_gated_mlp_fwd_workspace_bytes(const PalMlpDims *dims, int keeps); /* keeps: with t->kept */
 int pal_gated_mlp_fwd(const PalMlpDims *dims, const PalMlpTensors *t, void *workspace, size_t workspace_bytes, void *stream);

@@ -136,6 +136,10 @@ class PalMlpGrads(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("dy", "dx", "dw_gate", "dw_up", "dw_down")]
 
 
+class PalMlpForms(C.Structure):
+    _fields_ = [(n, C.c_int32 * 5) for n in ("tile_rows", "tile_cols", "shares", "tiles")]
+
+
 class PalMatrixCopy(C.Structure):
     _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p)] + [(n, C.c_int64) for n in ("src_ld", "dst_ld", "rows", "cols", "dst_rows", "dst_cols")]
 
@@ -234,6 +238,8 @@ def load() -> C.CDLL:
     lib.pal_gated_mlp_fwd.restype = lib.pal_gated_mlp_bwd.restype = C.c_int
     lib.pal_gated_mlp_fwd.argtypes = [P(PalMlpDims), P(PalMlpTensors), C.c_void_p, C.c_size_t, C.c_void_p]
     lib.pal_gated_mlp_bwd.argtypes = [P(PalMlpDims), P(PalMlpTensors), P(PalMlpGrads), C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.pal_gated_mlp_forms.restype = C.c_int
+    lib.pal_gated_mlp_forms.argtypes = [P(PalMlpDims), P(PalMlpGrads), P(PalMlpForms)]
     lib.pal_copy_matrices.restype = C.c_int
     lib.pal_copy_matrices.argtypes = [P(PalMatrixCopy), C.c_int32, C.c_int32, C.c_void_p]
     lib.pal_layer_norm_fwd.restype = lib.pal_layer_norm_bwd.restype = lib.pal_dropout.restype = C.c_int

@@ -540,6 +540,31 @@ extern "C" int pal_copy_matrices(const PalMatrixCopy* m, int32_t n, int32_t dtyp
   return PAL_OK;
 }
 
+extern "C" int pal_gated_mlp_forms(const PalMlpDims* d, const PalMlpGrads* g, PalMlpForms* forms) {
+  using namespace pal;
+  if (int rc = check_mlp(d)) return rc;
+  if (!forms) return PAL_E_NULL;
+  *forms = PalMlpForms{};
+  MlpPlan m;
+  PalMlpTensors t{};
+  auto put = [&](int i, const TilePlan& p, int kind) {
+    if (!p.tiles) return;
+    forms->tile_rows[i] = kTileShapes[p.form].m;
+    forms->tile_cols[i] = tile_cols(p.form, kind);
+    forms->shares[i] = p.splits;
+    forms->tiles[i] = p.tiles;
+  };
+  if (!plan_few(d, &t, nullptr, m)) {
+    put(0, m.p_up, kTileGated);
+    put(1, m.p_down, kTilePlain);
+  }
+  if (!g) return PAL_OK;
+  plan_bwd(d, &t, g, nullptr, nullptr, m);
+  put(2, m.p_grad, kTileGrad);
+  put(3, m.p_dx, kTileTwice);
+  put(4, m.p_dw, kTilePlain);
+  return PAL_OK;
+}
 extern "C" size_t pal_gated_mlp_kept_bytes(const PalMlpDims* d) {
   using namespace pal;
   return check_mlp(d) == PAL_OK ? 3 * rows_bytes(d) : 0;
