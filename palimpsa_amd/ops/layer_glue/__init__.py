@@ -558,8 +558,9 @@ class Dropout(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         p, seed, site = ctx.meta
-        cm.check_saved(ctx.saved_tensors, ctx.form, "dropout")
-        return Dropout._run(dy, p, seed, ctx.saved_tensors[0], site), None, None, None, None
+        saved = ctx.saved_tensors
+        cm.check_saved(saved, ctx.form, "dropout")
+        return Dropout._run(dy, p, seed, saved[0], site), None, None, None, None
 
 
 def dropout(x: torch.Tensor, p: float, seed, site: int = 0) -> torch.Tensor:
@@ -634,8 +635,8 @@ class LayerNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dres=None):
-        cm.check_saved(ctx.saved_tensors, ctx.form, "layer_norm")
-        rows, w, stats, seed_t = ctx.saved_tensors
+        rows, w, stats, seed_t = saved = ctx.saved_tensors
+        cm.check_saved(saved, ctx.form, "layer_norm")
         m = ctx.meta
         w, stats = w.contiguous(), stats.contiguous()
         rows, stride = _norm_rows(rows.contiguous() if m["handed_on"] else rows, rows.dtype)
