@@ -245,10 +245,10 @@ __global__ __launch_bounds__(256) void copy_matrices_kernel(CopyArgs A) {
 // workgroup a compute unit; 128 x 128 by four, two of them, where there are few tiles; of fp32 rows 64 x 64 (64 x 128 of gated products).
 // Products of bf16 rows are bound by the reads and writes of LDS, of which a large tile has less per number; those of fp32 rows by the matrix units,
 // whose share of a compute unit a tile of any size uses in full: they take the tiles that spread best, and a unit's tiles count one by one.
-// Measured with 256 x 256, 256 x 192 and 128 x 128: 16384 rows of bf16, 768 -> 2048 gated 134, -, 148 us, back to 768 65, 57, 67, gradient of h 121, 131,
-// 118, of x 138, 129, 142, of the weights with shares 208, 229, 237; 8192 rows, 5632 -> 2048 170, 227, 217.  1503 rows of fp32, the
-// weights' gradients (771 x 2058, three) with 256, 128 and 64: 217, 167, 157.  Shares of k against none: those of the 16384 rows 213 and 311 us, 48 rows
-// of bf16 2048 -> 5632 gated 23 and 29, back 20 and 65.
+// Measured (a kernel between two events, in a pass over the whole block) with 256 x 256, 256 x 192 and 128 x 128: 16384 rows of bf16, 768 -> 2048 gated 127, -,
+// 142 us, back to 768 63, 56, 63, gradient of h 112, 131, 117, of x 135, 125, 138, of the weights with shares 185, 200, 206; 8192 rows, 5632 -> 2048 145, 203,
+// 197.  1503 rows of fp32, the weights' gradients (771 x 2058, three) with 256, 128 and 64: 193, 148, 146.  Shares of k, with their sum, against none: the
+// weights' gradients of the 16384 rows 185 + 13 and 292 us, 48 rows of bf16 2048 -> 5632 gated 17 + 7 and 27, back 14 + 7 and 61.
 enum TileForm { kTileBig = 0, kTileNarrow, kTileSmall, kTileTiny, kTileForms };
 struct TileShape {
   int m, n, slots;           // of the chip, bf16 rows

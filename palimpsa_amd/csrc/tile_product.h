@@ -21,8 +21,8 @@
 //
 // Bound by LDS: a step of 256 x 256 of bf16 rows keeps the matrix units busy for 2048 cycles, and its loads (16 cycles a KB) and reads (10 a KB of 16-byte
 // ones, 13 of transposing ones) with them take 2950 cycles with both operands in rows, 3200 with one and 3700 with both in columns; under a long load
-// by power too (clocks of 1.4 to 2.1 GHz).  8192 rows of 5632 by 2048 columns: 160 us, 1.18 PFLOP/s, where a large library product reaches 1.43.  fp32
-// rows are bound by the matrix units: 127 to 143 TFLOP/s where tiles fill the chip, the library's 153.
+// by power too (clocks of 1.4 to 2.1 GHz).  8192 rows of 5632 by 2048 columns: 145 us, 1.30 PFLOP/s, and 160 us among many of them, where a large library
+// product reaches 1.43.  fp32 rows are bound by the matrix units: 127 to 143 TFLOP/s where tiles fill the chip, the library's 153.
 //
 // Whatever lies behind a matrix (rows behind the last one, k behind the end) is read as zero: by the bounds of the buffer for whole rows,
 // by an address beyond all bounds for the rest of a row.
@@ -86,9 +86,10 @@ __device__ __forceinline__ void act_silu(float g, float& a, float& d) {
   a = g * f;
   if (GRAD) d = f * fmaf(g, 1.f - f, 1.f);
 }
+// (erfc: 1 + erf(-x) has no bits left from x = 4 on.  The fp32 training step of 1503 rows, 771 -> 2058 -> 771: 512 us with erf, 516 so.)
 template <bool GRAD>
 __device__ __forceinline__ void act_gelu(float g, float& a, float& d) {
-  const float f = 0.5f * erfcf(g * -0.70710678118654752f);   // (1 + erf(-x) has no bits left from x = 4 on; the fp32 training step of 1503 rows, 771 -> 2058: 512 us with it, 516 so)
+  const float f = 0.5f * erfcf(g * -0.70710678118654752f);
   a = g * f;
   if (GRAD) d = fmaf(g * 0.39894228040143268f, __expf(-0.5f * g * g), f);
 }
