@@ -135,8 +135,9 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 
     Gradients for x and the weights.  The product of the two projections is rounded once to the type of the rows between the kernels, and so
     are the gradients of the projections; sums are in fp32.  For the backward pass the two projections and their product are kept, six bytes per
-    row and hidden entry of bf16 rows, twelve of fp32 rows.  Rows and weights all in bf16, or everything is computed from fp32.  Dims that
-    are no multiple of eight, up to 2^20, are padded by a copy; up to 2^30 rows.  Calls of few rows are bound by the reading of the weights."""
+    row and hidden entry of bf16 rows, twelve of fp32 rows.  Rows and weights all in bf16, or everything is computed from fp32, under autocast too
+    (fp32 master weights beside bf16 rows: pass ``w.bfloat16()``, a sixth of the time).  Dims that are no multiple of eight, up to 2^20, are padded by
+    a copy; up to 2^30 rows.  Calls of few rows are bound by the reading of the weights."""
     if not torch.compiler.is_compiling() and x.is_cuda and activation in L.PAL_ACT:
         r = L.host().gated_mlp(x, w_gate, w_up, w_down, L.PAL_ACT[activation])
         if r is not None:
