@@ -7,7 +7,7 @@ import torch
 PRODUCTS = ("up", "down", "grad", "dx", "dw")
 STEP = {"bf16": 64, "fp32": 32}          # k of a step
 SIZES = {                                # rows, dim, hidden, out_dim
-    "bf16": [(935, 542, 197, 164), (168, 249, 2056, 748), (39591, 526, 144, 173), (22126, 1670, 8, 1101), (53986, 130, 197, 271), (30729, 1185, 174, 400),
+    "bf16": [(935, 542, 197, 164), (168, 249, 2056, 748), (39591, 526, 144, 173), (22126, 1670, 8, 1101), (53986, 130, 197, 271), (30801, 1185, 174, 400),
              (16638, 11, 1993, 151), (32877, 251, 338, 299), (10480, 161, 5422, 398), (10953, 8, 133, 2282), (159, 2850, 5530, 1860), (1700, 2385, 1677, 16),
              (36313, 135, 1861, 21), (131, 2572, 2129, 128), (39373, 276, 68, 32), (133, 1299, 4909, 149), (131, 1540, 4957, 16), (11079, 507, 5063, 30)],
     "fp32": [(78, 82, 65, 75), (74, 624, 1803, 463), (27381, 77, 76, 82), (4150, 90, 1508, 65), (4230, 1327, 94, 2891), (18367, 65, 2015, 94),
